@@ -7,6 +7,8 @@ values it actually used to the backward; the backward allocates dQ/dK/dV(/dB) an
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 import warnings
 
 import torch
@@ -28,7 +30,19 @@ except ImportError as e:      # (built where torch was missing, had no CUDA or w
             return None
 
         @staticmethod
+        def relative_bias(*args):
+            return None
+
+        @staticmethod
+        def dropout(*args):
+            return None
+
+        @staticmethod
         def set_python_backward(fn):
+            pass
+
+        @staticmethod
+        def set_python_function(name, fn):
             pass
 
         @classmethod
@@ -296,3 +310,202 @@ def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.
     ct, wl, wr = flash.translate_causal(bool(is_causal))
     return op_attn_fwd(query, key, value, attn_mask, float(scale), float(dropout_p), ct, wl, wr, philox_seed,
                        philox_offset1)[0]
+
+
+# ---------------------------------------------------------------------------------------------
+# What stands around attention in a layer.  The reference has neither.
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _launch(fn, device, args):
+    """An entry point of the C-ABI on the device's current stream."""
+    return fn(args, torch.cuda.current_stream(device).cuda_stream)
+
+
+@functools.lru_cache(maxsize=None)
+def relative_position_borders(buckets, max_distance):
+    """The smallest distance of each bucket of one direction but the first, as a tuple of whole numbers: the first half of the buckets (e)
+    has a distance each, bucket k beyond takes the distances from e * (max_distance / e) ** ((k - e) / (buckets - e)) on.  Compared in
+    whole numbers: a logarithm in floating point puts distances next to a border on either side of it."""
+    e = buckets // 2
+    if buckets < 2 or max_distance <= e:
+        raise ValueError(f"relative position buckets: {buckets} a direction up to distance {max_distance}: at least 2, and a distance above {e}, are needed")
+    borders = list(range(1, e + 1))
+    for k in range(e + 1, buckets):
+        lo, hi = borders[-1], max_distance      # the smallest r with (r / e) ** (buckets - e) >= (max_distance / e) ** (k - e)
+        most = e ** (buckets - k) * max_distance ** (k - e)
+        while lo < hi:
+            mid = (lo + hi) // 2
+            if mid ** (buckets - e) >= most:
+                hi = mid
+            else:
+                lo = mid + 1
+        borders.append(lo)
+    return tuple(borders)
+
+
+@functools.lru_cache(maxsize=None)
+def _borders_bytes(buckets, max_distance):
+    return bytes((ctypes.c_int32 * (buckets - 1))(*relative_position_borders(buckets, max_distance)))
+
+
+def _bias_rows(heads, sq, sk, dtype, device):
+    """(1, heads, sq, sk) with rows of a multiple of 32 bytes, which the kernels that read and write it take 16 or 32 bytes at a time."""
+    per = 32 // dtype.itemsize
+    return torch.empty((1, heads, sq, (sk + per - 1) // per * per), device=device, dtype=dtype)[..., :sk]
+
+
+class _RelativeBias(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, sq, sk, batch, borders, bidirectional, query_offset, dtype):
+        bias = _bias_rows(table.shape[1], sq, sk, dtype, table.device)
+        if bias.numel():
+            a = cabi.make_relative_bias_args(table, bias, borders, bidirectional=bidirectional, query_offset=query_offset)
+            _check(hipError_t(_launch(cabi.lib().ab200_relative_bias_fwd, table.device, a)), "relative_bias_fwd")
+        ctx.args = (borders, bidirectional, query_offset)
+        ctx.like = (table.shape, table.dtype)
+        return bias.expand(batch, -1, -1, -1)
+
+    @staticmethod
+    def backward(ctx, grad):
+        return (_RelativeBiasGrad.apply(grad, *ctx.like, *ctx.args),) + (None,) * 7
+
+
+class _RelativeBiasGrad(torch.autograd.Function):
+    """The table's gradient; linear in its input, its own derivative is the bias again."""
+
+    @staticmethod
+    def forward(ctx, grad, shape, dtype, borders, bidirectional, query_offset):
+        table = torch.empty(shape, device=grad.device, dtype=dtype)
+        ctx.args = (*grad.shape[2:], grad.shape[0], borders, bidirectional, query_offset, grad.dtype)
+        if not grad.numel():
+            return table.zero_()
+        kw = dict(bidirectional=bidirectional, query_offset=query_offset)
+        need = _launch(cabi.lib().ab200_relative_bias_workspace, grad.device, cabi.make_relative_bias_args(table, grad, borders, **kw))
+        if need < 0:
+            _check(hipError_t(-need), "relative_bias_bwd")
+        workspace = torch.empty([need], device=grad.device, dtype=torch.float32)
+        a = cabi.make_relative_bias_args(table, grad, borders, workspace=workspace, **kw)
+        _check(hipError_t(_launch(cabi.lib().ab200_relative_bias_bwd, grad.device, a)), "relative_bias_bwd")
+        return table
+
+    @staticmethod
+    def backward(ctx, grad):
+        return (_RelativeBias.apply(grad, *ctx.args),) + (None,) * 5
+
+
+def relative_position_bias(table, seqlen_q, seqlen_k, batch=1, max_distance=128, bidirectional=True, query_offset=0, dtype=None):
+    """The additive bias of `attention` from a learned (buckets, heads) table: (batch, heads, seqlen_q, seqlen_k), the batch axis
+    with stride 0, bias[b, h, m, n] = table[bucket(n - m - query_offset), h].
+
+    Distances r have a bucket each up to half of a direction's buckets, and share the others evenly over their logarithm up to
+    max_distance, beyond which all have the last (relative_position_borders).  Bidirectional: r = |n - m - query_offset|, keys behind
+    the query's position take the second half of the table (whose size is even); otherwise later keys count as distance 0.  query_offset is the position of
+    query 0 among the keys: seqlen_k - 1 for the last token alone.  `dtype`: of the bias, the table's own where not given; fp32, fp16 or
+    bf16 each.  The table's gradient is summed over the batch in fp32, in a fixed order."""
+    if table.dim() != 2 or table.dtype not in _FLOATS or not table.is_cuda:
+        raise ValueError("relative_position_bias: the table is a (buckets, heads) CUDA tensor of fp32, fp16 or bf16")
+    dtype = table.dtype if dtype is None else dtype
+    if dtype not in _FLOATS:
+        raise ValueError(f"relative_position_bias: a bias of {dtype} is not supported")
+    buckets = table.shape[0]
+    if bidirectional:
+        if buckets % 2:
+            raise ValueError("relative_position_bias: two directions need an even number of buckets")
+        buckets //= 2
+    if min(seqlen_q, seqlen_k, batch) < 0 or table.shape[1] < 1:
+        raise ValueError("relative_position_bias: negative sizes, or no heads")
+    if buckets > 128:
+        raise ValueError("relative_position_bias: at most 128 buckets a direction")
+    if abs(query_offset) >= 1 << 31:
+        raise ValueError("relative_position_bias: query_offset beyond 32 bits")
+    borders = relative_position_borders(buckets, max_distance)
+    if not torch.compiler.is_compiling():
+        r = _native.relative_bias(table, seqlen_q, seqlen_k, batch, _borders_bytes(buckets, max_distance), bool(bidirectional), query_offset, dtype)
+        if r is not None:
+            return r
+    return _RelativeBias.apply(table, seqlen_q, seqlen_k, batch, borders, bool(bidirectional), query_offset, dtype)
+
+
+def _as_rows(t):
+    """t as (rows, cols) with rows of unit stride: a view where its strides allow one, else a copy."""
+    if t.dim() == 0:
+        return t.view(1, 1)
+    if t.is_contiguous():
+        return t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, 1)
+    try:
+        rows = t.view(-1, t.shape[-1])
+    except RuntimeError:
+        rows = None
+    return rows if rows is not None and (rows.stride(1) == 1 or rows.shape[1] == 1) else t.contiguous().view(-1, t.shape[-1])
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, dropout_p, seed, offset):
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        tensors = [t if isinstance(t, torch.Tensor) else None for t in (seed, offset)]
+        if x.numel():
+            rows, to = _as_rows(x), _as_rows(out)
+            add = None if residual is None else _as_rows(residual)
+            numbers = [0 if isinstance(t, torch.Tensor) else t for t in (seed, offset)]
+            stream = torch.cuda.current_stream(x.device).cuda_stream
+            _check(hipError_t(cabi.dropout(rows, to, dropout_p, residual=add, philox_seed=tensors[0], philox_offset1=tensors[1],
+                                           philox_seed_value=numbers[0], philox_offset2=numbers[1], stream=stream)), "dropout")
+        ctx.save_for_backward(*tensors)      # (changed in place before the backward: refused there)
+        ctx.numbers = (seed, offset)
+        ctx.dropout_p = dropout_p
+        ctx.residual = residual is not None
+        return out
+
+    @staticmethod
+    def backward(ctx, grad):
+        saved = [t if t is not None else n for t, n in zip(ctx.saved_tensors, ctx.numbers)]
+        dx = _Dropout.apply(grad, None, ctx.dropout_p, *saved) if ctx.needs_input_grad[0] else None
+        return dx, grad if ctx.residual and ctx.needs_input_grad[1] else None, None, None, None
+
+
+def _python_dropout(grad, dropout_p, seed, offset):
+    """The gradient of a native call whose own gradient or modes are not ordinary ones (csrc/torch_ops.cc)."""
+    return _Dropout.apply(grad, None, dropout_p, seed, offset)
+
+
+def _python_relative_bias_grad(grad, buckets, heads, dtype, borders, bidirectional, query_offset):
+    borders = tuple((ctypes.c_int32 * (len(borders) // 4)).from_buffer_copy(borders))
+    return _RelativeBiasGrad.apply(grad, (buckets, heads), dtype, borders, bidirectional, query_offset)
+
+
+_native.set_python_function("dropout", _python_dropout)
+_native.set_python_function("relative_bias", _python_relative_bias_grad)
+
+
+def _philox_number(x, what, device):
+    if isinstance(x, torch.Tensor):
+        if x.numel() != 1 or x.dtype not in (torch.int64, torch.uint64) or x.device != device:
+            raise ValueError(f"dropout: {what} is a 64-bit number or a tensor of one on the device of x")
+        return x
+    if type(x) is not int or not 0 <= x < 1 << 64:
+        raise ValueError(f"dropout: {what} is a number from 0 to 2**64 - 1, or a tensor of one")
+    return x
+
+
+def dropout(x, dropout_p, residual=None, philox_seed=DEFAULT_PHILOX_SEED, philox_offset=DEFAULT_PHILOX_OFFSET_1):
+    """residual + dropout(x), for hidden states of any shape: element i in logical order is kept (and divided by 1 - dropout_p) or dropped by word
+    (0, 2, 1, 3)[i % 4] of Philox counter philox_offset + i // 4, the attention's generator and threshold.  The mask is never stored: the backward
+    draws it again.  A layer's calls take offsets at least x.numel() // 4 + 1 apart.
+
+    Seed and offset are numbers, or 64-bit tensors of one element on x's device, which a captured call reads when it is replayed.  x and residual
+    (the same shape and type: fp32, fp16 or bf16) need no particular strides, but what is not rows of unit stride is copied first.
+    The output is contiguous."""
+    if x.dtype not in _FLOATS or not x.is_cuda:
+        raise ValueError("dropout: x is a CUDA tensor of fp32, fp16 or bf16")
+    if not 0.0 <= dropout_p <= 1.0:
+        raise ValueError(f"dropout: dropout_p is {dropout_p}, not a probability")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("dropout: the residual has another shape, type or device than x")
+    if not torch.compiler.is_compiling():
+        r = _native.dropout(x, residual, dropout_p, philox_seed, philox_offset)
+        if r is not None:
+            return r
+    seed, offset = _philox_number(philox_seed, "philox_seed", x.device), _philox_number(philox_offset, "philox_offset", x.device)
+    return _Dropout.apply(x, residual, float(dropout_p), seed, offset)

@@ -29,7 +29,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "build"
 LIB = PKG / "libaotriton_v2.so"
 
-CUDA_SOURCES = ["cabi.cu", "general_kernels.cu", "sm100_fwd.cu", "sm100_bwd.cu"]
+CUDA_SOURCES = ["cabi.cu", "general_kernels.cu", "layer_ops.cu", "sm100_fwd.cu", "sm100_bwd.cu"]
 CXX_SOURCES = ["api.cc"]
 HEADERS = sorted(list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((ROOT / "include").rglob("*.h")))
 

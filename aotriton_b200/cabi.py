@@ -22,7 +22,8 @@ SELECT_ALIGNED, SELECT_DBIAS, SELECT_FUSED_REQUESTED, SELECT_FORCE_GENERAL, SELE
 SYMBOLS = [
     "ab200_attn_fwd", "ab200_attn_bwd", "ab200_attn_bwd_static_scratch", "ab200_bwd_uses_dq_acc",
     "ab200_bwd_fused", "ab200_bwd_postprocess", "ab200_bwd_preprocess", "ab200_bwd_dkdv", "ab200_bwd_dq",
-    "ab200_debug_simulate_encoded_softmax", "ab200_check_gpu", "ab200_multiprocessor_count",
+    "ab200_debug_simulate_encoded_softmax", "ab200_relative_bias_fwd", "ab200_relative_bias_bwd",
+    "ab200_relative_bias_workspace", "ab200_dropout", "ab200_check_gpu", "ab200_multiprocessor_count",
     "ab200_set_kernel_family", "ab200_select_variant", "ab200_last_fwd_family", "ab200_last_bwd_family",
     "ab200_kernel_status", "ab200_stream_check", "ab200_debug_bounded_wait_test", "ab200_debug_keep_tiles",
     "ab200_debug_dk_from_dbias", "ab200_debug_split_keys",
@@ -64,6 +65,23 @@ class BwdArgs(C.Structure):
     ]
 
 
+class RelativeBiasArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("table_dtype", C.c_int32), ("num_buckets", C.c_int32), ("num_heads", C.c_int32),
+        ("bidirectional", C.c_int32), ("query_offset", C.c_int32), ("borders", C.POINTER(C.c_int32)), ("table", C.c_void_p),
+        ("table_stride", C.c_int64 * 2), ("bias", View4), ("workspace", C.c_void_p), ("workspace_floats", C.c_uint64),
+    ]
+
+
+class DropoutArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("dropout_p", C.c_float), ("rows", C.c_int64), ("cols", C.c_int64), ("x", C.c_void_p),
+        ("residual", C.c_void_p), ("out", C.c_void_p), ("x_stride", C.c_int64), ("residual_stride", C.c_int64),
+        ("out_stride", C.c_int64), ("philox_seed", C.c_void_p), ("philox_offset1", C.c_void_p),
+        ("philox_seed_value", C.c_uint64), ("philox_offset2", C.c_uint64),
+    ]
+
+
 _lib = None
 
 
@@ -82,6 +100,10 @@ def lib() -> C.CDLL:
         L.ab200_debug_simulate_encoded_softmax.argtypes = [
             C.POINTER(View4), C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float,
             C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
+        for name in ("ab200_relative_bias_fwd", "ab200_relative_bias_bwd", "ab200_relative_bias_workspace"):
+            getattr(L, name).argtypes = [C.POINTER(RelativeBiasArgs), C.c_void_p]
+        L.ab200_relative_bias_workspace.restype = C.c_int64
+        L.ab200_dropout.argtypes = [C.POINTER(DropoutArgs), C.c_void_p]
         L.ab200_check_gpu.argtypes = [C.c_void_p]
         L.ab200_multiprocessor_count.argtypes = [C.c_void_p]
         L.ab200_select_variant.argtypes = [C.c_int] * 5
@@ -200,3 +222,48 @@ def debug_simulate_encoded_softmax(r, dropout_p, philox_seed, philox_offset1, ph
         C.byref(v), _torch_dtype_code(r), r.shape[0], r.shape[1], r.shape[2], r.shape[3], dropout_p,
         _ptr(philox_seed), _ptr(philox_offset1), philox_offset2,
         stream if stream is not None else current_stream_handle())
+
+
+def make_relative_bias_args(table, bias, borders, *, bidirectional=True, query_offset=0, workspace=None) -> RelativeBiasArgs:
+    """`borders`: the smallest distance of each bucket of a direction but the first.  `bias`: rank 4, written or (its gradient) read."""
+    a = RelativeBiasArgs()
+    a.dtype, a.table_dtype = _torch_dtype_code(bias), _torch_dtype_code(table)
+    a.num_buckets, a.num_heads = table.shape
+    a.bidirectional, a.query_offset = int(bidirectional), query_offset
+    a.borders = (C.c_int32 * len(borders))(*borders)
+    a.table = table.data_ptr()
+    a.table_stride[0], a.table_stride[1] = table.stride()
+    a.bias = view4(bias)
+    if workspace is not None:
+        a.workspace, a.workspace_floats = workspace.data_ptr(), workspace.numel()
+    return a
+
+
+def relative_bias_fwd(table, bias, borders, *, stream=None, **kw) -> int:
+    a = make_relative_bias_args(table, bias, borders, **kw)
+    return lib().ab200_relative_bias_fwd(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def relative_bias_workspace(table, bias, borders, *, stream=None, **kw) -> int:
+    """Floats the backward needs; negative: an error code."""
+    a = make_relative_bias_args(table, bias, borders, **kw)
+    return lib().ab200_relative_bias_workspace(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def relative_bias_bwd(table_grad, bias_grad, borders, *, stream=None, **kw) -> int:
+    a = make_relative_bias_args(table_grad, bias_grad, borders, **kw)
+    return lib().ab200_relative_bias_bwd(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def dropout(x, out, dropout_p, *, residual=None, philox_seed=None, philox_offset1=None, philox_seed_value=0, philox_offset2=0,
+            stream=None) -> int:
+    """x, residual and out: (rows, cols) with unit innermost stride."""
+    a = DropoutArgs()
+    a.dtype, a.dropout_p = _torch_dtype_code(x), dropout_p
+    a.rows, a.cols = x.shape
+    a.x, a.out, a.x_stride, a.out_stride = x.data_ptr(), out.data_ptr(), x.stride(0), out.stride(0)
+    if residual is not None:
+        a.residual, a.residual_stride = residual.data_ptr(), residual.stride(0)
+    a.philox_seed, a.philox_offset1 = _ptr(philox_seed), _ptr(philox_offset1)
+    a.philox_seed_value, a.philox_offset2 = philox_seed_value, philox_offset2
+    return lib().ab200_dropout(C.byref(a), stream if stream is not None else current_stream_handle())

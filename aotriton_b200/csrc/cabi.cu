@@ -14,6 +14,7 @@
 
 #include "../../include/aotriton_b200.h"
 #include "launch.h"
+#include "layer_ops.h"
 
 namespace ab200 {
 
@@ -796,6 +797,86 @@ int ab200_attn_bwd_static_scratch(const ab200_attn_bwd_args* a, void* stream) {
   ab200_attn_bwd_args b = *a;
   b.delta = delta;
   return ab200_attn_bwd(&b, stream);
+}
+
+// --- relative position bias, dropout of hidden states (layer_ops.cu) ----------------------------
+static int fill_relative_bias(const ab200_relative_bias_args* a, RelativeBias& r, bool backward) {
+  if (a == nullptr || a->borders == nullptr || a->table == nullptr || a->bias.ptr == nullptr) return kErrInvalidValue;
+  for (int t : {a->dtype, a->table_dtype})
+    if (t < AB200_DTYPE_FP32 || t > AB200_DTYPE_BF16) return kErrNotSupported;
+  if (a->num_heads <= 0 || a->num_buckets <= 0 || (a->bidirectional && a->num_buckets % 2 != 0)) return kErrInvalidValue;
+  const int per = a->bidirectional ? a->num_buckets / 2 : a->num_buckets;
+  if (per < 2) return kErrInvalidValue;
+  if (per > kMaxBorders + 1) return kErrNotSupported;
+  const int64_t* n = a->bias.size;
+  if (n[0] < 0 || n[2] < 0 || n[3] < 0 || n[1] != a->num_heads || (!backward && n[0] != 1)) return kErrInvalidValue;
+  // (sequence lengths in 32 bits with room for a tile; heads and row tiles are grid dimensions of 16 bits)
+  if (n[2] > 4000000 || n[3] > 1 << 30 || a->num_heads > 65535 || n[0] > INT32_MAX) return kErrNotSupported;
+  r.bias = to_view(a->bias);
+  r.table = a->table;
+  r.table_stride[0] = a->table_stride[0];
+  r.table_stride[1] = a->table_stride[1];
+  r.heads = a->num_heads; r.batch = (int32_t)n[0]; r.sq = (int32_t)n[2]; r.sk = (int32_t)n[3];
+  r.offset = a->query_offset;
+  r.per_direction = per; r.both = a->bidirectional != 0;
+  for (int k = 0; k + 1 < per; ++k) {
+    r.borders[k] = a->borders[k];
+    if (r.borders[k] < (k > 0 ? r.borders[k - 1] : 1)) return kErrInvalidValue;
+  }
+  const int per_vec = a->dtype == AB200_DTYPE_FP32 ? 4 : 8;
+  r.vec = (reinterpret_cast<uintptr_t>(a->bias.ptr) & 15u) == 0 && a->bias.stride[3] == 1;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && a->bias.stride[i] % per_vec != 0) r.vec = 0;
+  return 0;
+}
+
+int ab200_relative_bias_fwd(const ab200_relative_bias_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  RelativeBias r{};
+  if (int e = fill_relative_bias(a, r, false)) return e;
+  if (int e = check_device(st)) return e;
+  DeviceGuard guard(st);
+  return (int)launch_relative_bias(a->dtype, a->table_dtype, r, st);
+}
+
+int64_t ab200_relative_bias_workspace(const ab200_relative_bias_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  RelativeBias r{};
+  if (int e = fill_relative_bias(a, r, true)) return -e;
+  if (int e = check_device(st)) return -e;
+  return plan_relative_bias_backward(a->dtype, r, device_info(stream_device(st)).sms);
+}
+
+int ab200_relative_bias_bwd(const ab200_relative_bias_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  RelativeBias r{};
+  if (int e = fill_relative_bias(a, r, true)) return e;
+  if (int e = check_device(st)) return e;
+  const int64_t need = plan_relative_bias_backward(a->dtype, r, device_info(stream_device(st)).sms);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_floats < (uint64_t)need)) return kErrInvalidValue;
+  r.partial = a->workspace;
+  DeviceGuard guard(st);
+  return (int)launch_relative_bias_backward(a->dtype, a->table_dtype, r, st);
+}
+
+int ab200_dropout(const ab200_dropout_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a == nullptr || a->rows < 0 || a->cols < 0) return kErrInvalidValue;
+  if (a->dtype < AB200_DTYPE_FP32 || a->dtype > AB200_DTYPE_BF16) return kErrNotSupported;
+  if (!(a->dropout_p >= 0.f) || a->dropout_p > 1.f) return kErrInvalidValue;
+  if (a->rows > 0 && a->cols > 0 && (a->x == nullptr || a->out == nullptr)) return kErrInvalidValue;
+  if (a->cols > 0 && a->rows > (INT64_MAX >> 12) / a->cols) return kErrInvalidValue;
+  if (a->rows * a->cols > (int64_t)INT32_MAX << 10) return kErrNotSupported;      // (a grid's width)
+  Dropout d{};
+  d.x = a->x; d.residual = a->residual; d.out = a->out;
+  d.rows = a->rows; d.cols = a->cols; d.sx = a->x_stride; d.sr = a->residual_stride; d.so = a->out_stride;
+  d.seed_ptr = a->philox_seed; d.offset_ptr = a->philox_offset1; d.seed = a->philox_seed_value; d.offset = a->philox_offset2;
+  d.on = a->dropout_p > 0.f;
+  d.scale = d.on ? 1.0f / (1.0f - a->dropout_p) : 1.0f;
+  d.threshold = dropout_threshold(a->dropout_p);
+  if (int e = check_device(st)) return e;
+  DeviceGuard guard(st);
+  return (int)launch_dropout(a->dtype, d, st);
 }
 
 // --- HIP-named runtime helpers used by the Python tests of the reference

@@ -11,6 +11,8 @@
 // one type on the current device with unit innermost stride, and every mode in which an operator call means more than its kernels
 // (dispatch and function modes, functorch transforms, forward-mode gradients, tracing).  The backward asks the same of its
 // gradient, of what was saved and of the modes it runs under, and otherwise leaves itself to the operator or to the Python Function's.
+#include <torch/csrc/Dtype.h>
+#include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -29,6 +31,7 @@
 #include <aotriton_b200.h>
 
 #include <atomic>
+#include <map>
 #include <string>
 
 namespace aotriton = AOTRITON_NS;
@@ -270,6 +273,180 @@ struct Attend : torch::autograd::Function<Attend> {
   }
 };
 
+// ---- what stands around attention -------------------------------------------------------------------------
+// The Python Functions that stand for these operators' backwards where the gradient or the modes are not ordinary ones, or where the
+// backward is to be differentiated in turn.  By name, set at import, kept for the life of the process.
+std::map<std::string, PyObject*>& python_functions() {
+  static std::map<std::string, PyObject*> table;
+  return table;
+}
+pybind11::object wrapped(const Tensor& t) {
+  return t.defined() ? pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(t)) : pybind11::object(pybind11::none());
+}
+// (the GIL is held)
+pybind11::object call_python(const char* name, const pybind11::tuple& args) {
+  auto r = pybind11::reinterpret_steal<pybind11::object>(PyObject_CallObject(python_functions()[name], args.ptr()));
+  if (!r) {
+    python_error e;
+    e.persist();
+    throw e;
+  }
+  return r;
+}
+PyObject* dtype_object(at::ScalarType t) { return reinterpret_cast<PyObject*>(torch::getTHPDtype(t)); }
+
+int32_t code_of(at::ScalarType t) { return t == at::kFloat ? AB200_DTYPE_FP32 : (t == at::kHalf ? AB200_DTYPE_FP16 : AB200_DTYPE_BF16); }
+bool floating(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+void* stream_handle() { return c10::cuda::getCurrentCUDAStream().stream(); }
+ab200_view4 c_view(const Tensor& t) {
+  ab200_view4 v;
+  v.ptr = t.data_ptr();
+  for (int i = 0; i < 4; ++i) { v.size[i] = t.size(i); v.stride[i] = t.stride(i); }
+  return v;
+}
+// A gradient that this file's backwards take as it is.
+bool ordinary_gradient(const Tensor& g, at::ScalarType type) {
+  return !at::GradMode::is_enabled() && plain_modes() && plain(g, c10::cuda::current_device()) && g.scalar_type() == type;
+}
+
+// ---- dropout with the residual's addition ----
+// t as rows of unit stride: (rows, cols, stride between rows); false where its strides give none.
+bool rows_of(const Tensor& t, int64_t* rows, int64_t* cols, int64_t* stride) {
+  if (t.is_contiguous()) {
+    *cols = t.dim() ? t.size(-1) : 1;
+    *rows = t.numel() / *cols;
+    *stride = *cols;
+    return true;
+  }
+  if (t.stride(-1) != 1 && t.size(-1) != 1) return false;
+  *cols = t.size(-1);
+  *rows = 1;
+  *stride = *cols;
+  for (int64_t i = t.dim() - 2; i >= 0; --i) {      // (from the innermost: one stride for all rows)
+    if (t.size(i) == 1) continue;
+    if (*rows == 1) *stride = t.stride(i);
+    else if (t.stride(i) != *stride * *rows) return false;
+    *rows *= t.size(i);
+  }
+  return true;
+}
+Tensor drop(const Tensor& x, const Tensor& residual, double p, uint64_t seed, uint64_t offset) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor out = fresh(x.sizes(), x.scalar_type()), from = x, add = residual;
+  ab200_dropout_args a{};
+  a.dtype = code_of(x.scalar_type());
+  a.dropout_p = (float)p;
+  if (!rows_of(from, &a.rows, &a.cols, &a.x_stride)) {
+    from = from.contiguous();
+    rows_of(from, &a.rows, &a.cols, &a.x_stride);
+  }
+  int64_t rows, cols;
+  if (add.defined() && !rows_of(add, &rows, &cols, &a.residual_stride)) {
+    add = add.contiguous();
+    rows_of(add, &rows, &cols, &a.residual_stride);
+  }
+  a.x = from.data_ptr();
+  a.residual = add.defined() ? add.data_ptr() : nullptr;
+  a.out = out.data_ptr();
+  a.out_stride = a.cols;
+  a.philox_seed_value = seed;
+  a.philox_offset2 = offset;
+  check((hipError_t)ab200_dropout(&a, stream_handle()), "dropout");
+  return out;
+}
+
+struct Drop : torch::autograd::Function<Drop> {
+  using Maybe = std::optional<Tensor>;
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Maybe& residual, double p, uint64_t seed, uint64_t offset) {
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["numbers"] = std::vector<int64_t>{(int64_t)seed, (int64_t)offset, residual.has_value(), (int64_t)x.scalar_type()};
+    ctx->set_materialize_grads(false);
+    return drop(x, residual.value_or(Tensor()), p, seed, offset);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list r(5);
+    const Tensor& g = grads[0];
+    if (!g.defined()) return r;
+    const double p = ctx->saved_data["p"].toDouble();
+    const auto n = ctx->saved_data["numbers"].toIntVector();
+    if (n[2] && ctx->needs_input_grad(1)) r[1] = g;
+    if (!ctx->needs_input_grad(0)) return r;
+    if (ordinary_gradient(g, (at::ScalarType)n[3])) {
+      r[0] = drop(g, Tensor(), p, (uint64_t)n[0], (uint64_t)n[1]);
+    } else {
+      pybind11::gil_scoped_acquire gil;
+      const auto o = call_python("dropout", pybind11::make_tuple(wrapped(g), p, (uint64_t)n[0], (uint64_t)n[1]));
+      r[0] = THPVariable_Unpack(o.ptr());
+    }
+    return r;
+  }
+};
+
+// ---- learned relative position bias ----
+struct BiasCall {
+  int64_t sq, sk, batch, offset;
+  bool both;
+  at::ScalarType type;
+  std::string borders;      // int32 each
+};
+ab200_relative_bias_args bias_args(const Tensor& table, const Tensor& bias, const std::string& borders, bool both, int64_t offset) {
+  ab200_relative_bias_args a{};
+  a.dtype = code_of(bias.scalar_type());
+  a.table_dtype = code_of(table.scalar_type());
+  a.num_buckets = (int32_t)table.size(0);
+  a.num_heads = (int32_t)table.size(1);
+  a.bidirectional = both;
+  a.query_offset = (int32_t)offset;
+  a.borders = reinterpret_cast<const int32_t*>(borders.data());
+  a.table = table.data_ptr();
+  a.table_stride[0] = table.stride(0);
+  a.table_stride[1] = table.stride(1);
+  a.bias = c_view(bias);
+  return a;
+}
+// Rows of a multiple of 32 bytes, which the kernels that write and read them take 16 or 32 bytes at a time.
+Tensor make_bias(const Tensor& table, const BiasCall& c) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const int64_t per = c.type == at::kFloat ? 8 : 16, heads = table.size(1), pitch = (c.sk + per - 1) / per * per;
+  const Tensor store = fresh({heads, c.sq, pitch}, c.type);
+  const Tensor one = store.as_strided({1, heads, c.sq, c.sk}, {0, c.sq * pitch, pitch, 1});
+  const auto a = bias_args(table, one, c.borders, c.both, c.offset);
+  check((hipError_t)ab200_relative_bias_fwd(&a, stream_handle()), "relative_bias_fwd");
+  return store.as_strided({c.batch, heads, c.sq, c.sk}, {0, c.sq * pitch, pitch, 1});
+}
+struct RelativeBias : torch::autograd::Function<RelativeBias> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const BiasCall& c) {
+    ctx->saved_data["numbers"] = std::vector<int64_t>{table.size(0), table.size(1), (int64_t)table.scalar_type(), (int64_t)c.type, c.both, c.offset};
+    ctx->saved_data["borders"] = c.borders;
+    ctx->set_materialize_grads(false);
+    return make_bias(table, c);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list r(2);
+    const Tensor& g = grads[0];
+    if (!g.defined()) return r;
+    const auto n = ctx->saved_data["numbers"].toIntVector();
+    const std::string& borders = ctx->saved_data["borders"].toStringRef();
+    const auto table_type = (at::ScalarType)n[2];
+    if (!ordinary_gradient(g, (at::ScalarType)n[3])) {
+      pybind11::gil_scoped_acquire gil;
+      const auto dt = pybind11::reinterpret_borrow<pybind11::object>(dtype_object(table_type));
+      const auto o = call_python("relative_bias", pybind11::make_tuple(wrapped(g), n[0], n[1], dt, pybind11::bytes(borders), n[4] != 0, n[5]));
+      r[0] = THPVariable_Unpack(o.ptr());
+      return r;
+    }
+    r[0] = fresh({n[0], n[1]}, table_type);
+    auto a = bias_args(r[0], g, borders, n[4] != 0, n[5]);
+    const int64_t need = ab200_relative_bias_workspace(&a, stream_handle());
+    if (need < 0) check((hipError_t)-need, "relative_bias_bwd");
+    const Tensor workspace = fresh({need}, at::kFloat);
+    a.workspace = static_cast<float*>(workspace.data_ptr());
+    a.workspace_floats = (uint64_t)need;
+    check((hipError_t)ab200_relative_bias_bwd(&a, stream_handle()), "relative_bias_bwd");
+    return r;
+  }
+};
+
 // ---- from Python ------------------------------------------------------------------------------------------
 
 // A torch.Tensor or Parameter (no subclass) that is plain().  The tensor itself goes to *out.
@@ -357,6 +534,84 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// A floating-point tensor this file's operators take, of any shape and strides; or not.
+bool floating_tensor(PyObject* o, int dev, Tensor* out) {
+  if (!THPVariable_CheckExact(o)) return false;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!plain(t, dev) || !floating(t.scalar_type())) return false;
+  *out = t;
+  return true;
+}
+bool ordinary_first(PyObject* o) { return THPVariable_CheckExact(o) && THPVariable_Unpack(o).is_cuda() && plain_modes(); }
+
+// dropout(x, residual, dropout_p, philox_seed, philox_offset): the output, or None: not an ordinary call.
+PyObject* dropout(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "dropout takes 5 arguments");
+    return nullptr;
+  }
+  if (!ordinary_first(a[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  Tensor x, residual;
+  double p;
+  uint64_t seed, offset;
+  if (!floating_tensor(a[0], dev, &x) || (a[1] != Py_None && !floating_tensor(a[1], dev, &residual))) Py_RETURN_NONE;
+  if (!number(a[2], &p) || !u64(a[3], &seed) || !u64(a[4], &offset)) Py_RETURN_NONE;
+  Tensor out;
+  {
+    pybind11::gil_scoped_release release;
+    if (at::GradMode::is_enabled() && (x.requires_grad() || (residual.defined() && residual.requires_grad())))
+      out = Drop::apply(x, residual.defined() ? Drop::Maybe(residual) : Drop::Maybe(), p, seed, offset);
+    else
+      out = drop(x, residual, p, seed, offset);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// relative_bias(table, seqlen_q, seqlen_k, batch, borders, bidirectional, query_offset, dtype): the bias, or None: not an ordinary call.
+PyObject* relative_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) {
+    PyErr_SetString(PyExc_TypeError, "relative_bias takes 8 arguments");
+    return nullptr;
+  }
+  if (!ordinary_first(a[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  Tensor table;
+  BiasCall c{};
+  if (!floating_tensor(a[0], dev, &table) || table.dim() != 2) Py_RETURN_NONE;
+  if (!small_int(a[1], &c.sq) || !small_int(a[2], &c.sk) || !small_int(a[3], &c.batch) || !small_int(a[6], &c.offset)) Py_RETURN_NONE;
+  if (c.sq <= 0 || c.sk <= 0 || c.batch <= 0 || !PyBytes_CheckExact(a[4]) || !THPDtype_Check(a[7])) Py_RETURN_NONE;
+  c.borders.assign(PyBytes_AS_STRING(a[4]), PyBytes_GET_SIZE(a[4]));
+  c.both = a[5] == Py_True;
+  c.type = reinterpret_cast<THPDtype*>(a[7])->scalar_type;
+  if (!floating(c.type)) Py_RETURN_NONE;
+  Tensor out;
+  {
+    pybind11::gil_scoped_release release;
+    out = at::GradMode::is_enabled() && table.requires_grad() ? RelativeBias::apply(table, c) : make_bias(table, c);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// set_python_function(name, fn): what python_functions() holds.
+PyObject* set_python_function(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2 || !PyUnicode_Check(a[0])) {
+    PyErr_SetString(PyExc_TypeError, "set_python_function takes a name and a function");
+    return nullptr;
+  }
+  Py_INCREF(a[1]);
+  PyObject*& slot = python_functions()[PyUnicode_AsUTF8(a[0])];
+  Py_XDECREF(slot);
+  slot = a[1];
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* last_bwd_family(PyObject*, PyObject*) { return PyLong_FromLong(g_last_bwd_family.load(std::memory_order_relaxed)); }
 // ... of a backward that ran on this thread by the Python way
 PyObject* note_bwd_family(PyObject*, PyObject*) {
@@ -374,6 +629,9 @@ PyObject* set_python_backward(PyObject*, PyObject* fn) {
 }
 
 PyMethodDef kMethods[] = {{"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&attend)), METH_FASTCALL, nullptr},
+                          {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&dropout)), METH_FASTCALL, nullptr},
+                          {"relative_bias", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&relative_bias)), METH_FASTCALL, nullptr},
+                          {"set_python_function", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&set_python_function)), METH_FASTCALL, nullptr},
                           {"set_python_backward", &set_python_backward, METH_O, nullptr},
                           {"last_bwd_family", &last_bwd_family, METH_NOARGS, nullptr},
                           {"note_bwd_family", &note_bwd_family, METH_NOARGS, nullptr},

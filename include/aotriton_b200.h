@@ -190,6 +190,54 @@ AB200_API int ab200_debug_simulate_encoded_softmax(const ab200_view4* r, int32_t
                                                    const uint64_t* philox_offset1,
                                                    uint64_t philox_offset2, void* stream);
 
+/* ---- what stands around attention in a layer; the reference has none of these -------------------------------- */
+
+/* Learned relative position bias by buckets: the additive bias of ab200_attn_fwd from a table,
+ *   bias[b, h, m, n] = table[bucket(n - m - query_offset), h],
+ * and the gradient of the table from that of the bias.  A distance d = n - m - query_offset has, per direction, the bucket
+ * #{k : borders[k] <= r}; bidirectional: r = |d|, and d > 0 takes the second half of the table; else r = max(-d, 0). */
+typedef struct ab200_relative_bias_args {
+  int32_t dtype;            /* ab200_dtype of the bias, or of its gradient                                     */
+  int32_t table_dtype;      /* ab200_dtype of the table, or of its gradient                                    */
+  int32_t num_buckets;      /* of the whole table; per direction (half of it when bidirectional) 2 to 128      */
+  int32_t num_heads;
+  int32_t bidirectional;
+  int32_t query_offset;     /* position of query 0 among the keys                                              */
+  const int32_t* borders;   /* HOST pointer, positive, none below the one before: buckets of a direction less one */
+  void* table;              /* forward: read; backward: the gradient, every entry written                      */
+  int64_t table_stride[2];  /* between buckets, between heads                                                  */
+  ab200_view4 bias;         /* forward: (1, num_heads, Sq, Sk), written (a batch reads it with stride 0);
+                             * backward: (batch, num_heads, Sq, Sk), read.  Any strides; 16-byte aligned rows of unit stride are fastest. */
+  float* workspace;         /* backward: ab200_relative_bias_workspace() floats; contents do not matter         */
+  uint64_t workspace_floats;
+} ab200_relative_bias_args;
+
+AB200_API int ab200_relative_bias_fwd(const ab200_relative_bias_args* args, void* stream);
+/* Sums are fp32 in a fixed order: the same inputs give the same bits. */
+AB200_API int ab200_relative_bias_bwd(const ab200_relative_bias_args* args, void* stream);
+/* Floats of workspace the backward needs, or the negated error code.  Launches nothing. */
+AB200_API int64_t ab200_relative_bias_workspace(const ab200_relative_bias_args* args, void* stream);
+
+/* out = residual + keep(x) / (1 - dropout_p) over (rows, cols) elements, each tensor with rows of unit stride.  Element
+ * i in row-major order takes word (0, 2, 1, 3)[i % 4] of Philox counter offset + i / 4, as column i of a score row would,
+ * and the attention's threshold.  The mask is not stored: the backward is the same call on the output's gradient, without a
+ * residual.  `out` may be x or residual itself (same strides). */
+typedef struct ab200_dropout_args {
+  int32_t dtype;
+  float dropout_p;                  /* 0 to 1; 0 keeps everything, 1 nothing   */
+  int64_t rows, cols;
+  const void* x;
+  const void* residual;             /* NULL: none                              */
+  void* out;
+  int64_t x_stride, residual_stride, out_stride;   /* between rows, in elements */
+  const uint64_t* philox_seed;      /* device scalars, NULL -> 0; what they hold when the kernel runs counts */
+  const uint64_t* philox_offset1;
+  uint64_t philox_seed_value;       /* added to them                           */
+  uint64_t philox_offset2;
+} ab200_dropout_args;
+
+AB200_API int ab200_dropout(const ab200_dropout_args* args, void* stream);
+
 /* Replaces aotriton::v2::flash::check_gpu (modules/flash/csrc/attn_check.cc:36-46):
  * 0 when the stream's device is an sm_100 part, hipErrorNoBinaryForGpu (209) otherwise. */
 AB200_API int ab200_check_gpu(void* stream);
