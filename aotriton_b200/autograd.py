@@ -30,6 +30,10 @@ except ImportError as e:      # (built where torch was missing, had no CUDA or w
             return None
 
         @staticmethod
+        def sink_attend(*args):
+            return None
+
+        @staticmethod
         def relative_bias(*args):
             return None
 
@@ -320,6 +324,131 @@ _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 def _launch(fn, device, args):
     """An entry point of the C-ABI on the device's current stream."""
     return fn(args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def _sink_problem(cu_q, cu_k, max_q, max_k, varlen, sm_scale):
+    kw = dict(sm_scale=sm_scale)
+    if varlen:
+        kw.update(cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=max_q, max_seqlen_k=max_k, varlen_type=varlen)
+    return kw
+
+
+class _SinkAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, return_lse, varlen):
+        b, hq, sq, _ = q.shape
+        packed = varlen == cabi.VARLEN_COMPACT
+        if packed:      # (1, H, tokens, D) views of (tokens, H, D) storage
+            o = torch.empty((1, sq, hq, v.shape[3]), device=q.device, dtype=q.dtype).transpose(1, 2)
+        else:
+            o = torch.empty((b, hq, sq, v.shape[3]), device=q.device, dtype=q.dtype)
+        lse = torch.empty((hq, sq) if packed else (b * hq, sq), device=q.device, dtype=torch.float32)
+        if not q.numel() or not k.numel() or not v.numel():      # nobody, or nothing to see
+            o.zero_()
+            lse.fill_(float("inf"))
+        else:
+            kw = _sink_problem(cu_q, cu_k, max_q, max_k, varlen, sm_scale)
+            stream = torch.cuda.current_stream(q.device).cuda_stream
+            _check(hipError_t(cabi.sink_attn_fwd(q, k, v, o, lse, window, sinks, stream=stream, **kw)), "sink_attn_fwd")
+        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        ctx.args = (max_q, max_k, window, sinks, sm_scale, varlen)
+        ctx.mark_non_differentiable(lse)
+        return (o, lse) if return_lse else o
+
+    @staticmethod
+    def backward(ctx, do, *unused):
+        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        return _SinkAttentionGrad.apply(q, k, v, o, do, lse, cu_q, cu_k, *ctx.args) + (None,) * 9
+
+
+class _SinkAttentionGrad(torch.autograd.Function):
+    """(dq, dk, dv): an operator of its own, which knows that it has no derivative."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, o, do, lse, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, varlen):
+        if not q.numel() or not k.numel() or not v.numel():
+            return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+        do = do if do.stride(-1) == 1 else do.contiguous()
+        # (a padded batch's rows behind their sequences have gradient zero)
+        make = torch.zeros_like if varlen == cabi.VARLEN_PADDED else torch.empty_like
+        dq, dk, dv = make(q), make(k), make(v)
+        delta = torch.empty_like(lse)
+        kw = _sink_problem(cu_q, cu_k, max_q, max_k, varlen, sm_scale)
+        args = (q, k, v, o, do, dq, dk, dv, lse, delta, window, sinks)
+        stream = torch.cuda.current_stream(q.device).cuda_stream
+        need = cabi.sink_attn_bwd_workspace(*args, stream=stream, **kw)
+        if need < 0:
+            _check(hipError_t(-need), "sink_attn_bwd")
+        workspace = torch.empty([need], device=q.device, dtype=torch.float32) if need else None
+        _check(hipError_t(cabi.sink_attn_bwd(*args, workspace=workspace, stream=stream, **kw)), "sink_attn_bwd")
+        _native.note_bwd_family()
+        return dq, dk, dv
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("sink_attention has no second derivative")
+
+
+def _python_sink_grad(q, k, v, o, do, lse, cu_q, cu_k, *numbers):
+    """The gradients of a native call whose own gradient or modes are not ordinary ones (csrc/torch_ops.cc)."""
+    return _SinkAttentionGrad.apply(q, k, v, o, do, lse, cu_q, cu_k, *numbers)
+
+
+_native.set_python_function("sink_attention", _python_sink_grad)
+
+
+def _sink_attention(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, return_lse, varlen):
+    if not torch.compiler.is_compiling():
+        r = _native.sink_attend(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, return_lse, varlen)
+        if r is not None:
+            return r
+    for t in (q, k, v):
+        if t.dim() != 4 or t.dtype not in _FLOATS or not t.is_cuda or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError("sink_attention: q, k and v are (batch, heads, tokens, head dim) CUDA tensors of one device and type, fp32, fp16 or bf16")
+    if type(window) is not int or type(sinks) is not int or window < 1 or sinks < 0:
+        raise ValueError(f"sink_attention: window {window} and sinks {sinks}: whole numbers, 1 or more and 0 or more")
+    if k.shape[0] != q.shape[0] or v.shape[:3] != k.shape[:3] or k.shape[3] != q.shape[3] or not k.shape[1] or q.shape[1] % k.shape[1]:
+        raise ValueError(f"sink_attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not go together")
+    if not 1 <= q.shape[3] <= 512 or not 1 <= v.shape[3] <= 512:
+        raise ValueError("sink_attention: head dims from 1 to 512 are supported")
+    if varlen:
+        for t in (cu_q, cu_k):
+            if t.dim() != 1 or t.numel() < 2 or t.numel() != cu_q.numel() or t.dtype != torch.int32 or t.device != q.device or t.stride(0) != 1:
+                raise ValueError("sink_attention: the cumulative lengths are contiguous int32 tensors on q's device, one entry more than there are sequences")
+        if varlen == cabi.VARLEN_COMPACT and q.shape[0] != 1:
+            raise ValueError("sink_attention: packed tokens are (1, heads, tokens, head dim)")
+        if varlen == cabi.VARLEN_PADDED and cu_q.numel() != q.shape[0] + 1:
+            raise ValueError("sink_attention: a padded batch has one sequence for each entry of the batch axis")
+        if not 0 <= max_q <= q.shape[2] or not 0 <= max_k <= k.shape[2]:
+            raise ValueError(f"sink_attention: longest sequences {max_q} and {max_k} do not fit {q.shape[2]} and {k.shape[2]} tokens")
+        max_q = q.shape[2] if varlen == cabi.VARLEN_PADDED else max(max_q, 1)
+        max_k = max(max_k, 1)
+    window, sinks = min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)
+    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    return _SinkAttention.apply(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, float(sm_scale), bool(return_lse), varlen)
+
+
+def sink_attention(q, k, v, window, sinks, sm_scale=None, return_lse=False):
+    """Attention with a sliding window and `sinks` first keys that stay visible, for (B, H, S, D) tensors of any strides.  Query m of Sq
+    stands at the key position P = m + Sk - Sq (queries are the last of the keys' positions: Sq = Sk in training, Sq = 1 for one token against a cache)
+    and sees the keys n <= P with n > P - window or n < sinks.  A query that sees nothing gives zeros (log-sum-exp +inf).  GQA by fewer
+    heads in k and v; no bias, no dropout.  Only keys that some query sees are read, whole blocks of them; of a cache's others, what they hold (NaN too) does
+    not matter in fp16 and bf16 with head dims up to 256 that are multiples of 8.  The log-sum-exp has no gradient."""
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
+    return _sink_attention(q, k, v, None, None, 0, 0, window, sinks, sm_scale, return_lse, 0)
+
+
+def varlen_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks, sm_scale=None, return_lse=False,
+                          varlen_type="compact"):
+    """sink_attention over sequences of different lengths, each with its own positions.  varlen_type "compact": token-packed (1, H, tokens, D)
+    tensors, as for varlen_attention.  "padded": (B, H, S, D) tensors, such as a batch of caches, sequence z having the first
+    cu_seqlens[z + 1] - cu_seqlens[z] tokens of its row; what lies behind them is not looked at, output rows behind the last query are
+    zero (log-sum-exp +inf) and gradients there are zero.  max_seqlen_q and _k are at least the longest lengths."""
+    if varlen_type not in ("compact", "padded"):
+        raise ValueError(f"varlen_sink_attention: varlen_type {varlen_type!r} is not \"compact\" or \"padded\"")
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
+    return _sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks, sm_scale, return_lse,
+                           flash.IVARLEN_TYPE[varlen_type])
 
 
 @functools.lru_cache(maxsize=None)

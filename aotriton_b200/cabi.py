@@ -22,7 +22,8 @@ SELECT_ALIGNED, SELECT_DBIAS, SELECT_FUSED_REQUESTED, SELECT_FORCE_GENERAL, SELE
 SYMBOLS = [
     "ab200_attn_fwd", "ab200_attn_bwd", "ab200_attn_bwd_static_scratch", "ab200_bwd_uses_dq_acc",
     "ab200_bwd_fused", "ab200_bwd_postprocess", "ab200_bwd_preprocess", "ab200_bwd_dkdv", "ab200_bwd_dq",
-    "ab200_debug_simulate_encoded_softmax", "ab200_relative_bias_fwd", "ab200_relative_bias_bwd",
+    "ab200_debug_simulate_encoded_softmax", "ab200_sink_attn_fwd", "ab200_sink_attn_bwd",
+    "ab200_sink_attn_bwd_workspace", "ab200_relative_bias_fwd", "ab200_relative_bias_bwd",
     "ab200_relative_bias_workspace", "ab200_dropout", "ab200_check_gpu", "ab200_multiprocessor_count",
     "ab200_set_kernel_family", "ab200_select_variant", "ab200_last_fwd_family", "ab200_last_bwd_family",
     "ab200_kernel_status", "ab200_stream_check", "ab200_debug_bounded_wait_test", "ab200_debug_keep_tiles",
@@ -100,6 +101,10 @@ def lib() -> C.CDLL:
         L.ab200_debug_simulate_encoded_softmax.argtypes = [
             C.POINTER(View4), C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_float,
             C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
+        L.ab200_sink_attn_fwd.argtypes = [C.POINTER(FwdArgs), C.c_int32, C.c_int32, C.c_void_p]
+        L.ab200_sink_attn_bwd.argtypes = [C.POINTER(BwdArgs), C.c_int32, C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]
+        L.ab200_sink_attn_bwd_workspace.argtypes = [C.POINTER(BwdArgs), C.c_int32, C.c_int32, C.c_void_p]
+        L.ab200_sink_attn_bwd_workspace.restype = C.c_int64
         for name in ("ab200_relative_bias_fwd", "ab200_relative_bias_bwd", "ab200_relative_bias_workspace"):
             getattr(L, name).argtypes = [C.POINTER(RelativeBiasArgs), C.c_void_p]
         L.ab200_relative_bias_workspace.restype = C.c_int64
@@ -222,6 +227,23 @@ def debug_simulate_encoded_softmax(r, dropout_p, philox_seed, philox_offset1, ph
         C.byref(v), _torch_dtype_code(r), r.shape[0], r.shape[1], r.shape[2], r.shape[3], dropout_p,
         _ptr(philox_seed), _ptr(philox_offset1), philox_offset2,
         stream if stream is not None else current_stream_handle())
+
+
+def sink_attn_fwd(q, k, v, out, lse, window, sinks, *, stream=None, **kw) -> int:
+    a = make_fwd_args(q, k, v, out, lse, **kw)
+    return lib().ab200_sink_attn_fwd(C.byref(a), window, sinks, stream if stream is not None else current_stream_handle())
+
+
+def sink_attn_bwd_workspace(q, k, v, out, dout, dq, dk, dv, lse, delta, window, sinks, *, stream=None, **kw) -> int:
+    """Floats the backward needs; negative: an error code."""
+    a = make_bwd_args(q, k, v, out, dout, dq, dk, dv, lse, delta, **kw)
+    return lib().ab200_sink_attn_bwd_workspace(C.byref(a), window, sinks, stream if stream is not None else current_stream_handle())
+
+
+def sink_attn_bwd(q, k, v, out, dout, dq, dk, dv, lse, delta, window, sinks, *, workspace=None, stream=None, **kw) -> int:
+    a = make_bwd_args(q, k, v, out, dout, dq, dk, dv, lse, delta, **kw)
+    return lib().ab200_sink_attn_bwd(C.byref(a), window, sinks, _ptr(workspace), workspace.numel() if workspace is not None else 0,
+                                     stream if stream is not None else current_stream_handle())
 
 
 def make_relative_bias_args(table, bias, borders, *, bidirectional=True, query_offset=0, workspace=None) -> RelativeBiasArgs:

@@ -7,6 +7,7 @@
 // Error vocabulary follows ROCm/aotriton (python/codegen/template/op.cc:21-71):
 // unknown GPU -> hipErrorNoBinaryForGpu (209), unsupported functional ->
 // hipErrorNotSupported (801), malformed arguments -> hipErrorInvalidValue (1).
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 #include <cstdio>
@@ -797,6 +798,96 @@ int ab200_attn_bwd_static_scratch(const ab200_attn_bwd_args* a, void* stream) {
   ab200_attn_bwd_args b = *a;
   b.delta = delta;
   return ab200_attn_bwd(&b, stream);
+}
+
+// --- attention with a sliding window and first keys that stay visible -----------------------------
+// The window and the first keys of a call, after its problem.
+static int fill_sinks(const ab200_attn_problem& a, int window, int sinks, Params& p) {
+  if (window < 1 || sinks < 0 || (p.batch > 0 && (p.max_sq < 1 || p.max_sk < 1))) return kErrInvalidValue;
+  if (p.has_bias || p.has_dbias || a.dropout_p != 0.f) return kErrNotSupported;
+  p.causal = 1;
+  p.causal_type = AB200_CAUSAL_WINDOWED;
+  p.window_left = p.window_right = 0;      // (each sequence's own: seq_for)
+  p.sink_on = 1;
+  const bool all = (int64_t)window + sinks >= p.max_sk;      // nothing is ever out of sight
+  p.sink_window = all ? (p.max_sk > 0 ? p.max_sk : 1) : window;
+  p.sinks = all ? 0 : sinks;
+  return 0;
+}
+
+int ab200_sink_attn_fwd(const ab200_attn_fwd_args* a, int32_t window, int32_t sinks, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Params p{};
+  if (int e = fill_fwd(a, p)) return e;
+  if (int e = fill_sinks(a->prob, window, sinks, p)) return e;
+  if (a->encoded_softmax.ptr != nullptr) return kErrNotSupported;
+  if (int e = check_device(st)) return e;
+  DeviceGuard guard(st);
+  const int sel = select_fwd(a, p);
+  if (sel < 0) return -sel;
+  const bool tc = (sel & 0xff) >= kVarTcgen05;
+  t_last_fwd = tc ? 2 : 1;
+  return (int)(tc ? launch_sm100_fwd(a->prob.dtype, p, st) : launch_general(0, a->prob.dtype, p, st));
+}
+
+// The backward's kernels and how dK/dV shares the first keys' queries out (dkdv_item).  Returns the floats of workspace: the items'
+// partial sums and, behind them, dK/dV's ticket counter (not one of the library's pool: a captured call keeps its counter for good, and
+// replays of several may run side by side).
+constexpr int kTicketFloats = 4;
+static int64_t plan_sink_bwd(const ab200_attn_bwd_args* a, Params& p, int* sel) {
+  *sel = ab200_select_variant(kOpBwd, a->prob.dtype, p.dqk, p.dvo,
+                              family_flags(g_family) | (sm100_bwd_supported(a->prob.dtype, p) ? AB200_SELECT_ALIGNED : 0));
+  if (*sel < 0 || (*sel & 0xff) < kVarTcgen05 || p.dqk > 128 || p.dvo > 128) return 0;
+  if (p.sinks == 0) return kTicketFloats;
+  // as many query blocks to an item as a window's worth gives the other key blocks, eight at least
+  const int64_t all = ((int64_t)p.max_sq + 127) / 128 * p.group, own = ((int64_t)p.sink_window + 127) / 128 * p.group + p.group;
+  const int64_t each = own > 8 ? own : 8;
+  // (no more than fill the chip a few times over: each costs a row of partial sums for every first key)
+  const int64_t blocks = (int64_t)p.batch * p.hk * ((p.sinks + 127) / 128), most = blocks > 0 ? (592 + blocks - 1) / blocks : 1;
+  p.sink_chunks = (int)std::min<int64_t>(std::min<int64_t>(64, most), (all + each - 1) / each);
+  return (int64_t)p.batch * p.hk * (p.sink_chunks + 1) * p.sinks * (p.dqk + p.dvo) + kTicketFloats;
+}
+
+int64_t ab200_sink_attn_bwd_workspace(const ab200_attn_bwd_args* a, int32_t window, int32_t sinks, void* stream) {
+  Params p{};
+  int sel = 0;
+  if (int e = fill_bwd(a, p, true)) return -e;
+  if (int e = fill_sinks(a->prob, window, sinks, p)) return -e;
+  if (int e = check_device(static_cast<cudaStream_t>(stream))) return -e;
+  const int64_t floats = plan_sink_bwd(a, p, &sel);
+  return sel < 0 ? sel : floats;
+}
+
+int ab200_sink_attn_bwd(const ab200_attn_bwd_args* a, int32_t window, int32_t sinks, float* workspace, uint64_t workspace_floats,
+                        void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Params p{};
+  int sel = 0;
+  if (int e = fill_bwd(a, p, true)) return e;
+  if (!a->dq.ptr || !a->dk.ptr || !a->dv.ptr) return kErrInvalidValue;
+  if (int e = fill_sinks(a->prob, window, sinks, p)) return e;
+  if (int e = check_device(st)) return e;
+  DeviceGuard guard(st);
+  const int dtype = a->prob.dtype;
+  const int64_t floats = plan_sink_bwd(a, p, &sel);
+  if (sel < 0) return -sel;
+  if (p.batch == 0) return 0;
+  if (floats > 0) {
+    if (workspace == nullptr || workspace_floats < (uint64_t)floats || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return kErrInvalidValue;
+    p.sink_partial = workspace;
+    p.ticket = reinterpret_cast<unsigned int*>(workspace + floats - kTicketFloats);
+  }
+  cudaError_t e = launch_preprocess(dtype, p, st);
+  if (e != cudaSuccess) return (int)e;
+  const bool tc = (sel & 0xff) >= kVarTcgen05;
+  t_last_bwd = tc ? 2 : 1;
+  if (tc) {
+    if ((e = launch_sm100_bwd_dkdv(dtype, p, st)) != cudaSuccess) return (int)e;
+    return (int)launch_sm100_bwd_dq(dtype, p, st);
+  }
+  if (apart_from_inputs(p.dq, p, dtype == AB200_DTYPE_FP32 ? 4 : 2)) return (int)launch_general(3, dtype, p, st);
+  if ((e = launch_general(1, dtype, p, st)) != cudaSuccess) return (int)e;
+  return (int)launch_general(2, dtype, p, st);
 }
 
 // --- relative position bias, dropout of hidden states (layer_ops.cu) ----------------------------

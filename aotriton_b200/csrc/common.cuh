@@ -67,6 +67,10 @@ struct Params {
   int32_t dk_from_db;             // dK = sm_scale * dBias^T Q, after the dQ kernel has written dBias (sm100_bwd_dk_db.cuh)
   int32_t keep_tiles, keep_shift; // keep bits of the first keep_tiles 32-key tiles pass through dQ's rows (0: none), or, with
                                   // keep_shift kKeepInDbias, through dBias; see KeepShare
+  // Sink attention: query m of a sequence stands at key P = m + sk - sq and sees keys n <= P with n > P - sink_window or n < sinks.
+  int32_t sink_on, sinks, sink_window;
+  int32_t sink_chunks;            // dK/dV: items that share the queries beyond a first block's window (0: no such queries)
+  float* sink_partial;            // ... and the fp32 sums of each for the first keys (sink_partial_row)
 };
 
 // Geometry of one (sequence z) slice.
@@ -74,8 +78,9 @@ struct Params {
 // dropout (generator state, keep bits) and bias (its tile, pointers, strides) need is spilled around every block even where a
 // call uses neither, so each combination has instantiations of its own.  kAll leaves everything to the run time (dBias without
 // bias too).
-enum : int { kPlain = 0, kBias = 1, kDropout = 2, kAll = 3 };      // bias, and its gradient or not; dropout; anything
+enum : int { kPlain = 0, kBias = 1, kDropout = 2, kAll = 3, kSinks = 4 };      // bias, and its gradient or not; dropout; anything; sink attention
 inline int features(const Params& p) {
+  if (p.sink_on) return kSinks;
   if (p.has_dbias && !p.has_bias) return kAll;
   return (p.has_bias ? kBias : 0) | (p.dropout_on ? kDropout : 0);
 }
@@ -119,6 +124,59 @@ __device__ __forceinline__ Seq resolve_seq(const Params& p, int z) {
   int4 ends = make_int4(0, 0, 0, 0);
   if (p.varlen_mode != 0) ends = make_int4(p.cu_q[z], p.cu_q[z + 1], p.cu_k[z], p.cu_k[z + 1]);
   return seq_from_ends(p, z, ends);
+}
+
+// ---- sink attention -------------------------------------------------------------------------------------------
+// A window that moves with the queries, aligned to the last key, and the first keys.  The kernels walk the blocks the window
+// reaches as for any window, and before them the blocks of first keys that lie wholly in front of it; only a block with first keys
+// in it pays for a second comparison.  In dK/dV a first key is one whose window has no end.
+template <int FEAT>
+__device__ __forceinline__ Seq seq_for(const Params& p, int z, int4 ends) {
+  Seq s = seq_from_ends(p, z, ends);
+  if constexpr ((FEAT & kSinks) != 0) {
+    s.wr = s.sk - s.sq;
+    const int64_t wl = (int64_t)p.sink_window - 1 - s.wr;
+    s.wl = (int)(wl > 0x7fffffffLL ? 0x7fffffffLL : (wl < -0x7fffffffLL ? -0x7fffffffLL : wl));
+  }
+  return s;
+}
+template <int FEAT>
+__device__ __forceinline__ Seq resolve_seq_for(const Params& p, int z) {
+  int4 ends = make_int4(0, 0, 0, 0);
+  if (p.varlen_mode != 0) ends = make_int4(p.cu_q[z], p.cu_q[z + 1], p.cu_k[z], p.cu_k[z + 1]);
+  return seq_for<FEAT>(p, z, ends);
+}
+// Blocks of `block` keys that hold first keys and lie in front of block `first`, the window's; n_hi: the last key that is seen.
+template <int FEAT>
+__device__ __forceinline__ int blocks_before(const Params& p, int n_hi, int first, int block) {
+  if constexpr ((FEAT & kSinks) == 0) return 0;
+  return min((min(p.sinks, n_hi + 1) + block - 1) / block, first);
+}
+// Block j of the walk.
+template <int FEAT>
+__device__ __forceinline__ int block_at(int j, int before, int first) {
+  if constexpr ((FEAT & kSinks) == 0) return first + j;
+  return j < before ? j : first + (j - before);
+}
+// Keys that no query of the sequence sees, [from, to): between the first keys and the first query's window.  Their rows of V (and K,
+// where it is contracted over) are zeroed in shared memory: a cache may hold anything there, and zero times NaN is NaN.
+__device__ __forceinline__ void hidden_keys(const Params& p, const Seq& s, int& from, int& to) {
+  from = p.sinks;
+  to = -s.wl;
+}
+// mask_columns in a block that holds first keys
+template <int N>
+__device__ __forceinline__ void mask_sink_columns(float* x, int first, int lo, int hi, int sinks, float fill) {
+  lo -= first;
+  hi -= first;
+  sinks -= first;
+#pragma unroll
+  for (int c = 0; c < N; ++c) x[c] = (c <= hi && (c >= lo || c < sinks)) ? x[c] : fill;
+}
+// fp32 sums of first key n for dK (dqk floats, without sm_scale) and dV (dvo) by one of the items that share its queries: 0 is
+// the key block's own, 1..sink_chunks the others.
+__device__ __forceinline__ float* sink_partial_row(const Params& p, int z, int hk, int chunk, int n) {
+  return p.sink_partial + ((((int64_t)z * p.hk + hk) * (p.sink_chunks + 1) + chunk) * p.sinks + n) * (p.dqk + p.dvo);
 }
 
 // Row tile `tile` of a token-packed batch, when the tiles of all sequences are counted through (within a
@@ -207,6 +265,12 @@ __device__ __forceinline__ bool score_valid(const Params& p, const Seq& s, int m
   bool ok = (m < s.sq) && (n < s.sk);
   if (p.causal) ok = ok && (n <= m + s.wr) && (n >= m - s.wl);
   return ok;
+}
+
+template <bool SINKS>
+__device__ __forceinline__ bool score_valid_for(const Params& p, const Seq& s, int m, int n) {
+  if constexpr (!SINKS) return score_valid(p, s, m, n);
+  return m < s.sq && n < s.sk && n <= (int64_t)m + s.wr && (n >= (int64_t)m - s.wl || n < p.sinks);
 }
 
 // Closed range of key indices that can be valid for query rows [m_lo, m_hi].
@@ -447,6 +511,18 @@ template <typename T> __device__ __forceinline__ T from_f32(float x);
 template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// Rows behind a padded sequence's last query: O = 0, LSE = +inf, as for rows that see no key (sink attention; the other entries leave
+// them as they are).
+template <typename T>
+__device__ void write_rows_behind(const Params& p, const Seq& sq, int h, int m0, int rows) {
+  const int end = min(m0 + rows, p.max_sq);
+  for (int m = max(m0, sq.sq) + (int)threadIdx.x; m < end; m += blockDim.x) {
+    T* op = reinterpret_cast<T*>(p.out.ptr) + (int64_t)sq.bidx * p.out.s[0] + (int64_t)h * p.out.s[1] + (int64_t)m * p.out.s[2];
+    for (int d = 0; d < p.dvo; ++d) op[d] = from_f32<T>(0.f);
+    if (p.lse) p.lse[lse_offset(p, sq, h) + m] = INFINITY;
+  }
+}
 
 // dBias of query rows [m0, m0 + rows) outside the key columns [c_lo, c_hi) that the calling CTA's
 // block loop visits.  A causal or windowed problem skips whole key blocks; the gradient of the bias

@@ -75,7 +75,7 @@ __device__ __forceinline__ float half_warp_sum(float x) {
 
 // ---------------------------------------------------------------------------
 // Forward.  grid = (cdiv(max_sq, 16), Hq, batch)
-template <typename T, int DJ>
+template <typename T, int DJ, int FEAT>
 __global__ void __launch_bounds__(kThreads) general_fwd_kernel(const __grid_constant__ Params p) {
   wait_for_earlier_grids();
   extern __shared__ float smem[];
@@ -97,7 +97,10 @@ __global__ void __launch_bounds__(kThreads) general_fwd_kernel(const __grid_cons
     if (p.seed_out) *p.seed_out = seed;
     if (p.off_out) *p.off_out = base;
   }
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
+  if constexpr ((FEAT & kSinks) != 0) {
+    if (p.varlen_mode == 2 && m0 + kTile > sq.sq) write_rows_behind<T>(p, sq, h, m0, kTile);
+  }
   if (m0 >= sq.sq) return;
   const int hk = h / p.group;
   const int tid = threadIdx.x, r = tid >> 4, c = tid & 15, warp = tid >> 5, lane = tid & 31;
@@ -116,15 +119,16 @@ __global__ void __launch_bounds__(kThreads) general_fwd_kernel(const __grid_cons
   int n_lo, n_hi;
   key_range(p, sq, m0, min(m0 + kTile, sq.sq) - 1, n_lo, n_hi);
   const int m = m0 + r;
-  for (int nb = n_lo / kTile; nb * kTile <= n_hi; ++nb) {
-    const int n0 = nb * kTile;
+  const int nb_lo = n_lo / kTile, before = blocks_before<FEAT>(p, n_hi, nb_lo, kTile);
+  for (int j = 0; block_at<FEAT>(j, before, nb_lo) * kTile <= n_hi; ++j) {
+    const int n0 = block_at<FEAT>(j, before, nb_lo) * kTile;
     __syncthreads();   // previous accumulate phase done (and Qs staged on first trip)
     stage_rows<T>(Ks, LD, DPAD, p.k, sq.bidx, hk, sq.k0, n0, sq.sk, p.dqk);
     stage_rows<T>(Vs, LD, DPAD, p.v, sq.bidx, hk, sq.k0, n0, sq.sk, p.dvo);
     __syncthreads();
     const int n = n0 + c;
     float s = -INFINITY;
-    if (score_valid(p, sq, m, n)) {
+    if (score_valid_for<(FEAT & kSinks) != 0>(p, sq, m, n)) {
       s = dot_rows(Qs + r * LD, Ks + c * LD, DPAD) * p.qk_scale;
       if (p.has_bias) {
         const T* bp = reinterpret_cast<const T*>(p.bias.ptr) + (int64_t)sq.bidx * p.bias.s[0] +
@@ -184,13 +188,13 @@ __global__ void __launch_bounds__(kThreads) general_fwd_kernel(const __grid_cons
 // ---------------------------------------------------------------------------
 // Pair phase shared by both backward kernels: recompute P, dP and dS for pair (m, n).
 // pd_out = dropped-and-scaled P (for dV), ds_out = dS (for dK, dQ, dBias).
-template <typename T>
+template <typename T, int FEAT>
 __device__ __forceinline__ void bwd_pair(const Params& p, const Seq& sq, const DropoutCtx& dctx, int h,
                                          int m, int n, const float* qrow, const float* krow,
                                          const float* dorow, const float* vrow, int dpad,
                                          float lse_m, float delta_m, float& pd_out, float& ds_out) {
   pd_out = 0.f; ds_out = 0.f;
-  if (!score_valid(p, sq, m, n)) return;
+  if (!score_valid_for<(FEAT & kSinks) != 0>(p, sq, m, n)) return;
   float s = dot_rows(qrow, krow, dpad) * p.qk_scale;
   if (p.has_bias) {
     const T* bp = reinterpret_cast<const T*>(p.bias.ptr) + (int64_t)sq.bidx * p.bias.s[0] +
@@ -210,7 +214,7 @@ __device__ __forceinline__ void bwd_pair(const Params& p, const Seq& sq, const D
 }
 
 // dK / dV.  grid = (cdiv(max_sk, 16), Hk, batch)
-template <typename T, int DJ>
+template <typename T, int DJ, int FEAT>
 __global__ void __launch_bounds__(kThreads) general_bwd_dkdv_kernel(const __grid_constant__ Params p) {
   wait_for_earlier_grids();
   extern __shared__ float smem[];
@@ -226,7 +230,7 @@ __global__ void __launch_bounds__(kThreads) general_bwd_dkdv_kernel(const __grid
   float* dl_s = lse_s + kTile;         // [16]
 
   const int z = blockIdx.z, hk = blockIdx.y, n0 = blockIdx.x * kTile;
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
   if (n0 >= sq.sk) return;
   const int tid = threadIdx.x, r = tid >> 4, c = tid & 15, warp = tid >> 5, lane = tid & 31;
 
@@ -241,6 +245,7 @@ __global__ void __launch_bounds__(kThreads) general_bwd_dkdv_kernel(const __grid
 
   int m_lo, m_hi;
   query_range(p, sq, n0, min(n0 + kTile, sq.sk) - 1, m_lo, m_hi);
+  if ((FEAT & kSinks) != 0 && n0 < p.sinks) m_hi = sq.sq - 1;      // first keys: every query behind them
   for (int g = 0; g < p.group; ++g) {
     const int h = hk * p.group + g;
     DropoutCtx dctx;
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(kThreads) general_bwd_dkdv_kernel(const __grid
       }
       __syncthreads();
       float pd, ds;
-      bwd_pair<T>(p, sq, dctx, h, m0 + r, n0 + c, Qs + r * LD, Ks + c * LD, dOs + r * LD, Vs + c * LD, DPAD,
+      bwd_pair<T, FEAT>(p, sq, dctx, h, m0 + r, n0 + c, Qs + r * LD, Ks + c * LD, dOs + r * LD, Vs + c * LD, DPAD,
                   lse_s[r], dl_s[r], pd, ds);
       Ps[r * kTile + c] = round_to<T>(pd);
       dSs[r * kTile + c] = round_to<T>(ds);
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(kThreads) general_bwd_dkdv_kernel(const __grid
 }
 
 // dQ (+ dBias).  grid = (cdiv(max_sq, 16), Hq, batch)
-template <typename T, int DJ>
+template <typename T, int DJ, int FEAT>
 __global__ void __launch_bounds__(kThreads) general_bwd_dq_kernel(const __grid_constant__ Params p) {
   wait_for_earlier_grids();
   extern __shared__ float smem[];
@@ -308,7 +313,7 @@ __global__ void __launch_bounds__(kThreads) general_bwd_dq_kernel(const __grid_c
   float* dl_s = lse_s + kTile;
 
   const int z = blockIdx.z, h = blockIdx.y, m0 = blockIdx.x * kTile;
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
   if (m0 >= sq.sq) return;
   const int hk = h / p.group;
   const int tid = threadIdx.x, r = tid >> 4, c = tid & 15, warp = tid >> 5, lane = tid & 31;
@@ -335,15 +340,16 @@ __global__ void __launch_bounds__(kThreads) general_bwd_dq_kernel(const __grid_c
   if (n_hi >= n_lo) zero_dbias_outside<T>(p, sq, h, m0, kTile, (n_lo / kTile) * kTile, (n_hi / kTile + 1) * kTile);
   else zero_dbias_outside<T>(p, sq, h, m0, kTile, 0, 0);
   const int m = m0 + r;
-  for (int nb = n_lo / kTile; nb * kTile <= n_hi; ++nb) {
-    const int n0 = nb * kTile;
+  const int nb_lo = n_lo / kTile, before = blocks_before<FEAT>(p, n_hi, nb_lo, kTile);
+  for (int j = 0; block_at<FEAT>(j, before, nb_lo) * kTile <= n_hi; ++j) {
+    const int n0 = block_at<FEAT>(j, before, nb_lo) * kTile;
     __syncthreads();
     stage_rows<T>(Ks, LD, DPAD, p.k, sq.bidx, hk, sq.k0, n0, sq.sk, p.dqk);
     stage_rows<T>(Vs, LD, DPAD, p.v, sq.bidx, hk, sq.k0, n0, sq.sk, p.dvo);
     __syncthreads();
     const int n = n0 + c;
     float pd, ds;
-    bwd_pair<T>(p, sq, dctx, h, m, n, Qs + r * LD, Ks + c * LD, dOs + r * LD, Vs + c * LD, DPAD, lse_s[r],
+    bwd_pair<T, FEAT>(p, sq, dctx, h, m, n, Qs + r * LD, Ks + c * LD, dOs + r * LD, Vs + c * LD, DPAD, lse_s[r],
                 dl_s[r], pd, ds);
     if (p.has_dbias && m < sq.sq && n < sq.sk) {
       T* dbp = reinterpret_cast<T*>(p.dbias.ptr) + (int64_t)sq.bidx * p.dbias.s[0] + (int64_t)h * p.dbias.s[1] +
@@ -516,27 +522,32 @@ cudaError_t set_smem(K kernel, size_t bytes) {
   return host().func_set_smem(reinterpret_cast<const void*>(kernel), (int)bytes);
 }
 
-template <typename T, int DJ>
-cudaError_t launch_general_T(int which, const Params& p, cudaStream_t st) {
+template <typename T, int DJ, int FEAT>
+cudaError_t launch_general_F(int which, const Params& p, cudaStream_t st) {
   cudaError_t e;
   if (which == 0) {
     size_t sm = fwd_smem<T, DJ>();
-    if ((e = set_smem(general_fwd_kernel<T, DJ>, sm)) != cudaSuccess) return e;
+    if ((e = set_smem(general_fwd_kernel<T, DJ, FEAT>, sm)) != cudaSuccess) return e;
     dim3 grid((p.max_sq + kTile - 1) / kTile, p.hq, p.batch);
-    e = launch_kernel_as<false>(general_fwd_kernel<T, DJ>, dim3(grid), dim3(kThreads), sm, st, p);
+    e = launch_kernel_as<false>(general_fwd_kernel<T, DJ, FEAT>, dim3(grid), dim3(kThreads), sm, st, p);
   } else if (which == 1) {
     size_t sm = bwd_smem<T, DJ>();
-    if ((e = set_smem(general_bwd_dkdv_kernel<T, DJ>, sm)) != cudaSuccess) return e;
+    if ((e = set_smem(general_bwd_dkdv_kernel<T, DJ, FEAT>, sm)) != cudaSuccess) return e;
     dim3 grid((p.max_sk + kTile - 1) / kTile, p.hk, p.batch);
-    e = launch_kernel_as<false>(general_bwd_dkdv_kernel<T, DJ>, dim3(grid), dim3(kThreads), sm, st, p);
+    e = launch_kernel_as<false>(general_bwd_dkdv_kernel<T, DJ, FEAT>, dim3(grid), dim3(kThreads), sm, st, p);
   } else {
     size_t sm = bwd_smem<T, DJ>();
-    if ((e = set_smem(general_bwd_dq_kernel<T, DJ>, sm)) != cudaSuccess) return e;
+    if ((e = set_smem(general_bwd_dq_kernel<T, DJ, FEAT>, sm)) != cudaSuccess) return e;
     dim3 grid((p.max_sq + kTile - 1) / kTile, p.hq, p.batch);
-    e = launch_kernel_as<false>(general_bwd_dq_kernel<T, DJ>, dim3(grid), dim3(kThreads), sm, st, p);
+    e = launch_kernel_as<false>(general_bwd_dq_kernel<T, DJ, FEAT>, dim3(grid), dim3(kThreads), sm, st, p);
   }
   if (e == cudaSuccess) count_launch();
   return e;
+}
+
+template <typename T, int DJ>
+cudaError_t launch_general_T(int which, const Params& p, cudaStream_t st) {
+  return p.sink_on ? launch_general_F<T, DJ, kSinks>(which, p, st) : launch_general_F<T, DJ, kPlain>(which, p, st);
 }
 
 template <int DP>
@@ -562,21 +573,21 @@ bool joint_backward(const Params& p) { return sizeof(T) != 2 || DP <= 64 || row_
 template <int DP>
 bool split_backward(const Params& p) { return row_tiles<DP>(p) < 1536; }
 
-template <typename T, int DP>
-cudaError_t launch_tiled_T(int which, const Params& p, cudaStream_t st) {
+template <typename T, int DP, int FEAT>
+cudaError_t launch_tiled_F(int which, const Params& p, cudaStream_t st) {
   using C = Tiled<DP>;
   if (which == 3 && !joint_backward<T, DP>(p)) {
-    const cudaError_t e = launch_tiled_T<T, DP>(1, p, st);
-    return e != cudaSuccess ? e : launch_tiled_T<T, DP>(2, p, st);
+    const cudaError_t e = launch_tiled_F<T, DP, FEAT>(1, p, st);
+    return e != cudaSuccess ? e : launch_tiled_F<T, DP, FEAT>(2, p, st);
   }
   const bool split = which != 0 && split_backward<DP>(p);
   const size_t rows = which == 0 ? C::kBM + kFwdGroups * 2 * C::kBN : 2 * C::kBM + 2 * C::kBN;      // staged rows of DP + 4 floats
   const size_t tiles = which == 0 ? kFwdGroups : (which & 1 ? 2 : 1);                              // P and dS, or one of them
   const size_t sm = (rows * C::kLd + tiles * C::kBM * C::kLdP + (which & 1 ? 2 * C::kBN : 0)) * sizeof(float);
-  auto kern = which == 0   ? tiled_fwd_kernel<T, DP>
-              : which == 1 ? (split ? tiled_bwd_kernel<T, DP, 1, 2> : tiled_bwd_kernel<T, DP, 1, 1>)
-              : which == 2 ? (split ? tiled_bwd_kernel<T, DP, 2, 2> : tiled_bwd_kernel<T, DP, 2, 1>)
-                           : (split ? tiled_bwd_kernel<T, DP, 3, 2> : tiled_bwd_kernel<T, DP, 3, 1>);
+  auto kern = which == 0   ? tiled_fwd_kernel<T, DP, FEAT>
+              : which == 1 ? (split ? tiled_bwd_kernel<T, DP, 1, 2, FEAT> : tiled_bwd_kernel<T, DP, 1, 1, FEAT>)
+              : which == 2 ? (split ? tiled_bwd_kernel<T, DP, 2, 2, FEAT> : tiled_bwd_kernel<T, DP, 2, 1, FEAT>)
+                           : (split ? tiled_bwd_kernel<T, DP, 3, 2, FEAT> : tiled_bwd_kernel<T, DP, 3, 1, FEAT>);
   cudaError_t e = set_smem(kern, sm);
   if (e != cudaSuccess) return e;
   const int rows_total = which == 1 ? p.max_sk : (which == 3 && p.max_sk > p.max_sq ? p.max_sk : p.max_sq);
@@ -585,6 +596,11 @@ cudaError_t launch_tiled_T(int which, const Params& p, cudaStream_t st) {
   e = launch_kernel_as<false>(kern, grid, dim3(which == 0 ? kFwdGroups * C::kThreads : C::kThreads), sm, st, p);
   if (e == cudaSuccess) count_launch();
   return e;
+}
+
+template <typename T, int DP>
+cudaError_t launch_tiled_T(int which, const Params& p, cudaStream_t st) {
+  return p.sink_on ? launch_tiled_F<T, DP, kSinks>(which, p, st) : launch_tiled_F<T, DP, kPlain>(which, p, st);
 }
 
 template <typename T>

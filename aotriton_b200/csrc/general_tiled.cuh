@@ -178,6 +178,46 @@ __device__ __forceinline__ void tile_accumulate(float4 (&acc)[4][Tiled<DP>::kND]
   }
 }
 
+// The blocks of keys of a row tile, from n_lo's to n_hi's, `rank`th first, and before them those of the first keys.  Block starts
+// at or below n_hi are blocks.
+template <int DP, int FEAT> struct BlockWalk {
+  static constexpr int kBN = Tiled<DP>::kBN;
+  int start, j, before, first;
+  __device__ __forceinline__ BlockWalk(const Params& p, int n_lo, int n_hi, int rank) : j(rank), first(n_lo / kBN) {
+    before = blocks_before<FEAT>(p, n_hi, first, kBN);
+    if constexpr ((FEAT & kSinks) == 0) start = n_lo / kBN * kBN + rank * kBN;
+    else start = block_at<FEAT>(rank, before, first) * kBN;
+  }
+  __device__ __forceinline__ int next(int n0, int step) const {
+    if constexpr ((FEAT & kSinks) == 0) return n0 + step * kBN;
+    return block_at<FEAT>(j + step, before, first) * kBN;
+  }
+  __device__ __forceinline__ int advance(int n0, int step) {
+    const int n = next(n0, step);
+    if constexpr ((FEAT & kSinks) != 0) j += step;
+    return n;
+  }
+};
+
+// acc += P X over the columns of the block at col0 that some row of the warp's eight sees: [lo, hi], and the first `sinks` up to hi
+template <int DP, int FEAT>
+__device__ __forceinline__ void accumulate_seen(float4 (&acc)[4][Tiled<DP>::kND], const float* P, const float* X, int lo, int hi, int col0, int sinks,
+                                                int ty, int tx) {
+  int k0, k1;
+  if constexpr ((FEAT & kSinks) != 0) {
+    if (col0 < sinks) {
+      seen_columns<DP>(0, min(sinks - 1, hi), col0, k0, k1);
+      tile_accumulate<DP>(acc, P, X, k0, k1, ty, tx);
+      const int end = max(k1 + 7, 0) & ~7;      // (rounded up as the accumulation was)
+      seen_columns<DP>(lo, hi, col0, k0, k1);
+      tile_accumulate<DP>(acc, P, X, max(k0, end), k1, ty, tx);
+      return;
+    }
+  }
+  seen_columns<DP>(lo, hi, col0, k0, k1);
+  tile_accumulate<DP>(acc, P, X, k0, k1, ty, tx);
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void store_acc_row(T* dst, const float4 (&acc)[Tiled<DP>::kND], float scale, int d, int tx) {
 #pragma unroll
@@ -219,7 +259,7 @@ __device__ __forceinline__ const T* bias_at(const Params& p, const Seq& sq, int 
 // as long, and an SM has 16 warps instead of 12.  Within a group the copy of V runs under the scores, that of the next K
 // under the accumulation.
 constexpr int kFwdGroups = 2;
-template <typename T, int DP>
+template <typename T, int DP, int FEAT>
 __global__ void __launch_bounds__(kFwdGroups * 128, 2) tiled_fwd_kernel(const __grid_constant__ Params p) {
   wait_for_earlier_grids();
   using C = Tiled<DP>;
@@ -239,7 +279,10 @@ __global__ void __launch_bounds__(kFwdGroups * 128, 2) tiled_fwd_kernel(const __
   int x, h, z;
   tile_of_block<true>((int)blockIdx.x, (int)blockIdx.y, (int)blockIdx.z, (int)gridDim.x, (int)gridDim.y, (int)gridDim.z, x, h, z);
   const int m0 = ((int)gridDim.x - 1 - x) * C::kBM;
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
+  if constexpr ((FEAT & kSinks) != 0) {
+    if (p.varlen_mode == 2 && m0 + C::kBM > sq.sq) write_rows_behind<T>(p, sq, h, m0, C::kBM);
+  }
   if (m0 >= sq.sq) return;
   const int hk = h / p.group, ty = tid >> 4, tx = tid & 15;
   const bool kvec = rows_vec4<T>(p.k, p.dqk), vvec = rows_vec4<T>(p.v, p.dvo);
@@ -251,7 +294,8 @@ __global__ void __launch_bounds__(kFwdGroups * 128, 2) tiled_fwd_kernel(const __
   const int wm = m0 + (tid >> 5) * kWarpRows;
   if (wm < sq.sq) key_range(p, sq, wm, min(wm + kWarpRows, sq.sq) - 1, w_lo, w_hi);
   const int d4 = (p.dqk + 3) >> 2;
-  int n0 = n_lo / C::kBN * C::kBN + grp * C::kBN;
+  BlockWalk<DP, FEAT> walk(p, n_lo, n_hi, grp);
+  int n0 = walk.start;
   stage_tile<T, DP, C::kBM, kFwdGroups * 128>(Qs, p.q, sq.bidx, h, sq.q0, m0, sq.sq, p.dqk, rows_vec4<T>(p.q, p.dqk), threadIdx.x);
   if (n0 <= n_hi) stage_tile<T, DP, C::kBN, 128>(Ks, p.k, sq.bidx, hk, sq.k0, n0, sq.sk, p.dqk, kvec, tid);
   float m_i[4], l_i[4];
@@ -265,7 +309,7 @@ __global__ void __launch_bounds__(kFwdGroups * 128, 2) tiled_fwd_kernel(const __
   }
   stage_wait<0>();
   __syncthreads();      // (Q is staged by both groups)
-  for (; n0 <= n_hi; n0 += kFwdGroups * C::kBN) {
+  for (; n0 <= n_hi; n0 = walk.advance(n0, kFwdGroups)) {
     stage_wait<0>();
     group_sync();       // K has landed, the previous block's V has been read
     stage_tile<T, DP, C::kBN, 128>(Vs, p.v, sq.bidx, hk, sq.k0, n0, sq.sk, p.dvo, vvec, tid);
@@ -279,7 +323,7 @@ __global__ void __launch_bounds__(kFwdGroups * 128, 2) tiled_fwd_kernel(const __
 #pragma unroll
       for (int j = 0; j < C::kNC; ++j) {
         const int n = n0 + tx + 16 * j;
-        const bool ok = score_valid(p, sq, m, n);
+        const bool ok = score_valid_for<(FEAT & kSinks) != 0>(p, sq, m, n);
         s[i][j] *= p.qk_scale;
         if (ok && p.has_bias) s[i][j] += to_f32<T>(*bias_at<T>(p, sq, h, m, n)) * kLog2e;
         if (!ok) s[i][j] = -INFINITY;
@@ -304,11 +348,9 @@ __global__ void __launch_bounds__(kFwdGroups * 128, 2) tiled_fwd_kernel(const __
     }
     stage_wait<0>();
     group_sync();       // V has landed, K has been read
-    if (n0 + kFwdGroups * C::kBN <= n_hi)
-      stage_tile<T, DP, C::kBN, 128>(Ks, p.k, sq.bidx, hk, sq.k0, n0 + kFwdGroups * C::kBN, sq.sk, p.dqk, kvec, tid);
-    int k0, k1;
-    seen_columns<DP>(w_lo, w_hi, n0, k0, k1);
-    tile_accumulate<DP>(acc, Ps, Vs, k0, k1, ty, tx);
+    if (walk.next(n0, kFwdGroups) <= n_hi)
+      stage_tile<T, DP, C::kBN, 128>(Ks, p.k, sq.bidx, hk, sq.k0, walk.next(n0, kFwdGroups), sq.sk, p.dqk, kvec, tid);
+    accumulate_seen<DP, FEAT>(acc, Ps, Vs, w_lo, w_hi, n0, p.sinks, ty, tx);
     __syncwarp();
   }
 #pragma unroll
@@ -380,7 +422,7 @@ __device__ __forceinline__ void pair_exchange(float* buf, float4 (&keep)[N], con
 
 // dK / dV of 32 keys of one kv head.  The scores of dO V^T come first: its tile is the first to be free again, so that the
 // next block's dO is on its way under the accumulation of dK, Q behind it.
-template <typename T, int DP, int SPLIT>
+template <typename T, int DP, int SPLIT, int FEAT>
 __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int z, int hk, int n0) {
   using C = Tiled<DP>;
   constexpr int kThr = C::kThreads;
@@ -392,7 +434,7 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
   float* dSs = Ps + C::kBM * C::kLdP;
   float* lse_s = dSs + C::kBM * C::kLdP;  // [BN]
   float* dl_s = lse_s + C::kBN;
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
   if (n0 >= sq.sk) return;
   const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   const bool qvec = rows_vec4<T>(p.q, p.dqk), dovec = rows_vec4<T>(p.dout, p.dvo);
@@ -405,6 +447,10 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
   query_range(p, sq, n0, min(n0 + C::kBM, sq.sk) - 1, m_lo, m_hi);
   const int wn = n0 + (tid >> 5) * kWarpRows;
   if (wn < sq.sk) query_range(p, sq, wn, min(wn + kWarpRows, sq.sk) - 1, w_lo, w_hi);
+  if constexpr ((FEAT & kSinks) != 0) {      // first keys: every query behind them
+    if (n0 < p.sinks) m_hi = sq.sq - 1;
+    if (wn < p.sinks && wn < sq.sk) w_hi = sq.sq - 1;
+  }
   const int dq4 = (p.dqk + 3) >> 2, dv4 = (p.dvo + 3) >> 2;
   const int first = m_lo / C::kBN * C::kBN;
   auto stage_q = [&](int h, int m0) {      // Q, and the rows' logsumexp and delta
@@ -456,7 +502,7 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
         for (int i = 0; i < 4; ++i) {
           const int n = n0 + ty * 4 + i;
           float pd = 0.f, ds = 0.f;
-          if (score_valid(p, sq, m, n)) {
+          if (score_valid_for<(FEAT & kSinks) != 0>(p, sq, m, n)) {
             float x = s[i][j] * p.qk_scale;
             if (p.has_bias) x += to_f32<T>(*bias_at<T>(p, sq, h, m, n)) * kLog2e;
             const float pr = exp2f(x - lse);      // lse = +inf on dead rows -> 0
@@ -512,7 +558,7 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
 
 // dQ (+ dBias) of 32 query rows of one head.  V is read by the scores only: the next block's is on its way for the rest
 // of a block.
-template <typename T, int DP, int SPLIT>
+template <typename T, int DP, int SPLIT, int FEAT>
 __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z, int h, int m0) {
   using C = Tiled<DP>;
   constexpr int kThr = C::kThreads;
@@ -521,7 +567,7 @@ __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z
   float* Ks = dOs + C::kBM * C::kLd;      // [BN][LD]
   float* Vs = Ks + C::kBN * C::kLd;
   float* dSs = Vs + C::kBN * C::kLd;      // [32][BN + 4]
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
   if (m0 >= sq.sq) return;
   const int tid = threadIdx.x, hk = h / p.group, ty = tid >> 4, tx = tid & 15;
   const bool kvec = rows_vec4<T>(p.k, p.dqk), vvec = rows_vec4<T>(p.v, p.dvo);
@@ -530,7 +576,8 @@ __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z
   int n_lo, n_hi, w_lo = 1, w_hi = 0;
   key_range(p, sq, m0, min(m0 + C::kBM, sq.sq) - 1, n_lo, n_hi);
   const uint32_t rank = SPLIT == 2 ? pair_rank() : 0u;
-  const int first = n_lo / C::kBN * C::kBN + (int)rank * C::kBN;      // (this CTA's)
+  BlockWalk<DP, FEAT> walk(p, n_lo, n_hi, (int)rank);
+  const int first = walk.start;      // (this CTA's)
   auto stage_k = [&](int n0) { stage_tile<T, DP, C::kBN, kThr>(Ks, p.k, sq.bidx, hk, sq.k0, n0, sq.sk, p.dqk, kvec, tid); };
   auto stage_v = [&](int n0) { stage_tile<T, DP, C::kBN, kThr>(Vs, p.v, sq.bidx, hk, sq.k0, n0, sq.sk, p.dvo, vvec, tid); };
   if (first <= n_hi) {
@@ -559,13 +606,14 @@ __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z
   const int dq4 = (p.dqk + 3) >> 2, dv4 = (p.dvo + 3) >> 2;
   stage_wait<2>();      // dO and V
   __syncthreads();
-  for (int n0 = first; n0 <= n_hi; n0 += SPLIT * C::kBN) {
-    const bool more = n0 + SPLIT * C::kBN <= n_hi;
+  for (int n0 = first; n0 <= n_hi; n0 = walk.advance(n0, SPLIT)) {
+    const int next = walk.next(n0, SPLIT);
+    const bool more = next <= n_hi;
     float s[4][C::kNC], dp[4][C::kNC];
     tile_dots<DP>(dp, dOs, Vs, dv4, ty, tx);
     stage_wait<0>();
     __syncthreads();      // V has been read, K (and Q) is there
-    if (more) stage_v(n0 + SPLIT * C::kBN);
+    if (more) stage_v(next);
     tile_dots<DP>(s, Qs, Ks, dq4, ty, tx);
     const uint32_t keep = p.dropout_on ? tile_keep_bits<C::kNC>(dctx, m0 + ty * 4, n0, tx) : 0xffffffffu;
 #pragma unroll
@@ -575,7 +623,7 @@ __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z
       for (int j = 0; j < C::kNC; ++j) {
         const int n = n0 + tx + 16 * j;
         float ds = 0.f;
-        if (score_valid(p, sq, m, n)) {
+        if (score_valid_for<(FEAT & kSinks) != 0>(p, sq, m, n)) {
           float x = s[i][j] * p.qk_scale;
           if (p.has_bias) x += to_f32<T>(*bias_at<T>(p, sq, h, m, n)) * kLog2e;
           const float pr = exp2f(x - lse[i]);
@@ -590,12 +638,10 @@ __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z
       }
     }
     __syncwarp();
-    int k0, k1;
-    seen_columns<DP>(w_lo, w_hi, n0, k0, k1);
-    tile_accumulate<DP>(adq, dSs, Ks, k0, k1, ty, tx);
+    accumulate_seen<DP, FEAT>(adq, dSs, Ks, w_lo, w_hi, n0, p.sinks, ty, tx);
     stage_wait<0>();
     __syncthreads();      // K has been read, the next V is there
-    if (more) stage_k(n0 + SPLIT * C::kBN);
+    if (more) stage_k(next);
   }
   if constexpr (SPLIT == 2) {      // the first CTA finishes two of a thread's rows, the second the others (K's and V's tiles are free)
     float4 mine[2 * C::kND], theirs[2 * C::kND];
@@ -628,7 +674,7 @@ __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z
 // Hq, batch), last rows first.  3: both in one launch, x alternating between the two (neither reads what the other
 // writes); joint_backward() says when.  At the sizes single precision is used at, each of the two alone leaves most of the chip idle: 2 x 8
 // heads x 500 tokens are 256 CTAs of four warps, 7 warps an SM, waiting for their own loads and barriers.
-template <typename T, int DP, int WHICH, int SPLIT>
+template <typename T, int DP, int WHICH, int SPLIT, int FEAT>
 __global__ void __cluster_dims__(SPLIT, 1, 1) __launch_bounds__(128, DP <= 64 || WHICH == 2 ? 3 : 2)
 tiled_bwd_kernel(const __grid_constant__ Params p) {
   wait_for_earlier_grids();
@@ -638,15 +684,15 @@ tiled_bwd_kernel(const __grid_constant__ Params p) {
   int x, h, z;
   tile_of_block<false>((int)blockIdx.x / SPLIT, (int)blockIdx.y, (int)blockIdx.z, nx, (int)gridDim.y, (int)gridDim.z, x, h, z);
   if constexpr (WHICH == 1) {
-    tiled_bwd_dkdv<T, DP, SPLIT>(p, smem, z, h, x * kBM);
+    tiled_bwd_dkdv<T, DP, SPLIT, FEAT>(p, smem, z, h, x * kBM);
   } else if constexpr (WHICH == 2) {
-    tiled_bwd_dq<T, DP, SPLIT>(p, smem, z, h, (nx - 1 - x) * kBM);
+    tiled_bwd_dq<T, DP, SPLIT, FEAT>(p, smem, z, h, (nx - 1 - x) * kBM);
   } else {
     if (x & 1) {
       const int m0 = (nx / 2 - 1 - (x >> 1)) * kBM;
-      if (m0 < p.max_sq) tiled_bwd_dq<T, DP, SPLIT>(p, smem, z, h, m0);
+      if (m0 < p.max_sq) tiled_bwd_dq<T, DP, SPLIT, FEAT>(p, smem, z, h, m0);
     } else if (h < p.hk) {
-      tiled_bwd_dkdv<T, DP, SPLIT>(p, smem, z, h, (x >> 1) * kBM);
+      tiled_bwd_dkdv<T, DP, SPLIT, FEAT>(p, smem, z, h, (x >> 1) * kBM);
     }
   }
 }

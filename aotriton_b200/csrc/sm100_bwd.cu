@@ -188,18 +188,55 @@ struct DkdvItem {
   Seq sq;
   int mb_lo, nmb, niter;   // niter == 0: keys no query attends to (gradients are zero)
   bool valid;              // false: key block beyond this sequence
+  int hg0, mb0;            // head of the group and query block of the first iteration
+  int chunk;               // sink attention: 0 the key block's own item, else the chunk-th that shares the queries beyond its window
 };
 
+// Sink attention: first keys are seen by all queries behind them, the others by a window's worth, so a block of first keys would
+// keep its CTA long after the others are done (8 kv heads of a group of 8, 16384 tokens, window 1024: 1024 query blocks against 72 of every
+// other block, of which a CTA gets some 550 in all).  Its own item stops at the window like any other; the query blocks beyond are shared
+// out over sink_chunks items, drawn first.  Each leaves its fp32 sums for the first keys in the workspace, which a last launch adds up
+// in their order (sink_finish_kernel).
+template <int FEAT>
 __device__ __forceinline__ DkdvItem dkdv_item(const Params& p, int w) {
   DkdvItem it;
+  it.hg0 = it.mb0 = it.chunk = 0;
   const int per = p.batch * p.hk;
+  if constexpr ((FEAT & kSinks) != 0) {
+    const int extra = per * ((p.sinks + kBlk - 1) / kBlk) * p.sink_chunks;
+    if (w < extra) {
+      const int zh = w % per, r = w / per;
+      it.z = zh / p.hk;
+      it.hk = zh - it.z * p.hk;
+      it.chunk = r % p.sink_chunks + 1;
+      it.n0 = r / p.sink_chunks * kBlk;
+      it.sq = resolve_seq_for<FEAT>(p, it.z);
+      it.valid = it.n0 < it.sq.sk;
+      it.mb_lo = it.nmb = it.niter = 0;
+      if (it.valid && it.sq.sq > 0) {
+        int m_lo, m_hi;
+        query_range(p, it.sq, it.n0, min(it.n0 + kBlk, it.sq.sk) - 1, m_lo, m_hi);
+        it.mb_lo = m_hi >= m_lo ? m_hi / kBlk + 1 : m_lo / kBlk;
+        it.nmb = max(0, (it.sq.sq - 1) / kBlk - it.mb_lo + 1);
+        const int64_t total = (int64_t)it.nmb * p.group;
+        const int from = (int)(total * (it.chunk - 1) / p.sink_chunks), to = (int)(total * it.chunk / p.sink_chunks);
+        it.niter = to - from;
+        if (it.niter > 0) {
+          it.hg0 = from / it.nmb;
+          it.mb0 = from - it.hg0 * it.nmb;
+        }
+      }
+      return it;
+    }
+    w -= extra;
+  }
   const int nkb = (p.max_sk + kBlk - 1) / kBlk;
   const int grp = quick_div_any(w, nkb * 8), r = w - grp * (nkb * 8);
   const int kb = r >> 3, rem = grp * 8 + (r & 7);
   it.z = quick_div(min(rem, per - 1), p.hk);
   it.hk = min(rem, per - 1) - it.z * p.hk;
   it.n0 = kb * kBlk;
-  it.sq = resolve_seq(p, it.z);
+  it.sq = resolve_seq_for<FEAT>(p, it.z);
   it.valid = rem < per && it.n0 < it.sq.sk;
   it.mb_lo = it.nmb = it.niter = 0;
   if (it.valid) {
@@ -286,7 +323,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       uint32_t G = 0, live = 0, drawn = 0;
       bool ok = true;
       for (int w = blockIdx.x; ok && w < nitems; w = next_item(drawn++, false)) {
-        const DkdvItem it = dkdv_item(p, w);
+        const DkdvItem it = dkdv_item<FEAT>(p, w);
         if (!it.valid || it.niter == 0) continue;
         // K and V of the previous item are free once its last S and dP GEMMs have run.
         if (!mbar_wait(&bars[L::bResEmpty], (live & 1u) ^ 1u, abort_flag, status, 0x1000)) break;
@@ -296,7 +333,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           tma_load_4d(smem + L::kResA + hf * 16384, &tm_k, &bars[L::bResFull], hf * 64, krow, it.hk, it.sq.bidx);
           tma_load_4d(smem + L::kResB + hf * 16384, &tm_v, &bars[L::bResFull], hf * 64, krow, it.hk, it.sq.bidx);
         }
-        for (int i = 0, hg = 0, mb = 0; i < it.niter; ++i, ++G) {     // hg, mb: i / nmb, i % nmb
+        for (int i = 0, hg = it.hg0, mb = it.mb0; i < it.niter; ++i, ++G) {     // hg, mb: i / nmb, i % nmb
           const int s = (int)(G & 1u);
           const int h = it.hk * p.group + hg;
           const int mrow = (int)(it.sq.q0 + (int64_t)(it.mb_lo + mb) * kBlk);
@@ -372,7 +409,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     uint32_t G = 0, live = 0, drawn = 0;
     bool ok = true;
     for (int w = blockIdx.x; ok && w < nitems; w = next_item(drawn++, true)) {
-      const DkdvItem it = dkdv_item(p, w);
+      const DkdvItem it = dkdv_item<FEAT>(p, w);
       if (!it.valid || it.niter == 0) continue;
       // first iteration of the item: K/V resident, Q/dO block landed, S buffer read out by the
       // compute warps (the dP buffer is released in issue order by the previous item's dV/dK)
@@ -403,7 +440,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           }
         }
       };
-      zero_ring_tail(G, 0);
+      zero_ring_tail(G, it.mb0);
       tc_fence_after();
       issue_s(G);
       issue_dp(G, !FUSED && it.niter == 1);
@@ -419,7 +456,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         }
         __syncwarp();
       };
-      for (int i = 0, mb_next = 1; i < it.niter; ++i, ++G, ++mb_next) {     // mb_next: (i + 1) % nmb
+      for (int i = 0, mb_next = it.mb0 + 1; i < it.niter; ++i, ++G, ++mb_next) {     // mb_next: (i + 1) % nmb
         const uint32_t s = G & 1u, par = G & 1u;
         if (mb_next == it.nmb) mb_next = 0;
         if constexpr (FUSED) {
@@ -496,9 +533,9 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     uint32_t G = 0, drawn = 0;
     bool ok = true;
     for (int w = blockIdx.x; ok && w < nitems; w = next_item(drawn++, true)) {
-      const DkdvItem it = dkdv_item(p, w);
+      const DkdvItem it = dkdv_item<FEAT>(p, w);
       if (!it.valid || it.niter == 0) continue;
-      for (int i = 0, hg = 0, mb = 0; i < it.niter; ++i, ++G) {     // hg, mb: i / nmb, i % nmb
+      for (int i = 0, hg = it.hg0, mb = it.mb0; i < it.niter; ++i, ++G) {     // hg, mb: i / nmb, i % nmb
         const int s = (int)(G & 1u);
         if (!mbar_wait_relaxed(&bars[L::bAuxEmpty + s], ((G >> 1) & 1u) ^ 1u, abort_flag, status, 0x1600)) { ok = false; break; }
         const int h = it.hk * p.group + hg;
@@ -556,13 +593,19 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     const uint64_t ph_seed = (drop_on && p.seed_ptr) ? *p.seed_ptr : 0ull;
     const uint64_t ph_off = p.off2 + ((drop_on && p.off1_ptr) ? *p.off1_ptr : 0ull);
     for (int w = blockIdx.x; ok && w < nitems; w = next_item(drawn++, true)) {
-      const DkdvItem it = dkdv_item(p, w);
+      const DkdvItem it = dkdv_item<FEAT>(p, w);
       if (!it.valid) continue;
       const Seq& sq = it.sq;
       const int hk = it.hk, z = it.z;
       const int n = it.n0 + r;
       if (it.niter == 0) {          // no query attends to these keys
-        if (wg == 0 && n < sq.sk) {
+        if constexpr ((FEAT & kSinks) != 0) {
+          if (wg == 0 && n < min(p.sinks, sq.sk)) {
+            float* sums = sink_partial_row(p, z, hk, it.chunk, n);
+            for (int c = 0; c < p.dqk + p.dvo; ++c) sums[c] = 0.f;
+          }
+        }
+        if (wg == 0 && n < sq.sk && it.chunk == 0) {
           T* dkp = reinterpret_cast<T*>(p.dk.ptr) + (int64_t)sq.bidx * p.dk.s[0] + (int64_t)hk * p.dk.s[1] +
                    (sq.k0 + n) * p.dk.s[2];
           T* dvp = reinterpret_cast<T*>(p.dv.ptr) + (int64_t)sq.bidx * p.dv.s[0] + (int64_t)hk * p.dv.s[1] +
@@ -583,6 +626,10 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         if (hi < col_hi) col_hi = (int)(hi < -1 ? -1 : hi);
       }
       if (FUSED && n >= sq.sk) { col_lo = 1; col_hi = 0; }
+      if constexpr ((FEAT & kSinks) != 0) {
+        if (n < p.sinks) col_hi = sq.sq - 1;
+        else if (it.chunk > 0) { col_lo = 1; col_hi = 0; }
+      }
       // the tightest bounds over the warp's rows: a block needs masking iff it is not inside them
       const int warp_lo = __reduce_max_sync(0xffffffffu, col_lo), warp_hi = __reduce_min_sync(0xffffffffu, col_hi);
       // Fused form: the dQ^T partial of iteration g (head dim x queries, in the S columns) is taken
@@ -601,7 +648,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           }
         }
       };
-      for (int i = 0, hg = 0, mb = 0; i < it.niter; ++i, ++G) {     // hg, mb: i / nmb, i % nmb
+      for (int i = 0, hg = it.hg0, mb = it.mb0; i < it.niter; ++i, ++G) {     // hg, mb: i / nmb, i % nmb
         const int s = (int)(G & 1u);
         const uint32_t par = G & 1u;
         const int h = hk * p.group + hg;
@@ -830,12 +877,25 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         // Each warp transposes its 32 rows x 32 columns through the staging tile, so that the global
         // stores are 64-byte row segments instead of 16 bytes per row.
         const uint32_t stage = smem_u32(smem + L::kStage);
-        const int nrows = min(kBlk, sq.sk - it.n0);
+        const int nrows = (FEAT & kSinks) != 0 && it.chunk > 0 ? 0 : min(kBlk, sq.sk - it.n0);
         const int d0 = wg * 32;
         float v[32];
+        // a first key's sums (the 16-bit row written below is overwritten by the last launch)
+        auto keep_sums = [&](int at, int d) {
+          if constexpr ((FEAT & kSinks) != 0) {
+            if (n < min(p.sinks, sq.sk)) {
+              float* sums = sink_partial_row(p, z, hk, it.chunk, n) + at + d0;
+#pragma unroll
+              for (int c = 0; c < 32; c += 4)
+                if (d0 + c < d) *reinterpret_cast<float4*>(sums + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+            }
+            __syncwarp();
+          }
+        };
         tc_fence_after();
         tmem_ld32f(tmem_base + lane_addr + kColAcc0 + d0, v);
         tmem_wait_ld();
+        keep_sums(p.dqk, p.dvo);
         stage_put32<T>(stage, r, d0, v, 1.0f, HD * 2);
         __syncwarp();
         warp_copy_out<T, 4>(stage, reinterpret_cast<T*>(p.dv.ptr) + (int64_t)sq.bidx * p.dv.s[0] + (int64_t)hk * p.dv.s[1] +
@@ -847,6 +907,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         // zero) are only issued after this thread's next hand-off, i.e. after these loads.
         tc_fence_before();
         __syncwarp();
+        keep_sums(0, p.dqk);
         stage_put32<T>(stage, r, d0, v, p.sm_scale, HD * 2);
         __syncwarp();
         warp_copy_out<T, 4>(stage, reinterpret_cast<T*>(p.dk.ptr) + (int64_t)sq.bidx * p.dk.s[0] + (int64_t)hk * p.dk.s[1] +
@@ -868,6 +929,31 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, kTmemCols);
+  }
+}
+
+// dK and dV of the first keys: the sums of the items that shared their queries, in the items' order.  A few hundred kilobytes at most,
+// in L2.  grid = (sinks, Hk, batch), a thread four columns.
+template <typename T>
+__global__ void __launch_bounds__(128) sink_finish_kernel(const __grid_constant__ Params p) {
+  wait_for_earlier_grids();
+  const int n = blockIdx.x, hk = blockIdx.y, z = blockIdx.z;
+  const Seq sq = resolve_seq_for<kSinks>(p, z);
+  if (n >= sq.sk) return;
+  const int64_t step = (int64_t)p.sinks * (p.dqk + p.dvo);
+  for (int c = threadIdx.x * 4; c < p.dqk + p.dvo; c += 512) {
+    const float* from = sink_partial_row(p, z, hk, 0, n) + c;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i <= p.sink_chunks; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(from + i * step);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+    const bool is_k = c < p.dqk;
+    const View4& v = is_k ? p.dk : p.dv;
+    const float scale = is_k ? p.sm_scale : 1.f;
+    T* to = reinterpret_cast<T*>(v.ptr) + (int64_t)sq.bidx * v.s[0] + (int64_t)hk * v.s[1] + (sq.k0 + n) * v.s[2] + (is_k ? c : c - p.dqk);
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack2<T>(s.x * scale, s.y * scale), pack2<T>(s.z * scale, s.w * scale));
   }
 }
 
@@ -931,7 +1017,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
   // on behind the set-up, which so runs under the read.
   const unsigned int failed_before = *reinterpret_cast<volatile unsigned int*>(status);
   if (warp == 2 && lane == 0) { prefetch_tmap(&tm_q); prefetch_tmap(&tm_do); prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
   if (m0 >= sq.sq) return;
   const int hk = quick_div(h, p.group);
   int n_lo, n_hi;
@@ -942,7 +1028,9 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
     return;
   }
   const int jb_lo = n_lo / kBlk;
-  const int niter = n_hi / kBlk - jb_lo + 1;
+  const int before = blocks_before<FEAT>(p, n_hi, jb_lo, kBlk);
+  const int niter = before + n_hi / kBlk - jb_lo + 1;
+  auto block = [&](int i) { return block_at<FEAT>(i, before, jb_lo); };
   if (dbias_on) zero_dbias_outside<T>(p, sq, h, m0, kBlk, jb_lo * kBlk, (jb_lo + niter) * kBlk);
 
   if (threadIdx.x == 0) {
@@ -968,7 +1056,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
       tma_load_4d(smem + L::kResA + hf * 16384, &tm_q, &bars[L::bResFull], hf * 64, qrow, h, sq.bidx);
       tma_load_4d(smem + L::kResB + hf * 16384, &tm_do, &bars[L::bResFull], hf * 64, qrow, h, sq.bidx);
     }
-    const int krow = (int)(sq.k0 + (int64_t)jb_lo * kBlk);
+    const int krow = (int)(sq.k0 + (int64_t)block(0) * kBlk);
     mbar_expect_tx(&bars[L::bKFull], L::kTile);
     for (int hf = 0; hf < L::kHalves; ++hf)
       tma_load_4d(smem + L::kK + hf * 16384, &tm_k, &bars[L::bKFull], hf * 64, krow, hk, sq.bidx);
@@ -1003,7 +1091,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
       int issued_k = 1, issued_v = 1;
       for (int i = 1; i < niter; ++i) {
         const int sv = i & 1, sk = i % L::kKStages;
-        const int krow = (int)(sq.k0 + (int64_t)(jb_lo + i) * kBlk);
+        const int krow = (int)(sq.k0 + (int64_t)block(i) * kBlk);
         if (!mbar_wait(&bars[L::bKEmpty + sk], ((uint32_t)(i / L::kKStages) & 1u) ^ 1u, abort_flag, status, 0x2180 + i)) break;
         mbar_expect_tx(&bars[L::bKFull + sk], L::kTile);
         for (int hf = 0; hf < L::kHalves; ++hf)
@@ -1044,13 +1132,20 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
     // dP and dQ products (a zero dS times a non-finite K row, or dO times a non-finite V row).
     auto zero_tail = [&](int base, int i, int stage) {
       if constexpr (!EXACT) {
-        const int valid = sq.sk - (jb_lo + i) * kBlk;
+        const int valid = sq.sk - block(i) * kBlk;
         if (valid < kBlk) zero_tail_rows(smem + base + stage * L::kTile, valid, L::kHalves, lane);
+      }
+      if constexpr ((FEAT & kSinks) != 0) {
+        int from, to;
+        hidden_keys(p, sq, from, to);
+        from = max(from - block(i) * kBlk, 0);
+        to = min(to - block(i) * kBlk, kBlk);
+        if (from < to) zero_rows_between(smem + base + stage * L::kTile, from, to, L::kHalves, 16384, lane);
       }
     };
     auto issue_s = [&](int i) {      // S = Q K_i^T
       zero_tail(L::kK, i, i % L::kKStages);
-      if constexpr (!EXACT) tc_fence_after();
+      if constexpr (!EXACT || (FEAT & kSinks) != 0) tc_fence_after();
       const uint64_t ka = k_km + (uint64_t)((uint32_t)(i % L::kKStages) * kStageStep);
       if (elect_one()) {
 #pragma unroll
@@ -1063,7 +1158,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
     };
     auto issue_dp = [&](int i) {     // dP = dO V_i^T, into dP buffer i & 1; frees V's ring stage
       zero_tail(L::kV, i, i & 1);
-      if constexpr (!EXACT) tc_fence_after();
+      if constexpr (!EXACT || (FEAT & kSinks) != 0) tc_fence_after();
       const uint64_t va = v_km + (uint64_t)((uint32_t)(i & 1) * kStageStep);
       const uint32_t d = tmem_base + kColDP + (uint32_t)(i & 1) * 128u;
       if (elect_one()) {
@@ -1171,7 +1266,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
     bool ok = true;
     for (int i = 0; i < niter; ++i) {
       const uint32_t par = (uint32_t)i & 1u;
-      const int nbase = (jb_lo + i) * kBlk + cbase;     // first key of this thread's columns
+      const int nbase = block(i) * kBlk + cbase;     // first key of this thread's columns
       if (threadIdx.x == AB200_TRACE_TID) AB200_STAMPQ(i, 4);
       // keep bits the dK/dV kernel left behind: on their way while the tensor pipe computes S
       const bool shared = drop_on && keep_shared(p, sq, m0 + quarter * 32, nbase);
@@ -1217,7 +1312,8 @@ sm100_bwd_dq_kernel(const __grid_constant__ Params p, const __grid_constant__ CU
         for (int c = 0; c < 32; ++c) pr[c] = ex2(pr[c] - lse2);
       }
       if (any_mask) {
-        mask_columns<32, FEAT != kAll>(pr, nbase, row_lo, row_hi, nbase >= warp_lo, 0.f);
+        if ((FEAT & kSinks) != 0 && nbase < p.sinks) mask_sink_columns<32>(pr, nbase, row_lo, row_hi, p.sinks, 0.f);
+        else mask_columns<32, FEAT != kAll>(pr, nbase, row_lo, row_hi, nbase >= warp_lo, 0.f);
       }
       uint32_t keep = 0xffffffffu;
       if (shared) {
@@ -1330,7 +1426,7 @@ cudaError_t launch_bwd_T(int which, const Params& p, cudaStream_t st, float* dq_
   // make the stream's device, and remembered.
   struct PerDevice { std::atomic<unsigned int*> status{nullptr}; std::atomic<int> sms{0}; };
   static PerDevice per_device[64];
-  static std::atomic<bool> attr_set[64][20];
+  static std::atomic<bool> attr_set[64][24];
   const bool exact = p.varlen_mode == 0 && p.max_sq % 128 == 0 && p.max_sk % 128 == 0 && p.dqk == HD && p.dvo == HD;
   const int feat = features(p);
   int dev = 0;
@@ -1354,20 +1450,23 @@ cudaError_t launch_bwd_T(int which, const Params& p, cudaStream_t st, float* dq_
   };
   if (which == 1 || which == 3) {
     const bool fused = which == 3;
-    if (fused && HD != 128) return cudaErrorInvalidValue;
+    if (fused && (HD != 128 || feat == kSinks)) return cudaErrorInvalidValue;
     using Kernel = decltype(&sm100_bwd_dkdv_kernel<T, HD, false, true, kPlain>);
-    static constexpr Kernel kSplit[2][4] = {
+    static constexpr Kernel kSplit[2][5] = {
         {sm100_bwd_dkdv_kernel<T, HD, false, false, kPlain>, sm100_bwd_dkdv_kernel<T, HD, false, false, kBias>,
-         sm100_bwd_dkdv_kernel<T, HD, false, false, kDropout>, sm100_bwd_dkdv_kernel<T, HD, false, false, kAll>},
+         sm100_bwd_dkdv_kernel<T, HD, false, false, kDropout>, sm100_bwd_dkdv_kernel<T, HD, false, false, kAll>,
+         sm100_bwd_dkdv_kernel<T, HD, false, false, kSinks>},
         {sm100_bwd_dkdv_kernel<T, HD, false, true, kPlain>, sm100_bwd_dkdv_kernel<T, HD, false, true, kBias>,
-         sm100_bwd_dkdv_kernel<T, HD, false, true, kDropout>, sm100_bwd_dkdv_kernel<T, HD, false, true, kAll>}};
+         sm100_bwd_dkdv_kernel<T, HD, false, true, kDropout>, sm100_bwd_dkdv_kernel<T, HD, false, true, kAll>,
+         sm100_bwd_dkdv_kernel<T, HD, false, true, kSinks>}};
     static constexpr Kernel kFused[4] = {sm100_bwd_dkdv_kernel<T, 128, true, false, kPlain>, sm100_bwd_dkdv_kernel<T, 128, true, false, kBias>,
                                          sm100_bwd_dkdv_kernel<T, 128, true, false, kDropout>, sm100_bwd_dkdv_kernel<T, 128, true, false, kAll>};
-    const Kernel kern_split = kSplit[exact][feat], kern_fused = kFused[feat];
+    const Kernel kern_split = kSplit[exact][feat], kern_fused = kFused[feat & 3];
     e = fused ? set_smem(16 + feat, reinterpret_cast<const void*>(kern_fused), BwdSmem<128>::kDynamic)
-              : set_smem(2 * feat + exact, reinterpret_cast<const void*>(kern_split), L::kDynamic);
+              : set_smem(feat == kSinks ? 20 + exact : 2 * feat + exact, reinterpret_cast<const void*>(kern_split), L::kDynamic);
     if (e != cudaSuccess) return e;
-    const int nitems = ((p.max_sk + kBlk - 1) / kBlk) * ((p.hk * p.batch + 7) / 8) * 8;
+    const int nitems = ((p.max_sk + kBlk - 1) / kBlk) * ((p.hk * p.batch + 7) / 8) * 8 +
+                       (feat == kSinks ? p.batch * p.hk * ((p.sinks + kBlk - 1) / kBlk) * p.sink_chunks : 0);
     int sms = pd.sms.load(std::memory_order_acquire);
     if (sms == 0) {
       if ((e = host().device_attr(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
@@ -1386,15 +1485,19 @@ cudaError_t launch_bwd_T(int which, const Params& p, cudaStream_t st, float* dq_
     else
       e = launch_kernel(kern_split, grid, dim3(kBwdThreads), L::kDynamic, st, p, tq, tk, tv, tdo, status, nitems, ticket,
                         static_cast<float*>(nullptr));
+    if (e == cudaSuccess && feat == kSinks && p.sinks > 0) {
+      count_launch();
+      e = launch_kernel(sink_finish_kernel<T>, dim3(p.sinks, p.hk, p.batch), dim3(128), 0, st, p);
+    }
   } else {
     using Kernel = decltype(&sm100_bwd_dq_kernel<T, HD, true, kPlain>);
-    static constexpr Kernel kDq[2][4] = {
+    static constexpr Kernel kDq[2][5] = {
         {sm100_bwd_dq_kernel<T, HD, false, kPlain>, sm100_bwd_dq_kernel<T, HD, false, kBias>,
-         sm100_bwd_dq_kernel<T, HD, false, kDropout>, sm100_bwd_dq_kernel<T, HD, false, kAll>},
+         sm100_bwd_dq_kernel<T, HD, false, kDropout>, sm100_bwd_dq_kernel<T, HD, false, kAll>, sm100_bwd_dq_kernel<T, HD, false, kSinks>},
         {sm100_bwd_dq_kernel<T, HD, true, kPlain>, sm100_bwd_dq_kernel<T, HD, true, kBias>,
-         sm100_bwd_dq_kernel<T, HD, true, kDropout>, sm100_bwd_dq_kernel<T, HD, true, kAll>}};
+         sm100_bwd_dq_kernel<T, HD, true, kDropout>, sm100_bwd_dq_kernel<T, HD, true, kAll>, sm100_bwd_dq_kernel<T, HD, true, kSinks>}};
     const Kernel kern_dq = kDq[exact][feat];
-    e = set_smem(8 + 2 * feat + exact, reinterpret_cast<const void*>(kern_dq), DqSmem<HD>::kDynamic);
+    e = set_smem(feat == kSinks ? 22 + exact : 8 + 2 * feat + exact, reinterpret_cast<const void*>(kern_dq), DqSmem<HD>::kDynamic);
     if (e != cudaSuccess) return e;
     dim3 grid((p.max_sq + kBlk - 1) / kBlk, p.hq, p.batch);
     e = launch_kernel(kern_dq, grid, dim3(kBwdThreads), DqSmem<HD>::kDynamic, st, p, tq, tk, tv, tdo, status);

@@ -104,12 +104,15 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
   // see the most keys.  Heavy CTAs start first.
   const int z = blockIdx.z, hrow = blockIdx.y;
   const int r0 = (kKeys ? (int)blockIdx.x : (int)(gridDim.x - 1 - blockIdx.x)) * kBlk;
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
   const int rows_total = kKeys ? sq.sk : sq.sq, cols_total = kKeys ? sq.sq : sq.sk;
   if (r0 >= rows_total) return;
   int c_lo, c_hi;
   if constexpr (kKeys) query_range(p, sq, r0, min(r0 + kBlk, sq.sk) - 1, c_lo, c_hi);
   else key_range(p, sq, r0, min(r0 + kBlk, sq.sq) - 1, c_lo, c_hi);
+  if constexpr (kKeys && (FEAT & kSinks) != 0) {
+    if (r0 < p.sinks) c_hi = sq.sq - 1;      // first keys: every query behind them
+  }
   const View4& outv = MODE == kWideDV ? p.dv : (MODE == kWideDK ? p.dk : p.dq);
   const int d_out = MODE == kWideDV ? p.dvo : p.dqk;
   const int64_t row_tok0 = kKeys ? sq.k0 : sq.q0, col_tok0 = kKeys ? sq.q0 : sq.k0;
@@ -119,7 +122,9 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     return;
   }
   const int cb_lo = c_lo / kNB;
-  const int ncb = c_hi / kNB - cb_lo + 1;
+  const int before = kKeys ? 0 : blocks_before<FEAT>(p, c_hi, cb_lo, kNB);
+  const int ncb = before + c_hi / kNB - cb_lo + 1;
+  auto block = [&](int c) { return kKeys ? cb_lo + c : block_at<FEAT>(c, before, cb_lo); };
   if constexpr (MODE == kWideDQ) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, cb_lo * kNB, (cb_lo + ncb) * kNB); }
   const int niter = kKeys ? ncb * p.group : ncb;      // dV / dK walk the q heads of the kv head's group
   const int hk = kKeys ? hrow : hrow / p.group;
@@ -170,7 +175,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       for (int i = 0, hg = 0, cb = 0; i < niter; ++i) {      // hg, cb: i / ncb, i % ncb
         const int s = i & 1;
         const int hs = kKeys ? hk * p.group + hg : hk;
-        const int srow = (int)(col_tok0 + (int64_t)(cb_lo + cb) * kNB);
+        const int srow = (int)(col_tok0 + (int64_t)block(cb) * kNB);
         if (++cb == ncb) { cb = 0; ++hg; }
         // the early tile first: it is what the block's first GEMM waits for
         const int es = i % kEarlyStages;
@@ -192,7 +197,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           // the next block's K and V towards L2 (their slots free up a block from now; measured: dQ 6 %
           // faster, while for dV and dK, whose streamed Q and dO are shared by fewer CTAs, it did not pay)
           if (i + 1 < niter) {
-            const int nrow = (int)(col_tok0 + (int64_t)(cb_lo + cb) * kNB);
+            const int nrow = (int)(col_tok0 + (int64_t)block(cb) * kNB);
             for (int b = 0; b < L::kBoxes; ++b) {
               tma_prefetch_4d(&tm_late, b * 64, nrow, hk, sq.bidx);
               tma_prefetch_4d(&tm_early, b * 64, nrow, hk, sq.bidx);
@@ -231,7 +236,16 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     };
     // rows of streamed block i that belong to the sequence (a partial last block holds a neighbour's
     // tokens or padding beyond them, which must not reach a product: they are zeroed in place)
-    auto valid_rows = [&](int i) { return cols_total - (cb_lo + (kKeys ? i % ncb : i)) * kNB; };
+    auto valid_rows = [&](int i) { return cols_total - block(kKeys ? i % ncb : i) * kNB; };
+    auto zero_hidden = [&](int i, uint8_t* tile) {      // (dQ) keys that no query sees
+      if constexpr (!kKeys && (FEAT & kSinks) != 0) {
+        int from, to;
+        hidden_keys(p, sq, from, to);
+        from = max(from - block(i) * kNB, 0);
+        to = min(to - block(i) * kNB, kNB);
+        if (from < to) zero_rows_between(tile, from, to, L::kBoxes, L::kStrBox, lane);
+      }
+    };
     // the GEMMs that only need the block's tiles: dP'_i into dP buffer i & 1, then S'_i into the one S'
     // buffer once the compute warps have copied S'_{i-1} out.  (dP' goes first: the late tile S' reads
     // was requested only when the accumulating GEMM of block i-2 had finished, and dP' gives that copy
@@ -259,6 +273,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         const int valid = valid_rows(i);
         if (!wait(L::bEarlyFull + es, epar, 0x3400)) return false;
         if (valid < kNB) zero_tail_rows_streamed(smem + kEarlyBase + es * L::kStr, valid, lane);
+        zero_hidden(i, smem + kEarlyBase + es * L::kStr);
         tc_fence_after();
         const uint64_t ea = early_km + (uint64_t)(es * kStageStep);
         if (elect_one()) {
@@ -273,6 +288,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         if (i > 0 && !wait(L::bSRead, (uint32_t)(i - 1) & 1u, 0x3800)) return false;
         if (!wait(L::bLateFull + s, (uint32_t)(i >> 1) & 1u, 0x3300)) return false;
         if (valid < kNB) zero_tail_rows_streamed(smem + L::kLate + s * L::kStr, valid, lane);
+        zero_hidden(i, smem + L::kLate + s * L::kStr);
         tc_fence_after();
         const uint64_t la = late_km + (uint64_t)(s * kStageStep);
         if (elect_one()) {
@@ -371,6 +387,9 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       const int64_t lo = (int64_t)rb - (kKeys ? sq.wr : sq.wl), hi = (int64_t)rb + (kKeys ? sq.wl : sq.wr);
       if (lo > v_lo) v_lo = (int)(lo > 0x7fffffffLL ? 0x7fffffffLL : lo);
       if (hi < v_hi) v_hi = (int)(hi < -1 ? -1 : hi);
+      if constexpr (kKeys && (FEAT & kSinks) != 0) {
+        if (rb < p.sinks) v_hi = cols_total - 1;
+      }
     }
     // the tightest bounds over the warp's rows: a block needs masking iff it is not inside them
     const int warp_lo = __reduce_max_sync(0xffffffffu, v_lo), warp_hi = __reduce_min_sync(0xffffffffu, v_hi);
@@ -528,7 +547,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       for (int i = 0; i < niter; ++i) {
         const int s = i & 1;
         const uint32_t par2 = (uint32_t)(i >> 1) & 1u;
-        const int nbase = (cb_lo + i) * kNB + cbase;     // first key of this thread's columns
+        const int nbase = block(i) * kNB + cbase;     // first key of this thread's columns
         const bool shared = drop_on && keep_shared(p, sq, r0 + quarter * 32, nbase);
         uint32_t shared_bits = 0u;
         if (shared) shared_bits = *keep_share_word<(FEAT & kBias) != 0>(p, sq, hrow, r0 + quarter * 32, nbase, lane);
@@ -565,7 +584,8 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           for (int c = 0; c < 32; ++c) pr[c] = ex2(pr[c] - lse2);
         }
         if (any_mask) {
-          mask_columns<32, true>(pr, nbase, v_lo, v_hi, nbase >= warp_lo, 0.f);
+          if ((FEAT & kSinks) != 0 && nbase < p.sinks) mask_sink_columns<32>(pr, nbase, v_lo, v_hi, p.sinks, 0.f);
+          else mask_columns<32, true>(pr, nbase, v_lo, v_hi, nbase >= warp_lo, 0.f);
         }
         uint32_t keep = 0xffffffffu;
         if (shared) {
@@ -665,7 +685,7 @@ cudaError_t launch_bwd_wide_T(int which, const Params& p, cudaStream_t st) {
       return cudaErrorInvalidValue;
   }
   static std::atomic<unsigned int*> status_of[64];
-  static std::atomic<bool> attr_set[64][13];
+  static std::atomic<bool> attr_set[64][16];
   const int feat = features(p);
   int dev = 0;
   cudaError_t e = host().get_device(&dev);
@@ -684,14 +704,17 @@ cudaError_t launch_bwd_wide_T(int which, const Params& p, cudaStream_t st) {
     return r;
   };
   using Kernel = decltype(&sm100_bwd_wide_kernel<T, kWideDV, kPlain>);
-  static constexpr Kernel kKernels[3][4] = {      // [kWide*][features]
-      {sm100_bwd_wide_kernel<T, 0, kPlain>, sm100_bwd_wide_kernel<T, 0, kBias>, sm100_bwd_wide_kernel<T, 0, kDropout>, sm100_bwd_wide_kernel<T, 0, kAll>},
-      {sm100_bwd_wide_kernel<T, 1, kPlain>, sm100_bwd_wide_kernel<T, 1, kBias>, sm100_bwd_wide_kernel<T, 1, kDropout>, sm100_bwd_wide_kernel<T, 1, kAll>},
-      {sm100_bwd_wide_kernel<T, 2, kPlain>, sm100_bwd_wide_kernel<T, 2, kBias>, sm100_bwd_wide_kernel<T, 2, kDropout>, sm100_bwd_wide_kernel<T, 2, kAll>}};
+  static constexpr Kernel kKernels[3][5] = {      // [kWide*][features]
+      {sm100_bwd_wide_kernel<T, 0, kPlain>, sm100_bwd_wide_kernel<T, 0, kBias>, sm100_bwd_wide_kernel<T, 0, kDropout>, sm100_bwd_wide_kernel<T, 0, kAll>,
+       sm100_bwd_wide_kernel<T, 0, kSinks>},
+      {sm100_bwd_wide_kernel<T, 1, kPlain>, sm100_bwd_wide_kernel<T, 1, kBias>, sm100_bwd_wide_kernel<T, 1, kDropout>, sm100_bwd_wide_kernel<T, 1, kAll>,
+       sm100_bwd_wide_kernel<T, 1, kSinks>},
+      {sm100_bwd_wide_kernel<T, 2, kPlain>, sm100_bwd_wide_kernel<T, 2, kBias>, sm100_bwd_wide_kernel<T, 2, kDropout>, sm100_bwd_wide_kernel<T, 2, kAll>,
+       sm100_bwd_wide_kernel<T, 2, kSinks>}};
   if (which == 1) {
     const Kernel kern_dv = kKernels[kWideDV][feat], kern_dk = kKernels[kWideDK][feat];
-    if ((e = set_smem(4 * kWideDV + feat, reinterpret_cast<const void*>(kern_dv))) != cudaSuccess) return e;
-    if ((e = set_smem(4 * kWideDK + feat, reinterpret_cast<const void*>(kern_dk))) != cudaSuccess) return e;
+    if ((e = set_smem(feat == kSinks ? 13 + kWideDV : 4 * kWideDV + feat, reinterpret_cast<const void*>(kern_dv))) != cudaSuccess) return e;
+    if ((e = set_smem(feat == kSinks ? 13 + kWideDK : 4 * kWideDK + feat, reinterpret_cast<const void*>(kern_dk))) != cudaSuccess) return e;
     dim3 grid((p.max_sk + kBlk - 1) / kBlk, p.hk, p.batch);
     e = launch_kernel(kern_dv, grid, dim3(wide_threads(kWideDV, feat)), L::kDynamic, st, p, k128, k128, do64, q64, status);
     if (e != cudaSuccess) return e;
@@ -701,7 +724,7 @@ cudaError_t launch_bwd_wide_T(int which, const Params& p, cudaStream_t st) {
     }
   } else {
     const Kernel kern_dq = kKernels[kWideDQ][feat];
-    if ((e = set_smem(4 * kWideDQ + feat, reinterpret_cast<const void*>(kern_dq))) != cudaSuccess) return e;
+    if ((e = set_smem(feat == kSinks ? 13 + kWideDQ : 4 * kWideDQ + feat, reinterpret_cast<const void*>(kern_dq))) != cudaSuccess) return e;
     dim3 grid((p.max_sq + kBlk - 1) / kBlk, p.hq, p.batch);
     e = launch_kernel(kern_dq, grid, dim3(wide_threads(kWideDQ, feat)), L::kDynamic, st, p, q128, do128, k64, v64, status);
     if (e == cudaSuccess && p.dk_from_db) {

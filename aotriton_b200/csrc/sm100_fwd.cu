@@ -174,7 +174,10 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
   } else if (p.varlen_mode != 0) {
     ends = make_int4(p.cu_q[z], p.cu_q[z + 1], p.cu_k[z], p.cu_k[z + 1]);
   }
-  const Seq sq = seq_from_ends(p, z, ends);
+  const Seq sq = seq_for<FEAT>(p, z, ends);
+  if constexpr ((FEAT & kSinks) != 0) {
+    if (p.varlen_mode == 2 && m0 + kCtaRows > sq.sq) write_rows_behind<T>(p, sq, h, m0, kCtaRows);
+  }
   if (m0 >= sq.sq) return;
   const int hk = quick_div(h, p.group);
   const int ntile = (L::kTiles == 2 && m0 + kBM < sq.sq) ? 2 : 1;   // the second tile may lie beyond the sequence
@@ -187,7 +190,9 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
     return;
   }
   const int jb_lo = n_lo / kBN;
-  const int nblk = n_hi / kBN - jb_lo + 1;
+  const int before = blocks_before<FEAT>(p, n_hi, jb_lo, kBN);
+  const int nblk = before + n_hi / kBN - jb_lo + 1;
+  auto block = [&](int j) { return block_at<FEAT>(j, before, jb_lo); };
 
   // ---- set-up -----------------------------------------------------------------------
   if (threadIdx.x == 0) {
@@ -220,7 +225,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
     }
     mbar_expect_tx(&bars[L::bKFull], L::kTileBytes);
     for (int hf = 0; hf < L::kHalves; ++hf)
-      tma_load_4d(smem + L::kK + hf * 16384, &tm_k, &bars[L::bKFull], hf * 64, (int)(sq.k0 + (int64_t)jb_lo * kBN), hk, sq.bidx);
+      tma_load_4d(smem + L::kK + hf * 16384, &tm_k, &bars[L::bKFull], hf * 64, (int)(sq.k0 + (int64_t)block(0) * kBN), hk, sq.bidx);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, kTmemCols);
@@ -250,7 +255,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
         for (int j = 0; j < nblk; ++j) {
           const int s = j % kStages;
           const uint32_t ph = (uint32_t)(j / kStages) & 1u;
-          const int krow = (int)(sq.k0 + (int64_t)(jb_lo + j) * kBN);
+          const int krow = (int)(sq.k0 + (int64_t)block(j) * kBN);
           if (j > 0) {
             if (!mbar_wait(&bars[L::bKEmpty + s], ph ^ 1u, abort_flag, status, 0x100 + j)) break;
             mbar_expect_tx(&bars[L::bKFull + s], L::kTileBytes);
@@ -316,7 +321,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       };
       // index of the sequence's last key block if it is a partial one (the only block whose V tile
       // holds rows beyond the sequence), else -1
-      const int tail_j = (sq.sk % kBN != 0) ? (sq.sk - 1) / kBN - jb_lo : -1;
+      const int tail_j = (sq.sk % kBN != 0) ? (sq.sk - 1) / kBN - jb_lo + before : -1;
       bool ok = true;
       for (int t = 0; ok && t < ntile; ++t) ok = wait(L::bQFull + t, 0, 0x300 + t);
       if (ok) ok = wait(L::bKFull + 0, 0, 0x400);
@@ -331,7 +336,14 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
         // Last, partial block of the sequence: the rows of V beyond its end must not reach P V.
         if constexpr (!EXACT) {
           if (j == tail_j)
-            zero_tail_rows(smem + L::kV + s * L::kTileBytes, sq.sk - (jb_lo + j) * kBN, L::kHalves, lane);
+            zero_tail_rows(smem + L::kV + s * L::kTileBytes, sq.sk - block(j) * kBN, L::kHalves, lane);
+        }
+        if constexpr ((FEAT & kSinks) != 0) {
+          int from, to;
+          hidden_keys(p, sq, from, to);
+          from = max(from - block(j) * kBN, 0);
+          to = min(to - block(j) * kBN, kBN);
+          if (from < to) zero_rows_between(smem + L::kV + s * L::kTileBytes, from, to, L::kHalves, 16384, lane);
         }
         if (j + 1 < nblk) {
           if (!wait(L::bKFull + ((j + 1) % kStages), (uint32_t)((j + 1) / kStages) & 1u, 0x400 + j + 1)) break;
@@ -434,7 +446,13 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     for (int j = 0; j < nblk; ++j) {
-      const int n0 = (jb_lo + j) * kBN;
+      const int n0 = block(j) * kBN;
+      auto mask = [&](float* x) {
+        if constexpr ((FEAT & kSinks) != 0) {
+          if (n0 < p.sinks) { mask_sink_columns<128>(x, n0, row_lo, row_hi, p.sinks, -INFINITY); return; }
+        }
+        mask_columns<128, kOneBound>(x, n0, row_lo, row_hi, n0 >= warp_lo, -INFINITY);
+      };
       const uint32_t par = (uint32_t)j & 1u;
       // The warp's four 32 x 32 tiles of bias: two on their way while the tensor pipe computes S, the others as these are used.
       // (All four are 64 registers beside 128 scores: 264 bytes spilled, head dim 72 877 -> 1231 us with the exchange.)
@@ -479,7 +497,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       bool simple = !bias_on && p.qk_scale > 0.f;
       float mx;
       if (simple) {
-        if (any_mask) mask_columns<128, kOneBound>(sc, n0, row_lo, row_hi, n0 >= warp_lo, -INFINITY);
+        if (any_mask) mask(sc);
         float m8[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) m8[c] = fmaxf(sc[2 * c], sc[2 * c + 1]);
@@ -495,7 +513,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
 #pragma unroll
           for (int c = 0; c < 128; ++c) sc[c] *= p.qk_scale;
         }
-        if (any_mask) mask_columns<128, kOneBound>(sc, n0, row_lo, row_hi, n0 >= warp_lo, -INFINITY);
+        if (any_mask) mask(sc);
         float m8[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) m8[c] = fmaxf(sc[2 * c], sc[2 * c + 1]);
@@ -747,6 +765,7 @@ cudaError_t launch_fwd_T(const Params& p, cudaStream_t st) {
     case kPlain: return exact ? launch_fwd_TE<T, HD, true, kPlain>(p, st) : launch_fwd_TE<T, HD, false, kPlain>(p, st);
     case kBias: return exact ? launch_fwd_TE<T, HD, true, kBias>(p, st) : launch_fwd_TE<T, HD, false, kBias>(p, st);
     case kDropout: return exact ? launch_fwd_TE<T, HD, true, kDropout>(p, st) : launch_fwd_TE<T, HD, false, kDropout>(p, st);
+    case kSinks: return exact ? launch_fwd_TE<T, HD, true, kSinks>(p, st) : launch_fwd_TE<T, HD, false, kSinks>(p, st);
     default: return exact ? launch_fwd_TE<T, HD, true, kAll>(p, st) : launch_fwd_TE<T, HD, false, kAll>(p, st);
   }
 }

@@ -92,7 +92,7 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t saddr, uint32_t rank
 }
 
 // grid = (CS, Hk * row chunks, batch); cluster = the CS CTAs of one x row
-template <typename T, int HD, int MT, int CS, int W>
+template <typename T, int HD, int MT, int CS, int W, int FEAT>
 __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(DecSmem<HD, MT, W>::kThreads, DecSmem<HD, MT, W>::kCtasPerSm)
 sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, unsigned int* status, int stages) {
@@ -109,7 +109,11 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
   const uint32_t rank = CS > 1 ? cluster_rank() : 0u;
   // Everything up to the stream depends on the sequence, the head and the chunk only: a cluster leaves
   // here as a whole or not at all.
-  const Seq sq = resolve_seq(p, z);
+  const Seq sq = resolve_seq_for<FEAT>(p, z);
+  if constexpr ((FEAT & kSinks) != 0) {
+    if (p.varlen_mode == 2 && sq.sq < p.max_sq && chunk == 0 && rank == 0)
+      for (int g = 0; g < p.group; ++g) write_rows_behind<T>(p, sq, hk * p.group + g, 0, p.max_sq);
+  }
   const int rows_total = p.group * sq.sq, row0 = chunk * L::kRows;
   if (row0 >= rows_total) return;
   const int nrows = min(L::kRows, rows_total - row0);
@@ -119,7 +123,8 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
   int n_lo, n_hi;
   key_range(p, sq, m_lo, m_hi, n_lo, n_hi);
   const int t_lo = n_lo / kDecKeys;
-  const int ntiles = n_hi < n_lo ? 0 : n_hi / kDecKeys - t_lo + 1;
+  const int before = n_hi < n_lo ? 0 : blocks_before<FEAT>(p, n_hi, t_lo, kDecKeys);
+  const int ntiles = n_hi < n_lo ? 0 : before + n_hi / kDecKeys - t_lo + 1;
   // this CTA's share of the tiles
   const int first = (int)((int64_t)ntiles * rank / CS), last = (int)((int64_t)ntiles * (rank + 1) / CS);
 
@@ -143,7 +148,7 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
     if (lane == 0) {
       int issued = 0;
       for (int i = 0, s = 0, ph = 1; i < n; ++i) {      // s, ph: ring stage and the parity that frees it
-        const int krow = (int)(sq.k0 + (int64_t)(t_lo + first + i) * kDecKeys);
+        const int krow = (int)(sq.k0 + (int64_t)block_at<FEAT>(first + i, before, t_lo) * kDecKeys);
         if (!mbar_wait(&bars[L::bEmpty + s], (uint32_t)ph, abort_flag, status, 0x5000)) break;
         if (!(p.drop_copy == 1 && i == 0 && rank == 0)) {      // (test hook: the cluster's first tile never arrives)
           uint8_t* kt = smem + L::kRing + s * (2 * L::kTile);
@@ -202,7 +207,7 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
           if (l64 > lo) lo = (int)(l64 > 0x7fffffffLL ? 0x7fffffffLL : l64);
           if (h64 < hi) hi = (int)(h64 < -1 ? -1 : h64);
         }
-        if (!in) { lo = 1; hi = 0; }
+        if (!in) { lo = 1; hi = (FEAT & kSinks) ? -1 : 0; }      // (first keys are bounded by hi alone)
         row_lo[2 * t + half] = lo;
         row_hi[2 * t + half] = hi;
       }
@@ -214,7 +219,7 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
     const int vrow = (warp & 3) * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), vchunk = lane >> 4;
     for (int i = warp >> 2, s = warp >> 2, ph = 0; i < n; i += W / 4) {
       if (!__all_sync(0xffffffffu, mbar_wait(&bars[L::bFull + s], (uint32_t)ph, abort_flag, status, 0x5100))) break;
-      const int key0 = (t_lo + first + i) * kDecKeys + (warp & 3) * 16;      // first key of this warp's 16
+      const int key0 = block_at<FEAT>(first + i, before, t_lo) * kDecKeys + (warp & 3) * 16;      // first key of this warp's 16
       const uint32_t kt = smem_s + L::kRing + s * (2 * L::kTile) + krow * 128;
       const uint32_t vt = smem_s + L::kRing + s * (2 * L::kTile) + L::kTile + vrow * 128;
       if (key0 + 16 > sq.sk) {
@@ -225,6 +230,17 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
           for (int c = lane; c < kBoxes * 8; c += 32)
             *reinterpret_cast<uint4*>(vtile + (c >> 3) * (kDecKeys * 128) + ((warp & 3) * 16 + rr) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
         __syncwarp();
+      }
+      if constexpr ((FEAT & kSinks) != 0) {
+        int from, to;
+        hidden_keys(p, sq, from, to);
+        if (from < key0 + 16 && to > key0) {      // keys that nobody sees: whatever the cache has there
+          uint8_t* vtile = smem + L::kRing + s * (2 * L::kTile) + L::kTile;
+          for (int rr = max(0, from - key0); rr < min(16, to - key0); ++rr)
+            for (int c = lane; c < kBoxes * 8; c += 32)
+              *reinterpret_cast<uint4*>(vtile + (c >> 3) * (kDecKeys * 128) + ((warp & 3) * 16 + rr) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+        }
       }
       // (two accumulators per 8 keys with one tile of rows: half the chain of dependent MMAs)
       constexpr int kChains = MT == 1 ? 2 : 1;
@@ -260,7 +276,7 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int nn = key0 + j * 8 + qc + (e & 1), half = e >> 1;
-            const bool ok = nn >= row_lo[2 * t + half] && nn <= row_hi[2 * t + half];
+            const bool ok = (nn >= row_lo[2 * t + half] || ((FEAT & kSinks) != 0 && nn < p.sinks)) && nn <= row_hi[2 * t + half];
             sc[t][j][e] = ok ? sc[t][j][e] * p.qk_scale : -INFINITY;
             mx[half] = fmaxf(mx[half], sc[t][j][e]);
           }
@@ -392,20 +408,27 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
   if constexpr (CS > 1) cluster_sync();      // no CTA leaves while a peer may still read its partial
 }
 
-template <typename T, int HD, int MT, int CS, int W>
-cudaError_t launch_decode_CS(const Params& p, int chunks, const CUtensorMap& tk, const CUtensorMap& tv, unsigned int* status,
+template <typename T, int HD, int MT, int CS, int W, int FEAT>
+cudaError_t launch_decode_F(const Params& p, int chunks, const CUtensorMap& tk, const CUtensorMap& tv, unsigned int* status,
                              int dev, bool remember, int stages, cudaStream_t st) {
   using L = DecSmem<HD, MT, W>;
   static std::atomic<bool> attr_set[64];
   if (!remember || !attr_set[dev].load(std::memory_order_acquire)) {
-    cudaError_t e = host().func_set_smem(reinterpret_cast<const void*>(sm100_fwd_decode_kernel<T, HD, MT, CS, W>), L::dynamic(L::kMaxStages));
+    cudaError_t e = host().func_set_smem(reinterpret_cast<const void*>(sm100_fwd_decode_kernel<T, HD, MT, CS, W, FEAT>), L::dynamic(L::kMaxStages));
     if (e != cudaSuccess) return e;
     if (remember) attr_set[dev].store(true, std::memory_order_release);
   }
-  cudaError_t e = launch_kernel(sm100_fwd_decode_kernel<T, HD, MT, CS, W>, dim3(CS, p.hk * chunks, p.batch), dim3(L::kThreads),
+  cudaError_t e = launch_kernel(sm100_fwd_decode_kernel<T, HD, MT, CS, W, FEAT>, dim3(CS, p.hk * chunks, p.batch), dim3(L::kThreads),
                                 L::dynamic(stages), st, p, tk, tv, status, stages);
   if (e == cudaSuccess) count_launch();
   return e;
+}
+
+template <typename T, int HD, int MT, int CS, int W>
+cudaError_t launch_decode_CS(const Params& p, int chunks, const CUtensorMap& tk, const CUtensorMap& tv, unsigned int* status,
+                             int dev, bool remember, int stages, cudaStream_t st) {
+  return p.sink_on ? launch_decode_F<T, HD, MT, CS, W, kSinks>(p, chunks, tk, tv, status, dev, remember, stages, st)
+                   : launch_decode_F<T, HD, MT, CS, W, kPlain>(p, chunks, tk, tv, status, dev, remember, stages, st);
 }
 
 // How a call is cut: pieces of the keys (CTAs of a cluster), consumer warps of a CTA, ring stages, row chunks.
@@ -414,7 +437,11 @@ SplitPlan split_plan(const Params& p, int sms) {
   using L = DecSmem<HD, MT, 4>;
   const int chunks = (p.group * p.max_sq + L::kRows - 1) / L::kRows;
   const int64_t clusters = (int64_t)p.hk * chunks * p.batch;
-  const int tiles = (p.max_sk + kDecKeys - 1) / kDecKeys;
+  int tiles = (p.max_sk + kDecKeys - 1) / kDecKeys;
+  if (p.sink_on) {      // those the window and the first keys reach
+    const int64_t seen = ((int64_t)p.sink_window + p.max_sq - 2 + kDecKeys) / kDecKeys + 1 + (p.sinks + kDecKeys - 1) / kDecKeys;
+    if (seen < tiles) tiles = (int)seen;
+  }
   // Cut the keys until the CTAs fill the chip once or a piece would fall below two tiles.  (More pieces than
   // that only add CTAs that wait for a slot: 2 x 8192 keys, 64:8 heads, 5 queries: 37 us with 4 pieces, 58 us with 8.)
   // The rule counts SMs; a cluster of eight also needs its SMs in one GPC, so a few counts just below the line leave

@@ -233,6 +233,15 @@ static __device__ __noinline__ void zero_tail_rows(uint8_t* tile, int valid_rows
   __syncwarp();
 }
 
+// Rows [from, to) of a tile of `boxes` boxes of 64 columns, box_bytes apart; not inlined for the same reason.
+static __device__ __noinline__ void zero_rows_between(uint8_t* tile, int from, int to, int boxes, int box_bytes, int lane) {
+  const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+  for (int b = 0; b < boxes; ++b)
+    for (int o = from * 128 + lane * 16; o < to * 128; o += 512) *reinterpret_cast<uint4*>(tile + b * box_bytes + o) = z;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 

@@ -309,6 +309,99 @@ bool ordinary_gradient(const Tensor& g, at::ScalarType type) {
   return !at::GradMode::is_enabled() && plain_modes() && plain(g, c10::cuda::current_device()) && g.scalar_type() == type;
 }
 
+// ---- attention with a sliding window and first keys that stay visible ----
+struct SinkCall {
+  int64_t max_q, max_k, window, sinks, varlen;      // varlen: AB200_VARLEN_*
+  double sm_scale;
+};
+ab200_attn_problem sink_problem(const SinkCall& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k) {
+  ab200_attn_problem p{};
+  p.dtype = code_of(q.scalar_type());
+  p.batch = (int32_t)q.size(0);
+  p.num_head_q = (int32_t)q.size(1);
+  p.num_head_k = (int32_t)k.size(1);
+  p.max_seqlen_q = (int32_t)q.size(2);
+  p.max_seqlen_k = (int32_t)k.size(2);
+  p.head_dim_qk = (int32_t)q.size(3);
+  p.head_dim_vo = (int32_t)v.size(3);
+  p.sm_scale = (float)c.sm_scale;
+  if (c.varlen) {
+    p.batch = (int32_t)cu_q.numel() - 1;
+    p.max_seqlen_q = (int32_t)c.max_q;
+    p.max_seqlen_k = (int32_t)c.max_k;
+    p.varlen_type = (int32_t)c.varlen;
+    p.cu_seqlens_q = cu_q.data_ptr<int32_t>();
+    p.cu_seqlens_k = cu_k.data_ptr<int32_t>();
+  }
+  return p;
+}
+// `lse` is left undefined where nobody will read it.
+void sink_forward(const SinkCall& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k, bool want_lse, Tensor& out,
+                  Tensor& lse) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  if (c.varlen == AB200_VARLEN_COMPACT) out = fresh({1, q.size(2), q.size(1), v.size(3)}, q.scalar_type()).transpose(1, 2);
+  else out = fresh({q.size(0), q.size(1), q.size(2), v.size(3)}, q.scalar_type());
+  if (want_lse) lse = fresh({q.size(0) * q.size(1), q.size(2)}, at::kFloat);
+  ab200_attn_fwd_args a{};
+  a.prob = sink_problem(c, q, k, v, cu_q, cu_k);
+  a.q = c_view(q); a.k = c_view(k); a.v = c_view(v); a.out = c_view(out);
+  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  check((hipError_t)ab200_sink_attn_fwd(&a, (int32_t)c.window, (int32_t)c.sinks, stream_handle()), "sink_attn_fwd");
+}
+struct SinkAttend : torch::autograd::Function<SinkAttend> {
+  using Maybe = std::optional<Tensor>;
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Maybe& seqs_q, const Maybe& seqs_k,
+                               const SinkCall& c, bool return_lse) {
+    const Tensor cu_q = seqs_q.value_or(Tensor()), cu_k = seqs_k.value_or(Tensor());
+    Tensor out, lse;
+    sink_forward(c, q, k, v, cu_q, cu_k, true, out, lse);
+    ctx->save_for_backward({q, k, v, out, lse, cu_q, cu_k});
+    ctx->saved_data["numbers"] = std::vector<int64_t>{c.max_q, c.max_k, c.window, c.sinks, c.varlen};
+    ctx->saved_data["scale"] = c.sm_scale;
+    ctx->mark_non_differentiable({lse});
+    ctx->set_materialize_grads(false);
+    return return_lse ? variable_list{out, lse} : variable_list{out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &cu_q = saved[5], &cu_k = saved[6];
+    const auto n = ctx->saved_data["numbers"].toIntVector();
+    const SinkCall c{n[0], n[1], n[2], n[3], n[4], ctx->saved_data["scale"].toDouble()};
+    variable_list r(7);
+    if (!grads[0].defined()) return r;
+    Tensor dout = grads[0];
+    // (create_graph: the operator, which knows that it has no derivative; the rest as in Attend::backward)
+    if (at::GradMode::is_enabled() || !Attend::as_saved(q, k, v, Tensor(), out, dout, lse, cu_q, cu_k)) {
+      pybind11::gil_scoped_acquire gil;
+      const auto o = call_python("sink_attention", pybind11::make_tuple(wrapped(q), wrapped(k), wrapped(v), wrapped(out), wrapped(dout), wrapped(lse),
+                                                                        wrapped(cu_q), wrapped(cu_k), c.max_q, c.max_k, c.window, c.sinks, c.sm_scale, c.varlen));
+      for (int i = 0; i < 3; ++i) r[i] = THPVariable_Unpack(PyTuple_GET_ITEM(o.ptr(), i));
+      return r;
+    }
+    if (dout.stride(-1) != 1) dout = dout.contiguous();
+    // (a padded batch's rows behind their sequences have gradient zero)
+    auto make = [&](const Tensor& t) { return c.varlen == AB200_VARLEN_PADDED ? at::zeros_like(t) : gradient_of(t); };
+    r[0] = make(q);
+    r[1] = make(k);
+    r[2] = make(v);
+    const Tensor delta = fresh(lse.sizes(), at::kFloat);
+    ab200_attn_bwd_args a{};
+    a.prob = sink_problem(c, q, k, v, cu_q, cu_k);
+    a.q = c_view(q); a.k = c_view(k); a.v = c_view(v); a.out = c_view(out); a.dout = c_view(dout);
+    a.dq = c_view(r[0]); a.dk = c_view(r[1]); a.dv = c_view(r[2]);
+    a.lse = lse.data_ptr<float>();
+    a.delta = delta.data_ptr<float>();
+    const int64_t need = ab200_sink_attn_bwd_workspace(&a, (int32_t)c.window, (int32_t)c.sinks, stream_handle());
+    if (need < 0) check((hipError_t)-need, "sink_attn_bwd");
+    const Tensor workspace = need > 0 ? fresh({need}, at::kFloat) : Tensor();
+    check((hipError_t)ab200_sink_attn_bwd(&a, (int32_t)c.window, (int32_t)c.sinks, need > 0 ? workspace.data_ptr<float>() : nullptr, (uint64_t)need,
+                                          stream_handle()),
+          "sink_attn_bwd");
+    g_last_bwd_family.store(ab200_last_bwd_family(), std::memory_order_relaxed);
+    return r;
+  }
+};
+
 // ---- dropout with the residual's addition ----
 // t as rows of unit stride: (rows, cols, stride between rows); false where its strides give none.
 bool rows_of(const Tensor& t, int64_t* rows, int64_t* cols, int64_t* stride) {
@@ -534,6 +627,54 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// sink_attend(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, window, sinks, sm_scale, return_lse, varlen): out, or (out, lse),
+// or None: not an ordinary call, or one whose arguments the caller is to look at.
+PyObject* sink_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) {
+    PyErr_SetString(PyExc_TypeError, "sink_attend takes 12 arguments");
+    return nullptr;
+  }
+  if (!THPVariable_CheckExact(a[0]) || !THPVariable_Unpack(a[0]).is_cuda() || !plain_modes()) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  SinkCall c{};
+  Tensor q, k, v, cu_q, cu_k;
+  if (!attention_operand(a[0], dev, &q) || !attention_operand(a[1], dev, &k) || !attention_operand(a[2], dev, &v)) Py_RETURN_NONE;
+  if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) Py_RETURN_NONE;
+  if (!small_int(a[11], &c.varlen) || !small_int(a[7], &c.window) || !small_int(a[8], &c.sinks) || !number(a[9], &c.sm_scale)) Py_RETURN_NONE;
+  const bool return_lse = a[10] == Py_True;
+  if (!return_lse && a[10] != Py_False) Py_RETURN_NONE;
+  if (c.window < 1 || c.sinks < 0 || k.size(0) != q.size(0) || v.size(0) != k.size(0) || v.size(1) != k.size(1) || v.size(2) != k.size(2) ||
+      k.size(3) != q.size(3) || q.size(1) % k.size(1) != 0 || q.size(3) > 512 || v.size(3) > 512)
+    Py_RETURN_NONE;
+  if (c.varlen) {
+    for (int i = 0; i < 2; ++i) {
+      Tensor& cu = i ? cu_k : cu_q;
+      if (!plain_tensor(a[3 + i], dev, &cu) || cu.dim() != 1 || cu.numel() < 2 || cu.scalar_type() != at::kInt) Py_RETURN_NONE;
+    }
+    if (cu_q.numel() != cu_k.numel() || !small_int(a[5], &c.max_q) || !small_int(a[6], &c.max_k)) Py_RETURN_NONE;
+    if (c.max_q < 1 || c.max_q > q.size(2) || c.max_k < 1 || c.max_k > k.size(2)) Py_RETURN_NONE;
+    if (c.varlen == AB200_VARLEN_COMPACT ? q.size(0) != 1 : cu_q.numel() != q.size(0) + 1) Py_RETURN_NONE;
+    if (c.varlen == AB200_VARLEN_PADDED) c.max_q = q.size(2);
+  }
+  Tensor out, lse;
+  {
+    pybind11::gil_scoped_release release;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+      auto maybe = [](const Tensor& t) { return t.defined() ? SinkAttend::Maybe(t) : SinkAttend::Maybe(); };
+      variable_list r = SinkAttend::apply(q, k, v, maybe(cu_q), maybe(cu_k), c, return_lse);
+      out = std::move(r[0]);
+      if (return_lse) lse = std::move(r[1]);
+    } else {
+      sink_forward(c, q, k, v, cu_q, cu_k, return_lse, out, lse);
+    }
+  }
+  if (!return_lse) return THPVariable_Wrap(std::move(out));
+  return PyTuple_Pack(2, pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(out))).ptr(),
+                      pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(lse))).ptr());
+  END_HANDLE_TH_ERRORS
+}
+
 // A floating-point tensor this file's operators take, of any shape and strides; or not.
 bool floating_tensor(PyObject* o, int dev, Tensor* out) {
   if (!THPVariable_CheckExact(o)) return false;
@@ -629,6 +770,7 @@ PyObject* set_python_backward(PyObject*, PyObject* fn) {
 }
 
 PyMethodDef kMethods[] = {{"attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&attend)), METH_FASTCALL, nullptr},
+                          {"sink_attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&sink_attend)), METH_FASTCALL, nullptr},
                           {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&dropout)), METH_FASTCALL, nullptr},
                           {"relative_bias", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&relative_bias)), METH_FASTCALL, nullptr},
                           {"set_python_function", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&set_python_function)), METH_FASTCALL, nullptr},

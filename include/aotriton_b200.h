@@ -192,6 +192,21 @@ AB200_API int ab200_debug_simulate_encoded_softmax(const ab200_view4* r, int32_t
 
 /* ---- what stands around attention in a layer; the reference has none of these -------------------------------- */
 
+/* Attention with a sliding window and a few first keys that stay visible.  Query m of a sequence of sq queries and sk keys stands at key
+ * P = m + sk - sq and sees the keys n <= P with n > P - window or n < sinks; window >= 1, sinks >= 0, max_seqlen_q and _k >= 1.  Arguments, layouts and
+ * types as in ab200_attn_fwd / ab200_attn_bwd, without bias, dropout and encoded_softmax; the problem's causal and window fields are not
+ * looked at.  Differences: rows of a padded batch behind a sequence's last query get O = 0 and LSE = +inf in the forward; keys that no query of
+ * the sequence sees (between the first ones and the first query's window) may hold anything, NaN included, without touching the outputs
+ * and dq of fp16 and bf16 tensors with head dims up to 256 that are multiples of 8. */
+AB200_API int ab200_sink_attn_fwd(const ab200_attn_fwd_args* args, int32_t window, int32_t sinks, void* stream);
+/* The fused form (dq_acc) does not apply.  Gradients are sums in a fixed order: the same inputs give the same bits.  `workspace`:
+ * ab200_sink_attn_bwd_workspace() floats, 16-byte aligned, for the partial gradients of the first keys and the kernels' work counter; contents do not
+ * matter, and calls that may overlap (two captured graphs, two streams) need one each. */
+AB200_API int ab200_sink_attn_bwd(const ab200_attn_bwd_args* args, int32_t window, int32_t sinks, float* workspace,
+                                  uint64_t workspace_floats, void* stream);
+/* Floats of workspace that call needs (0: none), or the negated error code.  Launches nothing. */
+AB200_API int64_t ab200_sink_attn_bwd_workspace(const ab200_attn_bwd_args* args, int32_t window, int32_t sinks, void* stream);
+
 /* Learned relative position bias by buckets: the additive bias of ab200_attn_fwd from a table,
  *   bias[b, h, m, n] = table[bucket(n - m - query_offset), h],
  * and the gradient of the table from that of the bias.  A distance d = n - m - query_offset has, per direction, the bucket

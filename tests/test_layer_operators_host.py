@@ -158,3 +158,96 @@ def test_dropout_entry_on_a_pretended_device(fake):
                       (dict(out=None), 1), (dict(dtype=0), 801), (dict(rows=1 << 40, cols=1 << 40), 1), (dict(rows=1 << 30, cols=1 << 20), 801)):
         assert f(_dropout_args(**bad), None) == code, bad
     assert f(None, None) == 1 and count() == 4
+
+
+def _attn_view(ptr, shape):
+    v = cabi.View4()
+    v.ptr = ptr
+    for i, s in enumerate((shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1)):
+        v.size[i], v.stride[i] = shape[i], s
+    return v
+
+
+def _sink_args(cls, dtype=cabi.DTYPE_BF16, B=2, Hq=4, Hk=2, S=1024, D=128):
+    a = cls()
+    p = a.prob
+    p.dtype, p.batch, p.num_head_q, p.num_head_k, p.max_seqlen_q, p.max_seqlen_k, p.head_dim_qk, p.head_dim_vo = dtype, B, Hq, Hk, S, S, D, D
+    p.sm_scale = 1.0
+    a.q, a.k, a.v, a.out = (_attn_view(0x10000000 * (i + 1), (B, h, S, D)) for i, h in enumerate((Hq, Hk, Hk, Hq)))
+    a.lse = 0x50000000
+    if cls is cabi.BwdArgs:
+        a.dout, a.dq, a.dk, a.dv = (_attn_view(0x60000000 + 0x10000000 * i, (B, h, S, D)) for i, h in enumerate((Hq, Hq, Hk, Hk)))
+        a.delta = 0xa0000000
+    return a
+
+
+def test_sink_entries_on_a_pretended_device(fake):
+    fwd, bwd, size = fake.ab200_sink_attn_fwd, fake.ab200_sink_attn_bwd, fake.ab200_sink_attn_bwd_workspace
+    count = lambda: fake.ab200_debug_host_call_count(7)
+    a, b = _sink_args(cabi.FwdArgs), _sink_args(cabi.BwdArgs)
+    assert fwd(a, 100, 4, None) == 0 and count() == 1 and fake.ab200_last_fwd_family() == 2
+    need = size(b, 100, 4, None)
+    assert need > 4 and size(b, 100, 0, None) == 4 and size(b, 1024, 4, None) == 4 and size(b, 2 ** 31 - 1, 2 ** 31 - 1, None) == 4
+    for ptr, n in ((None, need), (0x5000, need - 1), (0x5004, need)):
+        assert bwd(b, 100, 4, ptr, n, None) == 1 and count() == 1
+    assert bwd(b, 100, 4, 0x5000, need, None) == 0 and count() == 5      # delta, dK/dV, the first keys' sums, dQ
+    assert bwd(b, 100, 0, 0x5000, 4, None) == 0 and count() == 8
+    assert fake.ab200_debug_host_call_count(6) == 0      # (the work counter is zeroed by the first launch)
+    for window, sinks in ((0, 4), (-1, 4), (5, -1)):
+        assert fwd(a, window, sinks, None) == 1 and bwd(b, window, sinks, 0x5000, need, None) == 1 and size(b, window, sinks, None) == -1
+    for S in (0,):
+        assert fwd(_sink_args(cabi.FwdArgs, S=S), 5, 1, None) == 1 and size(_sink_args(cabi.BwdArgs, S=S), 5, 1, None) == -1
+    a.prob.dropout_p = b.prob.dropout_p = 0.1
+    assert fwd(a, 5, 1, None) == 801 and size(b, 5, 1, None) == -801
+    a.prob.dropout_p = b.prob.dropout_p = 0.0
+    a.bias.ptr = 0x1000
+    assert fwd(a, 5, 1, None) == 801
+    # wide heads and single precision need no workspace
+    for kw in (dict(D=256), dict(dtype=cabi.DTYPE_FP32)):
+        b = _sink_args(cabi.BwdArgs, **kw)
+        assert size(b, 100, 4, None) == 0 and bwd(b, 100, 4, None, 0, None) == 0
+    fake.ab200_debug_host_calls(1, 7, 98, 2)      # the third launch fails: nothing after it
+    b = _sink_args(cabi.BwdArgs)
+    assert bwd(b, 100, 4, 0x5000, need, None) == 98 and count() == 3
+
+
+@pytest.mark.parametrize("change", [
+    dict(window=0), dict(window=-3), dict(window=2.0), dict(window=True), dict(sinks=-1), dict(sinks=None), dict(heads=3), dict(kd=32), dict(vs=9), dict(kb=2),
+    dict(d=513), dict(dtype=torch.float64), dict(vdtype=torch.bfloat16), dict(cpu=True),
+])
+def test_sink_refusals(change):
+    class T:
+        def __init__(self, shape, dtype):
+            self.shape, self.dtype, self.is_cuda, self.device = torch.Size(shape), dtype, not change.get("cpu"), "cuda:0"
+
+        def dim(self):
+            return 4
+
+        def stride(self, i):
+            return 1
+
+    dt, d = change.get("dtype", torch.float16), change.get("d", 64)
+    q = T((1, 4, 8, d), dt)
+    k = T((change.get("kb", 1), change.get("heads", 2), 8, change.get("kd", d)), dt)
+    v = T((1, change.get("heads", 2), change.get("vs", 8), d), change.get("vdtype", dt))
+    with pytest.raises(ValueError):
+        autograd.sink_attention(q, k, v, change.get("window", 4), change.get("sinks", 1), sm_scale=1.0)
+
+
+def test_varlen_sink_refusals():
+    class T:
+        def __init__(self, shape, dtype=torch.float16):
+            self.shape, self.dtype, self.is_cuda, self.device = torch.Size(shape), dtype, True, torch.device("cpu")
+
+        def dim(self):
+            return 4
+
+        def stride(self, i):
+            return 1
+
+    q, ends = T((2, 4, 8, 64)), torch.tensor([0, 8, 16], dtype=torch.int32)
+    call = lambda q=q, a=ends, b=ends, mq=8, mk=8, how="padded": autograd.varlen_sink_attention(q, q, q, a, b, mq, mk, 4, 1, varlen_type=how)
+    for bad in (dict(how="strided"), dict(how="compact"), dict(a=ends[:2]), dict(b=ends[:2]), dict(a=ends[:1], b=ends[:1]), dict(a=ends.long()), dict(mq=9), dict(mk=9),
+                dict(mq=-1), dict(a=ends.view(1, 3)), dict(a=torch.zeros(6, dtype=torch.int32)[::2])):
+        with pytest.raises(ValueError):
+            call(**bad)
