@@ -915,9 +915,12 @@ static int fill_relative_bias(const ab200_relative_bias_args* a, RelativeBias& r
     if (r.borders[k] < (k > 0 ? r.borders[k - 1] : 1)) return kErrInvalidValue;
   }
   const int per_vec = a->dtype == AB200_DTYPE_FP32 ? 4 : 8;
-  r.vec = (reinterpret_cast<uintptr_t>(a->bias.ptr) & 15u) == 0 && a->bias.stride[3] == 1;
+  r.unit = a->bias.stride[3] == 1;
+  r.vec = r.unit && (reinterpret_cast<uintptr_t>(a->bias.ptr) & 15u) == 0;
   for (int i = 0; i < 3; ++i)
     if (n[i] > 1 && a->bias.stride[i] % per_vec != 0) r.vec = 0;
+  // (a row is read in elements of its type: addresses are multiples of their size)
+  if (reinterpret_cast<uintptr_t>(a->bias.ptr) % (a->dtype == AB200_DTYPE_FP32 ? 4 : 2) != 0) return kErrInvalidValue;
   return 0;
 }
 

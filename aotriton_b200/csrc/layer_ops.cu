@@ -3,16 +3,20 @@
 //
 // Relative bias.  bias[h, m, n] = table[bucket(n - m - offset), h] depends on the diagonal n - m only.  The forward is bound by its
 // stores: a CTA works out the few hundred values its tile's diagonals have, and a thread then takes an N x N piece of the tile from
-// 2N of them, held in registers and shifted by one element a row.  The backward is bound by reading the gradient once: a thread walks
-// down the tile diagonal, so that the 2N - 1 diagonals of its N x N pieces stay the same and one register each sums them; a CTA sums
-// those of its strip by buckets, and a second launch adds the CTAs' sums up in a fixed order (no atomics: the result does not
-// depend on who comes first).
+// 2N of them, held in registers and shifted by one element a row.  16 heads x 2048 x 2048 bf16: 21.5 us, 6.2 TB/s.  The backward is bound by reading
+// the gradient once: a warp walks down the diagonals in steps of eight rows, between which a 16-byte vector moves by whole vectors, so that each of its
+// elements stays on its diagonal and one register a diagonal sums them; a CTA sums those of its band by buckets, and a second launch adds
+// the CTAs' sums up in a fixed order (no atomics: the result does not depend on who comes first).  8 x 16 x 2048 x 2048 bf16, 1.07 GB: 180 us,
+// 6.0 TB/s.  (Pieces of 8 x 8 elements with 15 diagonals' registers took 217, and rows that start anywhere another kernel.)
 //
 // Dropout.  Element i in logical (row-major) order takes word (0, 2, 1, 3)[i % 4] of Philox counter offset + i / 4, as the columns of a
 // score row do (common.cuh): a mask follows from seed, offset and the logical index alone, not from strides, and is never stored; the
 // backward draws it again.  Ten rounds of the generator serve four elements; beside them the kernel moves two to three elements' bytes each.
+#include <algorithm>
+#include <type_traits>
 #include "launch.h"
 #include "layer_ops.h"
+#include "sm100_ptx.cuh"
 
 namespace ab200 {
 namespace {
@@ -103,144 +107,187 @@ __global__ void __launch_bounds__(kThreads) relative_bias_kernel(const __grid_co
 }
 
 // ---- relative bias, gradient of the table -----------------------------------------------------------------------
-// A strip: the diagonals n - m of 32 N columns' worth, seen from rows that are multiples of N.  Strip s of width W = 32 N starts at
-// column W s - (rows rounded up to N) of row 0; its CTA's pieces touch the N - 1 diagonals before it as well.
-template <typename T> struct Strip {
-  static constexpr int N = Vec<T>::N, W = 32 * N, kWarps = kThreads / 32;
-  static constexpr int kDiags = W + N - 1;      // diagonal i of a strip: n - m = first + i - (N - 1)
+// A band: kBand diagonals, first .. first + kBand - 1, of one head, in STRIPS strips of 31 N side by side.  A CTA takes the rows that pass
+// through it and have kResidues residues modulo 8 (kParts CTAs all of them), and of those chunk_rows' worth, counted through the batch (each of
+// its elements has the band's rows, padded to whole steps).
+template <typename T, int STRIPS> struct Band {
+  static constexpr int N = Vec<T>::N, kStrips = STRIPS, kStrip = 31 * N, kBand = STRIPS * kStrip;
+  static constexpr int kResidues = 8 / STRIPS, kParts = STRIPS, kStep = 64;      // rows of a step: eight of each residue
+  int64_t first;
+  int row_lo, rows;      // the rows some diagonal of the band passes through; `rows` in whole steps
+  __host__ __device__ Band(int sq, int sk, int band) {
+    first = (int64_t)band * kBand - (sq - 1);
+    const int64_t lo = -(first + kBand - 1), hi = (int64_t)sk - 1 - first;
+    row_lo = lo > 0 ? (int)lo : 0;
+    const int row_hi = hi < sq - 1 ? (int)hi : sq - 1;
+    rows = (row_hi - row_lo + kStep) / kStep * kStep;      // (at least one row: bands end with the last diagonal)
+  }
+  __host__ __device__ static int bands(int sq, int sk) { return (int)(((int64_t)sq + sk - 1 + kBand - 1) / kBand); }
 };
-__host__ __device__ inline int64_t first_diagonal(int strip, int width, int rows) { return (int64_t)strip * width - (rows + 7) / 8 * 8; }
 
-// grid = (strips * chunks, heads, batch_parts); partial[((h * batch_parts + part) * gridDim.x + x) * buckets + bucket]
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) relative_bias_sums_kernel(const __grid_constant__ RelativeBias a) {
+// Two elements of a word as fp32.
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// grid = (bands * chunks * kParts, heads); partial[(h * gridDim.x + x) * buckets + bucket], of chunks that have rows.
+// UNIT: rows of unit stride.  A warp takes every eighth row, all of whose starts are as far from a 16-byte boundary, whatever the rows'
+// stride: its lanes read aligned 16 bytes each, 32 of them from the one with the strip's first column on, and the diagonal of an element stays the
+// same from row to row.  N registers sum them; nothing is shifted, and odd row lengths cost what even ones do.  (The last of the 32 only
+// completes the first's: 31 N diagonals a strip.)  What is read beside the row lies in 16 bytes that hold some of it, and is not added.
+template <typename T, int STRIPS, bool UNIT>
+__global__ void __launch_bounds__(kThreads, 4) relative_bias_sums_kernel(const __grid_constant__ RelativeBias a) {
   wait_for_earlier_grids();
-  using S = Strip<T>;
+  using S = Band<T, STRIPS>;
   constexpr int N = S::N;
   __shared__ int borders[kMaxBorders];
-  __shared__ float sums[S::kWarps][S::kDiags + 1];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y, part = blockIdx.z;
-  const int strip = blockIdx.x / a.chunks, chunk = blockIdx.x - strip * a.chunks;
-  const int64_t first = first_diagonal(strip, S::W, a.sq);
+  __shared__ float sums[S::kResidues][S::kBand];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, h = blockIdx.y;
+  const int part = blockIdx.x % S::kParts, item = blockIdx.x / S::kParts, band = item / a.chunks, chunk = item - band * a.chunks;
+  const S st(a.sq, a.sk, band);
+  const int64_t begin = (int64_t)chunk * a.chunk_rows, end = min(begin + a.chunk_rows, (int64_t)st.rows * a.batch);
+  if (begin >= end) return;
   if (tid < a.per_direction - 1) borders[tid] = a.borders[tid];
-  // rows some diagonal of the strip passes through; the chunk's share of them, in whole pieces
-  const int64_t lo64 = -(first + S::W - 1), hi64 = (int64_t)a.sk - 1 - (first - (N - 1));
-  const int row_lo = lo64 > 0 ? (int)(lo64 / N * N) : 0, row_hi = (int)min((int64_t)a.sq - 1, hi64);
-  const int m_begin = row_lo + chunk * a.chunk_rows, m_end = (int)min((int64_t)row_hi + 1, (int64_t)m_begin + a.chunk_rows);
-  const int b0 = (int)((int64_t)a.batch * part / a.batch_parts), b1 = (int)((int64_t)a.batch * (part + 1) / a.batch_parts);
+  int b = (int)(begin / st.rows), row = (int)(begin - (int64_t)b * st.rows);      // the chunk's next step: rows row.. of the band's
   const T* g = reinterpret_cast<const T*>(a.bias.ptr) + (int64_t)h * a.bias.s[1];
-  if constexpr (VEC) {
-    float acc[2 * N - 1];      // acc[N - 1 + c - r]: column c, row r of a piece
-#pragma unroll
-    for (int i = 0; i < 2 * N - 1; ++i) acc[i] = 0.f;
-    for (int b = b0; b < b1; ++b) {
-      for (int m = m_begin + warp * N; m < m_end; m += S::kWarps * N) {
-        const int64_t n = first + m + lane * N;
-        if (n < 0 || n >= a.sk) continue;
-        const T* src = g + (int64_t)b * a.bias.s[0] + (int64_t)m * a.bias.s[2] + n;
-        Vec<T> v[N];
-        if (n + N <= a.sk) {
-#pragma unroll
-          for (int r = 0; r < N; ++r) {
-            if (m + r < m_end) *reinterpret_cast<uint4*>(&v[r]) = __ldcs(reinterpret_cast<const uint4*>(src + (int64_t)r * a.bias.s[2]));
-            else *reinterpret_cast<uint4*>(&v[r]) = make_uint4(0u, 0u, 0u, 0u);
-          }
-        } else {
-#pragma unroll
-          for (int r = 0; r < N; ++r)
-#pragma unroll
-            for (int c = 0; c < N; ++c) v[r].e[c] = m + r < m_end && n + c < a.sk ? src[(int64_t)r * a.bias.s[2] + c] : from_f32<T>(0.f);
-        }
-#pragma unroll
-        for (int r = 0; r < N; ++r)
-#pragma unroll
-          for (int c = 0; c < N; ++c) acc[N - 1 + c - r] += to_f32<T>(v[r].e[c]);
-      }
-    }
-    // lane l's diagonals are strip entries N l .. N l + 2N - 2: neighbours overlap, so the even lanes write and the odd ones add
-    float* mine = sums[warp];
-    if ((lane & 1) == 0) {
-#pragma unroll
-      for (int i = 0; i < 2 * N - 1; ++i) mine[N * lane + i] = acc[i];
-    }
-    __syncwarp();
-    if (lane & 1) {
-      // (between two even lanes' entries lies one that neither wrote)
-      mine[N * lane + N - 1] = acc[N - 1];
-#pragma unroll
-      for (int i = 0; i < 2 * N - 1; ++i)
-        if (i != N - 1 && (lane < 31 || i < N - 1)) mine[N * lane + i] += acc[i];
-      if (lane == 31) {
-#pragma unroll
-        for (int i = N; i < 2 * N - 1; ++i) mine[N * lane + i] = acc[i];
-      }
-    }
-  } else {
-    // a thread a diagonal (the strip's W, in passes of 256): rows whose starts are not 16-byte aligned
-    float* flat = &sums[0][0];
-    static_assert(S::W <= kThreads, "one pass");
-    float acc = 0.f;
-    const int64_t d = first + tid;
-    if (tid < S::W) {
-      const int lo = (int)max((int64_t)m_begin, -d), hi = (int)min((int64_t)m_end, (int64_t)a.sk - d);
-      for (int b = b0; b < b1; ++b) {
-        const T* src = g + (int64_t)b * a.bias.s[0] + (int64_t)lo * a.bias.s[2] + (lo + d) * a.bias.s[3];
-        const int64_t step = a.bias.s[2] + a.bias.s[3];
-        float part_sum[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) part_sum[i] = 0.f;
-        int m = lo;
-        for (; m + 8 <= hi; m += 8, src += 8 * step) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) part_sum[i] += to_f32<T>(__ldcs(src + i * step));
-        }
-        for (; m < hi; ++m, src += step) part_sum[0] += to_f32<T>(*src);
-        acc += ((part_sum[0] + part_sum[1]) + (part_sum[2] + part_sum[3])) + ((part_sum[4] + part_sum[5]) + (part_sum[6] + part_sum[7]));
-      }
-    }
-    for (int i = tid; i < S::kDiags; i += kThreads) flat[i] = 0.f;
-    __syncthreads();
-    if (tid < S::W) flat[N - 1 + tid] = acc;
-  }
+  for (int i = tid; i < S::kResidues * S::kBand; i += kThreads) (&sums[0][0])[i] = 0.f;
   __syncthreads();
-  if constexpr (VEC) {
-    for (int i = tid; i < S::kDiags; i += kThreads) {
+  if constexpr (UNIT) {
+    const int strip = warp % STRIPS, residue = S::kResidues * part + warp / STRIPS;
+    float* mine = sums[warp / STRIPS] + strip * S::kStrip;
+    float2 acc[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+    int shift = -1;      // of the rows summed so far: element e of lane l is the strip's diagonal N l + e - shift
+    auto flush = [&] {
+      if (shift < 0) return;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int i = N * lane + e - shift;
+        if (i >= 0 && i < S::kStrip) mine[i] += (e & 1) ? acc[e / 2].y : acc[e / 2].x;
+      }
+    };
+    const int64_t eight = 8 * (a.bias.s[2] + 1);
+    for (int64_t at = begin; at < end; at += S::kStep) {
+      const int m0 = st.row_lo + row + residue;
+      const int n0 = (int)(st.first + m0) + strip * S::kStrip;                        // the strip's first column in row m0
+      const T* p0 = g + (int64_t)b * a.bias.s[0] + (int64_t)m0 * a.bias.s[2];
+      if ((row += S::kStep) == st.rows) { row = 0; ++b; }
+      if (m0 >= a.sq || n0 - N >= a.sk || n0 + 56 + 32 * N <= 0) continue;      // (nothing of the row in the strip)
+      const uintptr_t from = reinterpret_cast<uintptr_t>(p0 + n0);
+      const int sh = (int)(from & 15) / (int)sizeof(T);
+      if (sh != shift) {      // (another element of the batch, a whole one of which is not a multiple of 16 bytes)
+        flush();
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) acc[i] = make_float2(0.f, 0.f);
+        shift = sh;
+      }
+      const int n = n0 - sh + N * lane;      // this lane's first column in row m0; one to the right in each further row
+      const T* src = reinterpret_cast<const T*>(from & ~uintptr_t(15)) + N * lane;
+      // adds a vector's elements; with `some`, those of them whose bits are set in `mask`
+      auto add = [&](const uint4& v, auto some, uint32_t mask) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+          float2 x;
+          if constexpr (sizeof(T) == 2) x = unpack2<T>(w[i]);
+          else x = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+          if constexpr (some.value) {
+            if (!(mask & (1u << (2 * i)))) x.x = 0.f;
+            if (!(mask & (2u << (2 * i)))) x.y = 0.f;
+          }
+          acc[i].x += x.x;
+          acc[i].y += x.y;
+        }
+      };
+      uint4 v[8];
+      // (all of it inside: no element lies beside its row, no row behind the last)
+      if (n0 - sh >= 0 && n0 - sh + 56 + 32 * N <= a.sk && m0 + 56 < a.sq) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = __ldg(reinterpret_cast<const uint4*>(src + r * eight));
+#pragma unroll
+        for (int r = 0; r < 8; ++r) add(v[r], std::false_type{}, 0u);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const bool in = m0 + 8 * r < a.sq && n + 8 * r + N > 0 && n + 8 * r < a.sk;
+          v[r] = in ? __ldg(reinterpret_cast<const uint4*>(src + r * eight)) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int before = -(n + 8 * r), behind = n + 8 * r + N - a.sk;      // elements of the vector on either side of the row, if above 0
+          const uint32_t mask = (0xffu << min(max(before, 0), N)) & (0xffu >> (8 - N + min(max(behind, 0), N)));
+          if (__any_sync(0xffffffffu, (before > 0 && before < N) || (behind > 0 && behind < N))) add(v[r], std::true_type{}, mask);
+          else add(v[r], std::false_type{}, 0u);      // (whole vectors beside the row are zero)
+        }
+      }
+    }
+    flush();
+    __syncthreads();
+    for (int i = tid; i < S::kBand; i += kThreads) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < S::kWarps; ++w) s += sums[w][i];
+      for (int r = 0; r < S::kResidues; ++r) s += sums[r][i];
       sums[0][i] = s;
     }
-    __syncthreads();
+  } else {
+    // a thread a diagonal, in turns: elements that are not next to each other
+    for (int64_t at = begin; at < end; at += S::kStep) {
+      for (int i = tid; i < S::kBand; i += kThreads) {
+        const int64_t d = st.first + i;
+        float s = 0.f;
+        const T* src = g + (int64_t)b * a.bias.s[0];
+#pragma unroll 4
+        for (int r = 0; r < 8 * S::kResidues; ++r) {
+          const int m = st.row_lo + row + 8 * (r / S::kResidues) + S::kResidues * part + r % S::kResidues;
+          const int64_t n = m + d;
+          if (m < a.sq && n >= 0 && n < a.sk) s += to_f32<T>(src[(int64_t)m * a.bias.s[2] + n * a.bias.s[3]]);
+        }
+        sums[0][i] += s;
+      }
+      if ((row += S::kStep) == st.rows) { row = 0; ++b; }
+    }
   }
-  // bucket by bucket: those between the strip's ends (buckets of a direction are intervals of distances)
+  __syncthreads();
+  // bucket by bucket (buckets of a direction are intervals of distances)
   const int buckets = a.per_direction * (a.both ? 2 : 1);
-  float* to = a.partial + (((int64_t)h * a.batch_parts + part) * gridDim.x + blockIdx.x) * buckets;
-  const int64_t d0 = first - (N - 1) - a.offset;      // distance of entry 0
-  for (int k = warp; k < buckets; k += S::kWarps) {
+  float* to = a.partial + ((int64_t)h * gridDim.x + blockIdx.x) * buckets;
+  const int64_t d0 = st.first - a.offset;      // distance of entry 0
+  for (int k = warp; k < buckets; k += kThreads / 32) {
     const int j = k < a.per_direction ? k : k - a.per_direction;
     const int64_t r_lo = j > 0 ? borders[j - 1] : 0, r_hi = j + 1 < a.per_direction ? (int64_t)borders[j] - 1 : INT64_MAX / 2;
     // distances [x, y] of the bucket
     int64_t x, y;
     if (k >= a.per_direction) { x = max(r_lo, (int64_t)1); y = r_hi; }
     else { x = -r_hi; y = j == 0 && !a.both ? INT64_MAX / 2 : -r_lo; }
-    const int i_lo = (int)max((int64_t)0, min(x - d0, (int64_t)S::kDiags)), i_hi = (int)min((int64_t)S::kDiags - 1, max(y - d0, (int64_t)-1));
+    const int i_lo = (int)max((int64_t)0, min(x - d0, (int64_t)S::kBand)), i_hi = (int)min((int64_t)S::kBand - 1, max(y - d0, (int64_t)-1));
     float s = 0.f;
-    for (int i = i_lo + lane; i <= i_hi; i += 32) s += sums[0][i];
+    if (i_lo <= i_hi) {
+      for (int i = i_lo + lane; i <= i_hi; i += 32) s += sums[0][i];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
     if (lane == 0) to[k] = s;
   }
 }
 
-// grid = (buckets, heads): the CTAs' sums, in their order
-template <typename TT>
-__global__ void __launch_bounds__(128) relative_bias_table_kernel(const __grid_constant__ RelativeBias a, int count) {
+// grid = (buckets, heads): the CTAs' sums, in their order.  T: the gradient's type, which the bands' width goes by
+template <typename T, int STRIPS, typename TT>
+__global__ void __launch_bounds__(128) relative_bias_table_kernel(const __grid_constant__ RelativeBias a) {
   wait_for_earlier_grids();
   __shared__ float sums[4];
-  const int k = blockIdx.x, h = blockIdx.y, buckets = gridDim.x;
-  const float* from = a.partial + (int64_t)h * count * buckets + k;
+  const int k = blockIdx.x, h = blockIdx.y, buckets = gridDim.x, items = a.bands * a.chunks;
+  const float* from = a.partial + (int64_t)h * items * Band<T, STRIPS>::kParts * buckets + k;
   float s = 0.f;
-  for (int i = threadIdx.x; i < count; i += 128) s += from[(int64_t)i * buckets];
+  for (int i = threadIdx.x; i < items; i += 128) {
+    const int band = i / a.chunks;
+    if ((int64_t)(i - band * a.chunks) * a.chunk_rows >= (int64_t)Band<T, STRIPS>(a.sq, a.sk, band).rows * a.batch) continue;
+#pragma unroll
+    for (int p = 0; p < Band<T, STRIPS>::kParts; ++p) s += from[((int64_t)i * Band<T, STRIPS>::kParts + p) * buckets];
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
@@ -251,94 +298,159 @@ __global__ void __launch_bounds__(128) relative_bias_table_kernel(const __grid_c
 }
 
 // ---- dropout ------------------------------------------------------------------------------------------------------
+// (selected, not multiplied by zero: what is dropped may be infinite, and so may be the scale)
 template <typename T>
-__device__ __forceinline__ T dropped(T x, bool keep, float scale, float residual) {
-  // (selected, not multiplied by zero: what is dropped may be infinite, and so may be the scale)
-  return from_f32<T>((keep ? to_f32<T>(x) * scale : 0.f) + residual);
+__device__ __forceinline__ float kept(T x, bool keep, float scale) { return keep ? to_f32<T>(x) * scale : 0.f; }
+
+// N counters of one seed side by side: c[n][0..1] in, the four words out.  The key of a call that passes its seed by value is the same
+// for the whole grid, and so are its twenty round keys: left in uniform registers they cost the threads nothing.
+template <int N>
+__device__ __forceinline__ void philox_words(uint32_t k0, uint32_t k1, uint32_t (&c)[N][4]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) c[n][2] = c[n][3] = 0u;
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const uint64_t pa = (uint64_t)0xD2511F53u * c[n][0], pb = (uint64_t)0xCD9E8D57u * c[n][2];
+      const uint32_t n0 = (uint32_t)(pb >> 32) ^ c[n][1] ^ k0, n2 = (uint32_t)(pa >> 32) ^ c[n][3] ^ k1;
+      c[n][1] = (uint32_t)pb; c[n][3] = (uint32_t)pa; c[n][0] = n0; c[n][2] = n2;
+    }
+    k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
+  }
 }
 
-// FLAT: everything is contiguous, one row.  Otherwise rows of cols elements, a multiple of N, with strides of their own.
-template <typename T, bool FLAT, bool RESIDUAL>
+// FLAT: everything is contiguous, one row.  Otherwise rows of cols elements, a multiple of N, with strides of their own.  POINTERS: seed and
+// offset are read from the device as well.
+template <typename T, bool FLAT, bool RESIDUAL, bool POINTERS>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant__ Dropout a, uint64_t vectors) {
   wait_for_earlier_grids();
-  constexpr int N = Vec<T>::N, U = 16 / N;      // sixteen elements a thread: four counters in lockstep
-  const uint64_t seed = a.seed + (a.seed_ptr ? *a.seed_ptr : 0ull), offset = a.offset + (a.offset_ptr ? *a.offset_ptr : 0ull);
+  constexpr int N = Vec<T>::N, U = 16 / N;      // sixteen elements a thread: four counters side by side
+  uint64_t seed = a.seed, offset = a.offset;
+  if constexpr (POINTERS) {
+    if (a.seed_ptr) seed += *a.seed_ptr;
+    if (a.offset_ptr) offset += *a.offset_ptr;
+  }
   const bool keep_all = !a.on;
-  const uint64_t v0 = (uint64_t)blockIdx.x * (kThreads * U) + threadIdx.x;
   const T* x = reinterpret_cast<const T*>(a.x);
   const T* res = reinterpret_cast<const T*>(a.residual);
   T* out = reinterpret_cast<T*>(a.out);
-  Vec<T> in[U], r[U];
-  int64_t row[U], col[U];
+  const uint64_t v0 = (uint64_t)blockIdx.x * (kThreads * U) + threadIdx.x;
+  auto body = [&](auto whole) {      // (no bounds but in the last CTA)
+    Vec<T> in[U], r[U];
+    int64_t row[U], col[U];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t v = v0 + (uint64_t)u * kThreads;
-    if (v >= vectors) continue;
-    if constexpr (FLAT) { row[u] = 0; col[u] = (int64_t)v * N; }
-    else {
-      const uint64_t per = (uint64_t)a.cols / N;
-      row[u] = vectors >> 32 ? (int64_t)(v / per) : (int64_t)((uint32_t)v / (uint32_t)per);
-      col[u] = ((int64_t)v - row[u] * (int64_t)per) * N;
+    for (int u = 0; u < U; ++u) {
+      const uint64_t v = v0 + (uint64_t)u * kThreads;
+      if (!whole.value && v >= vectors) continue;
+      if constexpr (FLAT) { row[u] = 0; col[u] = (int64_t)v * N; }
+      else {
+        const uint64_t per = (uint64_t)a.cols / N;
+        row[u] = vectors >> 32 ? (int64_t)(v / per) : (int64_t)((uint32_t)v / (uint32_t)per);
+        col[u] = ((int64_t)v - row[u] * (int64_t)per) * N;
+      }
+      *reinterpret_cast<uint4*>(&in[u]) = __ldcs(reinterpret_cast<const uint4*>(x + row[u] * a.sx + col[u]));
+      if constexpr (RESIDUAL) *reinterpret_cast<uint4*>(&r[u]) = __ldcs(reinterpret_cast<const uint4*>(res + row[u] * a.sr + col[u]));
     }
-    *reinterpret_cast<uint4*>(&in[u]) = __ldcs(reinterpret_cast<const uint4*>(x + row[u] * a.sx + col[u]));
-    if constexpr (RESIDUAL) *reinterpret_cast<uint4*>(&r[u]) = __ldcs(reinterpret_cast<const uint4*>(res + row[u] * a.sr + col[u]));
-  }
-  uint32_t c[4][4];
+    uint32_t c[4][4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint64_t counter = offset + (v0 + (uint64_t)(k / (N / 4)) * kThreads) * (N / 4) + (k % (N / 4));
-    c[k][0] = (uint32_t)counter;
-    c[k][1] = (uint32_t)(counter >> 32);
-  }
-  philox4x32_10_lockstep<4>(seed, c);
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (v0 + (uint64_t)u * kThreads >= vectors) continue;
-    Vec<T> w;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const uint32_t* words = c[u * (N / 4) + e / 4];
-      const uint32_t word = (e & 3) == 0 ? words[0] : ((e & 3) == 1 ? words[2] : ((e & 3) == 2 ? words[1] : words[3]));
-      w.e[e] = dropped<T>(in[u].e[e], keep_all || (int32_t)word > a.threshold, a.scale, RESIDUAL ? to_f32<T>(r[u].e[e]) : 0.f);
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t counter = offset + (v0 + (uint64_t)(k / (N / 4)) * kThreads) * (N / 4) + (k % (N / 4));
+      c[k][0] = (uint32_t)counter;
+      c[k][1] = (uint32_t)(counter >> 32);
     }
-    *reinterpret_cast<uint4*>(out + row[u] * a.so + col[u]) = *reinterpret_cast<const uint4*>(&w);
-  }
+    philox_words<4>((uint32_t)seed, (uint32_t)(seed >> 32), c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (!whole.value && v0 + (uint64_t)u * kThreads >= vectors) continue;
+      float y[N];
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const uint32_t* words = c[u * (N / 4) + e / 4];
+        const uint32_t word = (e & 3) == 0 ? words[0] : ((e & 3) == 1 ? words[2] : ((e & 3) == 2 ? words[1] : words[3]));
+        y[e] = kept<T>(in[u].e[e], keep_all || (int32_t)word > a.threshold, a.scale);
+        if constexpr (RESIDUAL) y[e] += to_f32<T>(r[u].e[e]);
+      }
+      uint4 w;
+      if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
+      else w = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[N - 4], y[N - 3]), pack2<T>(y[N - 2], y[N - 1]));
+      *reinterpret_cast<uint4*>(out + row[u] * a.so + col[u]) = w;
+    }
+  };
+  if ((uint64_t)(blockIdx.x + 1ull) * (kThreads * U) <= vectors) body(std::true_type{});
+  else body(std::false_type{});
 }
 
-// Any width, stride and alignment, from element `first` (a multiple of four) on: a warp takes 128 elements, one counter a lane, and
+// Any width, stride and alignment, from element `first` (a multiple of four) on: a warp takes 256 elements, two counters a lane, and
 // hands the bits round so that its accesses are to consecutive elements.
+constexpr int kElementsWarp = 256, kElementsCta = kElementsWarp * (kThreads / 32);
 template <typename T>
 __global__ void __launch_bounds__(kThreads) dropout_elements_kernel(const __grid_constant__ Dropout a, uint64_t first) {
   wait_for_earlier_grids();
   const uint64_t seed = a.seed + (a.seed_ptr ? *a.seed_ptr : 0ull), offset = a.offset + (a.offset_ptr ? *a.offset_ptr : 0ull);
   const int lane = threadIdx.x & 31;
-  const uint64_t n = (uint64_t)a.rows * (uint64_t)a.cols, base = first + ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * 128;
+  const uint64_t n = (uint64_t)a.rows * (uint64_t)a.cols, base = first + (uint64_t)blockIdx.x * kElementsCta + (threadIdx.x >> 5) * kElementsWarp;
   if (base >= n) return;
-  const Philox4 w = philox4x32_10(seed, offset + base / 4 + lane);
-  const uint32_t mine = !a.on ? 15u
-                              : ((int32_t)w.w[0] > a.threshold ? 1u : 0u) | ((int32_t)w.w[2] > a.threshold ? 2u : 0u) |
-                                    ((int32_t)w.w[1] > a.threshold ? 4u : 0u) | ((int32_t)w.w[3] > a.threshold ? 8u : 0u);
+  const T* x = reinterpret_cast<const T*>(a.x);
+  const T* res = reinterpret_cast<const T*>(a.residual);
+  T* out = reinterpret_cast<T*>(a.out);
+  constexpr int kPer = kElementsWarp / 32;
+  int64_t row[kPer], col[kPer];
+  T in[kPer], r[kPer];
+  {
+    const uint64_t i = base + lane;
+    row[0] = n >> 32 ? (int64_t)(i / (uint64_t)a.cols) : (int64_t)((uint32_t)i / (uint32_t)a.cols);
+    col[0] = (int64_t)i - row[0] * a.cols;
+  }
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t keep = __shfl_sync(0xffffffffu, mine, 8 * j + (lane >> 2)) >> (lane & 3);
-    const uint64_t i = base + 32 * j + lane;
-    if (i >= n) continue;
-    const int64_t row = n >> 32 ? (int64_t)(i / (uint64_t)a.cols) : (int64_t)((uint32_t)i / (uint32_t)a.cols), col = (int64_t)i - row * a.cols;
-    const float r = a.residual ? to_f32<T>(reinterpret_cast<const T*>(a.residual)[row * a.sr + col]) : 0.f;
-    reinterpret_cast<T*>(a.out)[row * a.so + col] = dropped<T>(reinterpret_cast<const T*>(a.x)[row * a.sx + col], keep & 1u, a.scale, r);
+  for (int j = 0; j < kPer; ++j) {
+    if (j > 0) {      // (32 elements further: the next row or, where rows are short, some rows on)
+      row[j] = row[j - 1];
+      col[j] = col[j - 1] + 32;
+      while (col[j] >= a.cols) { col[j] -= a.cols; ++row[j]; }
+    }
+    if (base + 32 * j + lane < n) {
+      in[j] = x[row[j] * a.sx + col[j]];
+      if (res) r[j] = res[row[j] * a.sr + col[j]];
+    }
+  }
+  uint32_t c[2][4], mine[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint64_t counter = offset + base / 4 + 32 * k + lane;
+    c[k][0] = (uint32_t)counter;
+    c[k][1] = (uint32_t)(counter >> 32);
+  }
+  philox_words<2>((uint32_t)seed, (uint32_t)(seed >> 32), c);
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    mine[k] = !a.on ? 15u
+                    : ((int32_t)c[k][0] > a.threshold ? 1u : 0u) | ((int32_t)c[k][2] > a.threshold ? 2u : 0u) |
+                          ((int32_t)c[k][1] > a.threshold ? 4u : 0u) | ((int32_t)c[k][3] > a.threshold ? 8u : 0u);
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const uint32_t keep = __shfl_sync(0xffffffffu, mine[j / 4], 8 * (j & 3) + (lane >> 2)) >> (lane & 3);
+    if (base + 32 * j + lane >= n) continue;
+    float y = kept<T>(in[j], keep & 1u, a.scale);
+    if (res) y += to_f32<T>(r[j]);
+    out[row[j] * a.so + col[j]] = from_f32<T>(y);
   }
 }
 
-// f.template operator()<T>() for the dtype's T
+// f.template operator()<T>() for the dtype's T (the entry points let no other through)
 template <typename F>
-cudaError_t with_type(int dtype, F f) {
-  switch (dtype) {
-    case 1: return f.template operator()<float>();
-    case 2: return f.template operator()<__half>();
-    case 3: return f.template operator()<__nv_bfloat16>();
-  }
-  return cudaErrorInvalidValue;
+auto with_type(int dtype, F f) {
+  return dtype == 1 ? f.template operator()<float>() : (dtype == 2 ? f.template operator()<__half>() : f.template operator()<__nv_bfloat16>());
 }
+template <typename F>
+auto with_band(int dtype, const RelativeBias& a, F f) {
+  return with_type(dtype, [&]<typename T>() { return a.strips == 4 ? f.template operator()<T, 4>() : f.template operator()<T, 1>(); });
+}
+// Four strips side by side, 2 KB of a row at once, where rows are long: memory gives 512 bytes here and there at 4.3 TB/s, 2 KB at 5.9.  In shorter
+// rows most of such a band lies beside them.  Measured, us, whole backward with nothing in L2, four strips / one: bf16, 8 x 16 heads x 513 44.0 / 37.9,
+// x 1000 75.8 / 67.6, 4 x 16 x 1536 80.9 / 77.8, x 2048 112.6 / 113.7, 8 x 16 x 2047 207.9 / 212.1; fp32, 8 x 16 x 768 72.8 / 72.7, x 1024 108.5 / 110.7,
+// x 2048 356 / 382.
+inline bool wide_bands(int dtype, const RelativeBias& a) { return (int64_t)std::min(a.sq, a.sk) * (dtype == 1 ? 4 : 2) >= 3584; }
 
 cudaError_t counted(cudaError_t e) {
   if (e == cudaSuccess) count_launch();
@@ -356,32 +468,39 @@ cudaError_t launch_relative_bias(int dtype, int table_dtype, const RelativeBias&
 }
 
 int64_t plan_relative_bias_backward(int dtype, RelativeBias& a, int sms) {
+  a.bands = a.chunks = a.chunk_rows = 0;
   if (a.sq <= 0 || a.sk <= 0 || a.heads <= 0 || a.batch <= 0) return 0;
-  const int n = dtype == 1 ? 4 : 8, width = 32 * n;
-  // strips cover the diagonals 1 - sq .. sk - 1
-  const int64_t strips = ((int64_t)a.sk + (a.sq + 7) / 8 * 8 + width - 1) / width;
-  const int most = a.sq < a.sk + width + 8 ? a.sq : a.sk + width + 8;      // rows of a strip
-  a.chunk_rows = 512;
-  a.strips = (int)strips;
-  a.chunks = (most + n + a.chunk_rows - 1) / a.chunk_rows;
-  a.batch_parts = a.batch;
-  while (a.batch_parts > 1 && strips * a.chunks * a.heads * (int64_t)a.batch_parts > 16ll * sms) a.batch_parts = (a.batch_parts + 1) / 2;
-  return strips * a.chunks * a.batch_parts * (int64_t)a.heads * a.per_direction * (a.both ? 2 : 1);
+  a.strips = wide_bands(dtype, a) ? 4 : 1;
+  return with_band(dtype, a, [&]<typename T, int STRIPS>() {
+    // Rows a CTA, whole steps: one round of the four CTAs an SM holds where the whole is small, three for long rows, whose bands are uneven.
+    // (Device us with 4 / 6 / 8 / 12 / 16 CTAs an SM: 16 x 12 x 391 bf16 27.4 / 28.0 / 29.9 / 31.7 / 31.7, 8 x 16 x 768 33.6 / 37.7 / 35.4 / 38.4 /
+    // 41.3, 4 x 16 x 2048 109.2 / 102.8 / 97.3 / 94.4 / 96.3.)  64 bands tell how many rows there are (neighbours differ little).
+    using B = Band<T, STRIPS>;
+    constexpr int step = B::kStep;
+    const int bands = B::bands(a.sq, a.sk), probe = std::min(bands, 64);
+    int64_t all = 0;
+    for (int i = 0; i < probe; ++i) all += B(a.sq, a.sk, (int)((int64_t)bands * i / probe)).rows;
+    const int64_t total = all * bands / probe * a.batch * a.heads * B::kParts, target = total / ((STRIPS == 4 ? 12ll : 4ll) * sms);
+    const int64_t rows = std::min<int64_t>(std::max<int64_t>((target + step - 1) / step * step, step), 1 << 30);
+    const int64_t most = (std::min<int64_t>(a.sq, (int64_t)a.sk + B::kBand - 1) + step - 1) / step * step;      // rows of a band
+    a.bands = bands;
+    a.chunk_rows = (int)rows;
+    a.chunks = (int)((most * a.batch + rows - 1) / rows);
+    return (int64_t)bands * a.chunks * B::kParts * a.heads * a.per_direction * (a.both ? 2 : 1);
+  });
 }
 
 cudaError_t launch_relative_bias_backward(int dtype, int table_dtype, const RelativeBias& a, cudaStream_t st) {
   const int buckets = a.per_direction * (a.both ? 2 : 1);
-  const bool empty = a.sq <= 0 || a.sk <= 0 || a.batch <= 0;
-  if (!empty) {
-    const dim3 grid(a.strips * a.chunks, a.heads, a.batch_parts);
-    const cudaError_t e = with_type(dtype, [&]<typename T>() {
-      return counted(launch_kernel(a.vec ? relative_bias_sums_kernel<T, true> : relative_bias_sums_kernel<T, false>, grid, dim3(kThreads), 0, st, a));
+  return with_band(dtype, a, [&]<typename T, int STRIPS>() {
+    if (a.bands > 0) {
+      const cudaError_t e = counted(launch_kernel(a.unit ? relative_bias_sums_kernel<T, STRIPS, true> : relative_bias_sums_kernel<T, STRIPS, false>,
+                                                  dim3(a.bands * a.chunks * Band<T, STRIPS>::kParts, a.heads), dim3(kThreads), 0, st, a));
+      if (e != cudaSuccess) return e;
+    }
+    return with_type(table_dtype, [&]<typename TT>() {
+      return counted(launch_kernel(relative_bias_table_kernel<T, STRIPS, TT>, dim3(buckets, a.heads), dim3(128), 0, st, a));
     });
-    if (e != cudaSuccess) return e;
-  }
-  const int count = empty ? 0 : a.strips * a.chunks * a.batch_parts;
-  return with_type(table_dtype, [&]<typename TT>() {
-    return counted(launch_kernel(relative_bias_table_kernel<TT>, dim3(buckets, a.heads), dim3(128), 0, st, a, count));
   });
 }
 
@@ -398,14 +517,17 @@ cudaError_t launch_dropout(int dtype, const Dropout& a, cudaStream_t st) {
     if (vec && total >= N) {
       const uint64_t vectors = (uint64_t)(total / N), per = kThreads * (16 / N);
       const dim3 grid((unsigned)((vectors + per - 1) / per));
-      auto kern = one_row ? (a.residual ? dropout_kernel<T, true, true> : dropout_kernel<T, true, false>)
-                          : (a.residual ? dropout_kernel<T, false, true> : dropout_kernel<T, false, false>);
+      using Kernel = void (*)(Dropout, uint64_t);
+      static constexpr Kernel kernels[2][2][2] = {      // [one row][residual][pointers]
+          {{dropout_kernel<T, false, false, false>, dropout_kernel<T, false, false, true>}, {dropout_kernel<T, false, true, false>, dropout_kernel<T, false, true, true>}},
+          {{dropout_kernel<T, true, false, false>, dropout_kernel<T, true, false, true>}, {dropout_kernel<T, true, true, false>, dropout_kernel<T, true, true, true>}}};
+      const Kernel kern = kernels[one_row][a.residual != nullptr][a.seed_ptr != nullptr || a.offset_ptr != nullptr];
       const cudaError_t e = counted(launch_kernel(kern, grid, dim3(kThreads), 0, st, a, vectors));
       if (e != cudaSuccess) return e;
       done = vectors * N;
     }
     if ((int64_t)done == total) return cudaSuccess;
-    const dim3 grid((unsigned)((total - done + 1023) / 1024));
+    const dim3 grid((unsigned)((total - done + kElementsCta - 1) / kElementsCta));
     return counted(launch_kernel(dropout_elements_kernel<T>, grid, dim3(kThreads), 0, st, a, done));
   });
 }

@@ -17,8 +17,8 @@ struct RelativeBias {
   int32_t per_direction, both;   // buckets of one direction; both: keys behind the query's position take the second half
   int32_t borders[kMaxBorders];  // borders[k - 1]: the smallest distance whose bucket is k or more
   float* partial;                // backward: bucket sums of each CTA
-  int32_t strips, chunks, chunk_rows, batch_parts;
-  int32_t vec;                   // rows allow 16-byte accesses
+  int32_t strips, bands, chunks, chunk_rows;
+  int32_t unit, vec;             // the bias' elements are next to each other in its rows; and those start on 16-byte boundaries
 };
 
 struct Dropout {
@@ -32,7 +32,7 @@ struct Dropout {
 };
 
 cudaError_t launch_relative_bias(int dtype, int table_dtype, const RelativeBias& a, cudaStream_t st);
-// How the backward is cut (strips, chunks, chunk_rows, batch_parts), for `sms` SMs; returns the floats of workspace it needs.
+// How the backward is cut (strips, bands, chunks, chunk_rows), for `sms` SMs; returns the floats of workspace it needs.
 int64_t plan_relative_bias_backward(int dtype, RelativeBias& a, int sms);
 cudaError_t launch_relative_bias_backward(int dtype, int table_dtype, const RelativeBias& a, cudaStream_t st);
 cudaError_t launch_dropout(int dtype, const Dropout& a, cudaStream_t st);
