@@ -11,7 +11,10 @@
 //
 // Dropout.  Element i in logical (row-major) order takes word (0, 2, 1, 3)[i % 4] of Philox counter offset + i / 4, as the columns of a
 // score row do (common.cuh): a mask follows from seed, offset and the logical index alone, not from strides, and is never stored; the
-// backward draws it again.  Ten rounds of the generator serve four elements; beside them the kernel moves two to three elements' bytes each.
+// backward draws it again.  Ten rounds of the generator serve four elements, beside which two (with a residual three) elements' bytes each move: the
+// wide multiplies, four of a round's eight issue slots' worth, and the exclusive ors bound the form without a residual in 16-bit types, memory the
+// others.  64M elements of bf16: 57 us without a residual (4.7 TB/s), 64 with one (6.3 TB/s); fp32, 32M, 36.6 and 53 (7.3 and 7.6 TB/s, a part of it from
+// L2).  (Round keys added up by each thread 68 and 74; CTAs that take several tiles in turn 57 to 63 and 64 to 75.)
 #include <algorithm>
 #include <type_traits>
 #include "launch.h"
@@ -22,6 +25,7 @@ namespace ab200 {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr uint32_t kPhiloxA = 0xD2511F53u, kPhiloxB = 0xCD9E8D57u;
 
 template <typename T> struct alignas(16) Vec {
   static constexpr int N = 16 / (int)sizeof(T);
@@ -129,7 +133,7 @@ template <typename T, int STRIPS> struct Band {
 template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  return make_float2(__uint_as_float(__byte_perm(w, 0u, 0x1044)), __uint_as_float(w & 0xffff0000u));
 }
 
 // grid = (bands * chunks * kParts, heads); partial[(h * gridDim.x + x) * buckets + bucket], of chunks that have rows.
@@ -302,79 +306,121 @@ __global__ void __launch_bounds__(128) relative_bias_table_kernel(const __grid_c
 template <typename T>
 __device__ __forceinline__ float kept(T x, bool keep, float scale) { return keep ? to_f32<T>(x) * scale : 0.f; }
 
-// N counters of one seed side by side: c[n][0..1] in, the four words out.  The key of a call that passes its seed by value is the same
-// for the whole grid, and so are its twenty round keys: left in uniform registers they cost the threads nothing.
-template <int N>
-__device__ __forceinline__ void philox_words(uint32_t k0, uint32_t k1, uint32_t (&c)[N][4]) {
+// Rounds FROM..9 of N counters of one seed side by side: c[n], four words in and out.  key(i): the i-th of the twenty round keys.
+template <int FROM, int N, typename K>
+__device__ __forceinline__ void philox_rounds(K key, uint32_t (&c)[N][4]) {
 #pragma unroll
-  for (int n = 0; n < N; ++n) c[n][2] = c[n][3] = 0u;
-#pragma unroll
-  for (int i = 0; i < 10; ++i) {
+  for (int i = FROM; i < 10; ++i) {
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const uint64_t pa = (uint64_t)0xD2511F53u * c[n][0], pb = (uint64_t)0xCD9E8D57u * c[n][2];
-      const uint32_t n0 = (uint32_t)(pb >> 32) ^ c[n][1] ^ k0, n2 = (uint32_t)(pa >> 32) ^ c[n][3] ^ k1;
+      const uint64_t pa = (uint64_t)kPhiloxA * c[n][0], pb = (uint64_t)kPhiloxB * c[n][2];
+      const uint32_t n0 = (uint32_t)(pb >> 32) ^ c[n][1] ^ key(2 * i), n2 = (uint32_t)(pa >> 32) ^ c[n][3] ^ key(2 * i + 1);
       c[n][1] = (uint32_t)pb; c[n][3] = (uint32_t)pa; c[n][0] = n0; c[n][2] = n2;
     }
-    k0 += 0x9E3779B9u; k1 += 0xBB67AE85u;
   }
 }
+__host__ __device__ constexpr uint32_t round_key(uint64_t seed, int i) {
+  return (i & 1) ? (uint32_t)(seed >> 32) + 0xBB67AE85u * (uint32_t)(i >> 1) : (uint32_t)seed + 0x9E3779B9u * (uint32_t)(i >> 1);
+}
+// The words of counters c[n][0..1], whatever they are.
+template <int N>
+__device__ __forceinline__ void philox_words(uint64_t seed, uint32_t (&c)[N][4]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) c[n][2] = c[n][3] = 0u;
+  philox_rounds<0, N>([&](int i) { return round_key(seed, i); }, c);
+}
+// The same for a call that passes its seed by value and all of whose counters have one high word: the keys come from the call's parameters, where
+// the exclusive ors read them for nothing, and of the first two rounds what the high word alone decides is in them already
+// (dropout_keys).  c[n][0]: the counter's low word in.
+template <int N>
+__device__ __forceinline__ void philox_words_by_value(const uint32_t (&keys)[20], uint32_t (&c)[N][4]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const uint64_t pa = (uint64_t)kPhiloxA * c[n][0], pb = (uint64_t)kPhiloxB * ((uint32_t)(pa >> 32) ^ keys[1]);
+    c[n][0] = (uint32_t)(pb >> 32) ^ keys[2];
+    c[n][1] = (uint32_t)pb;
+    c[n][2] = (uint32_t)pa ^ keys[3];
+    c[n][3] = 0u;      // (in keys[5])
+  }
+  philox_rounds<2, N>([&](int i) { return keys[i]; }, c);
+}
+// Round 1 leaves c0 = high ^ keys[0], the same for all counters; its product in round 2 goes into keys[3] and keys[5].
+void dropout_keys(uint64_t seed, uint32_t high, uint32_t (&keys)[20]) {
+  for (int i = 0; i < 20; ++i) keys[i] = round_key(seed, i);
+  const uint64_t product = (uint64_t)kPhiloxA * (high ^ keys[0]);
+  keys[3] ^= (uint32_t)(product >> 32);
+  keys[5] ^= (uint32_t)product;
+}
 
-// FLAT: everything is contiguous, one row.  Otherwise rows of cols elements, a multiple of N, with strides of their own.  POINTERS: seed and
-// offset are read from the device as well.
-template <typename T, bool FLAT, bool RESIDUAL, bool POINTERS>
+// FLAT: everything is contiguous, one row.  Otherwise rows of cols elements, a multiple of N, with strides of their own.  BY_VALUE: seed and
+// offset are the call's alone, and the counters' high word is one.
+template <typename T, bool FLAT, bool RESIDUAL, bool BY_VALUE>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant__ Dropout a, uint64_t vectors) {
   wait_for_earlier_grids();
   constexpr int N = Vec<T>::N, U = 16 / N;      // sixteen elements a thread: four counters side by side
   uint64_t seed = a.seed, offset = a.offset;
-  if constexpr (POINTERS) {
+  if constexpr (!BY_VALUE) {
     if (a.seed_ptr) seed += *a.seed_ptr;
     if (a.offset_ptr) offset += *a.offset_ptr;
   }
   const bool keep_all = !a.on;
-  const T* x = reinterpret_cast<const T*>(a.x);
-  const T* res = reinterpret_cast<const T*>(a.residual);
-  T* out = reinterpret_cast<T*>(a.out);
   const uint64_t v0 = (uint64_t)blockIdx.x * (kThreads * U) + threadIdx.x;
   auto body = [&](auto whole) {      // (no bounds but in the last CTA)
-    Vec<T> in[U], r[U];
-    int64_t row[U], col[U];
+    uint4 in[U], r[U], *to[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint64_t v = v0 + (uint64_t)u * kThreads;
       if (!whole.value && v >= vectors) continue;
-      if constexpr (FLAT) { row[u] = 0; col[u] = (int64_t)v * N; }
-      else {
+      const uint4 *from = reinterpret_cast<const uint4*>(a.x), *add = reinterpret_cast<const uint4*>(a.residual);
+      to[u] = reinterpret_cast<uint4*>(a.out);
+      if constexpr (FLAT) {
+        from += v0 + u * kThreads;
+        add += v0 + u * kThreads;
+        to[u] += v0 + u * kThreads;
+      } else {
         const uint64_t per = (uint64_t)a.cols / N;
-        row[u] = vectors >> 32 ? (int64_t)(v / per) : (int64_t)((uint32_t)v / (uint32_t)per);
-        col[u] = ((int64_t)v - row[u] * (int64_t)per) * N;
+        const int64_t row = vectors >> 32 ? (int64_t)(v / per) : (int64_t)((uint32_t)v / (uint32_t)per), col = (int64_t)v - row * (int64_t)per;
+        from += row * (a.sx / N) + col;
+        add += row * (a.sr / N) + col;
+        to[u] += row * (a.so / N) + col;
       }
-      *reinterpret_cast<uint4*>(&in[u]) = __ldcs(reinterpret_cast<const uint4*>(x + row[u] * a.sx + col[u]));
-      if constexpr (RESIDUAL) *reinterpret_cast<uint4*>(&r[u]) = __ldcs(reinterpret_cast<const uint4*>(res + row[u] * a.sr + col[u]));
+      in[u] = __ldcs(from);
+      if constexpr (RESIDUAL) r[u] = __ldcs(add);
     }
     uint32_t c[4][4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const uint64_t counter = offset + (v0 + (uint64_t)(k / (N / 4)) * kThreads) * (N / 4) + (k % (N / 4));
+      const uint64_t counter = offset + v0 * (N / 4) + (k / (N / 4)) * kThreads * (N / 4) + (k % (N / 4));
       c[k][0] = (uint32_t)counter;
       c[k][1] = (uint32_t)(counter >> 32);
     }
-    philox_words<4>((uint32_t)seed, (uint32_t)(seed >> 32), c);
+    if constexpr (BY_VALUE) philox_words_by_value<4>(a.keys, c);
+    else philox_words<4>(seed, c);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (!whole.value && v0 + (uint64_t)u * kThreads >= vectors) continue;
-      float y[N];
+      const uint32_t x[4] = {in[u].x, in[u].y, in[u].z, in[u].w}, res[4] = {r[u].x, r[u].y, r[u].z, r[u].w};
+      uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const uint32_t* words = c[u * (N / 4) + e / 4];
-        const uint32_t word = (e & 3) == 0 ? words[0] : ((e & 3) == 1 ? words[2] : ((e & 3) == 2 ? words[1] : words[3]));
-        y[e] = kept<T>(in[u].e[e], keep_all || (int32_t)word > a.threshold, a.scale);
-        if constexpr (RESIDUAL) y[e] += to_f32<T>(r[u].e[e]);
+      for (int i = 0; i < 4; ++i) {
+        constexpr int kPer = N / 4;      // elements of a word: one or two
+        auto keep = [&](int e) {
+          const uint32_t* words = c[u * (N / 4) + e / 4];
+          return keep_all || (int32_t)((e & 3) == 0 ? words[0] : ((e & 3) == 1 ? words[2] : ((e & 3) == 2 ? words[1] : words[3]))) > a.threshold;
+        };
+        if constexpr (kPer == 1) {
+          float y = keep(i) ? __uint_as_float(x[i]) * a.scale : 0.f;
+          if constexpr (RESIDUAL) y += __uint_as_float(res[i]);
+          w[i] = __float_as_uint(y);
+        } else {
+          float2 y = unpack2<T>(x[i]);
+          y.x = keep(2 * i) ? y.x * a.scale : 0.f;
+          y.y = keep(2 * i + 1) ? y.y * a.scale : 0.f;
+          if constexpr (RESIDUAL) y = ptx::add2(y, unpack2<T>(res[i]));
+          w[i] = pack2<T>(y.x, y.y);
+        }
       }
-      uint4 w;
-      if constexpr (sizeof(T) == 4) w = make_uint4(__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3]));
-      else w = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[N - 4], y[N - 3]), pack2<T>(y[N - 2], y[N - 1]));
-      *reinterpret_cast<uint4*>(out + row[u] * a.so + col[u]) = w;
+      *to[u] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   };
   if ((uint64_t)(blockIdx.x + 1ull) * (kThreads * U) <= vectors) body(std::true_type{});
@@ -382,36 +428,34 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(const __grid_constant
 }
 
 // Any width, stride and alignment, from element `first` (a multiple of four) on: a warp takes 256 elements, two counters a lane, and
-// hands the bits round so that its accesses are to consecutive elements.
+// hands the bits round so that its accesses are to consecutive elements.  WIDE: rows of 256 elements or more, so that a warp's lie in one row or
+// two.
 constexpr int kElementsWarp = 256, kElementsCta = kElementsWarp * (kThreads / 32);
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads) dropout_elements_kernel(const __grid_constant__ Dropout a, uint64_t first) {
   wait_for_earlier_grids();
   const uint64_t seed = a.seed + (a.seed_ptr ? *a.seed_ptr : 0ull), offset = a.offset + (a.offset_ptr ? *a.offset_ptr : 0ull);
   const int lane = threadIdx.x & 31;
   const uint64_t n = (uint64_t)a.rows * (uint64_t)a.cols, base = first + (uint64_t)blockIdx.x * kElementsCta + (threadIdx.x >> 5) * kElementsWarp;
   if (base >= n) return;
-  const T* x = reinterpret_cast<const T*>(a.x);
-  const T* res = reinterpret_cast<const T*>(a.residual);
-  T* out = reinterpret_cast<T*>(a.out);
   constexpr int kPer = kElementsWarp / 32;
-  int64_t row[kPer], col[kPer];
-  T in[kPer], r[kPer];
-  {
-    const uint64_t i = base + lane;
-    row[0] = n >> 32 ? (int64_t)(i / (uint64_t)a.cols) : (int64_t)((uint32_t)i / (uint32_t)a.cols);
-    col[0] = (int64_t)i - row[0] * a.cols;
-  }
+  const int left = (int)min(n - base, (uint64_t)kElementsWarp) - lane;      // element 32 j + lane is one where 32 j < left
+  // this lane's first element, and where its elements lie in a tensor with a stride of s between rows
+  uint64_t row = n >> 32 ? base / (uint64_t)a.cols : (uint64_t)((uint32_t)base / (uint32_t)a.cols);
+  const int64_t col = (int64_t)(base - row * (uint64_t)a.cols) + lane;
+  const int in_row = (int)min(a.cols - col, (int64_t)1 << 20);      // element j is in the next row where 32 j >= in_row (WIDE)
+  auto at = [&](int64_t s, int j) -> int64_t {
+    if constexpr (WIDE) return (int64_t)row * s + col + 32 * j + (32 * j >= in_row ? s - a.cols : 0);
+    const int64_t c = col + 32 * j, down = c / a.cols;
+    return ((int64_t)row + down) * s + c - down * a.cols;
+  };
+  const T *x = reinterpret_cast<const T*>(a.x), *res = reinterpret_cast<const T*>(a.residual);
+  T *out = reinterpret_cast<T*>(a.out), in[kPer], r[kPer];
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    if (j > 0) {      // (32 elements further: the next row or, where rows are short, some rows on)
-      row[j] = row[j - 1];
-      col[j] = col[j - 1] + 32;
-      while (col[j] >= a.cols) { col[j] -= a.cols; ++row[j]; }
-    }
-    if (base + 32 * j + lane < n) {
-      in[j] = x[row[j] * a.sx + col[j]];
-      if (res) r[j] = res[row[j] * a.sr + col[j]];
+    if (32 * j < left) {
+      in[j] = x[at(a.sx, j)];
+      if (res) r[j] = res[at(a.sr, j)];
     }
   }
   uint32_t c[2][4], mine[2];
@@ -421,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) dropout_elements_kernel(const __grid
     c[k][0] = (uint32_t)counter;
     c[k][1] = (uint32_t)(counter >> 32);
   }
-  philox_words<2>((uint32_t)seed, (uint32_t)(seed >> 32), c);
+  philox_words<2>(seed, c);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     mine[k] = !a.on ? 15u
@@ -430,10 +474,10 @@ __global__ void __launch_bounds__(kThreads) dropout_elements_kernel(const __grid
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     const uint32_t keep = __shfl_sync(0xffffffffu, mine[j / 4], 8 * (j & 3) + (lane >> 2)) >> (lane & 3);
-    if (base + 32 * j + lane >= n) continue;
+    if (32 * j >= left) continue;
     float y = kept<T>(in[j], keep & 1u, a.scale);
     if (res) y += to_f32<T>(r[j]);
-    out[row[j] * a.so + col[j]] = from_f32<T>(y);
+    out[at(a.so, j)] = from_f32<T>(y);
   }
 }
 
@@ -504,9 +548,12 @@ cudaError_t launch_relative_bias_backward(int dtype, int table_dtype, const Rela
   });
 }
 
-cudaError_t launch_dropout(int dtype, const Dropout& a, cudaStream_t st) {
+cudaError_t launch_dropout(int dtype, const Dropout& given, cudaStream_t st) {
+  Dropout a = given;
   const int64_t total = a.rows * a.cols;
   if (total <= 0) return cudaSuccess;
+  const bool by_value = a.seed_ptr == nullptr && a.offset_ptr == nullptr && (a.offset >> 32) == ((a.offset + (uint64_t)(total - 1) / 4) >> 32);
+  dropout_keys(a.seed, (uint32_t)(a.offset >> 32), a.keys);
   return with_type(dtype, [&]<typename T>() {
     constexpr int N = Vec<T>::N;
     auto aligned = [&](const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % N == 0; };
@@ -518,17 +565,17 @@ cudaError_t launch_dropout(int dtype, const Dropout& a, cudaStream_t st) {
       const uint64_t vectors = (uint64_t)(total / N), per = kThreads * (16 / N);
       const dim3 grid((unsigned)((vectors + per - 1) / per));
       using Kernel = void (*)(Dropout, uint64_t);
-      static constexpr Kernel kernels[2][2][2] = {      // [one row][residual][pointers]
+      static constexpr Kernel kernels[2][2][2] = {      // [one row][residual][by value]
           {{dropout_kernel<T, false, false, false>, dropout_kernel<T, false, false, true>}, {dropout_kernel<T, false, true, false>, dropout_kernel<T, false, true, true>}},
           {{dropout_kernel<T, true, false, false>, dropout_kernel<T, true, false, true>}, {dropout_kernel<T, true, true, false>, dropout_kernel<T, true, true, true>}}};
-      const Kernel kern = kernels[one_row][a.residual != nullptr][a.seed_ptr != nullptr || a.offset_ptr != nullptr];
+      const Kernel kern = kernels[one_row][a.residual != nullptr][by_value];
       const cudaError_t e = counted(launch_kernel(kern, grid, dim3(kThreads), 0, st, a, vectors));
       if (e != cudaSuccess) return e;
       done = vectors * N;
     }
     if ((int64_t)done == total) return cudaSuccess;
     const dim3 grid((unsigned)((total - done + kElementsCta - 1) / kElementsCta));
-    return counted(launch_kernel(dropout_elements_kernel<T>, grid, dim3(kThreads), 0, st, a, done));
+    return counted(launch_kernel(a.cols >= kElementsWarp ? dropout_elements_kernel<T, true> : dropout_elements_kernel<T, false>, grid, dim3(kThreads), 0, st, a, done));
   });
 }
 

@@ -29,6 +29,7 @@ struct Dropout {
   uint64_t seed, offset;               // added to what the pointers (may be null) say
   float scale;
   int32_t threshold, on;
+  uint32_t keys[20];                   // of calls without pointers (dropout_keys)
 };
 
 cudaError_t launch_relative_bias(int dtype, int table_dtype, const RelativeBias& a, cudaStream_t st);
