@@ -66,25 +66,17 @@ using namespace ptx;
 
 constexpr int kBM = 128, kBN = 128;
 constexpr int kFwdThreads = 384;
+constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleThreshold = 8.0f;
 
 // Head dims up to 128: two query tiles per CTA and two-stage K and V rings.  Head dims up to 256:
 // a tile is 64 KB, so one query tile per CTA (S in 128 and O in 256 tensor-memory columns) and one
 // stage each for K and V; the K copy of block j+1 then runs under the softmax and P V of block j,
 // the V copy under Q K^T and the softmax of block j+1.
-// Sink attention with head dims up to 128: one query tile per CTA and two CTAs on an SM.  A window is a few blocks, and of a CTA with two tiles
-// that has an SM to itself, 10 us went by setting up, filling and draining the pipeline and writing out, beside 2.2 us for each block of both; the two
-// tiles of a CTA each see a block that the other does not, as well.  With two CTAs one works while the other starts or ends, and a tile walks its own
-// blocks only; each has one stage of K and of V (two at head dims up to 64), 128 + 128 tensor-memory columns and half the registers.
-// Measured, us, two tiles / one: SINK_NUMBERS
-template <int HD, int FEAT>
+template <int HD>
 struct FwdSmem {
-  static constexpr bool kPair = (FEAT & kSinks) != 0 && HD <= 128;      // two CTAs an SM
-  static constexpr int kTiles = HD > 128 || kPair ? 1 : 2;
-  static constexpr int kStages = HD > 128 || (kPair && HD > 64) ? 1 : 2;
-  static constexpr int kThreads = kPair ? 256 : kFwdThreads, kCtasPerSm = kPair ? 2 : 1;
-  static constexpr uint32_t kTmemCols = kPair ? 256 : 512, kTmemO = kPair ? 128 : 256;      // tensor-memory columns, and the first of O
-  static constexpr int kSoftmaxRegs = kPair ? 200 : 216;      // (56 and 200 for each four warps are the 128 a thread of the launch)
+  static constexpr int kTiles = HD > 128 ? 1 : 2;
+  static constexpr int kStages = HD > 128 ? 1 : 2;
   static constexpr int kCtaRows = kTiles * kBM;
   static constexpr int kHalves = HD / 64;
   static constexpr int kTileBytes = kHalves * 128 * 128;     // 128 rows x HD x 2 bytes
@@ -100,7 +92,7 @@ struct FwdSmem {
   static constexpr int kAbort = kTmemSlot + 4;               // abort word, then the launch's wait limit
   static constexpr int kKeep = (kAbort + 8 + 15) & ~15;      // one tile: two buffers of keep bits of 128 rows x 128 keys
   static constexpr int kKeepTile = 128 * 16;
-  static constexpr int kTotal = kKeep + (HD > 128 ? 2 * kKeepTile : 0);
+  static constexpr int kTotal = kKeep + (kTiles == 1 ? 2 * kKeepTile : 0);
   static constexpr int kDynamic = kTotal + 1024;             // slack for manual 1024-byte alignment
 };
 
@@ -127,12 +119,12 @@ __device__ void write_dead_rows(const Params& p, const Seq& sq, int h, int m0, i
 // Bias' instantiation against the call's own, neither, of 256: 4 x 16:8 heads x 2048 327 -> 317, causal 201 -> 197, 2 x 16 x 4096 causal
 // 333 -> 329, 8 x 16 x 2048 637 -> 640.
 template <typename T, int HD, bool EXACT, int FEAT>
-__global__ void __launch_bounds__(FwdSmem<HD, FEAT>::kThreads, FwdSmem<HD, FEAT>::kCtasPerSm)
+__global__ void __launch_bounds__(kFwdThreads, 1)
 sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                  unsigned int* status) {
   wait_for_earlier_grids();
-  using L = FwdSmem<HD, FEAT>;
+  using L = FwdSmem<HD>;
   constexpr int kStages = L::kStages, kCtaRows = L::kCtaRows;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -201,9 +193,6 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
   const int before = blocks_before<FEAT>(p, n_hi, jb_lo, kBN);
   const int nblk = before + n_hi / kBN - jb_lo + 1;
   auto block = [&](int j) { return block_at<FEAT>(j, before, jb_lo); };
-  // A last block of first keys that lies in front of the window and has 32 of them at most is taken as 32 keys (-1: none).
-  constexpr bool kNarrow = (FEAT & kSinks) != 0;
-  const int narrow_j = kNarrow && before > 0 && p.sinks - (before - 1) * kBN <= 32 ? before - 1 : -1;
 
   // ---- set-up -----------------------------------------------------------------------
   if (threadIdx.x == 0) {
@@ -239,7 +228,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       tma_load_4d(smem + L::kK + hf * 16384, &tm_k, &bars[L::bKFull], hf * 64, (int)(sq.k0 + (int64_t)block(0) * kBN), hk, sq.bidx);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, L::kTmemCols);
+    tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -252,7 +241,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       mbar_wait_quiet(&bars[L::bKFull], 0, abort_flag);
     }
     __syncthreads();
-    if (warp == 1) tmem_dealloc(tmem_base, L::kTmemCols);
+    if (warp == 1) tmem_dealloc(tmem_base, kTmemCols);
     return;
   }
 
@@ -301,7 +290,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       // The contraction of Q K^T runs over the head dimension rounded up to 16 and P V produces the
       // value head dimension rounded up to 16 (the copies zero-fill up to the 64-column box), so a
       // padded head dimension costs its own size, not the kernel's.
-      constexpr uint32_t kIdescQK = instr_desc_f16(Fmt<T>::code, 128, 128, 0, 0), kIdescNarrow = instr_desc_f16(Fmt<T>::code, 128, 32, 0, 0);
+      constexpr uint32_t kIdescQK = instr_desc_f16(Fmt<T>::code, 128, 128, 0, 0);
       // (EXACT: both equal the kernel's head dimension, known at compile time)
       const uint32_t kIdescPV = instr_desc_f16(Fmt<T>::code, 128, EXACT ? (uint32_t)HD : (uint32_t)((p.dvo + 15) & ~15), 0, 1);
       const int ksteps = EXACT ? HD / 16 : (p.dqk + 15) >> 4;
@@ -318,13 +307,12 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       auto issue_qk = [&](int t, int j, bool release_k) {
         const uint64_t qd = q_desc + (uint64_t)((uint32_t)t * kStageStep);
         const uint64_t kd = k_desc + (uint64_t)((uint32_t)(j % kStages) * kStageStep);
-        const uint32_t idesc = kNarrow && j == narrow_j ? kIdescNarrow : kIdescQK;
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             constexpr uint32_t kHalfStep = 16384u >> 4, kInner = 32u >> 4;
             const uint32_t off = (uint32_t)(kk >> 2) * kHalfStep + (uint32_t)(kk & 3) * kInner;
-            if (kk < ksteps) mma_ss(tmem_base + (uint32_t)t * 128u, qd + off, kd + off, idesc, kk > 0 ? 1u : 0u);
+            if (kk < ksteps) mma_ss(tmem_base + (uint32_t)t * 128u, qd + off, kd + off, kIdescQK, kk > 0 ? 1u : 0u);
           }
           mma_commit(&bars[L::bSFull + t]);
           if (release_k) mma_commit(&bars[L::bKEmpty + (j % kStages)]);
@@ -362,19 +350,18 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
         }
         const uint64_t vd = v_desc + (uint64_t)((uint32_t)s * kStageStep);
         const uint32_t first = (j > 0) ? 1u : 0u;
-        const bool narrow = kNarrow && j == narrow_j;      // (P is 32 keys, two steps of 16, handed over at once)
         for (int t = 0; ok && t < ntile; ++t) {
           // P arrives in two halves of 64 keys: the first half of P V runs while the softmax warps
           // are still working on the second.
           const uint32_t pcol = tmem_base + (uint32_t)t * 128u;
-          const uint32_t ocol = tmem_base + L::kTmemO + (uint32_t)t * 128u;
+          const uint32_t ocol = tmem_base + 256u + (uint32_t)t * 128u;
           if (!wait(L::bPHalf + t, par, 0x580 + 2 * j + t)) { ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < kBN / 32; ++kk) {
               // 16 keys per step: 8 packed columns of P, 2048 bytes of V (two 8-key groups)
-              if (kk < 2 || !narrow) mma_ts(ocol, pcol + (uint32_t)kk * 8u, vd + (uint32_t)kk * (2048u >> 4), kIdescPV, kk > 0 ? 1u : first);
+              mma_ts(ocol, pcol + (uint32_t)kk * 8u, vd + (uint32_t)kk * (2048u >> 4), kIdescPV, kk > 0 ? 1u : first);
             }
           }
           __syncwarp();
@@ -383,7 +370,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
           if (elect_one()) {
 #pragma unroll
             for (int kk = kBN / 32; kk < kBN / 16; ++kk)
-              if (!narrow) mma_ts(ocol, pcol + (uint32_t)kk * 8u, vd + (uint32_t)kk * (2048u >> 4), kIdescPV, 1u);
+              mma_ts(ocol, pcol + (uint32_t)kk * 8u, vd + (uint32_t)kk * (2048u >> 4), kIdescPV, 1u);
             mma_commit(&bars[L::bPvDone + t]);
             if (t == ntile - 1) mma_commit(&bars[L::bVEmpty + s]);
           }
@@ -425,7 +412,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
     }
   } else {
     // ================================== softmax =====================================
-    reg_alloc<L::kSoftmaxRegs>();
+    reg_alloc<216>();
     const int t = (warp - 4) >> 2;              // tile of this warpgroup
     if (t < ntile) {
     const int quarter = warp & 3;
@@ -433,7 +420,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
     const int m = m0 + t * kBM + r;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_addr + (uint32_t)t * 128u;
-    const uint32_t o_addr = tmem_base + lane_addr + L::kTmemO + (uint32_t)t * 128u;
+    const uint32_t o_addr = tmem_base + lane_addr + 256u + (uint32_t)t * 128u;
     // Rows beyond the sequence's end take the last row's bounds: nothing of theirs is stored, a row of the products
     // depends on no other one, and bounds of their own (none) would make every block of their warps a masked one.
     // Measured, forward on the device, us: 24 packed prompts of 32 to 2048 tokens, 32:8 heads of 128, 379 -> 360; a prompt of
@@ -457,24 +444,6 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
                   (int64_t)row0 * p.bias.s[2];
 
     float m_used = -INFINITY, l = 0.f;
-    // O times alpha in front of block j: O must be complete up to block j-1.
-    // (S of block j was issued behind P V of block j-1, so the wait returns at once.)
-    auto rescale = [&](float alpha, int j) {
-      if (!mbar_wait(&bars[L::bPvDone + t], (uint32_t)(j - 1) & 1u, abort_flag, status, 0x800 + 2 * j + t)) return false;
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < HD / 32; ++c) {
-        if (c * 32 >= p.dvo) break;          // columns the P V product never writes
-        uint32_t o[32];
-        tmem_ld32(o_addr + c * 32, o);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-        tmem_st32(o_addr + c * 32, o);
-      }
-      tmem_wait_st();
-      return true;
-    };
     bool ok = true;
     for (int j = 0; j < nblk; ++j) {
       const int n0 = block(j) * kBN;
@@ -502,45 +471,6 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       if (!mbar_wait(&bars[L::bSFull + t], par, abort_flag, status, 0x700 + 2 * j + t)) { ok = false; break; }
       AB200_FSTAMP(j, 0);
       tc_fence_after();
-      if constexpr (kNarrow) {
-        if (j == narrow_j) {      // 32 keys, first keys and nothing else that is seen
-          float x[32];
-          tmem_ld32f(s_addr, x);
-          tmem_wait_ld();
-          float mx = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            x[c] = n0 + c < p.sinks && n0 + c <= row_hi ? x[c] * p.qk_scale : -INFINITY;
-            mx = fmaxf(mx, x[c]);
-          }
-          float alpha = 1.f;
-          const bool grow = mx > m_used + kRescaleThreshold;
-          if (grow) {
-            alpha = ex2(m_used - mx);
-            m_used = mx;
-          }
-          if (j > 0 && __any_sync(0xffffffffu, grow) && !rescale(alpha, j)) { ok = false; break; }
-          const float m_safe = (m_used == -INFINITY) ? 0.f : m_used;
-          float sum = 0.f;
-          uint32_t pk[16];
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float e0 = ex2(x[2 * c] - m_safe), e1 = ex2(x[2 * c + 1] - m_safe);
-            sum += e0 + e1;
-            pk[c] = pack2<T>(e0, e1);
-          }
-          l = l * alpha + sum;
-          tmem_st16(s_addr, pk);
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&bars[L::bPHalf + t]);
-            mbar_arrive(&bars[L::bPFull + t]);
-          }
-          continue;
-        }
-      }
       float sc[128];
       if (bias_on) {      // (a tile at a time: bias and scores of the whole block are more registers than there are)
 #pragma unroll
@@ -599,7 +529,23 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
         alpha = ex2(m_used - mx);                            // m_used == -inf -> 0
         m_used = mx;
       }
-      if (j > 0 && __any_sync(0xffffffffu, grow) && !rescale(alpha, j)) { ok = false; break; }
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        // O must be complete up to block j-1 before it is rescaled.
+        // (S of block j was issued behind P V of block j-1, so this wait returns at once.)
+        if (!mbar_wait(&bars[L::bPvDone + t], (uint32_t)(j - 1) & 1u, abort_flag, status, 0x800 + 2 * j + t)) { ok = false; break; }
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          if (c * 32 >= p.dvo) break;          // columns the P V product never writes
+          uint32_t o[32];
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(o_addr + c * 32, o);
+        }
+        tmem_wait_st();
+      }
       AB200_FSTAMP(j, 3);
       l *= alpha;
       const float m_safe = (m_used == -INFINITY) ? 0.f : m_used;
@@ -749,7 +695,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, L::kTmemCols);
+    tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
@@ -779,6 +725,7 @@ cudaError_t fwd_device_facts(int* dev, unsigned int** status, int* sms, bool* re
 }
 
 #include "sm100_fwd_decode.cuh"
+#include "sm100_fwd_sink.cuh"
 
 inline bool exact_tiles(const Params& p, int hd) {
   return p.varlen_mode == 0 && p.max_sq % 128 == 0 && p.max_sk % 128 == 0 && p.dqk == hd && p.dvo == hd;
@@ -786,10 +733,15 @@ inline bool exact_tiles(const Params& p, int hd) {
 
 template <typename T, int HD, bool EXACT, int FEAT>
 cudaError_t launch_fwd_TE(const Params& p, cudaStream_t st) {
-  using L = FwdSmem<HD, FEAT>;
+  constexpr bool kSink = (FEAT & kSinks) != 0 && HD <= 128;      // sm100_fwd_sink.cuh
+  constexpr int kRows = kSink ? kBM : FwdSmem<HD>::kCtaRows, kKeys = kSink ? kSinkBN : kBN, kBytes = kSink ? SinkSmem<HD>::kDynamic : FwdSmem<HD>::kDynamic;
+  const auto kern = [] {
+    if constexpr (kSink) return sm100_fwd_sink_kernel<T, HD, EXACT>;
+    else return sm100_fwd_kernel<T, HD, EXACT, FEAT>;
+  }();
   CUtensorMap tq, tk, tv;
-  if (!make_tile_map_16bit(&tq, p.q, p.dqk, p.q.n[2], kBM) || !make_tile_map_16bit(&tk, p.k, p.dqk, p.k.n[2], kBN) ||
-      !make_tile_map_16bit(&tv, p.v, p.dvo, p.v.n[2], kBN))
+  if (!make_tile_map_16bit(&tq, p.q, p.dqk, p.q.n[2], kBM) || !make_tile_map_16bit(&tk, p.k, p.dqk, p.k.n[2], kKeys) ||
+      !make_tile_map_16bit(&tv, p.v, p.dvo, p.v.n[2], kKeys))
     return cudaErrorInvalidValue;
   static std::atomic<bool> attr_set[64];
   int dev = 0;
@@ -798,16 +750,16 @@ cudaError_t launch_fwd_TE(const Params& p, cudaStream_t st) {
   cudaError_t e = fwd_device_facts(&dev, &status, nullptr, &remember);
   if (e != cudaSuccess) return e;
   if (!remember || !attr_set[dev].load(std::memory_order_acquire)) {
-    e = host().func_set_smem(reinterpret_cast<const void*>(sm100_fwd_kernel<T, HD, EXACT, FEAT>), L::kDynamic);
+    e = host().func_set_smem(reinterpret_cast<const void*>(kern), kBytes);
     if (e != cudaSuccess) return e;
     if (remember) attr_set[dev].store(true, std::memory_order_release);
   }
-  dim3 grid((p.max_sq + L::kCtaRows - 1) / L::kCtaRows, p.hq, p.batch);
+  dim3 grid((p.max_sq + kRows - 1) / kRows, p.hq, p.batch);
   Params pp = p;
-  pp.packed_tiles = packed_tiles_bound(p, L::kCtaRows);
+  pp.packed_tiles = packed_tiles_bound(p, kRows);
   if (pp.packed_tiles > 0) grid = dim3(pp.packed_tiles * p.hq);
   pp.hw_order = (int64_t)grid.x * grid.y * grid.z >= 1 << 24;
-  e = launch_kernel(sm100_fwd_kernel<T, HD, EXACT, FEAT>, grid, dim3(L::kThreads), L::kDynamic, st, pp, tq, tk, tv, status);
+  e = launch_kernel(kern, grid, dim3(kSink ? kSinkThreads : kFwdThreads), kBytes, st, pp, tq, tk, tv, status);
   if (e == cudaSuccess) count_launch();
   return e;
 }
