@@ -12,8 +12,9 @@
 // Tensor memory (256 columns): S0 [0,64)  S1 [64,128)  O [128,128+HD); P (32 packed columns) over its S.  Shared memory: Q, two stages each of K and V.
 // order on the tensor pipe:  S_0 S_1 | O += P_0 V_0, S_2 | O += P_1 V_1, S_3 | ...
 // Measured on the device, bf16, 1 x 32:8 heads x 8192 of 128, 4 first keys, us, two tiles to a CTA / one with blocks of 128 keys / this: window 2048
-// 310 / 282 / 249, 1024 229 / 192 / 167 (0.98 PFLOP/s of products that are issued), 512 151 / 140 / 122, 128 101 / 95 / 85.  What is left is the softmax:
-// 64 exponentials a row and step beside its products.  CTAs that stay and walk over the tiles (the next Q loaded under the last blocks, O staged beside
+// 310 / 282 / 249, 1024 229 / 192 / 167 (0.98 PFLOP/s of products that are issued), 512 151 / 140 / 122, 128 101 / 95 / 85.  At window 1024 the tensor pipe and the
+// exponential unit are each busy 45% of the time (56% in the tile kernel on a long row), L2 27%: what is left is a step's chain in a softmax warp, loads
+// from tensor memory, maximum, exponentials, store, of which two warps a scheduler overlap.  CTAs that stay and walk over the tiles (the next Q loaded under the last blocks, O staged beside
 // it) came out 1 to 5% slower: the second CTA of the SM covers a start as well, and the hardware hands tiles out in the order they end.
 // Every wait is bounded.
 
@@ -231,7 +232,9 @@ sm100_fwd_sink_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     for (int j = 0; j < nblk; ++j) {
       const int n0 = block(j) * kBlk;
       const uint32_t s_addr = lane_addr + (uint32_t)(j & 1) * kBlk;
-      if (!mbar_wait(&bars[L::bSFull + (j & 1)], (uint32_t)(j >> 1) & 1u, abort_flag, status, 0x700 + j)) { ok = false; break; }
+      // (a vote: the warp leaves as a whole)
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars[L::bSFull + (j & 1)], (uint32_t)(j >> 1) & 1u, abort_flag, status, 0x700 + j)) != 0;
+      if (!ok) break;
       tc_fence_after();
       float sc[kBlk];
       tmem_ld32f(s_addr, sc);
@@ -275,7 +278,8 @@ sm100_fwd_sink_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         m_used = mx;
       }
       if (j > 0 && __any_sync(0xffffffffu, grow)) {      // O must be complete up to block j-1 before it is rescaled
-        if (!mbar_wait(&bars[L::bPvDone + ((j - 1) & 1)], (uint32_t)((j - 1) >> 1) & 1u, abort_flag, status, 0x800 + j)) { ok = false; break; }
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars[L::bPvDone + ((j - 1) & 1)], (uint32_t)((j - 1) >> 1) & 1u, abort_flag, status, 0x800 + j)) != 0;
+        if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
@@ -310,7 +314,7 @@ sm100_fwd_sink_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       if (lane == 0) mbar_arrive(&bars[L::bPFull + (j & 1)]);
     }
     // ---- epilogue: as in the tile kernel, through the (now idle) Q tile ----------------
-    if (ok) ok = mbar_wait(&bars[L::bPvDone + ((nblk - 1) & 1)], (uint32_t)((nblk - 1) >> 1) & 1u, abort_flag, status, 0x900);
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&bars[L::bPvDone + ((nblk - 1) & 1)], (uint32_t)((nblk - 1) >> 1) & 1u, abort_flag, status, 0x900)) != 0;
     if (ok) {
       tc_fence_after();
       const float inv = (l > 0.f) ? 1.f / l : 0.f;
