@@ -5,7 +5,8 @@ API of ROCm/aotriton.
   aotriton_b200.flash     attn_fwd / attn_bwd / varlen / debug helpers over the pyaotriton
                           bindings, argument-for-argument like the reference's
                           modules/flash/tests/aotriton_flash.py
-  aotriton_b200.autograd  torch.autograd.Function wrappers (attention, varlen_attention)
+  aotriton_b200.autograd  torch.autograd.Function wrappers (attention, varlen_attention; sink_attention,
+                          varlen_sink_attention, relative_position_bias, dropout)
   aotriton_b200.sharding  batch x head partitioning for multi-GPU runs
   aotriton_b200.build     in-tree nvcc build
 

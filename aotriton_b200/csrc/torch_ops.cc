@@ -1,5 +1,5 @@
 // The autograd entry points' native route: attention on ordinary torch tensors, forward and backward, without Python in
-// between.  Outputs, gradients and scratch come from torch's caching allocator, launches go to torch's current stream
+// between; in the same way sink attention, the relative position bias and dropout of hidden states.  Outputs, gradients and scratch come from torch's caching allocator, launches go to torch's current stream
 // through the C++ operator API (include/aotriton/flash.h), the backward is a torch::autograd::Function: version checks and CUDA-graph
 // capture see what they see of the Python Function, saved-tensor hooks the inputs, the output and the log-sum-exp.
 //
