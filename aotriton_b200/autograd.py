@@ -369,9 +369,7 @@ class _SinkAttentionGrad(torch.autograd.Function):
         if not q.numel() or not k.numel() or not v.numel():
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
         do = do if do.stride(-1) == 1 else do.contiguous()
-        # (a padded batch's rows behind their sequences have gradient zero)
-        make = torch.zeros_like if varlen == cabi.VARLEN_PADDED else torch.empty_like
-        dq, dk, dv = make(q), make(k), make(v)
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         delta = torch.empty_like(lse)
         kw = _sink_problem(cu_q, cu_k, max_q, max_k, varlen, sm_scale)
         args = (q, k, v, o, do, dq, dk, dv, lse, delta, window, sinks)
@@ -442,7 +440,7 @@ def varlen_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max
                           varlen_type="compact"):
     """sink_attention over sequences of different lengths, each with its own positions.  varlen_type "compact": token-packed (1, H, tokens, D)
     tensors, as for varlen_attention.  "padded": (B, H, S, D) tensors, such as a batch of caches, sequence z having the first
-    cu_seqlens[z + 1] - cu_seqlens[z] tokens of its row; what lies behind them is not looked at, output rows behind the last query are
+    cu_seqlens[z + 1] - cu_seqlens[z] tokens of its row.  Of either, what lies behind the sequences is not looked at, output rows there are
     zero (log-sum-exp +inf) and gradients there are zero.  max_seqlen_q and _k are at least the longest lengths."""
     if varlen_type not in ("compact", "padded"):
         raise ValueError(f"varlen_sink_attention: varlen_type {varlen_type!r} is not \"compact\" or \"padded\"")

@@ -827,6 +827,7 @@ int ab200_sink_attn_fwd(const ab200_attn_fwd_args* a, int32_t window, int32_t si
   if (sel < 0) return -sel;
   const bool tc = (sel & 0xff) >= kVarTcgen05;
   t_last_fwd = tc ? 2 : 1;
+  if (const cudaError_t e = launch_rows_behind(a->prob.dtype, p, false, st)) return (int)e;
   return (int)(tc ? launch_sm100_fwd(a->prob.dtype, p, st) : launch_general(0, a->prob.dtype, p, st));
 }
 
@@ -877,7 +878,8 @@ int ab200_sink_attn_bwd(const ab200_attn_bwd_args* a, int32_t window, int32_t si
     p.sink_partial = workspace;
     p.ticket = reinterpret_cast<unsigned int*>(workspace + floats - kTicketFloats);
   }
-  cudaError_t e = launch_preprocess(dtype, p, st);
+  cudaError_t e = launch_rows_behind(dtype, p, true, st);
+  if (e == cudaSuccess) e = launch_preprocess(dtype, p, st);
   if (e != cudaSuccess) return (int)e;
   const bool tc = (sel & 0xff) >= kVarTcgen05;
   t_last_bwd = tc ? 2 : 1;

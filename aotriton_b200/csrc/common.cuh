@@ -130,6 +130,8 @@ __device__ __forceinline__ Seq resolve_seq(const Params& p, int z) {
 // A window that moves with the queries, aligned to the last key, and the first keys.  The kernels walk the blocks the window
 // reaches as for any window, and before them the blocks of first keys that lie wholly in front of it; only a block with first keys
 // in it pays for a second comparison.  In dK/dV a first key is one whose window has no end.
+// Sequences next to each other.  Their log-sum-exp has a row for each of q's tokens, those behind the last sequence too.
+__host__ __device__ __forceinline__ bool compact(const Params& p) { return p.varlen_mode != 0 && p.varlen_mode != 2 && p.ss_q == nullptr; }
 template <int FEAT>
 __device__ __forceinline__ Seq seq_for(const Params& p, int z, int4 ends) {
   Seq s = seq_from_ends(p, z, ends);
@@ -137,6 +139,7 @@ __device__ __forceinline__ Seq seq_for(const Params& p, int z, int4 ends) {
     s.wr = s.sk - s.sq;
     const int64_t wl = (int64_t)p.sink_window - 1 - s.wr;
     s.wl = (int)(wl > 0x7fffffffLL ? 0x7fffffffLL : (wl < -0x7fffffffLL ? -0x7fffffffLL : wl));
+    if (compact(p)) s.lse_row = p.q.n[2];
   }
   return s;
 }

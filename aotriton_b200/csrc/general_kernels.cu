@@ -396,7 +396,8 @@ __global__ void __launch_bounds__(256) bwd_preprocess_kernel(const __grid_consta
   constexpr int kWarpRows = 16, kPer = 16 / (int)sizeof(T);      // elements of a 16-byte load
   const int z = blockIdx.z, h = blockIdx.y;
   if (p.ticket != nullptr && blockIdx.x == 0 && h == 0 && z == 0 && threadIdx.x == 0) *p.ticket = 0u;
-  const Seq sq = resolve_seq(p, z);
+  Seq sq = resolve_seq(p, z);
+  if (p.sink_on && compact(p)) sq.lse_row = p.q.n[2];      // (as in seq_for)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int d = p.dvo;
   const int wrow0 = ((int)blockIdx.x * 8 + warp) * kWarpRows;
@@ -639,6 +640,66 @@ cudaError_t launch_preprocess(int dtype, const Params& p, cudaStream_t st) {
     case 3: e = launch_kernel(bwd_preprocess_kernel<__nv_bfloat16>, dim3(grid), dim3(256), 0, st, p); break;
     default: return cudaErrorInvalidValue;
   }
+  if (e == cudaSuccess) count_launch();
+  return e;
+}
+
+// Sink attention: what lies behind the sequences of a packed or padded batch, whose end only the device knows.  Zeros for O (log-sum-exp +inf) or the
+// gradients: the tensors are a caller's fresh ones as a rule, and garbage there would reach a layer's weights.  A few CTAs for each tensor and, padded, each
+// sequence; a packed batch without such tokens costs a launch that finds nothing.
+struct Behind {
+  View4 t[3];                    // extents and strides in units of `bytes` each
+  int32_t bytes[3];
+  const int32_t* cu[3];
+  float* lse;                    // beside t[0]; or null
+  int32_t batch, padded;
+};
+template <typename U>
+__device__ void zero_rows(const View4& t, int64_t b, int64_t from) {
+  const int64_t d = t.n[3], rows = t.n[2] - from, all = rows * d * t.n[1];
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / d, h = r / rows;
+    reinterpret_cast<U*>(t.ptr)[b * t.s[0] + h * t.s[1] + (from + (r - h * rows)) * t.s[2] + (i - r * d)] = U{};
+  }
+}
+// grid = (16, tensors, padded ? sequences : 1)
+__global__ void __launch_bounds__(256) rows_behind_kernel(const __grid_constant__ Behind a) {
+  wait_for_earlier_grids();
+  const int y = blockIdx.y, z = blockIdx.z;
+  const View4& t = a.t[y];
+  const int64_t from = a.padded ? a.cu[y][z + 1] - a.cu[y][z] : a.cu[y][a.batch];
+  if (from < 0 || from >= t.n[2]) return;
+  if (a.bytes[y] == 16) zero_rows<uint4>(t, z, from);
+  else if (a.bytes[y] == 4) zero_rows<uint32_t>(t, z, from);
+  else zero_rows<uint16_t>(t, z, from);
+  if (y == 0 && a.lse != nullptr) {
+    const int64_t rows = t.n[2] - from;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < rows * t.n[1]; i += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t h = i / rows;
+      a.lse[h * t.n[2] + from + (i - h * rows)] = INFINITY;
+    }
+  }
+}
+cudaError_t launch_rows_behind(int dtype, const Params& p, bool backward, cudaStream_t st) {
+  if (p.batch <= 0 || !(compact(p) || (backward && p.varlen_mode == 2))) return cudaSuccess;      // (the padded forward does it by itself)
+  const View4* t[3] = {backward ? &p.dq : &p.out, &p.dk, &p.dv};
+  const int count = backward ? 3 : 1, size = dtype == 1 ? 4 : 2;
+  Behind a{};
+  a.batch = p.batch;
+  a.padded = p.varlen_mode == 2;
+  a.lse = backward ? nullptr : p.lse;
+  for (int i = 0; i < count; ++i) {
+    View4& v = a.t[i] = *t[i];
+    a.cu[i] = i == 0 ? p.cu_q : p.cu_k;
+    const int64_t per = 16 / size;
+    const bool wide = reinterpret_cast<uintptr_t>(v.ptr) % 16 == 0 && v.n[3] % per == 0 && v.s[0] % per == 0 && v.s[1] % per == 0 && v.s[2] % per == 0;
+    a.bytes[i] = wide ? 16 : size;
+    if (wide) {
+      v.n[3] /= per;
+      for (int j = 0; j < 3; ++j) v.s[j] /= per;
+    }
+  }
+  const cudaError_t e = launch_kernel(rows_behind_kernel, dim3(16, count, a.padded ? p.batch : 1), dim3(256), 0, st, a);
   if (e == cudaSuccess) count_launch();
   return e;
 }

@@ -76,6 +76,8 @@ cudaError_t launch_kernel(A&&... a) { return launch_kernel_as<true>(std::forward
 // ab200_dtype value.
 cudaError_t launch_general(int which, int dtype, const Params& p, cudaStream_t st);
 cudaError_t launch_preprocess(int dtype, const Params& p, cudaStream_t st);
+// Sink attention: zeros behind the sequences of a packed or padded batch (`backward`: in the gradients).
+cudaError_t launch_rows_behind(int dtype, const Params& p, bool backward, cudaStream_t st);
 cudaError_t launch_dropout_sign(int dtype, const View4& r, int batch, int heads, int rows, int cols, float dropout_p,
                                 const uint64_t* seed, const uint64_t* off1, uint64_t off2, cudaStream_t st);
 

@@ -379,11 +379,9 @@ struct SinkAttend : torch::autograd::Function<SinkAttend> {
       return r;
     }
     if (dout.stride(-1) != 1) dout = dout.contiguous();
-    // (a padded batch's rows behind their sequences have gradient zero)
-    auto make = [&](const Tensor& t) { return c.varlen == AB200_VARLEN_PADDED ? at::zeros_like(t) : gradient_of(t); };
-    r[0] = make(q);
-    r[1] = make(k);
-    r[2] = make(v);
+    r[0] = gradient_of(q);
+    r[1] = gradient_of(k);
+    r[2] = gradient_of(v);
     const Tensor delta = fresh(lse.sizes(), at::kFloat);
     ab200_attn_bwd_args a{};
     a.prob = sink_problem(c, q, k, v, cu_q, cu_k);

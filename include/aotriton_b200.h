@@ -195,7 +195,8 @@ AB200_API int ab200_debug_simulate_encoded_softmax(const ab200_view4* r, int32_t
 /* Attention with a sliding window and a few first keys that stay visible.  Query m of a sequence of sq queries and sk keys stands at key
  * P = m + sk - sq and sees the keys n <= P with n > P - window or n < sinks; window >= 1, sinks >= 0, max_seqlen_q and _k >= 1.  Arguments, layouts and
  * types as in ab200_attn_fwd / ab200_attn_bwd, without bias, dropout and encoded_softmax; the problem's causal and window fields are not
- * looked at.  Differences: rows of a padded batch behind a sequence's last query get O = 0 and LSE = +inf in the forward; keys that no query of
+ * looked at.  Differences: rows behind the last query of a padded batch's sequence, or of a packed batch, get O = 0 and LSE = +inf, and zero
+ * gradients (up to max_seqlen_q in a padded batch's forward, else up to the views' sizes; packed tokens' LSE and delta have rows of q.size[2]); keys that no query of
  * the sequence sees (between the first ones and the first query's window) may hold anything, NaN included, without touching the outputs
  * and dq of fp16 and bf16 tensors with head dims up to 256 that are multiples of 8. */
 AB200_API int ab200_sink_attn_fwd(const ab200_attn_fwd_args* args, int32_t window, int32_t sinks, void* stream);

@@ -264,3 +264,43 @@ def test_long_cache_offsets():
     values, bounds = reference(q, near_k, near_v, window + sinks, 0, D ** -0.5)
     check("out", out, values, bounds)
     _healthy()
+
+
+@pytest.mark.parametrize("dt,D,layout", [(BF16, 128, "bshd"), (F16, 64, "bhsd"), (F16, 256, "bshd"), (F32, 64, "bshd"), (F32, 160, "bhsd"), (BF16, 60, "bshd")])
+@pytest.mark.parametrize("lens_q,lens_k", [([200, 7, 128], None), ([1, 1, 1], [300, 90, 1]), ([0, 0], [0, 0])])
+def test_packed_with_room_behind(lens_q, lens_k, dt, D, layout):
+    """Tokens behind the last sequence, as where buffers have one size for all batches: NaN there reaches nothing, and comes out as zero."""
+    from aotriton_b200 import autograd
+    lens_k = lens_k or lens_q
+    Hq, Hk, window, sinks, room = 4, 2, 60, 6, 75
+    tq, tk = sum(lens_q), sum(lens_k)
+    q, k, v, do = _rand((1, Hq, tq + room, D), (1, Hk, tk + room, D), (1, Hk, tk + room, D), (1, Hq, tq + room, D), dt=dt, seed=tq, layout=layout)
+    for t, n in ((q, tq), (k, tk), (v, tk), (do, tq)):
+        t[:, :, n:] = float("nan")
+    for t in (q, k, v):
+        t.requires_grad_()
+    max_q, max_k = max(*lens_q, 1), max(*lens_k, 1)
+    args = (_ends(lens_q), _ends(lens_k), max_q, max_k, window, sinks)
+    junk = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(8)]      # (what fresh tensors may hold)
+    del junk
+    for native in (True, False):
+        if native:
+            out, lse = autograd.varlen_sink_attention(q, k, v, *args, return_lse=True)
+        else:
+            out, lse = autograd._SinkAttention.apply(q, k, v, *args, D ** -0.5, True, 1)
+        grads = torch.autograd.grad(out, (q, k, v), do)
+        assert lse.shape == (Hq, tq + room)
+        assert bool((out[:, :, tq:] == 0).all()) and bool((lse[:, tq:] == float("inf")).all())
+        assert all(bool((t[:, :, n:] == 0).all()) for t, n in zip(grads, (tq, tk, tk)))
+        at_q = at_k = 0
+        for nq, nk in zip(lens_q, lens_k):
+            sl_q, sl_k = slice(at_q, at_q + nq), slice(at_k, at_k + nk)
+            at_q, at_k = at_q + nq, at_k + nk
+            if not nq:
+                continue
+            part = [t.detach()[:, :, sl] for t, sl in ((q, sl_q), (k, sl_k), (v, sl_k))]
+            values, bounds = reference(*part, window, sinks, D ** -0.5, do[:, :, sl_q])
+            for name, got in (("out", out.detach()[:, :, sl_q]), ("lse", lse[:, sl_q]), ("dq", grads[0][:, :, sl_q]), ("dk", grads[1][:, :, sl_k]),
+                              ("dv", grads[2][:, :, sl_k])):
+                check(name, got, values, bounds)
+    _healthy()
