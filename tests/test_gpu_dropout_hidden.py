@@ -144,3 +144,19 @@ def test_in_place_and_beside():
     assert torch.equal(view, want)
     view.fill_(7.0)
     assert bool((store == 7.0).all())
+
+
+@pytest.mark.parametrize("cols", [4096, 4093])
+def test_offsets_beyond_32_bits(cols):
+    """More than 2^31 elements: the last rows, forward and backward."""
+    from aotriton_b200 import autograd
+    n, p, seed = (2 ** 31 // cols + 40) // 4 * 4, 0.3, 7
+    x = torch.zeros(n, cols, device="cuda", dtype=BF16)
+    x[-4:] = torch.randn(4, cols, device="cuda").to(BF16)
+    x.requires_grad_()
+    y = autograd.dropout(x, p, philox_seed=seed, philox_offset=0)
+    first = (n - 4) * cols      # (a multiple of four: the rows start at a counter)
+    keep = O.dropout_keep(4 * cols, p, seed, first // 4)
+    _check(y.detach()[-4:], x.detach()[-4:], None, keep, p)
+    dx, = torch.autograd.grad(y, x, x.detach())
+    assert torch.equal(dx, y.detach())

@@ -168,3 +168,19 @@ def test_empty():
         assert bias.shape == (b, 4, sq, sk)
         got, = torch.autograd.grad(bias, t, torch.ones_like(bias))
         assert bool((got == 0).all())
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 entries: what the last rows hold, and a gradient that only they have."""
+    from aotriton_b200 import autograd
+    S, buckets, far, rows = 50001, 32, 128, 3
+    table = torch.randn(buckets, 1, device="cuda").to(BF16).requires_grad_()
+    bias = autograd.relative_position_bias(table, S, S, max_distance=far)
+    where = O.bucket_matrix(rows, S, buckets, far, True, S - rows)
+    assert torch.equal(bias[0, 0, -rows:].detach().cpu(), table.detach().cpu()[where][..., 0])
+    grad = torch.zeros(1, 1, S, S, device="cuda", dtype=BF16)
+    last = torch.randint(-1, 2, (rows, S), generator=torch.Generator().manual_seed(3))
+    grad[0, 0, -rows:] = last.to(BF16).cuda()
+    got, = torch.autograd.grad(bias, table, grad)
+    want = O.relative_bias_grad(last[None, None], where, buckets)      # (whole numbers, rounded once)
+    assert torch.equal(got.cpu(), want.to(BF16))
