@@ -126,6 +126,79 @@ __device__ __forceinline__ void tile_dots(float (&s)[4][Tiled<DP>::kNC], const f
     for (int j = 0; j < C::kNC; ++j) s[i][j] = t[i][j].x + t[i][j].y;
 }
 
+// Sink attention: tile_dots of the column groups [g0, g1) that some row of the warp's eight sees, the others zero.  A window of a hundred keys is a
+// few blocks of which a warp sees half the columns, and a block of first keys holds a handful.  One or two groups at a time: with
+// one, shared-memory reads are the bound (24 clocks of an SM a step, where four groups take 64 of arithmetic), with two about equal.
+// Device us, whole blocks / this, fp32, forward and backward: 2 x 8 x 500 of 64, window 100, 86.0 / 81.6; forward alone 26.4 / 24.5, 4 x 8:2 x 1000 of 128
+// 112.6 / 98.3, 2 x 8 x 1000 of 64 window 30 36.9 / 30.7, window 400 no change.
+template <int DP, int N>
+__device__ __forceinline__ void group_dots(float (&s)[4][Tiled<DP>::kNC], const float* A, const float* B, int d4, int ty, int tx, int g0) {
+  using C = Tiled<DP>;
+  float2 t[4][N];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) t[i][j] = make_float2(0.f, 0.f);
+  const float* a0 = A + ty * 4 * C::kLd;
+  const float* b0 = B + (tx + 16 * g0) * C::kLd;
+#pragma unroll 2
+  for (int c = 0; c < d4; ++c) {
+    float4 b[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) b[j] = *reinterpret_cast<const float4*>(b0 + j * 16 * C::kLd + c * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float4 a = *reinterpret_cast<const float4*>(a0 + i * C::kLd + c * 4);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        t[i][j] = ptx::fma2(make_float2(a.x, a.y), make_float2(b[j].x, b[j].y), t[i][j]);
+        t[i][j] = ptx::fma2(make_float2(a.z, a.w), make_float2(b[j].z, b[j].w), t[i][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < C::kNC; ++j) {
+      s[i][j] = 0.f;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (j == g0 + n) s[i][j] = t[i][n].x + t[i][n].y;
+    }
+}
+template <int DP, int FEAT>
+__device__ __forceinline__ void seen_dots(float (&s)[4][Tiled<DP>::kNC], const float* A, const float* B, int d4, int ty, int tx, int g0, int g1) {
+  using C = Tiled<DP>;
+  if constexpr ((FEAT & kSinks) != 0) {
+    if (g1 - g0 == 1) { group_dots<DP, 1>(s, A, B, d4, ty, tx, g0); return; }
+    if (C::kNC > 2 && g1 - g0 == 2) { group_dots<DP, 2>(s, A, B, d4, ty, tx, g0); return; }
+    if (g1 <= g0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < C::kNC; ++j) s[i][j] = 0.f;
+      return;
+    }
+  }
+  tile_dots<DP>(s, A, B, d4, ty, tx);
+}
+// The groups of 16 columns of the block at col0 that hold any of the columns [lo, hi], or of the first `sinks` up to hi.
+template <int DP, int FEAT>
+__device__ __forceinline__ void seen_groups(int lo, int hi, int col0, int sinks, int& g0, int& g1) {
+  g0 = g1 = 0;
+  if constexpr ((FEAT & kSinks) != 0) {
+    int first = max(lo - col0, 0), last = min(hi - col0, Tiled<DP>::kBN - 1);
+    if (col0 < sinks && hi >= col0) {
+      if (first > last) last = min(sinks - 1 - col0, last);      // the window is behind this block
+      first = 0;
+    }
+    if (first <= last) {
+      g0 = first >> 4;
+      g1 = (last >> 4) + 1;
+    }
+  }
+}
+
 // The part [k0, k1) of the block of BN columns at `col0` that some row of the warp's eight sees (columns lo..hi), k0
 // rounded down to eight.  The accumulations stop there.  A masked pair's weight is zero, but zero times a non-finite row
 // of X is not: a row must not depend on rows that neither it nor its neighbours in the warp see.  (The 16x16-tile
@@ -314,7 +387,9 @@ __global__ void __launch_bounds__(kFwdGroups * 128, 2) tiled_fwd_kernel(const __
     group_sync();       // K has landed, the previous block's V has been read
     stage_tile<T, DP, C::kBN, 128>(Vs, p.v, sq.bidx, hk, sq.k0, n0, sq.sk, p.dvo, vvec, tid);
     float s[4][C::kNC];
-    tile_dots<DP>(s, Qs, Ks, d4, ty, tx);
+    int g0, g1;
+    seen_groups<DP, FEAT>(w_lo, w_hi, n0, p.sinks, g0, g1);
+    seen_dots<DP, FEAT>(s, Qs, Ks, d4, ty, tx, g0, g1);
     const uint32_t keep = p.dropout_on ? tile_keep_bits<C::kNC>(dctx, m0 + ty * 4, n0, tx) : 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -488,10 +563,12 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
       const bool more = i + SPLIT < total;
       const int next_h = hk * p.group + g, next_m0 = first + mb * C::kBN;
       float s[4][C::kNC], dp[4][C::kNC];
-      tile_dots<DP>(dp, Vs, dOs, dv4, ty, tx);
+      int g0, g1;
+      seen_groups<DP, FEAT>(w_lo, w_hi, m0, 0, g0, g1);
+      seen_dots<DP, FEAT>(dp, Vs, dOs, dv4, ty, tx, g0, g1);
       stage_wait<0>();
       __syncthreads();      // K, Q, logsumexp and delta are there
-      tile_dots<DP>(s, Ks, Qs, dq4, ty, tx);
+      seen_dots<DP, FEAT>(s, Ks, Qs, dq4, ty, tx, g0, g1);
 #pragma unroll
       for (int j = 0; j < C::kNC; ++j) {
         const int c = tx + 16 * j, m = m0 + c;
@@ -610,11 +687,13 @@ __device__ __forceinline__ void tiled_bwd_dq(const Params& p, float* smem, int z
     const int next = walk.next(n0, SPLIT);
     const bool more = next <= n_hi;
     float s[4][C::kNC], dp[4][C::kNC];
-    tile_dots<DP>(dp, dOs, Vs, dv4, ty, tx);
+    int g0, g1;
+    seen_groups<DP, FEAT>(w_lo, w_hi, n0, p.sinks, g0, g1);
+    seen_dots<DP, FEAT>(dp, dOs, Vs, dv4, ty, tx, g0, g1);
     stage_wait<0>();
     __syncthreads();      // V has been read, K (and Q) is there
     if (more) stage_v(next);
-    tile_dots<DP>(s, Qs, Ks, dq4, ty, tx);
+    seen_dots<DP, FEAT>(s, Qs, Ks, dq4, ty, tx, g0, g1);
     const uint32_t keep = p.dropout_on ? tile_keep_bits<C::kNC>(dctx, m0 + ty * 4, n0, tx) : 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
