@@ -838,7 +838,13 @@ constexpr int kTicketFloats = 4;
 static int64_t plan_sink_bwd(const ab200_attn_bwd_args* a, Params& p, int* sel) {
   *sel = ab200_select_variant(kOpBwd, a->prob.dtype, p.dqk, p.dvo,
                               family_flags(g_family) | (sm100_bwd_supported(a->prob.dtype, p) ? AB200_SELECT_ALIGNED : 0));
-  if (*sel < 0 || (*sel & 0xff) < kVarTcgen05 || p.dqk > 128 || p.dvo > 128) return 0;
+  auto partials = [&] { return p.sink_chunks > 0 ? (int64_t)p.batch * p.hk * (p.sink_chunks + 1) * p.sinks * (p.dqk + p.dvo) : 0; };
+  if (*sel < 0) return 0;
+  if ((*sel & 0xff) < kVarTcgen05) {
+    p.sink_chunks = general_sink_chunks(p);
+    return partials();
+  }
+  if (p.dqk > 128 || p.dvo > 128) return 0;
   if (p.sinks == 0) return kTicketFloats;
   // as many query blocks to an item as a window's worth gives the other key blocks, eight at least
   const int64_t all = ((int64_t)p.max_sq + 127) / 128 * p.group, own = ((int64_t)p.sink_window + 127) / 128 * p.group + p.group;
@@ -846,7 +852,7 @@ static int64_t plan_sink_bwd(const ab200_attn_bwd_args* a, Params& p, int* sel) 
   // (no more than fill the chip a few times over: each costs a row of partial sums for every first key)
   const int64_t blocks = (int64_t)p.batch * p.hk * ((p.sinks + 127) / 128), most = blocks > 0 ? (592 + blocks - 1) / blocks : 1;
   p.sink_chunks = (int)std::min<int64_t>(std::min<int64_t>(64, most), (all + each - 1) / each);
-  return (int64_t)p.batch * p.hk * (p.sink_chunks + 1) * p.sinks * (p.dqk + p.dvo) + kTicketFloats;
+  return partials() + kTicketFloats;
 }
 
 int64_t ab200_sink_attn_bwd_workspace(const ab200_attn_bwd_args* a, int32_t window, int32_t sinks, void* stream) {
@@ -876,12 +882,12 @@ int ab200_sink_attn_bwd(const ab200_attn_bwd_args* a, int32_t window, int32_t si
   if (floats > 0) {
     if (workspace == nullptr || workspace_floats < (uint64_t)floats || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return kErrInvalidValue;
     p.sink_partial = workspace;
-    p.ticket = reinterpret_cast<unsigned int*>(workspace + floats - kTicketFloats);
   }
+  const bool tc = (sel & 0xff) >= kVarTcgen05;
+  if (tc && floats > 0) p.ticket = reinterpret_cast<unsigned int*>(workspace + floats - kTicketFloats);
   cudaError_t e = launch_rows_behind(dtype, p, true, st);
   if (e == cudaSuccess) e = launch_preprocess(dtype, p, st);
   if (e != cudaSuccess) return (int)e;
-  const bool tc = (sel & 0xff) >= kVarTcgen05;
   t_last_bwd = tc ? 2 : 1;
   if (tc) {
     if ((e = launch_sm100_bwd_dkdv(dtype, p, st)) != cudaSuccess) return (int)e;

@@ -78,7 +78,8 @@ struct Params {
 // dropout (generator state, keep bits) and bias (its tile, pointers, strides) need is spilled around every block even where a
 // call uses neither, so each combination has instantiations of its own.  kAll leaves everything to the run time (dBias without
 // bias too).
-enum : int { kPlain = 0, kBias = 1, kDropout = 2, kAll = 3, kSinks = 4 };      // bias, and its gradient or not; dropout; anything; sink attention
+enum : int { kPlain = 0, kBias = 1, kDropout = 2, kAll = 3, kSinks = 4,      // bias, and its gradient or not; dropout; anything; sink attention
+             kSharedSinks = 12 };      // ... whose first keys' queries several items share (register-tiled dK/dV)
 inline int features(const Params& p) {
   if (p.sink_on) return kSinks;
   if (p.has_dbias && !p.has_bias) return kAll;
@@ -181,6 +182,9 @@ __device__ __forceinline__ void mask_sink_columns(float* x, int first, int lo, i
 __device__ __forceinline__ float* sink_partial_row(const Params& p, int z, int hk, int chunk, int n) {
   return p.sink_partial + ((((int64_t)z * p.hk + hk) * (p.sink_chunks + 1) + chunk) * p.sinks + n) * (p.dqk + p.dvo);
 }
+
+// Items of dK/dV beside a key tile each (the kernels whose grids count them through): sink_chunks for every tile of `rows` keys with first ones.
+__host__ __device__ __forceinline__ int sink_items(const Params& p, int rows) { return (p.sinks + rows - 1) / rows * p.sink_chunks; }
 
 // Row tile `tile` of a token-packed batch, when the tiles of all sequences are counted through (within a
 // sequence the last rows, which a causal mask lets see the most keys, come first).  A grid of max_sq's tiles

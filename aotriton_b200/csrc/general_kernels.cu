@@ -16,6 +16,7 @@
 // Arithmetic follows ROCm/aotriton modules/flash/kernel/fwd_kernel_inner.py:126-277,
 // fwd_kernel.py:573-620, bwd_inner_dk_dv.py:117-256, bwd_inner_dq.py:117-205,
 // bwd_preprocess.py:118-133 and dropout_rng.py:86-126.
+#include <algorithm>
 #include "common.cuh"
 #include "launch.h"
 #include "sm100_ptx.cuh"
@@ -574,33 +575,64 @@ bool joint_backward(const Params& p) { return sizeof(T) != 2 || DP <= 64 || row_
 template <int DP>
 bool split_backward(const Params& p) { return row_tiles<DP>(p) < 1536; }
 
+// dK and dV of the first keys from the partial sums of the items that shared their queries, in the items' order.  grid = (sinks, Hk, batch)
+template <typename T>
+__global__ void __launch_bounds__(128) sink_finish_elements_kernel(const __grid_constant__ Params p) {
+  wait_for_earlier_grids();
+  const int n = blockIdx.x, hk = blockIdx.y, z = blockIdx.z;
+  const Seq sq = resolve_seq_for<kSinks>(p, z);
+  if (n >= sq.sk) return;
+  const int64_t step = (int64_t)p.sinks * (p.dqk + p.dvo);
+  for (int c = threadIdx.x; c < p.dqk + p.dvo; c += blockDim.x) {
+    const float* from = sink_partial_row(p, z, hk, 0, n) + c;
+    float sum = 0.f;
+#pragma unroll 4
+    for (int i = 0; i <= p.sink_chunks; ++i) sum += from[i * step];
+    if (c < p.dqk) row_ptr_mut<T>(p.dk, sq.bidx, hk, sq.k0 + n)[c] = from_f32<T>(sum * p.sm_scale);
+    else row_ptr_mut<T>(p.dv, sq.bidx, hk, sq.k0 + n)[c - p.dqk] = from_f32<T>(sum);
+  }
+}
+
+template <typename T, int DP>
+cudaError_t launch_tiled_T(int which, const Params& p, cudaStream_t st);
+
 template <typename T, int DP, int FEAT>
 cudaError_t launch_tiled_F(int which, const Params& p, cudaStream_t st) {
   using C = Tiled<DP>;
   if (which == 3 && !joint_backward<T, DP>(p)) {
-    const cudaError_t e = launch_tiled_F<T, DP, FEAT>(1, p, st);
-    return e != cudaSuccess ? e : launch_tiled_F<T, DP, FEAT>(2, p, st);
+    const cudaError_t e = launch_tiled_T<T, DP>(1, p, st);
+    return e != cudaSuccess ? e : launch_tiled_T<T, DP>(2, p, st);
   }
   const bool split = which != 0 && split_backward<DP>(p);
   const size_t rows = which == 0 ? C::kBM + kFwdGroups * 2 * C::kBN : 2 * C::kBM + 2 * C::kBN;      // staged rows of DP + 4 floats
   const size_t tiles = which == 0 ? kFwdGroups : (which & 1 ? 2 : 1);                              // P and dS, or one of them
   const size_t sm = (rows * C::kLd + tiles * C::kBM * C::kLdP + (which & 1 ? 2 * C::kBN : 0)) * sizeof(float);
-  auto kern = which == 0   ? tiled_fwd_kernel<T, DP, FEAT>
-              : which == 1 ? (split ? tiled_bwd_kernel<T, DP, 1, 2, FEAT> : tiled_bwd_kernel<T, DP, 1, 1, FEAT>)
-              : which == 2 ? (split ? tiled_bwd_kernel<T, DP, 2, 2, FEAT> : tiled_bwd_kernel<T, DP, 2, 1, FEAT>)
-                           : (split ? tiled_bwd_kernel<T, DP, 3, 2, FEAT> : tiled_bwd_kernel<T, DP, 3, 1, FEAT>);
+  const auto kern = [&] {
+    if constexpr (FEAT != kSharedSinks) {
+      if (which == 0) return tiled_fwd_kernel<T, DP, FEAT>;
+      if (which == 2) return split ? tiled_bwd_kernel<T, DP, 2, 2, FEAT> : tiled_bwd_kernel<T, DP, 2, 1, FEAT>;
+    }
+    if (which == 1) return split ? tiled_bwd_kernel<T, DP, 1, 2, FEAT> : tiled_bwd_kernel<T, DP, 1, 1, FEAT>;
+    return split ? tiled_bwd_kernel<T, DP, 3, 2, FEAT> : tiled_bwd_kernel<T, DP, 3, 1, FEAT>;
+  }();
   cudaError_t e = set_smem(kern, sm);
   if (e != cudaSuccess) return e;
   const int rows_total = which == 1 ? p.max_sk : (which == 3 && p.max_sk > p.max_sq ? p.max_sk : p.max_sq);
   const int blocks = (rows_total + C::kBM - 1) / C::kBM;
-  dim3 grid((which == 3 ? 2 : 1) * (split ? 2 : 1) * blocks, which == 1 ? p.hk : p.hq, p.batch);
+  const int extra = FEAT == kSharedSinks ? sink_items(p, C::kBM) : 0;
+  dim3 grid(((which == 3 ? 2 : 1) * blocks + extra) * (split ? 2 : 1), which == 1 ? p.hk : p.hq, p.batch);
   e = launch_kernel_as<false>(kern, grid, dim3(which == 0 ? kFwdGroups * C::kThreads : C::kThreads), sm, st, p);
   if (e == cudaSuccess) count_launch();
+  if (e == cudaSuccess && extra > 0) {
+    e = launch_kernel(sink_finish_elements_kernel<T>, dim3(p.sinks, p.hk, p.batch), dim3(128), 0, st, p);
+    if (e == cudaSuccess) count_launch();
+  }
   return e;
 }
 
 template <typename T, int DP>
 cudaError_t launch_tiled_T(int which, const Params& p, cudaStream_t st) {
+  if (p.sink_on && p.sink_chunks > 0 && (which & 1)) return launch_tiled_F<T, DP, kSharedSinks>(which, p, st);
   return p.sink_on ? launch_tiled_F<T, DP, kSinks>(which, p, st) : launch_tiled_F<T, DP, kPlain>(which, p, st);
 }
 
@@ -619,6 +651,29 @@ cudaError_t launch_general_D(int which, const Params& p, cudaStream_t st) {
 }
 
 }  // namespace
+
+// A first key's CTA walks over every query's block, those of other keys over a window's: shared out where that one takes eight blocks or more longer than the
+// chip needs for all of them, in pieces of a window's worth, four blocks at least, and no more than the chip has slots.
+// Device us of forward and backward, fp32, one CTA for all of a first key's queries / shared: 1 x 8:2 x 1024 of 64, window 64, 4 first keys 266 / 104; 4 x 8:2 x
+// 1000 of 128, window 100 585 / 463.  Shared below that rule: 2 x 8 x 500 of 64, window 100, 82 / 92.
+template <int DP>
+int tiled_sink_chunks(const Params& p) {
+  using C = Tiled<DP>;
+  const int64_t all = ((int64_t)p.max_sq + C::kBN - 1) / C::kBN * p.group, own = (((int64_t)p.sink_window + C::kBM) / C::kBN + 1) * p.group;
+  const int64_t slots = DP <= 64 ? 444 : 296, firsts = ((int64_t)p.sinks + C::kBM - 1) / C::kBM;
+  const auto rows = [](int n) { return ((int64_t)n + C::kBM - 1) / C::kBM; };
+  const int64_t steps = (int64_t)p.batch * p.hk * (rows(p.max_sq) + rows(p.max_sk)) * std::min(own, all);      // of dQ and of dK/dV, without the first keys
+  const int64_t tiles = (int64_t)p.batch * p.hk * firsts, each = std::max<int64_t>(own, 4);
+  if (all / (split_backward<DP>(p) ? 2 : 1) < (steps + tiles * all) / slots + 8) return 0;
+  const int64_t chunks = std::min(std::min<int64_t>(64, (slots + tiles - 1) / tiles), (all - own + each - 1) / each);
+  const int64_t blocks = ((int64_t)std::max(p.max_sq, p.max_sk) + C::kBM - 1) / C::kBM;
+  return chunks < 1 || beyond_tile_order(2 * blocks + chunks * firsts, p.hq, p.batch) ? 0 : (int)chunks;
+}
+int general_sink_chunks(const Params& p) {
+  const int d = std::max(p.dqk, p.dvo);
+  if (d > 128 || p.sinks == 0 || p.batch <= 0 || p.hk <= 0) return 0;
+  return d <= 64 ? tiled_sink_chunks<64>(p) : tiled_sink_chunks<128>(p);
+}
 
 cudaError_t launch_general(int which, int dtype, const Params& p, cudaStream_t st) {
   if (p.max_sq <= 0 || p.max_sk <= 0 || p.batch <= 0) return cudaSuccess;

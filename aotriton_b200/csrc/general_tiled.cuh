@@ -497,8 +497,11 @@ __device__ __forceinline__ void pair_exchange(float* buf, float4 (&keep)[N], con
 
 // dK / dV of 32 keys of one kv head.  The scores of dO V^T come first: its tile is the first to be free again, so that the
 // next block's dO is on its way under the accumulation of dK, Q behind it.
+// Sink attention: every query behind a first key sees it.  FEAT kSharedSinks: `chunk` 0 takes the queries of a window's worth of blocks, as for any tile, chunks
+// 1..p.sink_chunks share the others, and sink_finish_elements_kernel sums (sink_partial_row); else one CTA takes them all.  (In
+// one kernel, 2 x 8 x 500 of 64 with nothing to share: forward and backward 81.6 -> 92 us.)
 template <typename T, int DP, int SPLIT, int FEAT>
-__device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int z, int hk, int n0) {
+__device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int z, int hk, int n0, int chunk = 0) {
   using C = Tiled<DP>;
   constexpr int kThr = C::kThreads;
   float* Ks = smem;                       // [32][LD]
@@ -523,7 +526,12 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
   const int wn = n0 + (tid >> 5) * kWarpRows;
   if (wn < sq.sk) query_range(p, sq, wn, min(wn + kWarpRows, sq.sk) - 1, w_lo, w_hi);
   if constexpr ((FEAT & kSinks) != 0) {      // first keys: every query behind them
-    if (n0 < p.sinks) m_hi = sq.sq - 1;
+    if (n0 < p.sinks) {
+      const int own = m_lo <= m_hi ? (m_hi / C::kBN + 1) * C::kBN : m_lo / C::kBN * C::kBN;      // whole blocks
+      if (FEAT != kSharedSinks) m_hi = sq.sq - 1;
+      else if (chunk == 0) m_hi = min(own, sq.sq) - 1;
+      else { m_lo = own; m_hi = sq.sq - 1; }
+    }
     if (wn < p.sinks && wn < sq.sk) w_hi = sq.sq - 1;
   }
   const int dq4 = (p.dqk + 3) >> 2, dv4 = (p.dvo + 3) >> 2;
@@ -541,11 +549,21 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
     stage_tile<T, DP, C::kBN, kThr>(dOs, p.dout, sq.bidx, h, sq.q0, m0, sq.sq, p.dvo, dovec, tid);
   };
   const uint32_t rank = SPLIT == 2 ? pair_rank() : 0u;
-  const int nblk = m_lo <= m_hi ? m_hi / C::kBN - m_lo / C::kBN + 1 : 0, total = nblk * p.group;
+  const int nblk = m_lo <= m_hi ? m_hi / C::kBN - m_lo / C::kBN + 1 : 0;
+  int total = nblk * p.group, begin = 0;
   int g = 0, mb = 0;      // head of the group and block of it
+  if constexpr (FEAT == kSharedSinks) {
+    if (chunk > 0 && total > 0) {
+      const int each = (total + p.sink_chunks - 1) / p.sink_chunks;
+      begin = min((chunk - 1) * each, total);
+      total = min(begin + each, total);
+      g = begin / nblk;
+      mb = begin - g * nblk;
+    }
+  }
   auto advance = [&] { if (++mb == nblk) { mb = 0; ++g; } };
   if (rank == 1) advance();
-  if ((int)rank < total) {
+  if (begin + (int)rank < total) {
     stage_tile<T, DP, C::kBM, kThr>(Vs, p.v, sq.bidx, hk, sq.k0, n0, sq.sk, p.dvo, rows_vec4<T>(p.v, p.dvo), tid);
     stage_do(hk * p.group + g, first + mb * C::kBN);
     stage_tile<T, DP, C::kBM, kThr>(Ks, p.k, sq.bidx, hk, sq.k0, n0, sq.sk, p.dqk, rows_vec4<T>(p.k, p.dqk), tid);
@@ -553,7 +571,7 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
     __syncthreads();
     stage_q(hk * p.group + g, first + mb * C::kBN);
   }
-  for (int i = (int)rank; i < total; i += SPLIT) {
+  for (int i = begin + (int)rank; i < total; i += SPLIT) {
     {
       const int h = hk * p.group + g, m0 = first + mb * C::kBN;
       DropoutCtx dctx;
@@ -603,6 +621,17 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
       if (more) stage_q(next_h, next_m0);
     }
   }
+  // a row of dK (1) or dV (0), or of its partial sums
+  auto store = [&](int n, const float4 (&row)[C::kND], bool is_k) {
+    if constexpr (FEAT == kSharedSinks) {
+      if (n < p.sinks) {
+        store_acc_row<float, DP>(sink_partial_row(p, z, hk, chunk, n) + (is_k ? 0 : p.dqk), row, 1.f, is_k ? p.dqk : p.dvo, tx);
+        return;
+      }
+      if (chunk > 0) return;
+    }
+    store_acc_row<T, DP>(row_ptr_mut<T>(is_k ? p.dk : p.dv, sq.bidx, hk, sq.k0 + n), row, is_k ? p.sm_scale : 1.f, is_k ? p.dqk : p.dvo, tx);
+  };
   if constexpr (SPLIT == 2) {      // the first CTA finishes dK, the second dV (Q's and dO's tiles are free)
     float4 mine[4 * C::kND], theirs[4 * C::kND];
 #pragma unroll
@@ -620,7 +649,7 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
       float4 row[C::kND];
 #pragma unroll
       for (int j = 0; j < C::kND; ++j) row[j] = mine[i * C::kND + j];
-      store_acc_row<T, DP>(row_ptr_mut<T>(rank == 0 ? p.dk : p.dv, sq.bidx, hk, sq.k0 + n), row, rank == 0 ? p.sm_scale : 1.f, rank == 0 ? p.dqk : p.dvo, tx);
+      store(n, row, rank == 0);
     }
     return;
   }
@@ -628,8 +657,8 @@ __device__ __forceinline__ void tiled_bwd_dkdv(const Params& p, float* smem, int
   for (int i = 0; i < 4; ++i) {
     const int n = n0 + ty * 4 + i;
     if (n >= sq.sk) continue;
-    store_acc_row<T, DP>(row_ptr_mut<T>(p.dk, sq.bidx, hk, sq.k0 + n), adk[i], p.sm_scale, p.dqk, tx);
-    store_acc_row<T, DP>(row_ptr_mut<T>(p.dv, sq.bidx, hk, sq.k0 + n), adv[i], 1.f, p.dvo, tx);
+    store(n, adk[i], true);
+    store(n, adv[i], false);
   }
 }
 
@@ -759,16 +788,24 @@ tiled_bwd_kernel(const __grid_constant__ Params p) {
   wait_for_earlier_grids();
   extern __shared__ float smem[];
   constexpr int kBM = Tiled<DP>::kBM;
-  const int nx = (int)gridDim.x / SPLIT;
+  const int nx = (int)gridDim.x / SPLIT, extra = FEAT == kSharedSinks ? sink_items(p, kBM) : 0, base = nx - extra;
   int x, h, z;
   tile_of_block<false>((int)blockIdx.x / SPLIT, (int)blockIdx.y, (int)blockIdx.z, nx, (int)gridDim.y, (int)gridDim.z, x, h, z);
+  if constexpr (FEAT == kSharedSinks) {      // the items that share the first keys' queries, then the tiles
+    if (x < extra) {
+      const int t = x / p.sink_chunks;
+      if (h < p.hk) tiled_bwd_dkdv<T, DP, SPLIT, FEAT>(p, smem, z, h, t * kBM, x - t * p.sink_chunks + 1);
+      return;
+    }
+    x -= extra;
+  }
   if constexpr (WHICH == 1) {
     tiled_bwd_dkdv<T, DP, SPLIT, FEAT>(p, smem, z, h, x * kBM);
   } else if constexpr (WHICH == 2) {
     tiled_bwd_dq<T, DP, SPLIT, FEAT>(p, smem, z, h, (nx - 1 - x) * kBM);
   } else {
     if (x & 1) {
-      const int m0 = (nx / 2 - 1 - (x >> 1)) * kBM;
+      const int m0 = (base / 2 - 1 - (x >> 1)) * kBM;
       if (m0 < p.max_sq) tiled_bwd_dq<T, DP, SPLIT, FEAT>(p, smem, z, h, m0);
     } else if (h < p.hk) {
       tiled_bwd_dkdv<T, DP, SPLIT, FEAT>(p, smem, z, h, (x >> 1) * kBM);

@@ -75,6 +75,8 @@ cudaError_t launch_kernel(A&&... a) { return launch_kernel_as<true>(std::forward
 // which: 0 forward, 1 dK/dV, 2 dQ(+dBias), 3 both (dQ and dBias share no memory with an input).  dtype:
 // ab200_dtype value.
 cudaError_t launch_general(int which, int dtype, const Params& p, cudaStream_t st);
+// How many items share the queries beyond a first key's window in dK/dV (Params::sink_chunks).
+int general_sink_chunks(const Params& p);
 cudaError_t launch_preprocess(int dtype, const Params& p, cudaStream_t st);
 // Sink attention: zeros behind the sequences of a packed or padded batch (`backward`: in the gradients).
 cudaError_t launch_rows_behind(int dtype, const Params& p, bool backward, cudaStream_t st);

@@ -304,3 +304,38 @@ def test_packed_with_room_behind(lens_q, lens_k, dt, D, layout):
                               ("dv", grads[2][:, :, sl_k])):
                 check(name, got, values, bounds)
     _healthy()
+
+
+@pytest.mark.parametrize("dt,D", [(F32, 64), (F32, 128), (F32, 40), (BF16, 60), (F16, 124)])
+@pytest.mark.parametrize("window,sinks", [(30, 4), (100, 45)])
+@pytest.mark.parametrize("lens_q,lens_k", [([1000], None), ([1000, 0, 3, 200], None), ([40, 900], [1000, 950])])
+def test_first_keys_shared_by_many_queries(lens_q, lens_k, window, sinks, dt, D):
+    """Register-tiled backward: several CTAs share the queries of the first keys.  Short and empty sequences beside long ones."""
+    from aotriton_b200 import autograd, cabi
+    lens_k = lens_k or lens_q
+    Hq, Hk = 8, 2
+    tq, tk = sum(lens_q), sum(lens_k)
+    q, k, v, do = _rand((1, Hq, tq, D), (1, Hk, tk, D), (1, Hk, tk, D), (1, Hq, tq, D), dt=dt, seed=tq + sinks, layout="bshd")
+    for t in (q, k, v):
+        t.requires_grad_()
+    args = (_ends(lens_q), _ends(lens_k), max(lens_q), max(lens_k))
+    out, lse = autograd.varlen_sink_attention(q, k, v, *args, window, sinks, return_lse=True)
+    need = cabi.sink_attn_bwd_workspace(q, k, v, out, do, q, k, v, lse, torch.empty_like(lse), window, sinks, sm_scale=1.0, cu_seqlens_q=args[0],
+                                        cu_seqlens_k=args[1], max_seqlen_q=args[2], max_seqlen_k=args[3], varlen_type=1)
+    assert need > 0
+    poison = torch.full((need,), float("nan"), device="cuda")      # (the workspace that the backward gets next)
+    del poison
+    grads = torch.autograd.grad(out, (q, k, v), do, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(out, (q, k, v), do)))
+    at_q = at_k = 0
+    for nq, nk in zip(lens_q, lens_k):
+        sl_q, sl_k = slice(at_q, at_q + nq), slice(at_k, at_k + nk)
+        at_q, at_k = at_q + nq, at_k + nk
+        if not nq:
+            assert bool((grads[1][:, :, sl_k] == 0).all()) and bool((grads[2][:, :, sl_k] == 0).all())
+            continue
+        part = [t.detach()[:, :, sl] for t, sl in ((q, sl_q), (k, sl_k), (v, sl_k))]
+        values, bounds = reference(*part, window, sinks, D ** -0.5, do[:, :, sl_q])
+        for name, got in (("out", out.detach()[:, :, sl_q]), ("dq", grads[0][:, :, sl_q]), ("dk", grads[1][:, :, sl_k]), ("dv", grads[2][:, :, sl_k])):
+            check(name, got, values, bounds)
+    _healthy()
