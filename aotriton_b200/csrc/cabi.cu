@@ -844,7 +844,12 @@ static int64_t plan_sink_bwd(const ab200_attn_bwd_args* a, Params& p, int* sel) 
     p.sink_chunks = general_sink_chunks(p);
     return partials();
   }
-  if (p.dqk > 128 || p.dvo > 128) return 0;
+  if (p.dqk > 128 || p.dvo > 128) {      // (steps of 64 queries; the CTAs that share them start ahead of a kv head's others)
+    const int64_t all = ((int64_t)p.max_sq + 63) / 64 * p.group, own = (((int64_t)p.sink_window + 128) / 64 + 1) * p.group;
+    const int64_t tiles = (int64_t)p.batch * p.hk * ((p.sinks + 127) / 128), each = std::max<int64_t>(own, 16);
+    if (tiles > 0 && all >= own + 16) p.sink_chunks = (int)std::min(std::min<int64_t>(64, (592 + tiles - 1) / tiles), (all - own + each - 1) / each);
+    return partials();
+  }
   if (p.sinks == 0) return kTicketFloats;
   // as many query blocks to an item as a window's worth gives the other key blocks, eight at least
   const int64_t all = ((int64_t)p.max_sq + 127) / 128 * p.group, own = ((int64_t)p.sink_window + 127) / 128 * p.group + p.group;
@@ -884,7 +889,7 @@ int ab200_sink_attn_bwd(const ab200_attn_bwd_args* a, int32_t window, int32_t si
     p.sink_partial = workspace;
   }
   const bool tc = (sel & 0xff) >= kVarTcgen05;
-  if (tc && floats > 0) p.ticket = reinterpret_cast<unsigned int*>(workspace + floats - kTicketFloats);
+  if (tc && p.dqk <= 128 && p.dvo <= 128) p.ticket = reinterpret_cast<unsigned int*>(workspace + floats - kTicketFloats);
   cudaError_t e = launch_rows_behind(dtype, p, true, st);
   if (e == cudaSuccess) e = launch_preprocess(dtype, p, st);
   if (e != cudaSuccess) return (int)e;

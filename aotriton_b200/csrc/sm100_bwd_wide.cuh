@@ -103,7 +103,22 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
   // dV / dK: the first key blocks of a causal problem see the most queries; dQ: the last query blocks
   // see the most keys.  Heavy CTAs start first.
   const int z = blockIdx.z, hrow = blockIdx.y;
-  const int r0 = (kKeys ? (int)blockIdx.x : (int)(gridDim.x - 1 - blockIdx.x)) * kBlk;
+  int r0 = (kKeys ? (int)blockIdx.x : (int)(gridDim.x - 1 - blockIdx.x)) * kBlk;
+  // Sink attention: the queries behind a first key's window are shared out, as in dkdv_item: chunks 1..sink_chunks of a tile are CTAs ahead of
+  // the tiles, their partial sums meet in sink_finish_kernel.  Device us of a backward, bf16, 256, 4 first keys, one CTA for all queries / shared / no
+  // first keys at all: 1 x 32:8 x 8192, window 256 2046 / 742 / 650, window 2048 3094 / 2286 / 2126; 1 x 8 x 4096, window 256 306 / 174 / 153; 2 x 16:4 x 2048,
+  // window 128 484 / 240 / 178.
+  int chunk = 0;
+  if constexpr (kKeys && (FEAT & kSinks) != 0) {
+    const int extra = sink_items(p, kBlk), x = (int)blockIdx.x;
+    if (x < extra) {
+      const int t = x / p.sink_chunks;
+      chunk = x - t * p.sink_chunks + 1;
+      r0 = t * kBlk;
+    } else {
+      r0 = (x - extra) * kBlk;
+    }
+  }
   const Seq sq = resolve_seq_for<FEAT>(p, z);
   const int rows_total = kKeys ? sq.sk : sq.sq, cols_total = kKeys ? sq.sq : sq.sk;
   if (r0 >= rows_total) return;
@@ -111,12 +126,30 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
   if constexpr (kKeys) query_range(p, sq, r0, min(r0 + kBlk, sq.sk) - 1, c_lo, c_hi);
   else key_range(p, sq, r0, min(r0 + kBlk, sq.sq) - 1, c_lo, c_hi);
   if constexpr (kKeys && (FEAT & kSinks) != 0) {
-    if (r0 < p.sinks) c_hi = sq.sq - 1;      // first keys: every query behind them
+    if (r0 < p.sinks) {      // first keys: every query behind them
+      const int own = c_lo <= c_hi ? c_hi / kNB + 1 : c_lo / kNB;      // the first block that is shared
+      if (p.sink_chunks == 0) {
+        c_hi = sq.sq - 1;
+      } else if (chunk == 0) {
+        c_hi = min(own * kNB, sq.sq) - 1;
+      } else {
+        const int rest = max((sq.sq + kNB - 1) / kNB - own, 0), each = (rest + p.sink_chunks - 1) / p.sink_chunks, at = min((chunk - 1) * each, rest);
+        c_lo = (own + at) * kNB;
+        c_hi = min((own + min(at + each, rest)) * kNB, sq.sq) - 1;
+      }
+    }
   }
   const View4& outv = MODE == kWideDV ? p.dv : (MODE == kWideDK ? p.dk : p.dq);
   const int d_out = MODE == kWideDV ? p.dvo : p.dqk;
   const int64_t row_tok0 = kKeys ? sq.k0 : sq.q0, col_tok0 = kKeys ? sq.q0 : sq.k0;
   if (c_hi < c_lo) {      // rows nothing attends to / that attend to nothing: the gradient is zero
+    if constexpr (kKeys && (FEAT & kSinks) != 0) {
+      if (p.sink_chunks > 0) {
+        for (int n = r0 + warp; n < min(min(r0 + kBlk, p.sinks), sq.sk); n += (int)(blockDim.x >> 5))
+          for (int c = lane; c < d_out; c += 32) sink_partial_row(p, z, hrow, chunk, n)[(MODE == kWideDV ? p.dqk : 0) + c] = 0.f;
+      }
+      if (chunk > 0) return;
+    }
     zero_rows<T>(outv, sq.bidx, hrow, row_tok0, r0, rows_total, d_out);
     if constexpr (MODE == kWideDQ) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, 0, 0); }
     return;
@@ -640,7 +673,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     if (ok) {
       tc_fence_after();
       const uint32_t stage = smem_u32(smem + L::kResA);
-      const int nrows = min(kBlk, rows_total - r0);
+      const int nrows = kKeys && (FEAT & kSinks) != 0 && chunk > 0 ? 0 : min(kBlk, rows_total - r0);
       T* dst = reinterpret_cast<T*>(outv.ptr) + (int64_t)sq.bidx * outv.s[0] + (int64_t)hrow * outv.s[1] +
                (row_tok0 + r0) * outv.s[2];
       const float scale = MODE != kWideDV ? p.sm_scale : 1.0f;
@@ -648,6 +681,15 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         float v[32];
         tmem_ld32f(tmem_base + lane_addr + kWColAcc + c * 32, v);
         tmem_wait_ld();
+        if constexpr (kKeys && (FEAT & kSinks) != 0) {      // a first key's sums (the 16-bit row written below is overwritten by the last launch)
+          if (p.sink_chunks > 0 && r0 + r < min(p.sinks, sq.sk)) {
+            float* sums = sink_partial_row(p, z, hrow, chunk, r0 + r) + (MODE == kWideDV ? p.dqk : 0) + c * 32;
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (c * 32 + i < d_out) *reinterpret_cast<float4*>(sums + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          }
+          __syncwarp();
+        }
         stage_put32<T>(stage, r, c * 32, v, scale, 512);
         __syncwarp();
         warp_copy_out<T, 4>(stage, dst, outv.s[2], nrows, d_out, quarter * 32, c * 4, lane, 512);
@@ -715,12 +757,17 @@ cudaError_t launch_bwd_wide_T(int which, const Params& p, cudaStream_t st) {
     const Kernel kern_dv = kKernels[kWideDV][feat], kern_dk = kKernels[kWideDK][feat];
     if ((e = set_smem(feat == kSinks ? 13 + kWideDV : 4 * kWideDV + feat, reinterpret_cast<const void*>(kern_dv))) != cudaSuccess) return e;
     if ((e = set_smem(feat == kSinks ? 13 + kWideDK : 4 * kWideDK + feat, reinterpret_cast<const void*>(kern_dk))) != cudaSuccess) return e;
-    dim3 grid((p.max_sk + kBlk - 1) / kBlk, p.hk, p.batch);
+    const int extra = feat == kSinks ? sink_items(p, kBlk) : 0;
+    dim3 grid((p.max_sk + kBlk - 1) / kBlk + extra, p.hk, p.batch);
     e = launch_kernel(kern_dv, grid, dim3(wide_threads(kWideDV, feat)), L::kDynamic, st, p, k128, k128, do64, q64, status);
     if (e != cudaSuccess) return e;
     if (!p.dk_from_db) {
       count_launch();
       e = launch_kernel(kern_dk, grid, dim3(wide_threads(kWideDK, feat)), L::kDynamic, st, p, k128, v128, q64, do64, status);
+    }
+    if (e == cudaSuccess && extra > 0) {
+      count_launch();
+      e = launch_kernel(sink_finish_kernel<T>, dim3(p.sinks, p.hk, p.batch), dim3(128), 0, st, p);
     }
   } else {
     const Kernel kern_dq = kKernels[kWideDQ][feat];

@@ -306,11 +306,11 @@ def test_packed_with_room_behind(lens_q, lens_k, dt, D, layout):
     _healthy()
 
 
-@pytest.mark.parametrize("dt,D", [(F32, 64), (F32, 128), (F32, 40), (BF16, 60), (F16, 124)])
+@pytest.mark.parametrize("dt,D", [(F32, 64), (F32, 128), (F32, 40), (BF16, 60), (F16, 124), (BF16, 256), (F16, 160)])
 @pytest.mark.parametrize("window,sinks", [(30, 4), (100, 45)])
 @pytest.mark.parametrize("lens_q,lens_k", [([1000], None), ([1000, 0, 3, 200], None), ([40, 900], [1000, 950])])
 def test_first_keys_shared_by_many_queries(lens_q, lens_k, window, sinks, dt, D):
-    """Register-tiled backward: several CTAs share the queries of the first keys.  Short and empty sequences beside long ones."""
+    """Register-tiled backward and wide heads: several CTAs share the queries of the first keys.  Short and empty sequences beside long ones."""
     from aotriton_b200 import autograd, cabi
     lens_k = lens_k or lens_q
     Hq, Hk = 8, 2

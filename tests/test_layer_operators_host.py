@@ -202,15 +202,14 @@ def test_sink_entries_on_a_pretended_device(fake):
     a.prob.dropout_p = b.prob.dropout_p = 0.0
     a.bias.ptr = 0x1000
     assert fwd(a, 5, 1, None) == 801
-    # wide heads need no workspace, single precision for the first keys' partial sums alone
-    b = _sink_args(cabi.BwdArgs, D=256)
-    assert size(b, 100, 4, None) == 0 and bwd(b, 100, 4, None, 0, None) == 0
-    b = _sink_args(cabi.BwdArgs, dtype=cabi.DTYPE_FP32)
-    assert size(b, 100, 0, None) == 0 and size(b, 1000, 4, None) == 0
-    items = size(b, 100, 4, None)
-    assert items > 0 and items % (2 * 2 * 4 * 256) == 0 and bwd(b, 100, 4, 0x5000, items - 1, None) == 1
-    before = count()
-    assert bwd(b, 100, 4, 0x5000, items, None) == 0 and count() == before + 3      # delta, all gradients, the first keys' sums
+    # wide heads and single precision: for the first keys' partial sums alone
+    for kw, d, launches in ((dict(D=256), 512, 5), (dict(dtype=cabi.DTYPE_FP32), 256, 3)):      # delta, the gradients (dV, dK, dQ or all), the sums
+        b = _sink_args(cabi.BwdArgs, **kw)
+        assert size(b, 100, 0, None) == 0 and size(b, 1000, 4, None) == 0
+        items = size(b, 100, 4, None)
+        assert items > 0 and items % (2 * 2 * 4 * d) == 0 and bwd(b, 100, 4, 0x5000, items - 1, None) == 1
+        before = count()
+        assert bwd(b, 100, 4, 0x5000, items, None) == 0 and count() == before + launches
     fake.ab200_debug_host_calls(1, 7, 98, 2)      # the third launch fails: nothing after it
     b = _sink_args(cabi.BwdArgs)
     assert bwd(b, 100, 4, 0x5000, need, None) == 98 and count() == 3
