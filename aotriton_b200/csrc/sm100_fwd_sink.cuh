@@ -14,8 +14,8 @@
 // Measured on the device, bf16, 1 x 32:8 heads x 8192 of 128, 4 first keys, us, two tiles to a CTA / one with blocks of 128 keys / this: window 2048
 // 310 / 282 / 249, 1024 229 / 192 / 167 (0.98 PFLOP/s of products that are issued), 512 151 / 140 / 122, 128 101 / 95 / 85.  At window 1024 the tensor pipe and the
 // exponential unit are each busy 45% of the time (56% in the tile kernel on a long row), L2 27%: what is left is a step's chain in a softmax warp, loads
-// from tensor memory, maximum, exponentials, store, of which two warps a scheduler overlap.  CTAs that stay and walk over the tiles (the next Q loaded under the last blocks, O staged beside
-// it) came out 1 to 5% slower: the second CTA of the SM covers a start as well, and the hardware hands tiles out in the order they end.
+// from tensor memory, maximum, exponentials, store, of which two warps a scheduler overlap.  CTAs that stay and walk over the tiles (the
+// next Q loaded under the last blocks, O staged beside it) came out 1 to 5% slower: the second CTA of the SM covers a start as well, and the hardware hands tiles out in the order they end.
 // Every wait is bounded.
 
 constexpr int kSinkBN = 64, kSinkThreads = 256;
