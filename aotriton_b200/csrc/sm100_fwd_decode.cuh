@@ -239,6 +239,9 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
           for (int rr = max(0, from - key0); rr < min(16, to - key0); ++rr)
             for (int c = lane; c < kBoxes * 8; c += 32)
               *reinterpret_cast<uint4*>(vtile + (c >> 3) * (kDecKeys * 128) + ((warp & 3) * 16 + rr) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          // (these tiles are the walk's first: another is copied into their stage, and the barrier alone orders these stores for ordinary
+          // accesses, not for a copy's.  A sequence's last tile, zeroed above, is the last of its CTA)
+          fence_proxy_async_smem();
           __syncwarp();
         }
       }
