@@ -321,6 +321,16 @@ def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
+def _on_its_device(forward):
+    """forward(ctx, tensor, ...) of a Function with the tensor's device as the current one.  A default stream's handle is 0 on every device, and the
+    library takes it for the current device's."""
+    @functools.wraps(forward)
+    def run(ctx, tensor, *args):
+        with torch.cuda.device(tensor.device):
+            return forward(ctx, tensor, *args)
+    return run
+
+
 def _launch(fn, device, args):
     """An entry point of the C-ABI on the device's current stream."""
     return fn(args, torch.cuda.current_stream(device).cuda_stream)
@@ -335,6 +345,7 @@ def _sink_problem(cu_q, cu_k, max_q, max_k, varlen, sm_scale):
 
 class _SinkAttention(torch.autograd.Function):
     @staticmethod
+    @_on_its_device
     def forward(ctx, q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, return_lse, varlen):
         b, hq, sq, _ = q.shape
         packed = varlen == cabi.VARLEN_COMPACT
@@ -365,6 +376,7 @@ class _SinkAttentionGrad(torch.autograd.Function):
     """(dq, dk, dv): an operator of its own, which knows that it has no derivative."""
 
     @staticmethod
+    @_on_its_device
     def forward(ctx, q, k, v, o, do, lse, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, varlen):
         if not q.numel() or not k.numel() or not v.numel():
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
@@ -484,6 +496,7 @@ def _bias_rows(heads, sq, sk, dtype, device):
 
 class _RelativeBias(torch.autograd.Function):
     @staticmethod
+    @_on_its_device
     def forward(ctx, table, sq, sk, batch, borders, bidirectional, query_offset, dtype):
         bias = _bias_rows(table.shape[1], sq, sk, dtype, table.device)
         if bias.numel():
@@ -502,6 +515,7 @@ class _RelativeBiasGrad(torch.autograd.Function):
     """The table's gradient; linear in its input, its own derivative is the bias again."""
 
     @staticmethod
+    @_on_its_device
     def forward(ctx, grad, shape, dtype, borders, bidirectional, query_offset):
         table = torch.empty(shape, device=grad.device, dtype=dtype)
         ctx.args = (*grad.shape[2:], grad.shape[0], borders, bidirectional, query_offset, grad.dtype)
@@ -569,6 +583,7 @@ def _as_rows(t):
 
 class _Dropout(torch.autograd.Function):
     @staticmethod
+    @_on_its_device
     def forward(ctx, x, residual, dropout_p, seed, offset):
         out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
         tensors = [t if isinstance(t, torch.Tensor) else None for t in (seed, offset)]
