@@ -67,6 +67,16 @@ def _check(err, what):
         raise RuntimeError(f"{what} failed: {err}")
 
 
+def _on_its_device(fn):
+    """fn with the device of its first tensor as the current one.  A default stream's handle is 0 on every device, and the library takes it for
+    the current device's."""
+    @functools.wraps(fn)
+    def run(*args, **kw):
+        with torch.cuda.device(next(t for t in args if isinstance(t, torch.Tensor)).device):
+            return fn(*args, **kw)
+    return run
+
+
 # A null device scalar: no elements, so no address on any device.
 _NULL_SCALAR = torch.empty([0], dtype=torch.uint64)
 # The counter of a persistent kernel: the kernels bring their own.
@@ -118,6 +128,7 @@ def _attend(q, k, v, b, cu_q, cu_k, max_q, max_k, sm_scale, dropout_p, causal, r
     return _native.attend(q, k, v, b, cu_q, cu_k, max_q, max_k, sm_scale, dropout_p, ct, wl, wr, return_lse, seed, offset1, op)
 
 
+@_on_its_device
 def _backward(q, k, v, b, o, do, L, cu_q, cu_k, seed, offset1, offset2, sm_scale, dropout_p, causal, max_q, max_k):
     """(dq, dk, dv, dbias) of a dense or, with cumulative lengths, a token-packed call."""
     do = do if do.stride(-1) == 1 else do.contiguous()
@@ -146,6 +157,7 @@ _native.set_python_backward(_native_backward)
 
 class _Attention(torch.autograd.Function):
     @staticmethod
+    @_on_its_device
     def forward(ctx, q, k, v, b, causal, sm_scale, dropout_p, return_lse=False,
                 philox_seed=DEFAULT_PHILOX_SEED, philox_offset1=DEFAULT_PHILOX_OFFSET_1):
         o = torch.empty((q.shape[0], q.shape[1], q.shape[2], v.shape[3]), device=q.device, dtype=q.dtype)
@@ -177,6 +189,7 @@ def attention(q, k, v, b=None, causal=False, sm_scale=None, dropout_p=0.0, retur
 
 class _VarlenAttention(torch.autograd.Function):
     @staticmethod
+    @_on_its_device
     def forward(ctx, q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal, sm_scale,
                 dropout_p, return_lse=False, philox_seed=DEFAULT_PHILOX_SEED,
                 philox_offset1=DEFAULT_PHILOX_OFFSET_1):
@@ -221,6 +234,7 @@ def _lse_rows(q):
 
 
 @torch.library.custom_op("aotriton_b200::attn_fwd", mutates_args=())
+@_on_its_device
 def op_attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch.Tensor | None, sm_scale: float,
                 dropout_p: float, causal_type: int, window_left: int, window_right: int, philox_seed: int,
                 philox_offset1: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -246,6 +260,7 @@ def _(q, k, v, bias, sm_scale, dropout_p, causal_type, window_left, window_right
 
 
 @torch.library.custom_op("aotriton_b200::attn_bwd", mutates_args=())
+@_on_its_device
 def op_attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bias: torch.Tensor | None, out: torch.Tensor,
                 dout: torch.Tensor, lse: torch.Tensor, philox_seed: torch.Tensor, philox_offset: torch.Tensor,
                 sm_scale: float, dropout_p: float, causal_type: int, window_left: int, window_right: int,
@@ -319,16 +334,6 @@ def scaled_dot_product_attention(query, key, value, attn_mask=None, dropout_p=0.
 # ---------------------------------------------------------------------------------------------
 # What stands around attention in a layer.  The reference has neither.
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
-
-
-def _on_its_device(forward):
-    """forward(ctx, tensor, ...) of a Function with the tensor's device as the current one.  A default stream's handle is 0 on every device, and the
-    library takes it for the current device's."""
-    @functools.wraps(forward)
-    def run(ctx, tensor, *args):
-        with torch.cuda.device(tensor.device):
-            return forward(ctx, tensor, *args)
-    return run
 
 
 def _launch(fn, device, args):

@@ -5,7 +5,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from aotriton_b200 import autograd, cabi
+from aotriton_b200 import autograd, cabi, flash
 
 
 @pytest.fixture
@@ -35,6 +35,11 @@ def calls(monkeypatch):
         monkeypatch.setattr(cabi, name, entry(name, result))
     names = [("ab200_relative_bias_fwd", 0), ("ab200_relative_bias_bwd", 0), ("ab200_relative_bias_workspace", 8)]
     monkeypatch.setattr(cabi, "lib", lambda: SimpleNamespace(**{name: entry(name, result) for name, result in names}))
+    for name in ("attn_fwd", "attn_bwd", "attn_fwd_varlen", "attn_bwd_varlen"):
+        monkeypatch.setattr(flash, name, entry(name))
+    for name in ("eager_delta", "lazy_delta", "lazy_dq_acc"):
+        monkeypatch.setattr(flash, name, lambda t: None)
+    monkeypatch.setattr(autograd, "_check", lambda err, what: None)
     monkeypatch.setattr(autograd._native, "note_bwd_family", lambda: None)
     return seen
 
@@ -58,3 +63,20 @@ def test_dropout(calls):
     x, r = (torch.zeros(3, 4, requires_grad=True) for _ in range(2))
     autograd._Dropout.apply(x, r, 0.5, 1, 2).sum().backward()
     assert calls == [("dropout", HERE)] * 2
+
+
+def _qkv():
+    return [torch.zeros(1, 2, 5, 8, requires_grad=True) for _ in range(3)]
+
+
+@pytest.mark.parametrize("dropout_p", [0.0, 0.1])
+def test_attention(calls, dropout_p):
+    autograd._Attention.apply(*_qkv(), None, False, 1.0, dropout_p).sum().backward()
+    ends = torch.tensor([0, 2, 5], dtype=torch.int32)
+    autograd._VarlenAttention.apply(*_qkv(), ends, ends, 3, 3, False, 1.0, dropout_p).sum().backward()
+    assert calls == [(name, HERE) for name in ("attn_fwd", "attn_bwd", "attn_fwd_varlen", "attn_bwd_varlen")]
+
+
+def test_attention_operators(calls):
+    autograd.op_attn_fwd(*_qkv(), None, 1.0, 0.0, 0, 0, 0, 1, 2)[0].sum().backward()
+    assert calls == [(name, HERE) for name in ("attn_fwd", "attn_bwd")]
