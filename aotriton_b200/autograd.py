@@ -374,7 +374,7 @@ class _SinkAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do, *unused):
         q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
-        return _SinkAttentionGrad.apply(q, k, v, o, do, lse, cu_q, cu_k, *ctx.args) + (None,) * 9
+        return _sink_grad(q, k, v, o, do, lse, cu_q, cu_k, *ctx.args) + (None,) * 9
 
 
 class _SinkAttentionGrad(torch.autograd.Function):
@@ -404,12 +404,20 @@ class _SinkAttentionGrad(torch.autograd.Function):
         raise RuntimeError("sink_attention has no second derivative")
 
 
-def _python_sink_grad(q, k, v, o, do, lse, cu_q, cu_k, *numbers):
-    """The gradients of a native call whose own gradient or modes are not ordinary ones (csrc/torch_ops.cc)."""
+def _sink_grad(q, k, v, o, do, lse, cu_q, cu_k, *numbers):
+    """The gradients, of a Python call or of a native one whose own gradient or modes are not ordinary ones (csrc/torch_ops.cc).
+
+    A saved-tensor hook may have handed back anything; the kernels go by addresses and by the types and sizes that the gradient came with."""
+    bad = [t for t in (q, k, v, o) if t.dim() != 4 or t.dtype != do.dtype or t.device != do.device]
+    bad += [t for t in (cu_q, cu_k) if t is not None and (t.dtype != torch.int32 or t.device != do.device or t.shape != cu_q.shape or not t.is_contiguous())]
+    if (bad or lse.dim() != 2 or lse.dtype != torch.float32 or lse.device != do.device or not lse.is_contiguous()
+            or lse.numel() != q.shape[0] * q.shape[1] * q.shape[2] or not o.shape == do.shape == (*q.shape[:3], v.shape[3])
+            or k.shape[:3] != v.shape[:3] or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3] or k.shape[1] and q.shape[1] % k.shape[1]):
+        raise ValueError("sink_attention: what was saved for the backward came back with other types, sizes or devices")
     return _SinkAttentionGrad.apply(q, k, v, o, do, lse, cu_q, cu_k, *numbers)
 
 
-_native.set_python_function("sink_attention", _python_sink_grad)
+_native.set_python_function("sink_attention", _sink_grad)
 
 
 def _sink_attention(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, return_lse, varlen):
@@ -608,6 +616,8 @@ class _Dropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad):
         saved = [t if t is not None else n for t, n in zip(ctx.saved_tensors, ctx.numbers)]
+        for x, what in zip(saved, ("philox_seed", "philox_offset")):      # (a saved-tensor hook may hand back anything)
+            _philox_number(x, what, grad.device)
         dx = _Dropout.apply(grad, None, ctx.dropout_p, *saved) if ctx.needs_input_grad[0] else None
         return dx, grad if ctx.residual and ctx.needs_input_grad[1] else None, None, None, None
 

@@ -362,6 +362,13 @@ struct SinkAttend : torch::autograd::Function<SinkAttend> {
     ctx->set_materialize_grads(false);
     return return_lse ? variable_list{out, lse} : variable_list{out};
   }
+  // (a saved-tensor hook may hand back anything: what does not match is refused in Python)
+  static bool sizes_match(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out, const Tensor& cu_q, const Tensor& cu_k) {
+    for (int i = 0; i < 3; ++i)
+      if (k.size(i) != v.size(i) || q.size(i) != out.size(i)) return false;
+    return k.size(0) == q.size(0) && k.size(3) == q.size(3) && v.size(3) == out.size(3) && cu_q.defined() == cu_k.defined() &&
+           (!cu_q.defined() || cu_q.numel() == cu_k.numel());
+  }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &cu_q = saved[5], &cu_k = saved[6];
@@ -371,7 +378,7 @@ struct SinkAttend : torch::autograd::Function<SinkAttend> {
     if (!grads[0].defined()) return r;
     Tensor dout = grads[0];
     // (create_graph: the operator, which knows that it has no derivative; the rest as in Attend::backward)
-    if (at::GradMode::is_enabled() || !Attend::as_saved(q, k, v, Tensor(), out, dout, lse, cu_q, cu_k)) {
+    if (at::GradMode::is_enabled() || !Attend::as_saved(q, k, v, Tensor(), out, dout, lse, cu_q, cu_k) || !sizes_match(q, k, v, out, cu_q, cu_k)) {
       pybind11::gil_scoped_acquire gil;
       const auto o = call_python("sink_attention", pybind11::make_tuple(wrapped(q), wrapped(k), wrapped(v), wrapped(out), wrapped(dout), wrapped(lse),
                                                                         wrapped(cu_q), wrapped(cu_k), c.max_q, c.max_k, c.window, c.sinks, c.sm_scale, c.varlen));
