@@ -77,6 +77,17 @@ def _on_its_device(fn):
     return run
 
 
+# (torch.compiler.disable, with the three seconds of its import left to the first compiled call)
+@torch._disable_dynamo
+def _apply_untraced(function, *args):
+    return function.apply(*args)
+
+
+def _apply(function, *args):
+    """function.apply(*args); a compiled caller's graph breaks here.  (Traced, the Functions fail at the current stream's handle.)"""
+    return _apply_untraced(function, *args) if torch.compiler.is_compiling() else function.apply(*args)
+
+
 # A null device scalar: no elements, so no address on any device.
 _NULL_SCALAR = torch.empty([0], dtype=torch.uint64)
 # The counter of a persistent kernel: the kernels bring their own.
@@ -184,7 +195,7 @@ def attention(q, k, v, b=None, causal=False, sm_scale=None, dropout_p=0.0, retur
     unit innermost stride).  `causal` is a bool, a (left, right) window or a flash.CausalType."""
     sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
     r = _attend(q, k, v, b, None, None, 0, 0, sm_scale, dropout_p, causal, return_lse, philox_seed, philox_offset1, False)
-    return r if r is not None else _Attention.apply(q, k, v, b, causal, sm_scale, dropout_p, return_lse, philox_seed, philox_offset1)
+    return r if r is not None else _apply(_Attention, q, k, v, b, causal, sm_scale, dropout_p, return_lse, philox_seed, philox_offset1)
 
 
 class _VarlenAttention(torch.autograd.Function):
@@ -219,7 +230,7 @@ def varlen_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seql
     sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
     r = _attend(q, k, v, None, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, sm_scale, dropout_p, causal, return_lse,
                 DEFAULT_PHILOX_SEED, DEFAULT_PHILOX_OFFSET_1, False)
-    return r if r is not None else _VarlenAttention.apply(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal,
+    return r if r is not None else _apply(_VarlenAttention, q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal,
                                   sm_scale, dropout_p, return_lse)
 
 
@@ -448,7 +459,7 @@ def _sink_attention(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, 
         max_k = max(max_k, 1)
     window, sinks = min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)
     q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
-    return _SinkAttention.apply(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, float(sm_scale), bool(return_lse), varlen)
+    return _apply(_SinkAttention, q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, float(sm_scale), bool(return_lse), varlen)
 
 
 def sink_attention(q, k, v, window, sinks, sm_scale=None, return_lse=False):
@@ -578,7 +589,7 @@ def relative_position_bias(table, seqlen_q, seqlen_k, batch=1, max_distance=128,
         r = _native.relative_bias(table, seqlen_q, seqlen_k, batch, _borders_bytes(buckets, max_distance), bool(bidirectional), query_offset, dtype)
         if r is not None:
             return r
-    return _RelativeBias.apply(table, seqlen_q, seqlen_k, batch, borders, bool(bidirectional), query_offset, dtype)
+    return _apply(_RelativeBias, table, seqlen_q, seqlen_k, batch, borders, bool(bidirectional), query_offset, dtype)
 
 
 def _as_rows(t):
@@ -665,4 +676,4 @@ def dropout(x, dropout_p, residual=None, philox_seed=DEFAULT_PHILOX_SEED, philox
         if r is not None:
             return r
     seed, offset = _philox_number(philox_seed, "philox_seed", x.device), _philox_number(philox_offset, "philox_offset", x.device)
-    return _Dropout.apply(x, residual, float(dropout_p), seed, offset)
+    return _apply(_Dropout, x, residual, float(dropout_p), seed, offset)
