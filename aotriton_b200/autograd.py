@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import warnings
 
 import torch
@@ -485,11 +486,18 @@ def varlen_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max
                            flash.IVARLEN_TYPE[varlen_type])
 
 
-@functools.lru_cache(maxsize=None)
 def relative_position_borders(buckets, max_distance):
     """The smallest distance of each bucket of one direction but the first, as a tuple of whole numbers: the first half of the buckets (e)
     has a distance each, bucket k beyond takes the distances from e * (max_distance / e) ** ((k - e) / (buckets - e)) on.  Compared in
     whole numbers: a logarithm in floating point puts distances next to a border on either side of it."""
+    try:      # (as Python's own: other whole numbers overflow below, and whatever equals them would find their answer)
+        return _borders(operator.index(buckets), operator.index(max_distance))
+    except TypeError:
+        raise ValueError(f"relative position buckets: {buckets!r} and {max_distance!r} are not whole numbers") from None
+
+
+@functools.lru_cache(maxsize=None)
+def _borders(buckets, max_distance):
     e = buckets // 2
     if buckets < 2 or max_distance <= e:
         raise ValueError(f"relative position buckets: {buckets} a direction up to distance {max_distance}: at least 2, and a distance above {e}, are needed")
@@ -508,8 +516,8 @@ def relative_position_borders(buckets, max_distance):
 
 
 @functools.lru_cache(maxsize=None)
-def _borders_bytes(buckets, max_distance):
-    return bytes((ctypes.c_int32 * (buckets - 1))(*relative_position_borders(buckets, max_distance)))
+def _borders_bytes(borders):
+    return bytes((ctypes.c_int32 * len(borders))(*borders))
 
 
 def _bias_rows(heads, sq, sk, dtype, device):
@@ -586,7 +594,7 @@ def relative_position_bias(table, seqlen_q, seqlen_k, batch=1, max_distance=128,
         raise ValueError("relative_position_bias: query_offset beyond 32 bits")
     borders = relative_position_borders(buckets, max_distance)
     if not torch.compiler.is_compiling():
-        r = _native.relative_bias(table, seqlen_q, seqlen_k, batch, _borders_bytes(buckets, max_distance), bool(bidirectional), query_offset, dtype)
+        r = _native.relative_bias(table, seqlen_q, seqlen_k, batch, _borders_bytes(borders), bool(bidirectional), query_offset, dtype)
         if r is not None:
             return r
     return _apply(_RelativeBias, table, seqlen_q, seqlen_k, batch, borders, bool(bidirectional), query_offset, dtype)
