@@ -593,6 +593,8 @@ def relative_position_bias(table, seqlen_q, seqlen_k, batch=1, max_distance=128,
     if abs(query_offset) >= 1 << 31:
         raise ValueError("relative_position_bias: query_offset beyond 32 bits")
     borders = relative_position_borders(buckets, max_distance)
+    if borders[-1] >= 1 << 31:
+        raise ValueError(f"relative_position_bias: the last bucket starts at distance {borders[-1]}, beyond 32 bits")
     if not torch.compiler.is_compiling():
         r = _native.relative_bias(table, seqlen_q, seqlen_k, batch, _borders_bytes(borders), bool(bidirectional), query_offset, dtype)
         if r is not None:

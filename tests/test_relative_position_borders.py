@@ -1,6 +1,7 @@
-"""CPU: numbers for the bucket borders that are not Python's whole numbers."""
+"""CPU: numbers for the bucket borders that are not Python's whole numbers, and borders that the kernels' 32 bits do not hold."""
 import numpy as np
 import pytest
+import torch
 
 from aotriton_b200 import autograd
 
@@ -19,3 +20,17 @@ def test_not_whole_numbers(buckets, far):
     with pytest.raises(ValueError):
         autograd.relative_position_borders(buckets, far)
     assert all(type(b) is int for b in autograd.relative_position_borders(16, 777))
+
+
+def test_borders_beyond_32_bits():
+    class Table:      # (what the checks look at)
+        shape, dtype, is_cuda = torch.Size((6, 4)), torch.float32, True
+
+        def dim(self):
+            return 2
+
+    far = (2 ** 32 + 5) ** 2      # three buckets: the last from the square root on, whose low 32 bits are 5
+    assert autograd.relative_position_borders(3, far) == (1, 2 ** 32 + 5)
+    for edge in (far, (2 ** 31) ** 2):
+        with pytest.raises(ValueError, match="32 bits"):
+            autograd.relative_position_bias(Table(), 5, 6, max_distance=edge)
