@@ -360,6 +360,13 @@ def _sink_problem(cu_q, cu_k, max_q, max_k, varlen, sm_scale):
     return kw
 
 
+def _unit_rows(t):
+    """t with a unit innermost stride: itself or a copy.  A single column keeps any stride through contiguous()."""
+    if t.stride(-1) != 1:
+        t = t.squeeze(-1).unsqueeze(-1) if t.shape[-1] == 1 else t.contiguous()
+    return t
+
+
 class _SinkAttention(torch.autograd.Function):
     @staticmethod
     @_on_its_device
@@ -397,7 +404,7 @@ class _SinkAttentionGrad(torch.autograd.Function):
     def forward(ctx, q, k, v, o, do, lse, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, varlen):
         if not q.numel() or not k.numel() or not v.numel():
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
-        do = do if do.stride(-1) == 1 else do.contiguous()
+        do = _unit_rows(do)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         delta = torch.empty_like(lse)
         kw = _sink_problem(cu_q, cu_k, max_q, max_k, varlen, sm_scale)
@@ -459,7 +466,7 @@ def _sink_attention(q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, sm_scale, 
         max_q = q.shape[2] if varlen == cabi.VARLEN_PADDED else max(max_q, 1)
         max_k = max(max_k, 1)
     window, sinks = min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)
-    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    q, k, v = map(_unit_rows, (q, k, v))
     return _apply(_SinkAttention, q, k, v, cu_q, cu_k, max_q, max_k, window, sinks, float(sm_scale), bool(return_lse), varlen)
 
 

@@ -385,7 +385,7 @@ struct SinkAttend : torch::autograd::Function<SinkAttend> {
       for (int i = 0; i < 3; ++i) r[i] = THPVariable_Unpack(PyTuple_GET_ITEM(o.ptr(), i));
       return r;
     }
-    if (dout.stride(-1) != 1) dout = dout.contiguous();
+    if (dout.stride(-1) != 1) dout = dout.size(-1) == 1 ? dout.squeeze(-1).unsqueeze(-1) : dout.contiguous();      // (contiguous() leaves one column's stride)
     r[0] = gradient_of(q);
     r[1] = gradient_of(k);
     r[2] = gradient_of(v);
