@@ -579,7 +579,7 @@ def relative_position_bias(table, seqlen_q, seqlen_k, batch=1, max_distance=128,
     with stride 0, bias[b, h, m, n] = table[bucket(n - m - query_offset), h].
 
     Distances r have a bucket each up to half of a direction's buckets, and share the others evenly over their logarithm up to
-    max_distance, beyond which all have the last (relative_position_borders).  Bidirectional: r = |n - m - query_offset|, keys behind
+    max_distance, beyond which all have the last (relative_position_borders).  Bidirectional: r = |n - m - query_offset|, keys after
     the query's position take the second half of the table (whose size is even); otherwise later keys count as distance 0.  query_offset is the position of
     query 0 among the keys: seqlen_k - 1 for the last token alone.  `dtype`: of the bias, the table's own where not given; fp32, fp16 or
     bf16 each.  The table's gradient is summed over the batch in fp32, in a fixed order."""
@@ -677,7 +677,7 @@ def _philox_number(x, what, device):
 def dropout(x, dropout_p, residual=None, philox_seed=DEFAULT_PHILOX_SEED, philox_offset=DEFAULT_PHILOX_OFFSET_1):
     """residual + dropout(x), for hidden states of any shape: element i in logical order is kept (and divided by 1 - dropout_p) or dropped by word
     (0, 2, 1, 3)[i % 4] of Philox counter philox_offset + i // 4, the attention's generator and threshold.  The mask is never stored: the backward
-    draws it again.  A layer's calls take offsets at least x.numel() // 4 + 1 apart.
+    draws it again.  dropout_p is taken in 32 bits, as the attention takes it.  A layer's calls take offsets at least x.numel() // 4 + 1 apart.
 
     Seed and offset are numbers, or 64-bit tensors of one element on x's device, which a captured call reads when it is replayed.  x and residual
     (the same shape and type: fp32, fp16 or bf16) need no particular strides, but what is not rows of unit stride is copied first.

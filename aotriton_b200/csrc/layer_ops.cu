@@ -6,15 +6,15 @@
 // 2N of them, held in registers and shifted by one element a row.  16 heads x 2048 x 2048 bf16: 21.5 us, 6.2 TB/s.  The backward is bound by reading
 // the gradient once: a warp walks down the diagonals in steps of eight rows, between which a 16-byte vector moves by whole vectors, so that each of its
 // elements stays on its diagonal and one register a diagonal sums them; a CTA sums those of its band by buckets, and a second launch adds
-// the CTAs' sums up in a fixed order (no atomics: the result does not depend on who comes first).  8 x 16 x 2048 x 2048 bf16, 1.07 GB: 180 us,
-// 6.0 TB/s.  (Pieces of 8 x 8 elements with 15 diagonals' registers took 217, and rows that start anywhere another kernel.)
+// the CTAs' sums up in a fixed order (no atomics: the result does not depend on who comes first).  8 x 16 x 2048 x 2048 bf16, 1.07 GB: 185 to 188 us,
+// 5.7 to 5.8 TB/s.  Short rows are far from that: of 16 x 12 x 391 x 391 fp16 (27 us, 2.2 TB/s) 55 % of what the bands cover lies inside the matrix, and
+// nearly every step meets an edge.  (Pieces of 8 x 8 elements with 15 diagonals' registers took 217, and rows that start anywhere another kernel.)
 //
 // Dropout.  Element i in logical (row-major) order takes word (0, 2, 1, 3)[i % 4] of Philox counter offset + i / 4, as the columns of a
 // score row do (common.cuh): a mask follows from seed, offset and the logical index alone, not from strides, and is never stored; the
 // backward draws it again.  Ten rounds of the generator serve four elements, beside which two (with a residual three) elements' bytes each move: the
 // wide multiplies, four of a round's eight issue slots' worth, and the exclusive ors bound the form without a residual in 16-bit types, memory the
-// others.  64M elements of bf16: 57 us without a residual (4.7 TB/s), 64 with one (6.3 TB/s); fp32, 32M, 36.6 and 53 (7.3 and 7.6 TB/s, a part of it from
-// L2).  (Round keys added up by each thread 68 and 74; CTAs that take several tiles in turn 57 to 63 and 64 to 75.)
+// others.  64M elements of bf16: 55 to 58 us without a residual (4.6 to 4.9 TB/s), 65 with one (6.2 TB/s); fp32, 32M, 41 and 59 (6.6 and 6.8 TB/s).  (Round keys added up by each thread 68 and 74; CTAs that take several tiles in turn 57 to 63 and 64 to 75.)
 #include <algorithm>
 #include <type_traits>
 #include "launch.h"

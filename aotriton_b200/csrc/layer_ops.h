@@ -14,7 +14,7 @@ struct RelativeBias {
   void* table;                   // (buckets, heads): the table, or its gradient
   int64_t table_stride[2];
   int32_t heads, sq, sk, batch, offset;
-  int32_t per_direction, both;   // buckets of one direction; both: keys behind the query's position take the second half
+  int32_t per_direction, both;   // buckets of one direction; both: keys after the query's position take the second half
   int32_t borders[kMaxBorders];  // borders[k - 1]: the smallest distance whose bucket is k or more
   float* partial;                // backward: bucket sums of each CTA
   int32_t strips, bands, chunks, chunk_rows;

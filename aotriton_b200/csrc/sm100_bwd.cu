@@ -20,7 +20,8 @@
 //
 //   dK/dV, per query block i:   S^T = K Q_i^T      dP^T = V dO_i^T        (operands in smem)
 //                               P^T, dS^T computed in registers, written back over S^T / dP^T
-//                               as packed 16-bit
+//                               as packed 16-bit (the inputs' type, which the tensor pipe takes: half a step off each,
+//                               2^-8 of it in bf16; the sums over them are fp32)
 //                               dV += P^T dO_i     dK += dS^T Q_i         (A from TMEM)
 //   dQ, per key block i:        S = Q K_i^T        dP = dO V_i^T
 //                               dQ += dS K_i       dB = dS
@@ -932,8 +933,9 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
   }
 }
 
-// dK and dV of the first keys: the sums of the items that shared their queries, in the items' order.  A few hundred kilobytes at most,
-// in L2.  grid = (sinks, Hk, batch), a thread four columns.
+// dK and dV of the first keys: the sums of the items that shared their queries, in the items' order.  They are batch * Hk * (sink_chunks + 1) * sinks *
+// (dqk + dvo) floats: 0.3 MB with 4 first keys, 8 kv heads of 128 and 8 chunks, in L2, and growing with the first keys.  grid = (sinks, Hk, batch), a
+// thread four columns.
 template <typename T>
 __global__ void __launch_bounds__(128) sink_finish_kernel(const __grid_constant__ Params p) {
   wait_for_earlier_grids();

@@ -17,7 +17,7 @@
 // of the second resident tile); "late" tiles also feed the accumulating GEMM at the block's end and
 // live in two stages, so the dP' / S' GEMMs of block i+1 run while the compute warps work on block i.
 // Shared memory: 2 x 64 KB resident, 2 x 32 KB late, 32 KB early.  Tensor memory: [0,64) S', [64,128) and [128,192) two dP' buffers, whose first columns
-// then take the packed 16-bit P' / dS' (the A operand of the accumulating GEMM), [256,512) the
+// then take the packed 16-bit P' / dS' (the A operand of the accumulating GEMM, rounded to the inputs' type as in the 128-wide kernels), [256,512) the
 // accumulator; with two compute groups [0,64) and [64,128) a buffer of S' each, [128,192) and [192,256) those of P'.  Twelve warps: TMA producer, MMA issuer, logsumexp/delta stager (dV, dK), one idle,
 // eight compute warps (thread = one row of the 128 x 64 score tile, two warpgroups split its columns
 // 32 apiece); dV with bias and dropout has eight more and two S' buffers (wide_groups).  The arithmetic is that of the 128-wide kernels (see the head of sm100_bwd.cu); dK and dV

@@ -312,7 +312,7 @@ sm100_fwd_decode_kernel(const __grid_constant__ Params p, const __grid_constant_
           for (int j = 0; j < 2; ++j) {
             const float e0 = ex2(sc[t][j][2 * half] - ms), e1 = ex2(sc[t][j][2 * half + 1] - ms);
             sum += e0 + e1;
-            pa[t][2 * j + half] = pack2<T>(e0, e1);
+            pa[t][2 * j + half] = pack2<T>(e0, e1);      // (the type the products take: half a step off; the sum keeps 32 bits)
           }
           l_run[2 * t + half] += sum;      // this lane's columns; the quad's sums meet after the stream
         }

@@ -304,7 +304,7 @@ sm100_fwd_sink_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         const float2 a = fma2(make_float2(sc[c], sc[c + 1]), scale2, nm2);      // (times 1 is exact)
         const float2 e = make_float2(ex2(a.x), ex2(a.y));
         s4[(c >> 1) & 3] = add2(s4[(c >> 1) & 3], e);
-        pk[c >> 1] = pack2<T>(e.x, e.y);
+        pk[c >> 1] = pack2<T>(e.x, e.y);      // (the type the tensor pipe takes: half a step off, 2^-8 of P in bf16; the sum keeps 32 bits)
       }
       tmem_st32(s_addr, pk);
       l = l * alpha + (((s4[0].x + s4[0].y) + (s4[1].x + s4[1].y)) + ((s4[2].x + s4[2].y) + (s4[3].x + s4[3].y)));
