@@ -694,3 +694,73 @@ def dropout(x, dropout_p, residual=None, philox_seed=DEFAULT_PHILOX_SEED, philox
             return r
     seed, offset = _philox_number(philox_seed, "philox_seed", x.device), _philox_number(philox_offset, "philox_offset", x.device)
     return _apply(_Dropout, x, residual, float(dropout_p), seed, offset)
+
+
+class _JoinColumns(torch.autograd.Function):
+    """(k, shared) head by head: keys whose last columns all heads share."""
+
+    @staticmethod
+    @_on_its_device
+    def forward(ctx, k, shared):
+        b, h, s, dn = k.shape
+        joined = torch.empty((b, s, h, dn + shared.shape[3]), device=k.device, dtype=k.dtype).transpose(1, 2)
+        if joined.numel():
+            stream = torch.cuda.current_stream(k.device).cuda_stream
+            _check(hipError_t(cabi.shared_columns("join", k, shared, joined, stream=stream)), "join_columns")
+        ctx.width = dn
+        return joined
+
+    @staticmethod
+    def backward(ctx, grad):
+        return grad[..., :ctx.width], _SumColumns.apply(grad, ctx.width) if ctx.needs_input_grad[1] else None
+
+
+class _SumColumns(torch.autograd.Function):
+    """The sum over the heads of the columns from `width` on."""
+
+    @staticmethod
+    @_on_its_device
+    def forward(ctx, grad, width):
+        grad = _unit_rows(grad)
+        b, h, s, d = grad.shape
+        ctx.args = (h, width)
+        shared = torch.empty((b, 1, s, d - width), device=grad.device, dtype=grad.dtype)
+        if shared.numel():
+            stream = torch.cuda.current_stream(grad.device).cuda_stream
+            _check(hipError_t(cabi.shared_columns("sum", None, shared, grad, stream=stream)), "sum_columns")
+        return shared
+
+    @staticmethod
+    def backward(ctx, grad):
+        h, width = ctx.args
+        return torch.nn.functional.pad(grad.expand(-1, h, -1, -1), (width, 0)), None
+
+
+def _join_shared(q, k, k_shared, v, what):
+    for t in (q, k, k_shared, v):
+        if t.dim() != 4 or t.dtype not in _FLOATS or not t.is_cuda or t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{what}: q, k, k_shared and v are (batch, heads, tokens, dim) CUDA tensors of one device and type, fp32, fp16 or bf16")
+    if (k_shared.shape[0], *k_shared.shape[1:3]) != (k.shape[0], 1, k.shape[2]) or v.shape[:3] != k.shape[:3] or k.shape[0] != q.shape[0]:
+        raise ValueError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(k_shared.shape)}, {tuple(v.shape)} do not go together")
+    if not k.shape[1] or q.shape[1] % k.shape[1] or not k.shape[3] or not k_shared.shape[3] or q.shape[3] != k.shape[3] + k_shared.shape[3]:
+        raise ValueError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(k_shared.shape)} do not go together: a query is as wide as a head's key and the "
+                         "shared columns")
+    if q.shape[3] > 512 or not 1 <= v.shape[3] <= 512:
+        raise ValueError(f"{what}: head dims from 1 to 512 are supported")
+    return _apply(_JoinColumns, _unit_rows(k), _unit_rows(k_shared))
+
+
+def latent_attention(q, k, k_shared, v, causal=False, sm_scale=None, return_lse=False):
+    """Latent attention in its expanded form, for prompts and training: `attention` whose heads' keys are their own columns, expanded from a token's latent
+    vector, followed by columns that all heads share (its position columns).  q: (B, H, Sq, dn + dr), k: (B, Hk, Sk, dn), k_shared: (B, 1, Sk, dr),
+    v: (B, Hk, Sk, dv), of any strides; causal as for `attention`; sm_scale: (dn + dr) ** -0.5 where not given.  The gradient of k_shared is summed over the heads in fp32, in
+    their order.  paged.paged_latent_attention decodes from the latent vectors themselves."""
+    joined = _join_shared(q, k, k_shared, v, "latent_attention")
+    return attention(_unit_rows(q), joined, _unit_rows(v), causal=causal, sm_scale=sm_scale, return_lse=return_lse)
+
+
+def varlen_latent_attention(q, k, k_shared, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=False, sm_scale=None, return_lse=False):
+    """latent_attention over token-packed sequences, (1, H, tokens, dim) tensors, as varlen_attention has them."""
+    joined = _join_shared(q, k, k_shared, v, "varlen_latent_attention")
+    return varlen_attention(_unit_rows(q), joined, _unit_rows(v), cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=causal, sm_scale=sm_scale,
+                            return_lse=return_lse)

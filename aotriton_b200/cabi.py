@@ -24,7 +24,8 @@ SYMBOLS = [
     "ab200_bwd_fused", "ab200_bwd_postprocess", "ab200_bwd_preprocess", "ab200_bwd_dkdv", "ab200_bwd_dq",
     "ab200_debug_simulate_encoded_softmax", "ab200_sink_attn_fwd", "ab200_sink_attn_bwd",
     "ab200_sink_attn_bwd_workspace", "ab200_relative_bias_fwd", "ab200_relative_bias_bwd",
-    "ab200_relative_bias_workspace", "ab200_dropout", "ab200_check_gpu", "ab200_multiprocessor_count",
+    "ab200_relative_bias_workspace", "ab200_dropout", "ab200_block_tables", "ab200_paged_write", "ab200_paged_attn",
+    "ab200_paged_attn_workspace", "ab200_join_columns", "ab200_sum_columns", "ab200_check_gpu", "ab200_multiprocessor_count",
     "ab200_set_kernel_family", "ab200_select_variant", "ab200_last_fwd_family", "ab200_last_bwd_family",
     "ab200_kernel_status", "ab200_stream_check", "ab200_debug_bounded_wait_test", "ab200_debug_keep_tiles",
     "ab200_debug_dk_from_dbias", "ab200_debug_split_keys",
@@ -83,6 +84,37 @@ class DropoutArgs(C.Structure):
     ]
 
 
+class BlockTablesArgs(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int32), ("page_size", C.c_int32), ("table_width", C.c_int32), ("block_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("lengths", C.c_void_p), ("new_tokens", C.c_void_p), ("free_pages", C.c_void_p), ("num_free", C.c_int64), ("taken", C.c_void_p),
+        ("total_tokens", C.c_int64), ("slots", C.c_void_p), ("cu_seqlens", C.c_void_p), ("new_lengths", C.c_void_p), ("taken_out", C.c_void_p),
+    ]
+
+
+class PagedWriteArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("num_heads", C.c_int32), ("head_dim_k", C.c_int32), ("head_dim_v", C.c_int32), ("page_size", C.c_int32),
+        ("num_pages", C.c_int64), ("tokens", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 2),
+        ("v_stride", C.c_int64 * 2), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_cache_stride", C.c_int64 * 3),
+        ("v_cache_stride", C.c_int64 * 3), ("slots", C.c_void_p),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("batch", C.c_int32), ("num_head_q", C.c_int32), ("num_head_k", C.c_int32), ("seqlen_q", C.c_int32),
+        ("head_dim_qk", C.c_int32), ("head_dim_vo", C.c_int32), ("page_size", C.c_int32), ("sm_scale", C.c_float), ("window", C.c_int32),
+        ("sinks", C.c_int32), ("q", View4), ("out", View4), ("k_cache", View4), ("v_cache", View4), ("block_table", C.c_void_p),
+        ("table_stride", C.c_int64), ("table_width", C.c_int32), ("lengths", C.c_void_p), ("query_lengths", C.c_void_p), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_floats", C.c_uint64),
+    ]
+
+
+class SharedColumnsArgs(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("k", View4), ("shared", View4), ("joined", View4)]
+
+
 _lib = None
 
 
@@ -109,6 +141,11 @@ def lib() -> C.CDLL:
             getattr(L, name).argtypes = [C.POINTER(RelativeBiasArgs), C.c_void_p]
         L.ab200_relative_bias_workspace.restype = C.c_int64
         L.ab200_dropout.argtypes = [C.POINTER(DropoutArgs), C.c_void_p]
+        L.ab200_block_tables.argtypes = [C.POINTER(BlockTablesArgs), C.c_void_p]
+        L.ab200_paged_write.argtypes = [C.POINTER(PagedWriteArgs), C.c_void_p]
+        L.ab200_paged_attn.argtypes = L.ab200_paged_attn_workspace.argtypes = [C.POINTER(PagedAttnArgs), C.c_void_p]
+        L.ab200_paged_attn_workspace.restype = C.c_int64
+        L.ab200_join_columns.argtypes = L.ab200_sum_columns.argtypes = [C.POINTER(SharedColumnsArgs), C.c_void_p]
         L.ab200_check_gpu.argtypes = [C.c_void_p]
         L.ab200_multiprocessor_count.argtypes = [C.c_void_p]
         L.ab200_select_variant.argtypes = [C.c_int] * 5
@@ -289,3 +326,71 @@ def dropout(x, out, dropout_p, *, residual=None, philox_seed=None, philox_offset
     a.philox_seed, a.philox_offset1 = _ptr(philox_seed), _ptr(philox_offset1)
     a.philox_seed_value, a.philox_offset2 = philox_seed_value, philox_offset2
     return lib().ab200_dropout(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def make_block_tables_args(block_table, lengths, new_tokens, free_pages, page_size, slots, cu_seqlens, new_lengths, taken_out, *, taken=None) -> BlockTablesArgs:
+    a = BlockTablesArgs()
+    a.batch, a.table_width = block_table.shape
+    a.page_size, a.block_table, a.table_stride = page_size, _ptr(block_table), block_table.stride(0)
+    a.lengths, a.new_tokens = _ptr(lengths), _ptr(new_tokens)
+    a.free_pages, a.num_free, a.taken = _ptr(free_pages), free_pages.numel(), _ptr(taken)
+    a.total_tokens, a.slots = slots.numel(), _ptr(slots)
+    a.cu_seqlens, a.new_lengths, a.taken_out = _ptr(cu_seqlens), _ptr(new_lengths), _ptr(taken_out)
+    return a
+
+
+def block_tables(*args, stream=None, **kw) -> int:
+    a = make_block_tables_args(*args, **kw)
+    return lib().ab200_block_tables(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def make_paged_write_args(k, v, k_cache, v_cache, slots) -> PagedWriteArgs:
+    """k, v: (tokens, heads, dim); the caches (pages, page_size, heads, dim); v and v_cache may be None."""
+    a = PagedWriteArgs()
+    a.dtype = _torch_dtype_code(k)
+    a.tokens, a.num_heads, a.head_dim_k = k.shape
+    a.num_pages, a.page_size = k_cache.shape[:2]
+    a.k, a.k_cache, a.slots = _ptr(k), _ptr(k_cache), _ptr(slots)
+    a.k_stride[:], a.k_cache_stride[:] = k.stride()[:2], k_cache.stride()[:3]
+    if v is not None:
+        a.head_dim_v, a.v, a.v_cache = v.shape[2], _ptr(v), _ptr(v_cache)
+        a.v_stride[:], a.v_cache_stride[:] = v.stride()[:2], v_cache.stride()[:3]
+    return a
+
+
+def paged_write(k, v, k_cache, v_cache, slots, *, stream=None) -> int:
+    a = make_paged_write_args(k, v, k_cache, v_cache, slots)
+    return lib().ab200_paged_write(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def make_paged_attn_args(q, k_cache, v_cache, block_table, lengths, out, *, sm_scale, window=0, sinks=0, query_lengths=None, lse=None,
+                         workspace=None) -> PagedAttnArgs:
+    a = PagedAttnArgs()
+    a.dtype = _torch_dtype_code(q)
+    a.batch, a.num_head_q, a.seqlen_q, a.head_dim_qk = q.shape
+    a.page_size, a.num_head_k, a.head_dim_vo = k_cache.shape[1], k_cache.shape[2], v_cache.shape[3]
+    a.sm_scale, a.window, a.sinks = sm_scale, window, sinks
+    a.q, a.out, a.k_cache, a.v_cache = view4(q), view4(out), view4(k_cache), view4(v_cache)
+    a.block_table, a.table_stride, a.table_width = _ptr(block_table), block_table.stride(0), block_table.shape[1]
+    a.lengths, a.query_lengths, a.lse = _ptr(lengths), _ptr(query_lengths), _ptr(lse)
+    if workspace is not None:
+        a.workspace, a.workspace_floats = _ptr(workspace), workspace.numel()
+    return a
+
+
+def paged_attn_workspace(*args, stream=None, **kw) -> int:
+    """Floats the call needs; negative: an error code."""
+    a = make_paged_attn_args(*args, **kw)
+    return lib().ab200_paged_attn_workspace(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def paged_attn(*args, stream=None, **kw) -> int:
+    a = make_paged_attn_args(*args, **kw)
+    return lib().ab200_paged_attn(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def shared_columns(entry, k, shared, joined, *, stream=None) -> int:
+    """entry "join": joined = (k, shared) head by head; "sum": shared = the sum over heads of joined's last columns (k: None)."""
+    a = SharedColumnsArgs()
+    a.dtype, a.k, a.shared, a.joined = _torch_dtype_code(joined), view4(k), view4(shared), view4(joined)
+    return getattr(lib(), f"ab200_{entry}_columns")(C.byref(a), stream if stream is not None else current_stream_handle())

@@ -16,6 +16,7 @@
 #include "../../include/aotriton_b200.h"
 #include "launch.h"
 #include "layer_ops.h"
+#include "paged.h"
 
 namespace ab200 {
 
@@ -984,6 +985,152 @@ int ab200_dropout(const ab200_dropout_args* a, void* stream) {
   if (int e = check_device(st)) return e;
   DeviceGuard guard(st);
   return (int)launch_dropout(a->dtype, d, st);
+}
+
+// --- a cache in pages (paged.cu) -----------------------------------------------------------------
+int ab200_block_tables(const ab200_block_tables_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a == nullptr || a->batch < 0 || a->page_size < 1 || a->table_width < 0 || a->num_free < 0 || a->total_tokens < 0) return kErrInvalidValue;
+  if (a->cu_seqlens == nullptr || a->taken_out == nullptr || (a->total_tokens > 0 && a->slots == nullptr)) return kErrInvalidValue;
+  if (a->batch > 0 && (a->lengths == nullptr || a->new_tokens == nullptr || a->new_lengths == nullptr)) return kErrInvalidValue;
+  if ((a->batch > 0 && a->table_width > 0 && a->block_table == nullptr) || (a->num_free > 0 && a->free_pages == nullptr)) return kErrInvalidValue;
+  if (a->total_tokens > INT32_MAX) return kErrNotSupported;
+  BlockTables b{};
+  b.batch = a->batch; b.page = a->page_size; b.width = a->table_width; b.total = a->total_tokens; b.table_stride = a->table_stride; b.num_free = a->num_free;
+  b.table = a->block_table; b.lengths = a->lengths; b.new_tokens = a->new_tokens; b.free_pages = a->free_pages; b.taken = a->taken;
+  b.slots = a->slots; b.cu_seqlens = a->cu_seqlens; b.new_lengths = a->new_lengths; b.taken_out = a->taken_out;
+  if (int e = check_device(st)) return e;
+  DeviceGuard guard(st);
+  return (int)launch_block_tables(b, st);
+}
+
+int ab200_paged_write(const ab200_paged_write_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a == nullptr || a->num_heads < 1 || a->head_dim_k < 1 || a->head_dim_v < 0 || a->page_size < 1 || a->num_pages < 0 || a->tokens < 0) return kErrInvalidValue;
+  if (a->dtype < AB200_DTYPE_FP32 || a->dtype > AB200_DTYPE_BF16) return kErrNotSupported;
+  if (a->tokens == 0 || a->num_pages == 0) return 0;
+  if (a->k == nullptr || a->k_cache == nullptr || a->slots == nullptr || (a->head_dim_v > 0 && (a->v == nullptr || a->v_cache == nullptr))) return kErrInvalidValue;
+  if ((int64_t)a->num_heads * ((int64_t)a->head_dim_k + a->head_dim_v) > 1 << 24 || a->tokens > INT32_MAX || a->num_pages > INT64_MAX / a->page_size)
+    return kErrNotSupported;
+  PagedWrite w{};
+  w.tokens = a->tokens; w.slots_total = a->num_pages * a->page_size; w.page = a->page_size; w.heads = a->num_heads; w.dk = a->head_dim_k; w.dv = a->head_dim_v;
+  w.k = a->k; w.v = a->v; w.k_cache = a->k_cache; w.v_cache = a->v_cache; w.slots = a->slots;
+  for (int i = 0; i < 2; ++i) { w.sk[i] = a->k_stride[i]; w.sv[i] = a->v_stride[i]; }
+  for (int i = 0; i < 3; ++i) { w.ck[i] = a->k_cache_stride[i]; w.cv[i] = a->v_cache_stride[i]; }
+  // the widest vector that every row allows
+  const int elt = a->dtype == AB200_DTYPE_FP32 ? 4 : 2;
+  const int64_t extent[3] = {a->num_pages, a->page_size, a->num_heads}, rows[2] = {a->tokens, a->num_heads};
+  auto allows = [&](int bytes) {
+    auto fits = [&](const void* p, int dim, const int64_t* n, const int64_t* s, int rank) {
+      if (reinterpret_cast<uintptr_t>(p) % bytes != 0 || (int64_t)dim * elt % bytes != 0) return false;
+      for (int i = 0; i < rank; ++i)
+        if (n[i] > 1 && s[i] * elt % bytes != 0) return false;
+      return true;
+    };
+    return fits(w.k, w.dk, rows, w.sk, 2) && fits(w.k_cache, w.dk, extent, w.ck, 3) &&
+           (w.dv == 0 || (fits(w.v, w.dv, rows, w.sv, 2) && fits(w.v_cache, w.dv, extent, w.cv, 3)));
+  };
+  w.vec = allows(16) ? 16 : (elt == 4 || allows(4) ? 4 : 2);
+  if (!allows(elt)) return kErrInvalidValue;      // (addresses are multiples of the elements' size)
+  if (int e = check_device(st)) return e;
+  DeviceGuard guard(st);
+  return (int)launch_paged_write(a->dtype, w, st);
+}
+
+static int fill_paged(const ab200_paged_attn_args* a, PagedAttn& p) {
+  if (a == nullptr) return kErrInvalidValue;
+  if (a->dtype < AB200_DTYPE_FP32 || a->dtype > AB200_DTYPE_BF16) return kErrNotSupported;
+  if (a->batch < 0 || a->num_head_q < 1 || a->num_head_k < 1 || a->num_head_q % a->num_head_k != 0 || a->seqlen_q < 0 || a->page_size < 1 ||
+      a->table_width < 0 || a->window < 0 || a->sinks < 0 || a->head_dim_qk < 1 || a->head_dim_vo < 1)
+    return kErrInvalidValue;
+  if (a->head_dim_qk > 1024 || a->head_dim_vo > 1024) return kErrNotSupported;
+  const int64_t* n = a->k_cache.size;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] != a->v_cache.size[i]) return kErrInvalidValue;
+  if (n[0] < 0 || n[1] != a->page_size || n[2] != a->num_head_k) return kErrInvalidValue;
+  if (n[0] > INT32_MAX || (int64_t)a->num_head_q * a->seqlen_q > 1 << 30 || (int64_t)a->num_head_q * a->seqlen_q * a->batch > INT32_MAX) return kErrNotSupported;
+  if (a->batch > 0 && a->seqlen_q > 0) {
+    if (a->q.ptr == nullptr || a->out.ptr == nullptr || a->lengths == nullptr || (a->table_width > 0 && a->block_table == nullptr)) return kErrInvalidValue;
+    if (n[0] > 0 && (a->k_cache.ptr == nullptr || a->v_cache.ptr == nullptr)) return kErrInvalidValue;
+  }
+  for (const ab200_view4* v : {&a->q, &a->out, &a->k_cache, &a->v_cache}) {
+    if (!inner_contiguous(*v)) return kErrInvalidValue;
+    if (reinterpret_cast<uintptr_t>(v->ptr) % (a->dtype == AB200_DTYPE_FP32 ? 4 : 2) != 0) return kErrInvalidValue;
+  }
+  p.q = to_view(a->q); p.out = to_view(a->out); p.k = to_view(a->k_cache); p.v = to_view(a->v_cache);
+  p.q.n[0] = p.out.n[0] = a->batch; p.q.n[1] = p.out.n[1] = a->num_head_q; p.q.n[2] = p.out.n[2] = a->seqlen_q;
+  p.q.n[3] = p.k.n[3] = a->head_dim_qk; p.out.n[3] = p.v.n[3] = a->head_dim_vo;
+  p.table = a->block_table; p.table_stride = a->table_stride; p.width = a->table_width; p.page = a->page_size; p.num_pages = (int32_t)n[0];
+  p.lengths = a->lengths; p.query_lengths = a->query_lengths; p.lse = a->lse;
+  p.batch = a->batch; p.hq = a->num_head_q; p.hk = a->num_head_k; p.group = a->num_head_q / a->num_head_k; p.sq = a->seqlen_q;
+  p.dqk = a->head_dim_qk; p.dvo = a->head_dim_vo; p.qk_scale = a->sm_scale * kLog2e;
+  p.window = a->window > 0 ? a->window : INT32_MAX;
+  p.sinks = a->window > 0 ? a->sinks : 0;
+  p.wait_limit_kcycles = t_wait_limit_kcycles; p.drop_copy = t_drop_copy;
+  return 0;
+}
+
+int64_t ab200_paged_attn_workspace(const ab200_paged_attn_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  PagedAttn p{};
+  if (int e = fill_paged(a, p)) return -e;
+  if (int e = check_device(st)) return -e;
+  if (p.batch == 0 || p.sq == 0) return 0;
+  return plan_paged(a->dtype, p, device_info(stream_device(st)).sms);
+}
+
+int ab200_paged_attn(const ab200_paged_attn_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  PagedAttn p{};
+  if (int e = fill_paged(a, p)) return e;
+  if (int e = check_device(st)) return e;
+  if (p.batch == 0 || p.sq == 0) return 0;
+  const int64_t need = plan_paged(a->dtype, p, device_info(stream_device(st)).sms);
+  if (need > 0 && (a->workspace == nullptr || a->workspace_floats < (uint64_t)need || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0))
+    return kErrInvalidValue;
+  p.partial = a->workspace;
+  DeviceGuard guard(st);
+  return (int)launch_paged(a->dtype, p, st);
+}
+
+// --- keys that share columns (paged.cu) -----------------------------------------------------------
+static int fill_shared_columns(const ab200_shared_columns_args* a, SharedColumns& s, bool gradient) {
+  if (a == nullptr) return kErrInvalidValue;
+  if (a->dtype < AB200_DTYPE_FP32 || a->dtype > AB200_DTYPE_BF16) return kErrNotSupported;
+  s.k = to_view(a->k); s.shared = to_view(a->shared); s.out = to_view(a->joined);
+  const View4 &r = s.shared, &o = s.out;
+  for (const View4* v : {&r, &o})
+    for (int i = 0; i < 4; ++i)
+      if (v->n[i] < 0 || v->n[i] > INT32_MAX) return kErrInvalidValue;
+  if (r.n[0] != o.n[0] || r.n[1] != 1 || r.n[2] != o.n[2] || r.n[3] < 1 || r.n[3] >= o.n[3]) return kErrInvalidValue;
+  if (!gradient && (s.k.n[0] != o.n[0] || s.k.n[1] != o.n[1] || s.k.n[2] != o.n[2] || s.k.n[3] != o.n[3] - r.n[3])) return kErrInvalidValue;
+  const int elt = a->dtype == AB200_DTYPE_FP32 ? 4 : 2;
+  for (const ab200_view4* v : {&a->k, &a->shared, &a->joined}) {
+    if (v == &a->k && gradient) continue;
+    const bool empty = v->size[0] == 0 || v->size[1] == 0 || v->size[2] == 0;
+    if (v->stride[3] != 1 || reinterpret_cast<uintptr_t>(v->ptr) % elt != 0 || (!empty && v->ptr == nullptr)) return kErrInvalidValue;
+  }
+  return 0;
+}
+
+int ab200_join_columns(const ab200_shared_columns_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  SharedColumns s{};
+  if (int e = fill_shared_columns(a, s, false)) return e;
+  if (int e = check_device(st)) return e;
+  if (s.out.n[0] == 0 || s.out.n[1] == 0 || s.out.n[2] == 0) return 0;
+  DeviceGuard guard(st);
+  return (int)launch_join_columns(a->dtype, s, st);
+}
+
+int ab200_sum_columns(const ab200_shared_columns_args* a, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  SharedColumns s{};
+  if (int e = fill_shared_columns(a, s, true)) return e;
+  if (int e = check_device(st)) return e;
+  if (s.shared.n[0] == 0 || s.shared.n[2] == 0) return 0;
+  DeviceGuard guard(st);
+  return (int)launch_sum_columns(a->dtype, s, st);
 }
 
 // --- HIP-named runtime helpers used by the Python tests of the reference

@@ -1,0 +1,505 @@
+// Operators over a cache in pages: block tables and slot maps, the writing of new tokens, attention for any type and size, the sum of a split
+// sequence's pieces; and keys whose last columns all heads share.
+#include <algorithm>
+#include "launch.h"
+#include "paged.h"
+#include "paged_split.cuh"
+
+namespace ab200 {
+namespace {
+
+// ---- block tables and slot maps --------------------------------------------------------------------------------
+// Sequence z holds n tokens and takes m more; token i of them stands at position n + i, in page (n + i) / page of its row.  Pages that it has not
+// got yet are the next of the free list, in order of sequence and position, so that a token finds its page from two running sums over the sequences
+// ahead of it: tokens, which say whose it is, and pages taken.  Every CTA adds those up for itself, as far as its own tokens; nothing waits
+// for anything, and one launch does.
+constexpr int kTableThreads = 256, kTableTokens = 2048;
+
+__global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const __grid_constant__ BlockTables a) {
+  wait_for_earlier_grids();
+  __shared__ int64_t warp_tokens[kTableThreads / 32], warp_pages[kTableThreads / 32];
+  __shared__ int64_t start[kTableThreads], fresh[kTableThreads];
+  __shared__ int held[kTableThreads];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t t0 = (int64_t)blockIdx.x * kTableTokens, t1 = min(t0 + kTableTokens, a.total);
+  const bool sums = blockIdx.x == 0;
+  int64_t tokens = 0, pages = a.taken != nullptr ? max(a.taken[0], 0) : 0;      // of the sequences so far
+  for (int z0 = 0; z0 < a.batch && (sums || tokens < t1); z0 += kTableThreads) {
+    const int z = z0 + tid;
+    int n = 0, m = 0;
+    int64_t need = 0;
+    if (z < a.batch) {
+      n = max(a.lengths[z], 0);
+      m = max(a.new_tokens[z], 0);
+      const int64_t have = min(((int64_t)n + a.page - 1) / a.page, (int64_t)a.width);
+      need = min(((int64_t)n + m + a.page - 1) / a.page, (int64_t)a.width) - have;
+    }
+    int64_t up_t = m, up_p = need;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, up_t, d), y = __shfl_up_sync(0xffffffffu, up_p, d);
+      if (lane >= d) { up_t += x; up_p += y; }
+    }
+    __syncthreads();      // (the last chunk's tokens have been found)
+    if (lane == 31) { warp_tokens[warp] = up_t; warp_pages[warp] = up_p; }
+    __syncthreads();
+    int64_t all_t = 0, all_p = 0;
+    for (int w = 0; w < kTableThreads / 32; ++w) {
+      if (w < warp) { up_t += warp_tokens[w]; up_p += warp_pages[w]; }
+      all_t += warp_tokens[w];
+      all_p += warp_pages[w];
+    }
+    start[tid] = tokens + up_t - m;
+    fresh[tid] = pages + up_p - need;
+    held[tid] = n;
+    if (sums && z < a.batch) {
+      if (z == 0) a.cu_seqlens[0] = 0;
+      a.cu_seqlens[z + 1] = (int)min(tokens + up_t, (int64_t)0x7fffffff);
+      a.new_lengths[z] = (int)min((int64_t)n + m, (int64_t)0x7fffffff);
+    }
+    __syncthreads();
+    const int64_t end = min(tokens + all_t, t1);
+    for (int64_t t = max(tokens, t0) + tid; t < end; t += kTableThreads) {
+      int lo = 0, hi = kTableThreads - 1;      // the last sequence that starts at or ahead of the token: it has tokens, those behind it start later
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (start[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      const int64_t p = (int64_t)held[lo] + (t - start[lo]), page = p / a.page, have = min(((int64_t)held[lo] + a.page - 1) / a.page, (int64_t)a.width);
+      int64_t id = -1;
+      if (page < a.width) {
+        int32_t* entry = a.table + (int64_t)(z0 + lo) * a.table_stride + page;
+        if (page < have) {
+          id = *entry;
+        } else {
+          const int64_t i = fresh[lo] + page - have;
+          id = i < a.num_free ? a.free_pages[i] : -1;
+          if (p % a.page == 0) *entry = (int)id;      // (a page's first token enters it)
+        }
+      }
+      a.slots[t] = id < 0 ? -1 : id * a.page + p % a.page;
+    }
+    tokens += all_t;
+    pages += all_p;
+  }
+  for (int64_t t = max(tokens, t0) + tid; t < t1; t += kTableThreads) a.slots[t] = -1;
+  if (sums && tid == 0) {
+    if (a.batch == 0) a.cu_seqlens[0] = 0;
+    a.taken_out[0] = (int)min(pages, (int64_t)0x7fffffff);
+  }
+}
+
+// ---- new tokens into their slots --------------------------------------------------------------------------------
+// Rows are moved as they are: bound by their bytes, read once and written once.  A CTA takes a few tokens' rows, each thread kWriteBatch vectors whose
+// loads are on the way together.
+constexpr int kWriteThreads = 256, kWriteBatch = 4;
+
+template <typename V>
+__global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const __grid_constant__ PagedWrite a, int elt, int64_t vectors) {
+  wait_for_earlier_grids();
+  const int per = (int)sizeof(V) / elt;      // elements of a vector
+  const int vk = a.dk / per, vv = a.dv / per, of_k = a.heads * vk, of_token = of_k + a.heads * vv;
+  const int64_t first = ((int64_t)blockIdx.x * kWriteBatch * kWriteThreads) + threadIdx.x;
+  V value[kWriteBatch];
+  V* to[kWriteBatch];
+#pragma unroll
+  for (int b = 0; b < kWriteBatch; ++b) {
+    const int64_t i = first + b * kWriteThreads;
+    to[b] = nullptr;
+    if (i >= vectors) continue;
+    const int64_t t = i / of_token;
+    int e = (int)(i - t * of_token);
+    const int64_t slot = a.slots[t];
+    if (slot < 0 || slot >= a.slots_total) continue;
+    const int64_t page = slot / a.page, in = slot - page * a.page;
+    const bool is_k = e < of_k;
+    if (!is_k) e -= of_k;
+    const int wide = is_k ? vk : vv, h = e / wide, c = e - h * wide;
+    const int64_t from = t * (is_k ? a.sk[0] : a.sv[0]) + h * (is_k ? a.sk[1] : a.sv[1]) + (int64_t)c * per;
+    const int64_t dst = page * (is_k ? a.ck[0] : a.cv[0]) + in * (is_k ? a.ck[1] : a.cv[1]) + h * (is_k ? a.ck[2] : a.cv[2]) + (int64_t)c * per;
+    value[b] = *reinterpret_cast<const V*>(reinterpret_cast<const char*>(is_k ? a.k : a.v) + from * elt);
+    to[b] = reinterpret_cast<V*>(reinterpret_cast<char*>(is_k ? a.k_cache : a.v_cache) + dst * elt);
+  }
+#pragma unroll
+  for (int b = 0; b < kWriteBatch; ++b)
+    if (to[b] != nullptr) *to[b] = value[b];
+}
+
+// ---- attention, any type and size up to 1024 ----------------------------------------------------------------------
+// Tiles of 32 keys: eight lanes form a key's scores with the unit's rows, a warp a row takes their softmax on, and a thread a column adds up
+// the values; with fewer columns than threads, groups of threads share the keys.
+constexpr int kGenThreads = 256, kGenRows = 8, kGenKeys = 32, kGenMaxDim = 1024;
+
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* src, float (&x)[N]) {
+  if constexpr (N == 1) {
+    x[0] = to_f32<T>(*src);
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(src);
+    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = to_f32<T>(e[i]);
+  }
+}
+
+// J: columns of a thread.  N: elements of K that a lane reads at a time.
+template <typename T, int N, int J>
+__global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid_constant__ PagedAttn p) {
+  wait_for_earlier_grids();
+  extern __shared__ float q_s[];      // [kGenRows][dqk]
+  __shared__ float s[kGenRows][kGenKeys], alpha[kGenRows], m_s[kGenRows], l_s[kGenRows];
+  __shared__ float meet[J == 1 ? kGenThreads * kGenRows : 1];
+  __shared__ int64_t page_of[kGenKeys], scratch[kGenThreads / 32 + 4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Line line = find_in_line<kGenThreads>(p, -1, blockIdx.x, scratch);
+  if (line.z >= p.batch) return;
+  int64_t at = (int64_t)blockIdx.x * line.share;
+  const int64_t end = min(at + line.share, line.total);
+  int width = 32;      // threads that share the columns
+  while (width < p.dvo && width < kGenThreads) width <<= 1;
+  const int groups = kGenThreads / width, group = tid / width, col = tid - group * width;
+  int z = line.z;
+  int64_t base = line.base;
+  Walk w(p, z);
+  while (at < end) {
+    while (at >= base + (int64_t)w.tiles * p.hk * p.chunks) {
+      base += (int64_t)w.tiles * p.hk * p.chunks;
+      w = Walk(p, ++z);
+    }
+    const int u = (int)((at - base) / w.tiles), hk = u / p.chunks, chunk = u - hk * p.chunks;
+    const int64_t unit = base + (int64_t)u * w.tiles;
+    const int first = (int)(at - unit), last = (int)(min(end, unit + w.tiles) - unit);
+    at = unit + last;
+    const bool whole = first == 0 && last == w.tiles;
+    const Rows rows(p, w, chunk);
+    if (first == 0 && chunk == 0) zero_rows_behind<T, kGenThreads>(p, w, z, hk, tid);
+    if (rows.n == 0) continue;
+    __syncthreads();
+    for (int i = tid; i < rows.n * p.dqk; i += kGenThreads) {
+      const int r = i / p.dqk, d = i - r * p.dqk;
+      q_s[i] = to_f32<T>(reinterpret_cast<const T*>(p.q.ptr)[(int64_t)z * p.q.s[0] + (int64_t)rows.head(p, hk, r) * p.q.s[1] + (int64_t)rows.query(r) * p.q.s[2] + d]);
+    }
+    if (tid < kGenRows) { m_s[tid] = -INFINITY; l_s[tid] = 0.f; }
+    float acc[kGenRows][J];
+#pragma unroll
+    for (int r = 0; r < kGenRows; ++r)
+#pragma unroll
+      for (int j = 0; j < J; ++j) acc[r][j] = 0.f;
+    for (int i = first; i < last; ++i) {
+      const int n0 = w.tile(i) * kGenKeys;
+      __syncthreads();
+      if (tid < kGenKeys) {      // a key's place in the cache in slots, or -1: nobody sees it
+        int64_t place = -1;
+        const int n = n0 + tid;
+        if (w.seen(p, n)) {
+          const int id = p.table[(int64_t)z * p.table_stride + n / p.page];
+          if (id >= 0 && id < p.num_pages) place = (int64_t)id * p.page + n % p.page;
+        }
+        page_of[tid] = place;
+      }
+      __syncthreads();
+      {
+        const int key = tid >> 3, l8 = tid & 7;
+        const int64_t place = page_of[key];
+        float dot[kGenRows];
+#pragma unroll
+        for (int r = 0; r < kGenRows; ++r) dot[r] = 0.f;
+        if (place >= 0) {
+          const T* kr = reinterpret_cast<const T*>(p.k.ptr) + place / p.page * p.k.s[0] + place % p.page * p.k.s[1] + (int64_t)hk * p.k.s[2];
+          for (int d = l8 * N; d < p.dqk; d += 8 * N) {
+            float x[N];
+            load_vec<T, N>(kr + d, x);
+#pragma unroll
+            for (int r = 0; r < kGenRows; ++r)
+              if (r < rows.n)
+#pragma unroll
+                for (int e = 0; e < N; ++e) dot[r] = fmaf(q_s[r * p.dqk + d + e], x[e], dot[r]);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < kGenRows; ++r) {
+#pragma unroll
+          for (int o = 1; o < 8; o <<= 1) dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], o);
+          if (l8 == 0) s[r][key] = dot[r];
+        }
+      }
+      __syncthreads();
+      for (int r = warp; r < rows.n; r += kGenThreads / 32) {
+        const int n = n0 + lane;
+        const int64_t pos = (int64_t)w.len - w.queries + rows.query(r);
+        const bool ok = page_of[lane] >= 0 && n <= pos && (n > pos - p.window || n < p.sinks);
+        const float x = ok ? s[r][lane] * p.qk_scale : -INFINITY;
+        float mx = x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        const float was = m_s[r], now = fmaxf(was, mx), ref = now == -INFINITY ? 0.f : now;
+        const float e = exp2f(x - ref);
+        float sum = e;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        s[r][lane] = e;
+        __syncwarp();
+        if (lane == 0) {
+          alpha[r] = exp2f(was - ref);
+          m_s[r] = now;
+          l_s[r] = l_s[r] * alpha[r] + sum;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < kGenRows; ++r)
+        if (r < rows.n)
+#pragma unroll
+          for (int j = 0; j < J; ++j) acc[r][j] *= alpha[r];
+      for (int key = group; key < kGenKeys; key += groups) {
+        const int64_t place = page_of[key];
+        if (place < 0) continue;
+        const T* vr = reinterpret_cast<const T*>(p.v.ptr) + place / p.page * p.v.s[0] + place % p.page * p.v.s[1] + (int64_t)hk * p.v.s[2];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const int d = col + j * kGenThreads;
+          if (d < p.dvo) {
+            const float x = to_f32<T>(vr[d]);
+#pragma unroll
+            for (int r = 0; r < kGenRows; ++r)
+              if (r < rows.n) acc[r][j] = fmaf(s[r][key], x, acc[r][j]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (J == 1) {      // the groups' sums, in their order
+      if (groups > 1) {
+#pragma unroll
+        for (int r = 0; r < kGenRows; ++r) meet[r * kGenThreads + tid] = acc[r][0];
+        __syncthreads();
+        if (group == 0)
+#pragma unroll
+          for (int r = 0; r < kGenRows; ++r)
+            for (int g = 1; g < groups; ++g) acc[r][0] += meet[r * kGenThreads + g * width + col];
+        __syncthreads();
+      }
+    }
+    float* part = partial_of(p, 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0));
+#pragma unroll
+    for (int r = 0; r < kGenRows; ++r) {
+      if (r >= rows.n) continue;
+      const float l = l_s[r], inv = l > 0.f ? 1.f / l : 0.f;
+      const int h = rows.head(p, hk, r), m = rows.query(r);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int d = col + j * kGenThreads;
+        if (group != 0 || d >= p.dvo) continue;
+        if (whole) out_row<T>(p, z, h, m)[d] = from_f32<T>(acc[r][j] * inv);
+        else part[r * p.dvo + d] = acc[r][j];
+      }
+      if (tid == 0) {
+        if (whole) put_lse(p, z, h, m, m_s[r], l);
+        else { part[p.rows * p.dvo + r] = m_s[r]; part[p.rows * p.dvo + p.rows + r] = l; }
+      }
+    }
+  }
+}
+
+// ---- the pieces of split units ----------------------------------------------------------------------------------------
+// grid = (batch * hk * chunks, rows): a block a row.  Weighs the pieces' rows by their maxima and adds them up in the order of the keys.
+constexpr int kJoinThreads = 128;
+
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttn p) {
+  wait_for_earlier_grids();
+  __shared__ int64_t scratch[kJoinThreads / 32 + 4];
+  __shared__ float weight[kJoinThreads], red[2][kJoinThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, units = p.hk * p.chunks;
+  const int z = (int)(blockIdx.x / units), u = (int)(blockIdx.x - (unsigned)z * units), r = blockIdx.y;
+  const Walk w(p, z);
+  const Rows rows(p, w, u % p.chunks);
+  if (r >= rows.n) return;
+  const Line line = find_in_line<kJoinThreads>(p, z, 0, scratch);
+  const int64_t unit = line.base + (int64_t)u * w.tiles;
+  const int64_t c0 = unit / line.share, c1 = (unit + w.tiles - 1) / line.share;
+  if (c0 == c1) return;      // (finished where it was formed)
+  auto piece = [&](int64_t c) { return partial_of(p, 2 * c + (c == c0 ? 1 : 0)); };
+  const int64_t at_m = (int64_t)p.rows * p.dvo + r, at_l = at_m + p.rows;
+  float mx = -INFINITY;
+  for (int64_t c = c0 + tid; c <= c1; c += kJoinThreads) mx = fmaxf(mx, piece(c)[at_m]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (lane == 0) red[0][warp] = mx;
+  __syncthreads();
+  mx = red[0][0];
+#pragma unroll
+  for (int i = 1; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[0][i]);
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  constexpr int kCols = kGenMaxDim / kJoinThreads;
+  float acc[kCols], l = 0.f;
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+  for (int64_t from = c0; from <= c1; from += kJoinThreads) {
+    const int n = (int)min((int64_t)kJoinThreads, c1 - from + 1);
+    __syncthreads();
+    if (tid < n) {
+      const float* q = piece(from + tid);
+      const float x = exp2f(q[at_m] - ref);
+      weight[tid] = x;
+      l = fmaf(x, q[at_l], l);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      const int d = tid + j * kJoinThreads;
+      if (d >= p.dvo) break;
+      float a = acc[j];
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) a = fmaf(weight[i], piece(from + i)[(int64_t)r * p.dvo + d], a);
+      acc[j] = a;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  if (lane == 0) red[1][warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) l += red[1][i];
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int hk = u / p.chunks, h = rows.head(p, hk, r), m = rows.query(r);
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    const int d = tid + j * kJoinThreads;
+    if (d < p.dvo) out_row<T>(p, z, h, m)[d] = from_f32<T>(acc[j] * inv);
+  }
+  if (tid == 0) put_lse(p, z, h, m, mx, l);
+}
+
+// ---- keys that share columns --------------------------------------------------------------------------------------
+// out[b, h, s] = (k[b, h, s], shared[b, 0, s]): rows moved as they are.  V: the vector that all rows allow.
+template <typename V>
+__global__ void __launch_bounds__(256) join_columns_kernel(const __grid_constant__ SharedColumns a, int elt) {
+  wait_for_earlier_grids();
+  const int per = (int)sizeof(V) / elt, vn = (int)a.k.n[3] / per, vr = (int)a.shared.n[3] / per, wide = vn + vr;
+  const int64_t rows = a.out.n[0] * a.out.n[1] * a.out.n[2], total = rows * wide;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / wide;
+    const int c = (int)(i - row * wide);
+    const int64_t bs = row / a.out.n[1], h = row - bs * a.out.n[1], b = bs / a.out.n[2], s = bs - b * a.out.n[2];      // (heads next to each other)
+    const char* src = c < vn ? reinterpret_cast<const char*>(a.k.ptr) + (b * a.k.s[0] + h * a.k.s[1] + s * a.k.s[2]) * elt + (int64_t)c * sizeof(V)
+                             : reinterpret_cast<const char*>(a.shared.ptr) + (b * a.shared.s[0] + s * a.shared.s[2]) * elt + (int64_t)(c - vn) * sizeof(V);
+    char* dst = reinterpret_cast<char*>(a.out.ptr) + (b * a.out.s[0] + h * a.out.s[1] + s * a.out.s[2]) * elt + (int64_t)c * sizeof(V);
+    *reinterpret_cast<V*>(dst) = *reinterpret_cast<const V*>(src);
+  }
+}
+
+// shared[b, 0, s, c] = sum over the heads of out[b, h, s, dn + c], in their order, in 32 bits, rounded once.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_columns_kernel(const __grid_constant__ SharedColumns a) {
+  wait_for_earlier_grids();
+  const int dr = (int)a.shared.n[3];
+  const int64_t dn = a.out.n[3] - dr, total = a.shared.n[0] * a.shared.n[2] * dr;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / dr, b = row / a.shared.n[2], s = row - b * a.shared.n[2];
+    const int c = (int)(i - row * dr);
+    const T* src = reinterpret_cast<const T*>(a.out.ptr) + b * a.out.s[0] + s * a.out.s[2] + dn + c;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int h = 0; h < (int)a.out.n[1]; ++h) sum += to_f32<T>(src[(int64_t)h * a.out.s[1]]);
+    reinterpret_cast<T*>(a.shared.ptr)[b * a.shared.s[0] + s * a.shared.s[2] + c] = from_f32<T>(sum);
+  }
+}
+
+unsigned grid_for(int64_t items, int64_t per) { return (unsigned)std::min<int64_t>((items + per - 1) / per, 0x7fffffff); }
+
+template <typename... K, typename... A>
+cudaError_t launch_counted(void (*kernel)(K...), dim3 grid, int threads, size_t smem, cudaStream_t st, A&&... args) {
+  const cudaError_t e = launch_kernel(kernel, grid, dim3(threads), smem, st, std::forward<A>(args)...);
+  if (e == cudaSuccess) count_launch();
+  return e;
+}
+
+bool vec_rows(const View4& v, int elements) {
+  if (reinterpret_cast<uintptr_t>(v.ptr) % 16 != 0 || v.n[3] % elements != 0) return false;
+  for (int i = 0; i < 3; ++i)
+    if (v.n[i] > 1 && v.s[i] % elements != 0) return false;
+  return true;
+}
+
+template <typename T, int N, int J>
+cudaError_t launch_general_NJ(const PagedAttn& p, cudaStream_t st) {
+  return launch_counted(paged_general_kernel<T, N, J>, dim3(p.ctas), kGenThreads, (size_t)kGenRows * p.dqk * sizeof(float), st, p);
+}
+template <typename T>
+cudaError_t launch_general_T(const PagedAttn& p, cudaStream_t st) {
+  constexpr int N = 16 / (int)sizeof(T);
+  const bool vec = vec_rows(p.k, N);
+  if (p.dvo <= kGenThreads) return vec ? launch_general_NJ<T, N, 1>(p, st) : launch_general_NJ<T, 1, 1>(p, st);
+  return vec ? launch_general_NJ<T, N, 4>(p, st) : launch_general_NJ<T, 1, 4>(p, st);
+}
+template <typename T>
+cudaError_t launch_join_T(const PagedAttn& p, cudaStream_t st) {
+  return launch_counted(paged_join_kernel<T>, dim3((unsigned)((int64_t)p.batch * p.hk * p.chunks), p.rows), kJoinThreads, 0, st, p);
+}
+
+template <typename F>
+auto with_type(int dtype, F f) {
+  switch (dtype) {
+    case 1: return f.template operator()<float>();
+    case 2: return f.template operator()<__half>();
+    default: return f.template operator()<__nv_bfloat16>();
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_block_tables(const BlockTables& a, cudaStream_t st) {
+  return launch_counted(block_tables_kernel, dim3(std::max(1u, grid_for(a.total, kTableTokens))), kTableThreads, 0, st, a);
+}
+
+cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st) {
+  const int elt = dtype == 1 ? 4 : 2, per = a.vec / elt;
+  const int64_t vectors = a.tokens * a.heads * ((a.dk + a.dv) / per);
+  if (vectors == 0) return cudaSuccess;
+  const dim3 grid(grid_for(vectors, (int64_t)kWriteThreads * kWriteBatch));
+  switch (a.vec) {
+    case 16: return launch_counted(paged_write_kernel<uint4>, grid, kWriteThreads, 0, st, a, elt, vectors);
+    case 4: return launch_counted(paged_write_kernel<uint32_t>, grid, kWriteThreads, 0, st, a, elt, vectors);
+    default: return launch_counted(paged_write_kernel<uint16_t>, grid, kWriteThreads, 0, st, a, elt, vectors);
+  }
+}
+
+int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
+  (void)dtype;
+  p.kind = kPagedGeneral;
+  p.rows = kGenRows;
+  p.tile_keys = kGenKeys;
+  p.min_tiles = 2;
+  const int resident = 4;
+  p.chunks = (int)(((int64_t)p.group * p.sq + p.rows - 1) / p.rows);
+  const int64_t units = (int64_t)p.batch * p.hk * p.chunks;
+  const int64_t most = std::max<int64_t>(1, ((int64_t)p.width * p.page + p.tile_keys - 1) / p.tile_keys + 1);      // tiles of a unit (one more: a window across a border)
+  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sms * resident, units * most / p.min_tiles + 1));
+  p.join = most > 1;
+  return p.join ? 2 * (int64_t)p.ctas * partial_floats(p) : 0;
+}
+
+cudaError_t launch_paged(int dtype, const PagedAttn& p, cudaStream_t st) {
+  cudaError_t e = with_type(dtype, [&]<typename T>() { return launch_general_T<T>(p, st); });
+  if (e == cudaSuccess && p.join) e = with_type(dtype, [&]<typename T>() { return launch_join_T<T>(p, st); });
+  return e;
+}
+
+cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t st) {
+  const int elt = dtype == 1 ? 4 : 2, per = 16 / elt;
+  const int64_t elements = a.out.n[0] * a.out.n[1] * a.out.n[2] * a.out.n[3];
+  if (vec_rows(a.k, per) && vec_rows(a.shared, per) && vec_rows(a.out, per))
+    return launch_counted(join_columns_kernel<uint4>, dim3(grid_for(elements / per, 256)), 256, 0, st, a, elt);
+  if (elt == 4) return launch_counted(join_columns_kernel<uint32_t>, dim3(grid_for(elements, 256)), 256, 0, st, a, elt);
+  return launch_counted(join_columns_kernel<uint16_t>, dim3(grid_for(elements, 256)), 256, 0, st, a, elt);
+}
+
+cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st) {
+  const dim3 grid(grid_for(a.shared.n[0] * a.shared.n[2] * a.shared.n[3], 256));
+  return with_type(dtype, [&]<typename T>() { return launch_counted(sum_columns_kernel<T>, grid, 256, 0, st, a); });
+}
+
+}  // namespace ab200

@@ -1,0 +1,66 @@
+// Host-side declarations of the operators over a paged cache (paged.cu, sm100_paged.cu, sm100_latent.cu) and of keys that share columns.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include "common.cuh"
+
+namespace ab200 {
+
+struct BlockTables {
+  int32_t batch, page, width;
+  int64_t total, table_stride, num_free;
+  int32_t* table;
+  const int32_t *lengths, *new_tokens, *free_pages, *taken;
+  int64_t* slots;
+  int32_t *cu_seqlens, *new_lengths, *taken_out;
+};
+
+struct PagedWrite {
+  int64_t tokens, slots_total;       // slots of the cache: what lies outside them is not written
+  int32_t page, heads, dk, dv;       // dv 0: keys alone
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  int64_t sk[2], sv[2];              // strides of tokens and heads
+  int64_t ck[3], cv[3];              // strides of pages, slots and heads
+  const int64_t* slots;
+  int32_t vec;                       // bytes that every row allows at a time
+};
+
+// Attention of the last queries of each sequence over pages.  Sequence z has the first lengths[z] keys of its table's pages; its
+// query m stands at position lengths[z] - queries + m.
+struct PagedAttn {
+  View4 q, out;                      // (B, Hq, Sq, D)
+  View4 k, v;                        // (pages, page, Hk, D)
+  const int32_t* table;
+  int64_t table_stride;
+  int32_t width, page, num_pages;
+  const int32_t *lengths, *query_lengths;
+  float* lse;                        // (B * Hq, Sq), or null
+  int32_t batch, hq, hk, group, sq, dqk, dvo;
+  float qk_scale;                    // sm_scale * log2(e)
+  int32_t window, sinks;             // window INT32_MAX: none
+  // How the call is cut (plan_paged): the tiles of all units -- (sequence, kv head, chunk of `rows` query rows) -- stand in one line,
+  // of which each of `ctas` CTAs takes an equal piece, min_tiles at least.
+  int32_t kind, ctas, rows, chunks, tile_keys, min_tiles, join, stages;
+  float* partial;                    // two partial results a CTA: of the unit that it starts with, of the one that it ends with
+  uint32_t wait_limit_kcycles;
+  int32_t drop_copy;
+};
+
+enum PagedKind : int { kPagedGeneral = 1, kPagedSplit = 2, kPagedLatent = 3 };
+
+struct SharedColumns {
+  View4 k, shared, out;              // (B, H, S, dn), (B, 1, S, dr), (B, H, S, dn + dr)
+};
+
+cudaError_t launch_block_tables(const BlockTables& a, cudaStream_t st);
+cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st);
+// Chooses the kernel and how the call is cut for `sms` SMs; returns the floats of workspace it needs.
+int64_t plan_paged(int dtype, PagedAttn& a, int sms);
+cudaError_t launch_paged(int dtype, const PagedAttn& a, cudaStream_t st);
+cudaError_t launch_paged_general(int dtype, const PagedAttn& a, cudaStream_t st);
+cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t st);
+cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st);      // shared = sum over heads of out's last columns
+
+}  // namespace ab200

@@ -1,0 +1,131 @@
+// How the attention kernels over a paged cache share a call out, and how pieces of a sequence meet.
+//
+// Sequences of one batch have lengths between one token and a hundred thousand, which only the device knows.  So nothing is cut by a
+// bound on the lengths: the key tiles of all units -- (sequence, kv head, chunk of query rows) -- are put in one line, and each CTA takes an equal
+// piece of it, whatever sequences that crosses.  A unit that lies within a piece is finished there; the pieces of others leave row maximum,
+// row sum and unnormalised output in a workspace (at most two a CTA: of the unit it begins with and of the one it ends with, so that its size does not
+// depend on the lengths), which a second launch adds up in the order of the keys.  Every CTA works out its place from the lengths alone.
+#pragma once
+
+#include "paged.h"
+
+namespace ab200 {
+namespace {
+
+// What a sequence's queries see of its keys: the first `sinks` and those from `lo` on, in tiles of p.tile_keys.  At least one tile, so
+// that every unit has an owner.
+struct Walk {
+  int len, queries, lo, first, n_sink, tiles;
+  __device__ __forceinline__ Walk(const PagedAttn& p, int z) {
+    const int64_t room = (int64_t)p.width * p.page;
+    const int64_t most = room < 0x7fffffff ? room : 0x7fffffff;
+    int64_t l = p.lengths[z];
+    l = l < 0 ? 0 : (l < most ? l : most);
+    len = (int)l;
+    queries = p.query_lengths != nullptr ? min(max(p.query_lengths[z], 0), p.sq) : p.sq;
+    if (len == 0 || queries == 0) { lo = first = n_sink = 0; tiles = 1; return; }
+    const int64_t from = (int64_t)len - queries - p.window + 1;      // the first query's window
+    lo = from > 0 ? (int)from : 0;
+    first = lo / p.tile_keys;
+    n_sink = min((min(p.sinks, lo) + p.tile_keys - 1) / p.tile_keys, first);
+    tiles = n_sink + (len - 1) / p.tile_keys - first + 1;
+  }
+  __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
+  // Whether some query of the sequence sees key n, its page apart.
+  __device__ __forceinline__ bool seen(const PagedAttn& p, int n) const { return n < len && (n >= lo || n < p.sinks); }
+};
+
+// The line of tiles as one thread block sees it.
+struct Line {
+  int64_t total, share;      // tiles in all, and of a CTA
+  int64_t base;              // first tile of sequence z
+  int z;
+};
+
+// A block of NT threads (a multiple of 32) finds sequence `z`, or the one that tile `at` belongs to (z < 0).  `scratch`: NT / 32 + 4 words of 8 bytes.
+// Of a tile behind the last, z is the batch's size.
+template <int NT>
+__device__ __forceinline__ Line find_in_line(const PagedAttn& p, int z, int64_t cta, int64_t* scratch) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t units = (int64_t)p.hk * p.chunks;
+  const int each = (p.batch + NT - 1) / NT, z0 = min(tid * each, p.batch), z1 = min(z0 + each, p.batch);
+  int64_t mine = 0;
+  for (int i = z0; i < z1; ++i) mine += Walk(p, i).tiles;
+  int64_t up = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t o = __shfl_up_sync(0xffffffffu, up, d);
+    if (lane >= d) up += o;
+  }
+  if (lane == 31) scratch[warp] = up;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < NT / 32; ++w) {
+    const int64_t s = scratch[w];
+    if (w < warp) before += s;
+    total += s;
+  }
+  before += up - mine;
+  Line r;
+  r.total = total * units;
+  r.share = (r.total + p.ctas - 1) / p.ctas;
+  if (r.share < p.min_tiles) r.share = p.min_tiles;
+  const int64_t at = cta * r.share;
+  if (tid == 0) { scratch[NT / 32] = p.batch; scratch[NT / 32 + 1] = r.total; }
+  __syncthreads();
+  if (z >= 0 ? (z >= z0 && z < z1) : (mine > 0 && at >= before * units && at < (before + mine) * units)) {
+    int64_t b = before;
+    int i = z0;
+    for (; i + 1 < z1; ++i) {
+      if (i == z) break;
+      const int64_t t = Walk(p, i).tiles;
+      if (z < 0 && at < (b + t) * units) break;
+      b += t;
+    }
+    scratch[NT / 32] = i;
+    scratch[NT / 32 + 1] = b * units;
+  }
+  __syncthreads();
+  r.z = (int)scratch[NT / 32];
+  r.base = scratch[NT / 32 + 1];
+  return r;
+}
+
+// Rows of a unit's chunk: row r of it is query m of head h.
+struct Rows {
+  int row0, n, queries;
+  __device__ __forceinline__ Rows(const PagedAttn& p, const Walk& w, int chunk) {
+    queries = w.queries;
+    row0 = chunk * p.rows;
+    n = min(p.rows, p.group * w.queries - row0);
+    if (n < 0) n = 0;
+  }
+  __device__ __forceinline__ int head(const PagedAttn& p, int hk, int r) const { return hk * p.group + (row0 + r) / queries; }
+  __device__ __forceinline__ int query(int r) const { return (row0 + r) % queries; }
+};
+
+// Partial result `slot` (twice the CTA, one more for the unit that starts in it): rows x dvo outputs, then maxima, then sums.
+__host__ __device__ __forceinline__ int64_t partial_floats(const PagedAttn& p) { return ((int64_t)p.rows * (p.dvo + 2) + 3) / 4 * 4; }
+__device__ __forceinline__ float* partial_of(const PagedAttn& p, int64_t slot) { return p.partial + slot * partial_floats(p); }
+
+template <typename T>
+__device__ __forceinline__ T* out_row(const PagedAttn& p, int z, int h, int m) {
+  return reinterpret_cast<T*>(p.out.ptr) + (int64_t)z * p.out.s[0] + (int64_t)h * p.out.s[1] + (int64_t)m * p.out.s[2];
+}
+__device__ __forceinline__ void put_lse(const PagedAttn& p, int z, int h, int m, float mx, float l) {
+  if (p.lse != nullptr) p.lse[((int64_t)z * p.hq + h) * p.sq + m] = l > 0.f ? (mx + log2f(l)) * kLn2 : INFINITY;
+}
+
+// Rows of a kv head's queries behind the sequence's last, by the block that starts the head's first chunk: zeros.
+template <typename T, int NT>
+__device__ __forceinline__ void zero_rows_behind(const PagedAttn& p, const Walk& w, int z, int hk, int tid) {
+  const int behind = p.sq - w.queries;
+  for (int r = tid / 32; r < p.group * behind; r += NT / 32) {
+    const int h = hk * p.group + r / behind, m = w.queries + r % behind;
+    for (int d = tid & 31; d < p.dvo; d += 32) out_row<T>(p, z, h, m)[d] = from_f32<T>(0.f);
+    if ((tid & 31) == 0) put_lse(p, z, h, m, 0.f, 0.f);
+  }
+}
+
+}  // namespace
+}  // namespace ab200

@@ -254,6 +254,94 @@ typedef struct ab200_dropout_args {
 
 AB200_API int ab200_dropout(const ab200_dropout_args* args, void* stream);
 
+/* ---- attention over a cache in pages; the reference has none of these ------------------------------------------- */
+
+/* Books of a paged cache.  Sequence z holds lengths[z] tokens and takes new_tokens[z] more (below zero: none); token i of them stands at position
+ * p = lengths[z] + i, in page p / page_size of row z of the block table, and has the slot entry * page_size + p % page_size.  Pages that the sequence
+ * does not have yet, those behind the first ceil(lengths[z] / page_size), are the next of free_pages behind the first *taken, in order of sequence and
+ * position, and are entered into the table; the rest of it is left as it is.  A token has the slot -1 where its page would lie outside the row, where the
+ * free pages are used up (entry -1) or where the entry is negative.  Sums are below 2^31. */
+typedef struct ab200_block_tables_args {
+  int32_t batch;
+  int32_t page_size;
+  int32_t table_width;          /* entries of a row                                                      */
+  int32_t* block_table;         /* (batch, table_width)                                                  */
+  int64_t table_stride;         /* between rows                                                          */
+  const int32_t* lengths;
+  const int32_t* new_tokens;
+  const int32_t* free_pages;
+  int64_t num_free;
+  const int32_t* taken;         /* device scalar: how many of free_pages are gone already; NULL -> 0     */
+  int64_t total_tokens;         /* room of `slots`, at least the sum of new_tokens (what is beyond gets neither slot nor page) */
+  int64_t* slots;               /* packed in order of sequence; -1 behind the last token                 */
+  int32_t* cu_seqlens;          /* batch + 1: running sums of new_tokens                                 */
+  int32_t* new_lengths;         /* lengths + new_tokens                                                  */
+  int32_t* taken_out;           /* taken + pages taken now; above num_free: there were too few           */
+} ab200_block_tables_args;
+
+AB200_API int ab200_block_tables(const ab200_block_tables_args* args, void* stream);
+
+/* Rows of new tokens into their slots: k_cache[slot / page_size, slot % page_size, h] = k[t, h], and the same for v.  Slots outside the cache (-1) are
+ * skipped; the slots of one call differ from one another.  Rows have unit stride; a single latent cache is written as two column ranges of it. */
+typedef struct ab200_paged_write_args {
+  int32_t dtype;
+  int32_t num_heads;
+  int32_t head_dim_k, head_dim_v;      /* head_dim_v 0: no values                                */
+  int32_t page_size;
+  int64_t num_pages;
+  int64_t tokens;
+  const void *k, *v;                   /* (tokens, heads, dim)                                    */
+  int64_t k_stride[2], v_stride[2];    /* between tokens, between heads                           */
+  void *k_cache, *v_cache;             /* (pages, page_size, heads, dim)                          */
+  int64_t k_cache_stride[3], v_cache_stride[3];      /* between pages, slots, heads               */
+  const int64_t* slots;
+} ab200_paged_write_args;
+
+AB200_API int ab200_paged_write(const ab200_paged_write_args* args, void* stream);
+
+/* Attention of the last tokens of each sequence over its pages.  Sequence z has the keys 0 to lengths[z] - 1, key n in slot n % page_size of page
+ * block_table[z][n / page_size]; its queries are the last query_lengths[z] of them (NULL: seqlen_q), at positions lengths[z] - query_lengths[z] + m.  A query at
+ * position P sees the keys n <= P with n > P - window (window 0: all of them) or n < sinks.  Lengths are taken as 0 to the table's width, query lengths as 0 to
+ * seqlen_q; keys of pages outside the cache are seen by nobody.  Rows that see nothing, and those behind query_lengths[z], get O = 0 and LSE = +inf.
+ * What the cache holds in slots that no query of the sequence sees does not matter, NaN included.  With one kv head, values may be the
+ * first columns of the keys themselves (v_cache the same memory and strides): they are then read once.  The same inputs give the same bits. */
+typedef struct ab200_paged_attn_args {
+  int32_t dtype;
+  int32_t batch;
+  int32_t num_head_q, num_head_k;
+  int32_t seqlen_q;
+  int32_t head_dim_qk, head_dim_vo;    /* 1 to 1024                                               */
+  int32_t page_size;
+  float sm_scale;
+  int32_t window, sinks;
+  ab200_view4 q, out;                  /* (batch, Hq, seqlen_q, dim)                              */
+  ab200_view4 k_cache, v_cache;        /* (pages, page_size, Hk, dim)                             */
+  const int32_t* block_table;          /* (batch, table_width)                                    */
+  int64_t table_stride;
+  int32_t table_width;
+  const int32_t* lengths;
+  const int32_t* query_lengths;        /* NULL: all seqlen_q                                      */
+  float* lse;                          /* (batch * Hq, seqlen_q), natural logarithm; NULL: not written */
+  float* workspace;                    /* ab200_paged_attn_workspace() floats, 16-byte aligned; contents do not matter, calls that may overlap need one each */
+  uint64_t workspace_floats;
+} ab200_paged_attn_args;
+
+AB200_API int ab200_paged_attn(const ab200_paged_attn_args* args, void* stream);
+/* Floats of workspace the call needs (it does not depend on the lengths), or the negated error code.  Launches nothing. */
+AB200_API int64_t ab200_paged_attn_workspace(const ab200_paged_attn_args* args, void* stream);
+
+/* Keys whose last columns all heads share: joined[b, h, s] = (k[b, h, s], shared[b, 0, s]); and the gradient of the shared columns, shared[b, 0, s] = the sum
+ * over h of joined[b, h, s]'s last columns (fp32, in the order of the heads; `k` is not looked at). */
+typedef struct ab200_shared_columns_args {
+  int32_t dtype;
+  ab200_view4 k;         /* (B, H, S, dn), read                                     */
+  ab200_view4 shared;    /* (B, 1, S, dr): read, or the gradient, written           */
+  ab200_view4 joined;    /* (B, H, S, dn + dr): written, or its gradient, read      */
+} ab200_shared_columns_args;
+
+AB200_API int ab200_join_columns(const ab200_shared_columns_args* args, void* stream);
+AB200_API int ab200_sum_columns(const ab200_shared_columns_args* args, void* stream);
+
 /* Replaces aotriton::v2::flash::check_gpu (modules/flash/csrc/attn_check.cc:36-46):
  * 0 when the stream's device is an sm_100 part, hipErrorNoBinaryForGpu (209) otherwise. */
 AB200_API int ab200_check_gpu(void* stream);
