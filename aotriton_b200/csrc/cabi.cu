@@ -475,8 +475,8 @@ int ab200_set_kernel_family(int family) {
 int ab200_last_fwd_family(void) { return t_last_fwd; }
 int ab200_last_bwd_family(void) { return t_last_bwd; }
 unsigned int ab200_kernel_status(int reset) {
-  unsigned int f = sm100_fwd_status(reset != 0), b = sm100_bwd_status(reset != 0);
-  const unsigned int v = f ? f : b;
+  unsigned int f = sm100_fwd_status(reset != 0), b = sm100_bwd_status(reset != 0), g = sm100_paged_status(reset != 0);
+  const unsigned int v = f ? f : b ? b : g;
   int dev = -1;
   if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) {
     if (reset) g_failed_devices.fetch_and(~(uint64_t(1) << dev));

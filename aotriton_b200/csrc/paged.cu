@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   const int64_t unit = line.base + (int64_t)u * w.tiles;
   const int64_t c0 = unit / line.share, c1 = (unit + w.tiles - 1) / line.share;
   if (c0 == c1) return;      // (finished where it was formed)
+  if (p.status != nullptr && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
   auto piece = [&](int64_t c) { return partial_of(p, 2 * c + (c == c0 ? 1 : 0)); };
   const int64_t at_m = (int64_t)p.rows * p.dvo + r, at_l = at_m + p.rows;
   float mx = -INFINITY;
@@ -468,22 +469,23 @@ cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st) 
 }
 
 int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
-  (void)dtype;
-  p.kind = kPagedGeneral;
-  p.rows = kGenRows;
-  p.tile_keys = kGenKeys;
-  p.min_tiles = 2;
-  const int resident = 4;
+  if (!plan_paged_split(dtype, p, sms)) {
+    p.kind = kPagedGeneral;
+    p.rows = kGenRows;
+    p.tile_keys = kGenKeys;
+    p.min_tiles = 2;
+    p.ctas = sms * 4;
+  }
   p.chunks = (int)(((int64_t)p.group * p.sq + p.rows - 1) / p.rows);
   const int64_t units = (int64_t)p.batch * p.hk * p.chunks;
   const int64_t most = std::max<int64_t>(1, ((int64_t)p.width * p.page + p.tile_keys - 1) / p.tile_keys + 1);      // tiles of a unit (one more: a window across a border)
-  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sms * resident, units * most / p.min_tiles + 1));
+  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(p.ctas, units * most / p.min_tiles + 1));
   p.join = most > 1;
   return p.join ? 2 * (int64_t)p.ctas * partial_floats(p) : 0;
 }
 
-cudaError_t launch_paged(int dtype, const PagedAttn& p, cudaStream_t st) {
-  cudaError_t e = with_type(dtype, [&]<typename T>() { return launch_general_T<T>(p, st); });
+cudaError_t launch_paged(int dtype, PagedAttn& p, cudaStream_t st) {
+  cudaError_t e = p.kind == kPagedSplit ? launch_paged_split(dtype, p, st) : with_type(dtype, [&]<typename T>() { return launch_general_T<T>(p, st); });
   if (e == cudaSuccess && p.join) e = with_type(dtype, [&]<typename T>() { return launch_join_T<T>(p, st); });
   return e;
 }

@@ -42,7 +42,8 @@ struct PagedAttn {
   int32_t window, sinks;             // window INT32_MAX: none
   // How the call is cut (plan_paged): the tiles of all units -- (sequence, kv head, chunk of `rows` query rows) -- stand in one line,
   // of which each of `ctas` CTAs takes an equal piece, min_tiles at least.
-  int32_t kind, ctas, rows, chunks, tile_keys, min_tiles, join, stages;
+  int32_t kind, ctas, rows, chunks, tile_keys, min_tiles, join, stages, box;      // box: slots of a tile copy
+  unsigned int* status;              // the word in which a kernel records a wait that ran out (null: the general kernel has none)
   float* partial;                    // two partial results a CTA: of the unit that it starts with, of the one that it ends with
   uint32_t wait_limit_kcycles;
   int32_t drop_copy;
@@ -58,8 +59,13 @@ cudaError_t launch_block_tables(const BlockTables& a, cudaStream_t st);
 cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st);
 // Chooses the kernel and how the call is cut for `sms` SMs; returns the floats of workspace it needs.
 int64_t plan_paged(int dtype, PagedAttn& a, int sms);
-cudaError_t launch_paged(int dtype, const PagedAttn& a, cudaStream_t st);
-cudaError_t launch_paged_general(int dtype, const PagedAttn& a, cudaStream_t st);
+cudaError_t launch_paged(int dtype, PagedAttn& a, cudaStream_t st);
+// The tensor-core kernels: whether one takes the call, and if so how it cuts it (all but ctas' bound and the workspace); and its launch.
+bool plan_paged_split(int dtype, PagedAttn& a, int sms);
+cudaError_t launch_paged_split(int dtype, PagedAttn& a, cudaStream_t st);
+// The status word of the current device (sm100_paged.cu), as sm100_fwd_status has it.
+cudaError_t paged_status_word(unsigned int** word, int* dev, bool* remember);
+unsigned int sm100_paged_status(bool reset);
 cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t st);
 cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st);      // shared = sum over heads of out's last columns
 

@@ -39,6 +39,7 @@
 #include "launch.h"
 #include "sm100_ptx.cuh"
 #include "tile32.cuh"
+#include "warp_mma.cuh"
 
 namespace ab200 {
 

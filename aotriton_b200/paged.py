@@ -129,6 +129,15 @@ def _paged_attention(q, k_cache, v_cache, block_table, lengths, query_lengths, w
     return (out, lse) if return_lse else out
 
 
+def _aligned(q):
+    """q with a unit innermost stride and rows that start on 16 bytes where its type and head dim allow it: itself or a copy (a few rows, beside a cache)."""
+    q = _unit_rows(q)
+    per = 16 // q.itemsize
+    if q.shape[-1] % per == 0 and (q.data_ptr() % 16 or any(n > 1 and s % per for n, s in zip(q.shape[:3], q.stride()))):
+        q = q.clone(memory_format=torch.contiguous_format)
+    return q
+
+
 def _attend(q, k_cache, v_cache, block_table, lengths, query_lengths, window, sinks, sm_scale, return_lse, what):
     if q.dim() != 4 or q.dtype not in _FLOATS or not q.is_cuda:
         raise ValueError(f"{what}: q is a (batch, heads, tokens, head dim) CUDA tensor of fp32, fp16 or bf16")
@@ -149,7 +158,7 @@ def _attend(q, k_cache, v_cache, block_table, lengths, query_lengths, window, si
         raise ValueError(f"{what}: pages without slots")
     _no_gradient(what, q, k_cache, v_cache)
     window, sinks = 0 if window is None else min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1)
-    return _paged_attention(_unit_rows(q), k_cache, v_cache, block_table, lengths, query_lengths, window, sinks, float(sm_scale), bool(return_lse), what)
+    return _paged_attention(_aligned(q), k_cache, v_cache, block_table, lengths, query_lengths, window, sinks, float(sm_scale), bool(return_lse), what)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sinks=0, query_lengths=None, sm_scale=None, return_lse=False):
