@@ -29,7 +29,7 @@ CSRC = PKG / "csrc"
 OBJ = PKG / "build"
 LIB = PKG / "libaotriton_v2.so"
 
-CUDA_SOURCES = ["cabi.cu", "general_kernels.cu", "layer_ops.cu", "paged.cu", "sm100_fwd.cu", "sm100_bwd.cu", "sm100_paged.cu"]
+CUDA_SOURCES = ["cabi.cu", "general_kernels.cu", "layer_ops.cu", "paged.cu", "sm100_fwd.cu", "sm100_bwd.cu", "sm100_paged.cu", "sm100_latent.cu"]
 CXX_SOURCES = ["api.cc"]
 HEADERS = sorted(list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((ROOT / "include").rglob("*.h")))
 

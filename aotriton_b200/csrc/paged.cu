@@ -469,7 +469,7 @@ cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st) 
 }
 
 int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
-  if (!plan_paged_split(dtype, p, sms)) {
+  if (!plan_paged_latent(dtype, p, sms) && !plan_paged_split(dtype, p, sms)) {
     p.kind = kPagedGeneral;
     p.rows = kGenRows;
     p.tile_keys = kGenKeys;
@@ -485,7 +485,9 @@ int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
 }
 
 cudaError_t launch_paged(int dtype, PagedAttn& p, cudaStream_t st) {
-  cudaError_t e = p.kind == kPagedSplit ? launch_paged_split(dtype, p, st) : with_type(dtype, [&]<typename T>() { return launch_general_T<T>(p, st); });
+  cudaError_t e = p.kind == kPagedSplit    ? launch_paged_split(dtype, p, st)
+                  : p.kind == kPagedLatent ? launch_paged_latent(dtype, p, st)
+                                           : with_type(dtype, [&]<typename T>() { return launch_general_T<T>(p, st); });
   if (e == cudaSuccess && p.join) e = with_type(dtype, [&]<typename T>() { return launch_join_T<T>(p, st); });
   return e;
 }

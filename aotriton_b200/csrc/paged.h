@@ -63,6 +63,8 @@ cudaError_t launch_paged(int dtype, PagedAttn& a, cudaStream_t st);
 // The tensor-core kernels: whether one takes the call, and if so how it cuts it (all but ctas' bound and the workspace); and its launch.
 bool plan_paged_split(int dtype, PagedAttn& a, int sms);
 cudaError_t launch_paged_split(int dtype, PagedAttn& a, cudaStream_t st);
+bool plan_paged_latent(int dtype, PagedAttn& a, int sms);
+cudaError_t launch_paged_latent(int dtype, PagedAttn& a, cudaStream_t st);
 // The status word of the current device (sm100_paged.cu), as sm100_fwd_status has it.
 cudaError_t paged_status_word(unsigned int** word, int* dev, bool* remember);
 unsigned int sm100_paged_status(bool reset);

@@ -18,7 +18,7 @@ struct Walk {
   int len, queries, lo, first, n_sink, tiles;
   __device__ __forceinline__ Walk(const PagedAttn& p, int z) {
     const int64_t room = (int64_t)p.width * p.page;
-    const int64_t most = room < 0x7fffffff ? room : 0x7fffffff;
+    const int64_t most = room < 0x7fffff00 ? room : 0x7fffff00;      // (a last tile's keys are counted in 32 bits)
     int64_t l = p.lengths[z];
     l = l < 0 ? 0 : (l < most ? l : most);
     len = (int)l;
