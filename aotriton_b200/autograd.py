@@ -43,6 +43,22 @@ except ImportError as e:      # (built where torch was missing, had no CUDA or w
             return None
 
         @staticmethod
+        def join_columns(*args):
+            return None
+
+        @staticmethod
+        def paged_attention(*args):
+            return None
+
+        @staticmethod
+        def block_tables(*args):
+            return None
+
+        @staticmethod
+        def paged_write(*args):
+            return None
+
+        @staticmethod
         def set_python_backward(fn):
             pass
 
@@ -736,6 +752,14 @@ class _SumColumns(torch.autograd.Function):
         return torch.nn.functional.pad(grad.expand(-1, h, -1, -1), (width, 0)), None
 
 
+def _python_sum_columns(grad, width):
+    """The gradient of a native call whose own gradient or modes are not ordinary ones (csrc/torch_ops.cc)."""
+    return _SumColumns.apply(grad, width)
+
+
+_native.set_python_function("sum_columns", _python_sum_columns)
+
+
 def _join_shared(q, k, k_shared, v, what):
     for t in (q, k, k_shared, v):
         if t.dim() != 4 or t.dtype not in _FLOATS or not t.is_cuda or t.dtype != q.dtype or t.device != q.device:
@@ -747,6 +771,10 @@ def _join_shared(q, k, k_shared, v, what):
                          "shared columns")
     if q.shape[3] > 512 or not 1 <= v.shape[3] <= 512:
         raise ValueError(f"{what}: head dims from 1 to 512 are supported")
+    if not torch.compiler.is_compiling():
+        r = _native.join_columns(k, k_shared)
+        if r is not None:
+            return r
     return _apply(_JoinColumns, _unit_rows(k), _unit_rows(k_shared))
 
 

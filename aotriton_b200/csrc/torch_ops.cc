@@ -1,5 +1,5 @@
 // The autograd entry points' native route: attention on ordinary torch tensors, forward and backward, without Python in
-// between; in the same way sink attention, the relative position bias and dropout of hidden states.  Outputs, gradients and scratch
+// between; in the same way sink attention, the relative position bias, dropout of hidden states, the operators over a paged cache and keys that share columns.  Outputs, gradients and scratch
 // come from torch's caching allocator, launches go to torch's current stream through the C++ operator API (include/aotriton/flash.h), the backward is a torch::autograd::Function: version checks and CUDA-graph
 // capture see what they see of the Python Function, saved-tensor hooks the inputs, the output and the log-sum-exp.
 //
@@ -545,6 +545,101 @@ struct RelativeBias : torch::autograd::Function<RelativeBias> {
   }
 };
 
+// ---- keys that share columns ----
+ab200_shared_columns_args columns_args(const Tensor& k, const Tensor& shared, const Tensor& joined) {
+  ab200_shared_columns_args a{};
+  a.dtype = code_of(joined.scalar_type());
+  if (k.defined()) a.k = c_view(k);
+  a.shared = c_view(shared);
+  a.joined = c_view(joined);
+  return a;
+}
+Tensor join_columns(const Tensor& k, const Tensor& shared) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  const Tensor joined = fresh({k.size(0), k.size(2), k.size(1), k.size(3) + shared.size(3)}, k.scalar_type()).transpose(1, 2);
+  const auto a = columns_args(k, shared, joined);
+  check((hipError_t)ab200_join_columns(&a, stream_handle()), "join_columns");
+  return joined;
+}
+struct JoinColumns : torch::autograd::Function<JoinColumns> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& k, const Tensor& shared) {
+    ctx->saved_data["numbers"] = std::vector<int64_t>{k.size(3), (int64_t)k.scalar_type()};
+    ctx->set_materialize_grads(false);
+    return join_columns(k, shared);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list r(2);
+    Tensor g = grads[0];
+    if (!g.defined()) return r;
+    const auto n = ctx->saved_data["numbers"].toIntVector();
+    if (ctx->needs_input_grad(0)) r[0] = g.narrow(3, 0, n[0]);
+    if (!ctx->needs_input_grad(1)) return r;
+    if (ordinary_gradient(g, (at::ScalarType)n[1])) {
+      if (g.stride(-1) != 1) g = g.contiguous();
+      r[1] = fresh({g.size(0), 1, g.size(2), g.size(3) - n[0]}, g.scalar_type());
+      const auto a = columns_args(Tensor(), r[1], g);
+      check((hipError_t)ab200_sum_columns(&a, stream_handle()), "sum_columns");
+    } else {
+      pybind11::gil_scoped_acquire gil;
+      r[1] = THPVariable_Unpack(call_python("sum_columns", pybind11::make_tuple(wrapped(g), n[0])).ptr());
+    }
+    return r;
+  }
+};
+
+// ---- a cache in pages ----
+struct PagedCall {
+  int64_t window, sinks, value_dim;      // value_dim: of a latent cache, whose first columns are the values; 0: keys and values apart
+  double sm_scale;
+};
+Tensor paged_attend(const PagedCall& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths,
+                    const Tensor& query_lengths, Tensor* lse) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  ab200_paged_attn_args a{};
+  a.dtype = code_of(q.scalar_type());
+  a.batch = (int32_t)q.size(0); a.num_head_q = (int32_t)q.size(1); a.seqlen_q = (int32_t)q.size(2); a.head_dim_qk = (int32_t)q.size(3);
+  a.page_size = (int32_t)k.size(1);
+  a.sm_scale = (float)c.sm_scale;
+  a.window = (int32_t)c.window; a.sinks = (int32_t)c.sinks;
+  a.q = c_view(q);
+  if (c.value_dim) {
+    a.num_head_k = 1;
+    a.head_dim_vo = (int32_t)c.value_dim;
+    a.k_cache = ab200_view4{k.data_ptr(), {k.size(0), k.size(1), 1, k.size(2)}, {k.stride(0), k.stride(1), k.stride(1), 1}};
+    a.v_cache = a.k_cache;
+    a.v_cache.size[3] = c.value_dim;
+  } else {
+    a.num_head_k = (int32_t)k.size(2);
+    a.head_dim_vo = (int32_t)v.size(3);
+    a.k_cache = c_view(k);
+    a.v_cache = c_view(v);
+  }
+  // (tokens' heads next to each other)
+  const Tensor store = fresh({q.size(0), q.size(2), q.size(1), a.head_dim_vo}, q.scalar_type());
+  const Tensor out = store.transpose(1, 2);
+  a.out = c_view(out);
+  if (lse != nullptr) {
+    *lse = fresh({q.size(0) * q.size(1), q.size(2)}, at::kFloat);
+    a.lse = static_cast<float*>(lse->data_ptr());
+  }
+  a.block_table = static_cast<const int32_t*>(table.data_ptr());
+  a.table_stride = table.stride(0);
+  a.table_width = (int32_t)table.size(1);
+  a.lengths = static_cast<const int32_t*>(lengths.data_ptr());
+  a.query_lengths = query_lengths.defined() ? static_cast<const int32_t*>(query_lengths.data_ptr()) : nullptr;
+  const char* what = c.value_dim ? "paged_latent_attention" : "paged_attention";
+  const int64_t need = ab200_paged_attn_workspace(&a, stream_handle());
+  if (need < 0) check((hipError_t)-need, what);
+  Tensor workspace;
+  if (need > 0) {
+    workspace = fresh({need}, at::kFloat);
+    a.workspace = static_cast<float*>(workspace.data_ptr());
+    a.workspace_floats = (uint64_t)need;
+  }
+  check((hipError_t)ab200_paged_attn(&a, stream_handle()), what);
+  return out;
+}
+
 // ---- from Python ------------------------------------------------------------------------------------------
 
 // A torch.Tensor or Parameter (no subclass) that is plain().  The tensor itself goes to *out.
@@ -743,6 +838,186 @@ PyObject* relative_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// join_columns(k, shared): the joined keys, or None: not an ordinary call.  (The caller has looked at types and shapes.)
+PyObject* join_columns_from(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 2) {
+    PyErr_SetString(PyExc_TypeError, "join_columns takes 2 arguments");
+    return nullptr;
+  }
+  if (!ordinary_first(a[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  Tensor k, shared;
+  if (!attention_operand(a[0], dev, &k) || !attention_operand(a[1], dev, &shared)) Py_RETURN_NONE;
+  if (shared.scalar_type() != k.scalar_type() || shared.size(0) != k.size(0) || shared.size(1) != 1 || shared.size(2) != k.size(2)) Py_RETURN_NONE;
+  Tensor out;
+  {
+    pybind11::gil_scoped_release release;
+    out = at::GradMode::is_enabled() && (k.requires_grad() || shared.requires_grad()) ? JoinColumns::apply(k, shared) : join_columns(k, shared);
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// A contiguous tensor of whole numbers of this type and rank, without gradients; or not.
+bool whole_numbers(PyObject* o, int dev, at::ScalarType type, int64_t dim, Tensor* out) {
+  if (!plain_tensor(o, dev, out)) return false;
+  return out->scalar_type() == type && out->dim() == dim;
+}
+bool wants_gradient(std::initializer_list<const Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+// Rows that start on 16 bytes, where the type and the head dim allow it.
+bool aligned_rows(const Tensor& t) {
+  const int64_t per = 16 / (int64_t)t.element_size();
+  if (t.size(-1) % per != 0) return true;
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) return false;
+  for (int64_t i = 0; i + 1 < t.dim(); ++i)
+    if (t.size(i) > 1 && t.stride(i) % per != 0) return false;
+  return true;
+}
+
+// paged_attention(q, k_cache, v_cache, block_table, lengths, query_lengths, window, sinks, sm_scale, return_lse), or with a latent cache
+// paged_attention(q, cache, value_dim, ...): out, or (out, lse), or None: not an ordinary call, or one whose arguments the caller is to look at.
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) {
+    PyErr_SetString(PyExc_TypeError, "paged_attention takes 10 arguments");
+    return nullptr;
+  }
+  if (!ordinary_first(a[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  PagedCall c{};
+  Tensor q, k, v, table, lengths, query_lengths;
+  if (!attention_operand(a[0], dev, &q) || !plain_tensor(a[1], dev, &k) || k.scalar_type() != q.scalar_type()) Py_RETURN_NONE;
+  const bool latent = PyLong_CheckExact(a[2]);
+  if (latent) {
+    if (!small_int(a[2], &c.value_dim) || k.dim() != 3 || c.value_dim < 1 || c.value_dim > k.size(2)) Py_RETURN_NONE;
+  } else if (!attention_operand(a[2], dev, &v) || v.scalar_type() != q.scalar_type() || k.dim() != 4 || v.size(0) != k.size(0) || v.size(1) != k.size(1) ||
+             v.size(2) != k.size(2) || q.size(1) % k.size(2) != 0 || v.size(3) > 1024) {
+    Py_RETURN_NONE;
+  }
+  if (k.size(-1) != q.size(3) || q.size(3) > 1024 || !aligned_rows(q)) Py_RETURN_NONE;
+  if (!whole_numbers(a[3], dev, at::kInt, 2, &table) || !whole_numbers(a[4], dev, at::kInt, 1, &lengths) || table.size(0) != q.size(0) ||
+      lengths.size(0) != q.size(0))
+    Py_RETURN_NONE;
+  if (a[5] != Py_None && (!whole_numbers(a[5], dev, at::kInt, 1, &query_lengths) || query_lengths.size(0) != q.size(0))) Py_RETURN_NONE;
+  if (a[6] != Py_None && (!small_int(a[6], &c.window) || c.window < 1)) Py_RETURN_NONE;
+  if (!small_int(a[7], &c.sinks) || c.sinks < 0 || !number(a[8], &c.sm_scale)) Py_RETURN_NONE;
+  for (const Tensor* t : {&q, &k, &v, &table})
+    if (t->defined())
+      for (const int64_t x : t->sizes())
+        if (x > INT32_MAX) Py_RETURN_NONE;
+  const bool return_lse = a[9] == Py_True;
+  if ((!return_lse && a[9] != Py_False) || wants_gradient({&q, &k, &v})) Py_RETURN_NONE;
+  Tensor out, lse;
+  {
+    pybind11::gil_scoped_release release;
+    out = paged_attend(c, q, k, v, table, lengths, query_lengths, return_lse ? &lse : nullptr);
+  }
+  if (!return_lse) return THPVariable_Wrap(std::move(out));
+  return PyTuple_Pack(2, pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(out))).ptr(),
+                      pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(lse))).ptr());
+  END_HANDLE_TH_ERRORS
+}
+
+// block_tables(block_table, lengths, new_tokens, free_pages, page_size, total_tokens, taken): (slots, cu_seqlens, lengths, taken), or None as above.
+PyObject* block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) {
+    PyErr_SetString(PyExc_TypeError, "block_tables takes 7 arguments");
+    return nullptr;
+  }
+  if (!ordinary_first(a[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  Tensor table, lengths, new_tokens, free_pages, taken;
+  int64_t page, total;
+  if (!whole_numbers(a[0], dev, at::kInt, 2, &table) || !whole_numbers(a[1], dev, at::kInt, 1, &lengths) || !whole_numbers(a[2], dev, at::kInt, 1, &new_tokens) ||
+      !whole_numbers(a[3], dev, at::kInt, 1, &free_pages) || !small_int(a[4], &page) || !small_int(a[5], &total))
+    Py_RETURN_NONE;
+  if (a[6] != Py_None && (!whole_numbers(a[6], dev, at::kInt, 1, &taken) || taken.numel() != 1)) Py_RETURN_NONE;
+  const int64_t batch = table.size(0);
+  if (lengths.size(0) != batch || new_tokens.size(0) != batch || batch > INT32_MAX || table.size(1) > INT32_MAX || page < 1 || total < 1) Py_RETURN_NONE;
+  Tensor out[4];
+  {
+    pybind11::gil_scoped_release release;
+    at::AutoDispatchBelowADInplaceOrView guard;
+    out[0] = fresh({total}, at::kLong);
+    out[1] = fresh({batch + 1}, at::kInt);
+    out[2] = fresh({batch}, at::kInt);
+    out[3] = fresh({1}, at::kInt);
+    ab200_block_tables_args b{};
+    b.batch = (int32_t)batch; b.page_size = (int32_t)page; b.table_width = (int32_t)table.size(1);
+    b.block_table = static_cast<int32_t*>(table.data_ptr());
+    b.table_stride = table.stride(0);
+    b.lengths = static_cast<const int32_t*>(lengths.data_ptr());
+    b.new_tokens = static_cast<const int32_t*>(new_tokens.data_ptr());
+    b.free_pages = static_cast<const int32_t*>(free_pages.data_ptr());
+    b.num_free = free_pages.numel();
+    b.taken = taken.defined() ? static_cast<const int32_t*>(taken.data_ptr()) : nullptr;
+    b.total_tokens = total;
+    b.slots = static_cast<int64_t*>(out[0].data_ptr());
+    b.cu_seqlens = static_cast<int32_t*>(out[1].data_ptr());
+    b.new_lengths = static_cast<int32_t*>(out[2].data_ptr());
+    b.taken_out = static_cast<int32_t*>(out[3].data_ptr());
+    check((hipError_t)ab200_block_tables(&b, stream_handle()), "block_tables");
+    if (!table.is_inference()) table.unsafeGetTensorImpl()->bump_version();
+  }
+  PyObject* r = PyTuple_New(4);
+  if (r == nullptr) return nullptr;
+  for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(r, i, THPVariable_Wrap(std::move(out[i])));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_write(k, v, k_cache, v_cache, slots): True, or None as above.
+PyObject* paged_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) {
+    PyErr_SetString(PyExc_TypeError, "paged_write takes 5 arguments");
+    return nullptr;
+  }
+  if (!ordinary_first(a[0])) Py_RETURN_NONE;
+  const int dev = c10::cuda::current_device();
+  Tensor k, v, k_cache, v_cache, slots;
+  const bool values = a[1] != Py_None;
+  if (values != (a[3] != Py_None)) Py_RETURN_NONE;
+  auto pair = [&](PyObject* x, PyObject* cache, Tensor* xt, Tensor* ct) {
+    return plain_tensor(x, dev, xt) && floating(xt->scalar_type()) && xt->dim() == 3 && attention_operand(cache, dev, ct) && ct->scalar_type() == xt->scalar_type() &&
+           ct->size(2) == xt->size(1) && ct->size(3) == xt->size(2) && ct->size(1) <= INT32_MAX;
+  };
+  if (!pair(a[0], a[2], &k, &k_cache) || (values && !pair(a[1], a[3], &v, &v_cache))) Py_RETURN_NONE;
+  if (values && (v.scalar_type() != k.scalar_type() || v.size(0) != k.size(0) || v.size(1) != k.size(1) || v_cache.size(0) != k_cache.size(0) ||
+                 v_cache.size(1) != k_cache.size(1)))
+    Py_RETURN_NONE;
+  if (!whole_numbers(a[4], dev, at::kLong, 1, &slots) || slots.size(0) != k.size(0) || wants_gradient({&k, &v, &k_cache, &v_cache})) Py_RETURN_NONE;
+  {
+    pybind11::gil_scoped_release release;
+    ab200_paged_write_args w{};
+    w.dtype = code_of(k.scalar_type());
+    w.num_heads = (int32_t)k.size(1); w.head_dim_k = (int32_t)k.size(2); w.page_size = (int32_t)k_cache.size(1);
+    w.num_pages = k_cache.size(0); w.tokens = k.size(0);
+    w.k = k.data_ptr(); w.k_cache = k_cache.data_ptr();
+    w.slots = static_cast<const int64_t*>(slots.data_ptr());
+    for (int i = 0; i < 2; ++i) w.k_stride[i] = k.stride(i);
+    for (int i = 0; i < 3; ++i) w.k_cache_stride[i] = k_cache.stride(i);
+    if (values) {
+      w.head_dim_v = (int32_t)v.size(2);
+      w.v = v.data_ptr(); w.v_cache = v_cache.data_ptr();
+      for (int i = 0; i < 2; ++i) w.v_stride[i] = v.stride(i);
+      for (int i = 0; i < 3; ++i) w.v_cache_stride[i] = v_cache.stride(i);
+    }
+    check((hipError_t)ab200_paged_write(&w, stream_handle()), "paged_write");
+    for (const Tensor* t : {&k_cache, &v_cache})
+      if (t->defined() && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+  }
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // set_python_function(name, fn): what python_functions() holds.
 PyObject* set_python_function(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -778,6 +1053,10 @@ PyMethodDef kMethods[] = {{"attend", reinterpret_cast<PyCFunction>(reinterpret_c
                           {"sink_attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&sink_attend)), METH_FASTCALL, nullptr},
                           {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&dropout)), METH_FASTCALL, nullptr},
                           {"relative_bias", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&relative_bias)), METH_FASTCALL, nullptr},
+                          {"join_columns", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&join_columns_from)), METH_FASTCALL, nullptr},
+                          {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&paged_attention)), METH_FASTCALL, nullptr},
+                          {"block_tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&block_tables)), METH_FASTCALL, nullptr},
+                          {"paged_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&paged_write)), METH_FASTCALL, nullptr},
                           {"set_python_function", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&set_python_function)), METH_FASTCALL, nullptr},
                           {"set_python_backward", &set_python_backward, METH_O, nullptr},
                           {"last_bwd_family", &last_bwd_family, METH_NOARGS, nullptr},

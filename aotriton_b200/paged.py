@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from . import cabi
-from .autograd import _FLOATS, _check, _on_its_device, _unit_rows
+from .autograd import _FLOATS, _check, _native, _on_its_device, _unit_rows
 from .flash import hipError_t
 
 
@@ -51,6 +51,7 @@ def _block_tables(block_table, lengths, new_tokens, free_pages, page_size, total
                     torch.empty_like(lengths), torch.empty([1], device=device, dtype=torch.int32))
     stream = torch.cuda.current_stream(device).cuda_stream
     _check(hipError_t(cabi.block_tables(block_table, lengths, new_tokens, free_pages, page_size, *r, taken=taken, stream=stream)), "block_tables")
+    torch.autograd.graph.increment_version(block_table)
     return r
 
 
@@ -64,6 +65,10 @@ def block_tables(block_table, lengths, new_tokens, free_pages, page_size, total_
 
     total_tokens, a number, is at least the sum of new_tokens (what is beyond it gets neither slot nor page); slots behind that sum are -1.  Where the row is too
     short or the free list used up, tokens have the slot -1 (paged_write skips them), and `taken` exceeds the length of the free list in the second case."""
+    if not torch.compiler.is_compiling():
+        r = _native.block_tables(block_table, lengths, new_tokens, free_pages, page_size, total_tokens, taken)
+        if r is not None:
+            return BlockTables._make(r)
     if not isinstance(block_table, torch.Tensor) or not block_table.is_cuda or not _int32(block_table, 2, block_table.device):
         raise ValueError("block_tables: the block table is a (batch, width) int32 CUDA tensor with rows of unit stride")
     device, batch = block_table.device, block_table.shape[0]
@@ -95,6 +100,8 @@ def paged_write(k, v, k_cache, v_cache, slots):
     the cache (-1) is skipped; the slots of a call differ from one another (of two tokens with one slot, parts of either may be left).  v and
     v_cache may be None, and their dim another than the keys': a latent cache of (pages, page_size, width) is written from a latent vector and
     its position columns with cache[:, :, None, :n] and cache[:, :, None, n:]."""
+    if not torch.compiler.is_compiling() and _native.paged_write(k, v, k_cache, v_cache, slots):
+        return
     if (v is None) != (v_cache is None):
         raise ValueError("paged_write: values and their cache come together")
     for x, cache in ((k, k_cache), (v, v_cache)):
@@ -173,12 +180,16 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sink
     a batch of very different ones keeps the GPU busy.  The same inputs give the same bits.  No gradient.
 
     fp16 and bf16 with head dims up to 128 that are multiples of 8, 16-byte aligned caches, pages of a multiple of 8 slots and few queries are fastest."""
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
+    if not torch.compiler.is_compiling():
+        r = _native.paged_attention(q, k_cache, v_cache, block_table, lengths, query_lengths, window, sinks, sm_scale, return_lse)
+        if r is not None:
+            return r
     for t in (k_cache, v_cache):
         if not _is_cache(t, q) or t.shape[:3] != k_cache.shape[:3]:
             raise ValueError("paged_attention: the caches are (pages, page_size, heads, dim) tensors of q's device and type with unit innermost stride")
     if k_cache.shape[3] != q.shape[-1]:
         raise ValueError(f"paged_attention: head dims {q.shape[-1]} of q and {k_cache.shape[3]} of the keys")
-    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
     return _attend(q, k_cache, v_cache, block_table, lengths, query_lengths, window, sinks, sm_scale, return_lse, "paged_attention")
 
 
@@ -187,6 +198,10 @@ def paged_latent_attention(q, cache, block_table, lengths, value_dim, sm_scale, 
     q: (B, H, Sq, width), each head's queries already multiplied by its key expansion, followed by their position columns; cache: (pages, page_size, width); the
     output (B, H, Sq, value_dim) is still to be multiplied by each head's value expansion.  sm_scale is that of the expanded form, the inverse root of a
     head's key width there (autograd.latent_attention computes the same from expanded keys and values, with gradients).  The rest as in paged_attention."""
+    if not torch.compiler.is_compiling():
+        r = _native.paged_attention(q, cache, value_dim, block_table, lengths, query_lengths, None, 0, sm_scale, return_lse)
+        if r is not None:
+            return r
     if cache.dim() != 3 or not _is_cache(cache[:, :, None], q) or cache.shape[2] != q.shape[-1]:
         raise ValueError("paged_latent_attention: the cache is a (pages, page_size, width) tensor of q's device, type and width with unit innermost stride")
     if type(value_dim) is not int or not 1 <= value_dim <= cache.shape[2]:
