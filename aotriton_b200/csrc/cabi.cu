@@ -1076,7 +1076,8 @@ int64_t ab200_paged_attn_workspace(const ab200_paged_attn_args* a, void* stream)
   if (int e = fill_paged(a, p)) return -e;
   if (int e = check_device(st)) return -e;
   if (p.batch == 0 || p.sq == 0) return 0;
-  return plan_paged(a->dtype, p, device_info(stream_device(st)).sms);
+  const int64_t need = plan_paged(a->dtype, p, device_info(stream_device(st)).sms);
+  return need < 0 ? -kErrNotSupported : need;
 }
 
 int ab200_paged_attn(const ab200_paged_attn_args* a, void* stream) {
@@ -1086,6 +1087,7 @@ int ab200_paged_attn(const ab200_paged_attn_args* a, void* stream) {
   if (int e = check_device(st)) return e;
   if (p.batch == 0 || p.sq == 0) return 0;
   const int64_t need = plan_paged(a->dtype, p, device_info(stream_device(st)).sms);
+  if (need < 0) return kErrNotSupported;
   if (need > 0 && (a->workspace == nullptr || a->workspace_floats < (uint64_t)need || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0))
     return kErrInvalidValue;
   p.partial = a->workspace;

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const __grid
 // ---- attention, any type and size up to 1024 ----------------------------------------------------------------------
 // Tiles of 32 keys: eight lanes form a key's scores with the unit's rows, a warp a row takes their softmax on, and a thread a column adds up
 // the values; with fewer columns than threads, groups of threads share the keys.
-constexpr int kGenThreads = 256, kGenRows = 8, kGenKeys = 32, kGenMaxDim = 1024;
+constexpr int kGenThreads = 256, kGenRows = 8, kGenKeys = 32;
 
 template <typename T, int N>
 __device__ __forceinline__ void load_vec(const T* src, float (&x)[N]) {
@@ -150,30 +150,22 @@ __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid
   extern __shared__ float q_s[];      // [kGenRows][dqk]
   __shared__ float s[kGenRows][kGenKeys], alpha[kGenRows], m_s[kGenRows], l_s[kGenRows];
   __shared__ float meet[J == 1 ? kGenThreads * kGenRows : 1];
-  __shared__ int64_t page_of[kGenKeys], scratch[kGenThreads / 32 + 4];
+  __shared__ int64_t page_of[kGenKeys];
+  __shared__ int scratch[kGenThreads / 32 + 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Line line = find_in_line<kGenThreads>(p, -1, blockIdx.x, scratch);
+  const Line line = find_in_line<kGenThreads>(p, -1, blockIdx.x / p.lanes, scratch);
   if (line.z >= p.batch) return;
-  int64_t at = (int64_t)blockIdx.x * line.share;
-  const int64_t end = min(at + line.share, line.total);
   int width = 32;      // threads that share the columns
   while (width < p.dvo && width < kGenThreads) width <<= 1;
   const int groups = kGenThreads / width, group = tid / width, col = tid - group * width;
-  int z = line.z;
-  int64_t base = line.base;
-  Walk w(p, z);
-  while (at < end) {
-    while (at >= base + (int64_t)w.tiles * p.hk * p.chunks) {
-      base += (int64_t)w.tiles * p.hk * p.chunks;
-      w = Walk(p, ++z);
-    }
-    const int u = (int)((at - base) / w.tiles), hk = u / p.chunks, chunk = u - hk * p.chunks;
-    const int64_t unit = base + (int64_t)u * w.tiles;
-    const int first = (int)(at - unit), last = (int)(min(end, unit + w.tiles) - unit);
-    at = unit + last;
-    const bool whole = first == 0 && last == w.tiles;
-    const Rows rows(p, w, chunk);
-    if (first == 0 && chunk == 0) zero_rows_behind<T, kGenThreads>(p, w, z, hk, tid);
+  Piece c(p, line);
+  while (c.more()) {
+    c.next(p);
+    const Walk& w = c.w;
+    const int z = c.z, hk = c.hk, first = c.first, last = c.last;
+    const bool whole = c.whole();
+    const Rows rows(p, w, c.chunk);
+    if (first == 0 && c.chunk == 0) zero_rows_behind<T, kGenThreads>(p, w, z, hk, tid);
     if (rows.n == 0) continue;
     __syncthreads();
     for (int i = tid; i < rows.n * p.dqk; i += kGenThreads) {
@@ -281,7 +273,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid
         __syncthreads();
       }
     }
-    float* part = partial_of(p, 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0));
+    float* part = partial_of(p, c);
 #pragma unroll
     for (int r = 0; r < kGenRows; ++r) {
       if (r >= rows.n) continue;
@@ -303,75 +295,83 @@ __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid
 }
 
 // ---- the pieces of split units ----------------------------------------------------------------------------------------
-// grid = (batch * hk * chunks, rows): a block a row.  Weighs the pieces' rows by their maxima and adds them up in the order of the keys.
-constexpr int kJoinThreads = 128;
+// grid = (batch * hk * chunks, rows / 4): a warp a row.  Weighs the pieces' rows by their maxima and adds them up in the order of the keys, a few pieces'
+// columns on the way at a time.  V: float4, or float where the columns are not a multiple of 4; K: vectors of a lane.
+constexpr int kJoinThreads = 128, kJoinRows = kJoinThreads / 32;
 
-template <typename T>
+template <typename V> __device__ __forceinline__ void add_weighed(V& a, float w, const V& x);
+template <> __device__ __forceinline__ void add_weighed<float>(float& a, float w, const float& x) { a = fmaf(w, x, a); }
+template <> __device__ __forceinline__ void add_weighed<float4>(float4& a, float w, const float4& x) {
+  a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w);
+}
+
+template <typename T, typename V, int K>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttn p) {
+  constexpr int N = sizeof(V) / 4, kAhead = K > 4 ? 2 : (K > 1 ? 4 : 8);
+  __shared__ int scratch[kJoinThreads / 32 + 2];
+  const int tid = threadIdx.x, lane = tid & 31, units = p.hk * p.chunks;
   wait_for_earlier_grids();
-  __shared__ int64_t scratch[kJoinThreads / 32 + 4];
-  __shared__ float weight[kJoinThreads], red[2][kJoinThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, units = p.hk * p.chunks;
-  const int z = (int)(blockIdx.x / units), u = (int)(blockIdx.x - (unsigned)z * units), r = blockIdx.y;
-  const Walk w(p, z);
-  const Rows rows(p, w, u % p.chunks);
-  if (r >= rows.n) return;
+  const int z = (int)(blockIdx.x / (unsigned)units), u = (int)(blockIdx.x - (unsigned)z * units), r = blockIdx.y * kJoinRows + tid / 32;
   const Line line = find_in_line<kJoinThreads>(p, z, 0, scratch);
-  const int64_t unit = line.base + (int64_t)u * w.tiles;
-  const int64_t c0 = unit / line.share, c1 = (unit + w.tiles - 1) / line.share;
+  const Walk w(p, z);
+  const int hk = u / p.chunks, chunk = u - hk * p.chunks, along = hk * (p.chunks / p.lanes) + chunk / p.lanes;
+  const Rows rows(p, w, chunk);
+  if (r >= rows.n) return;
+  const int unit = line.base + along * w.tiles;
+  const int c0 = unit / line.share, c1 = (unit + w.tiles - 1) / line.share;
   if (c0 == c1) return;      // (finished where it was formed)
   if (p.status != nullptr && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
-  auto piece = [&](int64_t c) { return partial_of(p, 2 * c + (c == c0 ? 1 : 0)); };
+  auto piece = [&](int c) { return partial_of(p, 2 * ((int64_t)c * p.lanes + chunk % p.lanes) + (c == c0 ? 1 : 0)); };
   const int64_t at_m = (int64_t)p.rows * p.dvo + r, at_l = at_m + p.rows;
   float mx = -INFINITY;
-  for (int64_t c = c0 + tid; c <= c1; c += kJoinThreads) mx = fmaxf(mx, piece(c)[at_m]);
+  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, piece(c)[at_m]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  if (lane == 0) red[0][warp] = mx;
-  __syncthreads();
-  mx = red[0][0];
-#pragma unroll
-  for (int i = 1; i < kJoinThreads / 32; ++i) mx = fmaxf(mx, red[0][i]);
   const float ref = mx == -INFINITY ? 0.f : mx;
-  constexpr int kCols = kGenMaxDim / kJoinThreads;
-  float acc[kCols], l = 0.f;
+  V acc[K];
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
-  for (int64_t from = c0; from <= c1; from += kJoinThreads) {
-    const int n = (int)min((int64_t)kJoinThreads, c1 - from + 1);
-    __syncthreads();
-    if (tid < n) {
-      const float* q = piece(from + tid);
-      const float x = exp2f(q[at_m] - ref);
-      weight[tid] = x;
-      l = fmaf(x, q[at_l], l);
+  for (int k = 0; k < K; ++k) acc[k] = V{};
+  float l = 0.f;
+  for (int from = c0; from <= c1; from += 32) {
+    const int n = min(32, c1 - from + 1);
+    float weight = 0.f;
+    if (lane < n) {
+      const float* q = piece(from + lane);
+      weight = exp2f(q[at_m] - ref);
+      l = fmaf(weight, q[at_l], l);
     }
-    __syncthreads();
+    for (int i = 0; i < n; i += kAhead) {
+      V x[kAhead][K];
 #pragma unroll
-    for (int j = 0; j < kCols; ++j) {
-      const int d = tid + j * kJoinThreads;
-      if (d >= p.dvo) break;
-      float a = acc[j];
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) a = fmaf(weight[i], piece(from + i)[(int64_t)r * p.dvo + d], a);
-      acc[j] = a;
+      for (int a = 0; a < kAhead; ++a) {
+        const V* src = reinterpret_cast<const V*>(piece(from + min(i + a, n - 1)) + (int64_t)r * p.dvo);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+          if ((lane + 32 * k) * N < p.dvo) x[a][k] = src[lane + 32 * k];
+      }
+#pragma unroll
+      for (int a = 0; a < kAhead; ++a) {
+        const float f = __shfl_sync(0xffffffffu, weight, (i + a) & 31);
+        if (i + a < n)
+#pragma unroll
+          for (int k = 0; k < K; ++k)
+            if ((lane + 32 * k) * N < p.dvo) add_weighed(acc[k], f, x[a][k]);
+      }
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  if (lane == 0) red[1][warp] = l;
-  __syncthreads();
-  l = 0.f;
-#pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) l += red[1][i];
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  const int hk = u / p.chunks, h = rows.head(p, hk, r), m = rows.query(r);
+  const int h = rows.head(p, hk, r), m = rows.query(r);
+  T* out = out_row<T>(p, z, h, m);
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    const int d = tid + j * kJoinThreads;
-    if (d < p.dvo) out_row<T>(p, z, h, m)[d] = from_f32<T>(acc[j] * inv);
+  for (int k = 0; k < K; ++k) {
+    const float* e = reinterpret_cast<const float*>(&acc[k]);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if ((lane + 32 * k) * N < p.dvo) out[(lane + 32 * k) * N + j] = from_f32<T>(e[j] * inv);
   }
-  if (tid == 0) put_lse(p, z, h, m, mx, l);
+  if (lane == 0) put_lse(p, z, h, m, mx, l);
 }
 
 // ---- keys that share columns --------------------------------------------------------------------------------------
@@ -436,9 +436,16 @@ cudaError_t launch_general_T(const PagedAttn& p, cudaStream_t st) {
   if (p.dvo <= kGenThreads) return vec ? launch_general_NJ<T, N, 1>(p, st) : launch_general_NJ<T, 1, 1>(p, st);
   return vec ? launch_general_NJ<T, N, 4>(p, st) : launch_general_NJ<T, 1, 4>(p, st);
 }
+template <typename T, typename V, int K>
+cudaError_t launch_join_K(const PagedAttn& p, cudaStream_t st) {
+  const int rows = (int)std::min<int64_t>(p.rows, (int64_t)p.group * p.sq);
+  return launch_counted(paged_join_kernel<T, V, K>, dim3((unsigned)((int64_t)p.batch * p.hk * p.chunks), (rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, st, p);
+}
 template <typename T>
 cudaError_t launch_join_T(const PagedAttn& p, cudaStream_t st) {
-  return launch_counted(paged_join_kernel<T>, dim3((unsigned)((int64_t)p.batch * p.hk * p.chunks), p.rows), kJoinThreads, 0, st, p);
+  if (p.dvo % 4 != 0) return launch_join_K<T, float, 32>(p, st);
+  if (p.dvo <= 128) return launch_join_K<T, float4, 1>(p, st);
+  return p.dvo <= 512 ? launch_join_K<T, float4, 4>(p, st) : launch_join_K<T, float4, 8>(p, st);
 }
 
 template <typename F>
@@ -472,14 +479,20 @@ int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
   if (!plan_paged_latent(dtype, p, sms) && !plan_paged_split(dtype, p, sms)) {
     p.kind = kPagedGeneral;
     p.rows = kGenRows;
-    p.tile_keys = kGenKeys;
+    p.tile_log = 5;
     p.min_tiles = 2;
     p.ctas = sms * 4;
   }
-  p.chunks = (int)(((int64_t)p.group * p.sq + p.rows - 1) / p.rows);
-  const int64_t units = (int64_t)p.batch * p.hk * p.chunks;
-  const int64_t most = std::max<int64_t>(1, ((int64_t)p.width * p.page + p.tile_keys - 1) / p.tile_keys + 1);      // tiles of a unit (one more: a window across a border)
-  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(p.ctas, units * most / p.min_tiles + 1));
+  const int64_t chunks = ((int64_t)p.group * p.sq + p.rows - 1) / p.rows;
+  p.chunks = (int)chunks;
+  // (a last tile's keys are counted in 32 bits)
+  p.max_len = (int32_t)std::min<int64_t>((int64_t)p.width * p.page, 0x7fffff00);
+  const int64_t most = (p.max_len >> p.tile_log) + 2;      // tiles of a unit: a window may cross a border
+  const int64_t units = (int64_t)p.batch * p.hk * chunks;
+  if (units * most > 0x3fffffff) return -kPagedTooLarge;
+  // A kv head's chunks side by side, so that its keys come from memory once, unless that left too few CTAs to share a line out evenly.
+  p.lanes = chunks <= 8 ? (int)chunks : 1;
+  p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(p.ctas / p.lanes, units / p.lanes * most / p.min_tiles + 1)) * p.lanes;
   p.join = most > 1;
   return p.join ? 2 * (int64_t)p.ctas * partial_floats(p) : 0;
 }

@@ -40,9 +40,10 @@ struct PagedAttn {
   int32_t batch, hq, hk, group, sq, dqk, dvo;
   float qk_scale;                    // sm_scale * log2(e)
   int32_t window, sinks;             // window INT32_MAX: none
-  // How the call is cut (plan_paged): the tiles of all units -- (sequence, kv head, chunk of `rows` query rows) -- stand in one line,
-  // of which each of `ctas` CTAs takes an equal piece, min_tiles at least.
-  int32_t kind, ctas, rows, chunks, tile_keys, min_tiles, join, stages, box;      // box: slots of a tile copy
+  int32_t max_len;                   // what the table has room for
+  // How the call is cut (plan_paged, paged_split.cuh): into units -- (sequence, kv head, chunk of `rows` query rows) -- and tiles of 2^tile_log keys, for `ctas`
+  // CTAs, min_tiles a CTA at least; `lanes` chunks side by side (a divisor of the chunks, and of the CTAs).  box: slots of a tile copy.
+  int32_t kind, ctas, lanes, rows, chunks, tile_log, min_tiles, join, box;
   unsigned int* status;              // the word in which a kernel records a wait that ran out (null: the general kernel has none)
   float* partial;                    // two partial results a CTA: of the unit that it starts with, of the one that it ends with
   uint32_t wait_limit_kcycles;
@@ -57,7 +58,8 @@ struct SharedColumns {
 
 cudaError_t launch_block_tables(const BlockTables& a, cudaStream_t st);
 cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st);
-// Chooses the kernel and how the call is cut for `sms` SMs; returns the floats of workspace it needs.
+// Chooses the kernel and how the call is cut for `sms` SMs; returns the floats of workspace it needs, or -kPagedTooLarge: more tiles than are counted.
+constexpr int64_t kPagedTooLarge = 1;
 int64_t plan_paged(int dtype, PagedAttn& a, int sms);
 cudaError_t launch_paged(int dtype, PagedAttn& a, cudaStream_t st);
 // The tensor-core kernels: whether one takes the call, and if so how it cuts it (all but ctas' bound and the workspace); and its launch.

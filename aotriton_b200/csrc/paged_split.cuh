@@ -12,73 +12,69 @@
 namespace ab200 {
 namespace {
 
-// What a sequence's queries see of its keys: the first `sinks` and those from `lo` on, in tiles of p.tile_keys.  At least one tile, so
+// What a sequence's queries see of its keys: the first `sinks` and those from `lo` on, in tiles of 2^p.tile_log keys.  At least one tile, so
 // that every unit has an owner.
 struct Walk {
   int len, queries, lo, first, n_sink, tiles;
-  __device__ __forceinline__ Walk(const PagedAttn& p, int z) {
-    const int64_t room = (int64_t)p.width * p.page;
-    const int64_t most = room < 0x7fffff00 ? room : 0x7fffff00;      // (a last tile's keys are counted in 32 bits)
-    int64_t l = p.lengths[z];
-    l = l < 0 ? 0 : (l < most ? l : most);
-    len = (int)l;
-    queries = p.query_lengths != nullptr ? min(max(p.query_lengths[z], 0), p.sq) : p.sq;
+  __device__ __forceinline__ Walk(const PagedAttn& p, int z) : Walk(p, p.lengths[z], p.query_lengths != nullptr ? p.query_lengths[z] : p.sq) {}
+  __device__ __forceinline__ Walk(const PagedAttn& p, int length, int query_length) {
+    len = min(max(length, 0), p.max_len);
+    queries = min(max(query_length, 0), p.sq);
     if (len == 0 || queries == 0) { lo = first = n_sink = 0; tiles = 1; return; }
     const int64_t from = (int64_t)len - queries - p.window + 1;      // the first query's window
     lo = from > 0 ? (int)from : 0;
-    first = lo / p.tile_keys;
-    n_sink = min((min(p.sinks, lo) + p.tile_keys - 1) / p.tile_keys, first);
-    tiles = n_sink + (len - 1) / p.tile_keys - first + 1;
+    first = lo >> p.tile_log;
+    n_sink = min((min(p.sinks, lo) + (1 << p.tile_log) - 1) >> p.tile_log, first);
+    tiles = n_sink + ((len - 1) >> p.tile_log) - first + 1;
   }
   __device__ __forceinline__ int tile(int i) const { return i < n_sink ? i : first + i - n_sink; }
   // Whether some query of the sequence sees key n, its page apart.
   __device__ __forceinline__ bool seen(const PagedAttn& p, int n) const { return n < len && (n >= lo || n < p.sinks); }
 };
 
-// The line of tiles as one thread block sees it.
+// The line of tiles as one thread block sees it; the host has seen to it that 31 bits hold it.  `lanes` CTAs next to each other take the same piece of
+// a line without the chunks, a chunk each: they read the same keys at the same time.
 struct Line {
-  int64_t total, share;      // tiles in all, and of a CTA
-  int64_t base;              // first tile of sequence z
+  int total, share;      // tiles in all, and of a CTA
+  int base;              // first tile of sequence z
   int z;
 };
 
-// A block of NT threads (a multiple of 32) finds sequence `z`, or the one that tile `at` belongs to (z < 0).  `scratch`: NT / 32 + 4 words of 8 bytes.
-// Of a tile behind the last, z is the batch's size.
+// A block of NT threads (a multiple of 32) finds sequence `z`, or the one that the first tile of piece `piece` belongs to (z < 0).  `scratch`: NT / 32 + 2
+// words.  Behind the last tile, z is the batch's size.
 template <int NT>
-__device__ __forceinline__ Line find_in_line(const PagedAttn& p, int z, int64_t cta, int64_t* scratch) {
+__device__ __forceinline__ Line find_in_line(const PagedAttn& p, int z, int piece, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t units = (int64_t)p.hk * p.chunks;
+  const int units = p.hk * p.chunks / p.lanes;
   const int each = (p.batch + NT - 1) / NT, z0 = min(tid * each, p.batch), z1 = min(z0 + each, p.batch);
-  int64_t mine = 0;
+  int mine = 0;
   for (int i = z0; i < z1; ++i) mine += Walk(p, i).tiles;
-  int64_t up = mine;
+  int up = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t o = __shfl_up_sync(0xffffffffu, up, d);
+    const int o = __shfl_up_sync(0xffffffffu, up, d);
     if (lane >= d) up += o;
   }
   if (lane == 31) scratch[warp] = up;
+  if (tid == 0) scratch[NT / 32] = p.batch;
   __syncthreads();
-  int64_t before = 0, total = 0;
+  int before = 0, total = 0;
+#pragma unroll
   for (int w = 0; w < NT / 32; ++w) {
-    const int64_t s = scratch[w];
+    const int s = scratch[w];
     if (w < warp) before += s;
     total += s;
   }
   before += up - mine;
   Line r;
   r.total = total * units;
-  r.share = (r.total + p.ctas - 1) / p.ctas;
-  if (r.share < p.min_tiles) r.share = p.min_tiles;
-  const int64_t at = cta * r.share;
-  if (tid == 0) { scratch[NT / 32] = p.batch; scratch[NT / 32 + 1] = r.total; }
-  __syncthreads();
+  r.share = max((int)((unsigned)(r.total + p.ctas / p.lanes - 1) / (unsigned)(p.ctas / p.lanes)), p.min_tiles);
+  const int64_t at = (int64_t)piece * r.share;
   if (z >= 0 ? (z >= z0 && z < z1) : (mine > 0 && at >= before * units && at < (before + mine) * units)) {
-    int64_t b = before;
-    int i = z0;
+    int b = before, i = z0;
     for (; i + 1 < z1; ++i) {
       if (i == z) break;
-      const int64_t t = Walk(p, i).tiles;
+      const int t = Walk(p, i).tiles;
       if (z < 0 && at < (b + t) * units) break;
       b += t;
     }
@@ -86,10 +82,37 @@ __device__ __forceinline__ Line find_in_line(const PagedAttn& p, int z, int64_t 
     scratch[NT / 32 + 1] = b * units;
   }
   __syncthreads();
-  r.z = (int)scratch[NT / 32];
+  r.z = scratch[NT / 32];
   r.base = scratch[NT / 32 + 1];
   return r;
 }
+
+// A CTA's way along its piece of the line.
+struct Piece {
+  int at, end, z, base, lane;
+  Walk w;
+  int hk, chunk, first, last;      // the current unit, and its tiles in this piece
+  __device__ __forceinline__ Piece(const PagedAttn& p, const Line& line)
+      : at((int)(blockIdx.x / p.lanes) * line.share), end(min(at + line.share, line.total)), z(line.z), base(line.base),
+        lane((int)(blockIdx.x % p.lanes)), w(p, line.z), hk(0), chunk(0), first(0), last(0) {}
+  __device__ __forceinline__ bool more() const { return at < end; }
+  // The next unit; `at` is moved behind it.
+  __device__ __forceinline__ void next(const PagedAttn& p) {
+    const int chunks = p.chunks / p.lanes, units = p.hk * chunks;
+    while (at >= base + w.tiles * units) {
+      base += w.tiles * units;
+      w = Walk(p, ++z);
+    }
+    const int u = (int)((unsigned)(at - base) / (unsigned)w.tiles);
+    hk = (int)((unsigned)u / (unsigned)chunks);
+    chunk = (u - hk * chunks) * p.lanes + lane;
+    const int unit = base + u * w.tiles;
+    first = at - unit;
+    last = min(end, unit + w.tiles) - unit;
+    at = unit + last;
+  }
+  __device__ __forceinline__ bool whole() const { return first == 0 && last == w.tiles; }
+};
 
 // Rows of a unit's chunk: row r of it is query m of head h.
 struct Rows {
@@ -107,6 +130,9 @@ struct Rows {
 // Partial result `slot` (twice the CTA, one more for the unit that starts in it): rows x dvo outputs, then maxima, then sums.
 __host__ __device__ __forceinline__ int64_t partial_floats(const PagedAttn& p) { return ((int64_t)p.rows * (p.dvo + 2) + 3) / 4 * 4; }
 __device__ __forceinline__ float* partial_of(const PagedAttn& p, int64_t slot) { return p.partial + slot * partial_floats(p); }
+
+// ... of the unit that a CTA is at
+__device__ __forceinline__ float* partial_of(const PagedAttn& p, const Piece& c) { return partial_of(p, 2 * (int64_t)blockIdx.x + (c.first == 0 ? 1 : 0)); }
 
 template <typename T>
 __device__ __forceinline__ T* out_row(const PagedAttn& p, int z, int h, int m) {

@@ -37,7 +37,7 @@ struct LatentSmem {
                        bO = bP + 1, bDrain = bO + 1, bCount = bDrain + 1;
   static constexpr int kAbort = bCount * 8, kTmem = kAbort + 8;
   static constexpr int kScratch = (kTmem + 8 + 15) & ~15;
-  static constexpr int kRef = (kScratch + (kLatentThreads / 32 + 4) * 8 + 15) & ~15;      // [NR] references, rescales, inverse sums; [4][NR] of the warps
+  static constexpr int kRef = (kScratch + (kLatentThreads / 32 + 2) * 4 + 15) & ~15;      // [NR] references, rescales, inverse sums; [4][NR] of the warps
   static constexpr int kAlpha = kRef + NR * 4, kInv = kAlpha + NR * 4, kWarps = kInv + NR * 4;
   static constexpr int kPos = kWarps + 4 * NR * 4, kOut = kPos + NR * 4;                  // [NR] positions; offsets of the output's rows
   static constexpr int kQ = (kOut + NR * 8 + 1023) & ~1023;
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
     for (int b = 0; b < L::bCount; ++b) mbar_init(&bars[b], b == L::bQ || b == L::bP ? 4 : 1);
     fence_barrier_init();
   }
-  const Line line = find_in_line<kLatentThreads>(p, -1, blockIdx.x, reinterpret_cast<int64_t*>(smem + L::kScratch));
+  const Line line = find_in_line<kLatentThreads>(p, -1, blockIdx.x / p.lanes, reinterpret_cast<int*>(smem + L::kScratch));
   if (__syncthreads_or(tid == 0 && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u)) return;
   if (line.z >= p.batch) return;
   if (warp == 5) {
@@ -119,24 +119,8 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  int64_t at = (int64_t)blockIdx.x * line.share;
-  const int64_t end = min(at + line.share, line.total);
-  int z = line.z;
-  int64_t base = line.base;
-  Walk w(p, z);
-  // The next unit of this CTA's piece (one kv head); `at` is moved behind it.
-  int chunk = 0, first = 0, last = 0;
-  auto next_unit = [&] {
-    while (at >= base + (int64_t)w.tiles * p.chunks) {
-      base += (int64_t)w.tiles * p.chunks;
-      w = Walk(p, ++z);
-    }
-    chunk = (int)((at - base) / w.tiles);
-    const int64_t unit = base + (int64_t)chunk * w.tiles;
-    first = (int)(at - unit);
-    last = (int)(min(end, unit + w.tiles) - unit);
-    at = unit + last;
-  };
+  Piece run(p, line);
+  const Walk& w = run.w;
   const int blocks = p.dvo / 128;
 
   if (warp == 4) {
@@ -145,10 +129,11 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
     const bool leads = lane < 16 && lane % octets == 0;
     int vi = 0, ti = 0;      // blocks and tails requested
     bool stop = false;
-    while (at < end && !stop) {
-      next_unit();
-      if (Rows(p, w, chunk).n == 0) continue;
-      const int32_t* row = p.table + (int64_t)z * p.table_stride;
+    while (run.more() && !stop) {
+      run.next(p);
+      if (Rows(p, w, run.chunk).n == 0) continue;
+      const int first = run.first, last = run.last;
+      const int32_t* row = p.table + (int64_t)run.z * p.table_stride;
       auto look = [&](int i) {      // the page of this lane's eight keys in tile i
         const int n = i * kKeys + lane * 8;
         if (lane >= 16 || n >= w.len) return -1;
@@ -206,9 +191,10 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars[bar], parity, abort_flag, p.status, where)) != 0;
       return ok;
     };
-    while (at < end && ok) {
-      next_unit();
-      if (Rows(p, w, chunk).n == 0) continue;
+    while (run.more() && ok) {
+      run.next(p);
+      if (Rows(p, w, run.chunk).n == 0) continue;
+      const int first = run.first, last = run.last;
       if (!wait(L::bQ, (uint32_t)units & 1u, 0x7100)) break;
       ++units;
       for (int i = first; i < last; ++i) {
@@ -281,25 +267,27 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
     const int qboxes = (p.dqk + 63) / 64;
     int vi = 0, tiles = 0, units = 0;
     bool broken = false;
-    while (at < end && !broken) {
-      next_unit();
-      const Rows rows(p, w, chunk);
-      if (first == 0 && chunk == 0) zero_rows_behind<T, kSoftmax>(p, w, z, 0, tid);
+    while (run.more() && !broken) {
+      run.next(p);
+      const int z = run.z, first = run.first, last = run.last;
+      const Rows rows(p, w, run.chunk);
+      if (first == 0 && run.chunk == 0) zero_rows_behind<T, kSoftmax>(p, w, z, 0, tid);
       if (rows.n == 0) continue;
       // ---- the unit's queries, as the products read them ----
       for (int i = tid; i < NR * qboxes * 8; i += kSoftmax) {
-        const int c = i % (qboxes * 8), r = i / (qboxes * 8), d = c * 8;      // 16 bytes of a row
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows.n && d < p.dqk)
-          v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q.ptr) + (int64_t)z * p.q.s[0] + (int64_t)rows.head(p, 0, r) * p.q.s[1] +
-                                                   (int64_t)rows.query(r) * p.q.s[2] + d));
-        *reinterpret_cast<uint4*>(smem + L::kQ + (c >> 3) * L::kQBox + r * 128 + (((c ^ r) & 7) << 4)) = v;
+        const int r = i % NR, c = i / NR, d = c * 8;      // 16 bytes of a row; those that there are none of are zero
+        const bool in = r < rows.n && d < p.dqk;
+        const T* src = reinterpret_cast<const T*>(p.q.ptr);
+        if (in) src += (int64_t)z * p.q.s[0] + (int64_t)rows.head(p, 0, r) * p.q.s[1] + (int64_t)rows.query(r) * p.q.s[2] + d;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + L::kQ + (c >> 3) * L::kQBox + r * 128 + (((c ^ r) & 7) << 4))), "l"(src),
+                     "r"(in ? 16 : 0) : "memory");
       }
       if (tid < NR) {
         ref[tid] = kNoReference;
         pos[tid] = tid < rows.n ? w.len - rows.queries + rows.query(tid) : 0x7fffffff;
         out_at[tid] = tid < rows.n ? (int64_t)z * p.out.s[0] + (int64_t)rows.head(p, 0, tid) * p.out.s[1] + (int64_t)rows.query(tid) * p.out.s[2] : 0;
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[L::bQ]);
@@ -409,8 +397,8 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       if (NR != 16 || (lane & 1) == 0) warps[warp * NR + lane_column<NR>(lane)] = l[0];
       if (NR == 64) warps[warp * NR + lane_column<NR>(lane) + 1] = l[NR > 32 ? 1 : 0];
       softmax_sync();
-      const bool whole = first == 0 && last == w.tiles;
-      float* part = partial_of(p, 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0));
+      const bool whole = run.whole();
+      float* part = partial_of(p, run);
       if (tid < rows.n) {
         const float sum = (warps[tid] + warps[NR + tid]) + (warps[2 * NR + tid] + warps[3 * NR + tid]);
         inv[tid] = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
@@ -487,7 +475,7 @@ bool plan_paged_latent(int dtype, PagedAttn& p, int sms) {
   p.rows = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
   p.box = 128;
   while (p.page % p.box != 0) p.box /= 2;
-  p.tile_keys = kKeys;
+  p.tile_log = 7;
   p.min_tiles = 1;
   p.ctas = sms;
   return true;

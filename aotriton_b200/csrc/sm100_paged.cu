@@ -27,7 +27,7 @@ __device__ unsigned int g_sm100_paged_status = 0;
 namespace {
 using namespace ptx;
 
-constexpr int kTileKeys = 64, kConsumers = 4, kSplitThreads = (kConsumers + 1) * 32;
+constexpr int kTileKeys = 64, kTileLog = 6, kConsumers = 4, kSplitThreads = (kConsumers + 1) * 32;
 constexpr int kMergeCols = 32;
 
 template <int HD, int MT>
@@ -39,7 +39,7 @@ struct SplitSmem {
   static constexpr int kAbort = bCount * 8;
   static constexpr int kValid = kAbort + 8;                       // per stage: which eights of its keys are in the cache
   static constexpr int kScratch = (kValid + kStages * 4 + 15) & ~15;
-  static constexpr int kMl = kScratch + (kSplitThreads / 32 + 4) * 8;
+  static constexpr int kMl = kScratch + (kSplitThreads / 32 + 3) * 4;
   static constexpr int kLdO = kMergeCols + 4;
   static constexpr int kMerge = (kMl + kConsumers * 2 * kRows * 4 + 15) & ~15;
   static constexpr int kRing = (kMerge + kConsumers * kRows * kLdO * 4 + 1023) & ~1023;
@@ -76,30 +76,11 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
     }
     fence_barrier_init();
   }
-  const Line line = find_in_line<kSplitThreads>(p, -1, blockIdx.x, reinterpret_cast<int64_t*>(smem + L::kScratch));
+  const Line line = find_in_line<kSplitThreads>(p, -1, blockIdx.x / p.lanes, reinterpret_cast<int*>(smem + L::kScratch));
   if (__syncthreads_or(tid == 0 && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u)) return;
   if (line.z >= p.batch) return;
-  int64_t at = (int64_t)blockIdx.x * line.share;
-  const int64_t end = min(at + line.share, line.total);
-  int z = line.z;
-  int64_t base = line.base;
-  Walk w(p, z);
-  // The next unit of this CTA's piece; `at` is moved behind it.
-  int hk = 0, chunk = 0, first = 0, last = 0;
-  auto next_unit = [&] {
-    const int64_t units = (int64_t)p.hk * p.chunks;
-    while (at >= base + w.tiles * units) {
-      base += w.tiles * units;
-      w = Walk(p, ++z);
-    }
-    const int u = (int)((at - base) / w.tiles);
-    hk = u / p.chunks;
-    chunk = u - hk * p.chunks;
-    const int64_t unit = base + (int64_t)u * w.tiles;
-    first = (int)(at - unit);
-    last = (int)(min(end, unit + w.tiles) - unit);
-    at = unit + last;
-  };
+  Piece run(p, line);
+  const Walk& w = run.w;
 
   if (warp == kConsumers) {
     // ================================ TMA producer ===================================
@@ -107,11 +88,11 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
     const uint32_t mine = lane < 8 ? ((octets == 8 ? 0xffu : (1u << octets) - 1u) << (group * octets)) & 0xffu : 0u;
     int s = 0, ph = 1, issued = 0;
     bool stop = false;
-    while (at < end && !stop) {
-      next_unit();
-      const Rows rows(p, w, chunk);
-      if (rows.n == 0) continue;
-      const int32_t* row = p.table + (int64_t)z * p.table_stride;
+    while (run.more() && !stop) {
+      run.next(p);
+      if (Rows(p, w, run.chunk).n == 0) continue;
+      const int first = run.first, last = run.last, hk = run.hk;
+      const int32_t* row = p.table + (int64_t)run.z * p.table_stride;
       // the page of this lane's eight keys in tile i, -1 where there is none; `seen`: whether any of them is seen
       auto look = [&](int i, bool& seen) {
         const int n = w.tile(i) * kTileKeys + lane * 8;
@@ -166,10 +147,11 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
   float* merge = reinterpret_cast<float*>(smem + L::kMerge);
   int s = 0, ph = 0;
   bool broken = false;
-  while (at < end && !broken) {
-    next_unit();
-    const Rows rows(p, w, chunk);
-    if (first == 0 && chunk == 0) zero_rows_behind<T, kConsumers * 32>(p, w, z, hk, tid);
+  while (run.more() && !broken) {
+    run.next(p);
+    const int z = run.z, hk = run.hk, first = run.first, last = run.last;
+    const Rows rows(p, w, run.chunk);
+    if (first == 0 && run.chunk == 0) zero_rows_behind<T, kConsumers * 32>(p, w, z, hk, tid);
     if (rows.n == 0) continue;
     // Q as A fragments, straight from global memory (rows and columns beyond the ends are zero)
     uint32_t q[MT][kKsteps][4];
@@ -320,8 +302,8 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
           ml[warp * 2 * L::kRows + L::kRows + t * 16 + half * 8 + qr] = l;
         }
       }
-    const bool whole = first == 0 && last == w.tiles;
-    float* part = partial_of(p, 2 * (int64_t)blockIdx.x + (first == 0 ? 1 : 0));
+    const bool whole = run.whole();
+    float* part = partial_of(p, run);
 #pragma unroll
     for (int c0 = 0; c0 < HD; c0 += kMergeCols) {
       if (c0 >= p.dvo) break;
@@ -439,7 +421,7 @@ bool plan_paged_split(int dtype, PagedAttn& p, int sms) {
   p.kind = kPagedSplit;
   p.box = 64;
   while (p.page % p.box != 0) p.box /= 2;
-  p.tile_keys = kTileKeys;
+  p.tile_log = kTileLog;
   p.min_tiles = 2;
   with_split_tile(p, [&]<int HD, int MT>() {
     p.rows = SplitSmem<HD, MT>::kRows;
