@@ -159,8 +159,7 @@ __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid
   while (width < p.dvo && width < kGenThreads) width <<= 1;
   const int groups = kGenThreads / width, group = tid / width, col = tid - group * width;
   Piece c(p, line);
-  while (c.more()) {
-    c.next(p);
+  while (c.next(p)) {
     const Walk& w = c.w;
     const int z = c.z, hk = c.hk, first = c.first, last = c.last;
     const bool whole = c.whole();
@@ -310,16 +309,16 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   constexpr int N = sizeof(V) / 4, kAhead = K > 4 ? 2 : (K > 1 ? 4 : 8);
   __shared__ int scratch[kJoinThreads / 32 + 2];
   const int tid = threadIdx.x, lane = tid & 31, units = p.hk * p.chunks;
-  wait_for_earlier_grids();
+  // (the lengths are older than the attention's launch, which has waited for what was ahead of it: the places are worked out while that still runs)
   const int z = (int)(blockIdx.x / (unsigned)units), u = (int)(blockIdx.x - (unsigned)z * units), r = blockIdx.y * kJoinRows + tid / 32;
   const Line line = find_in_line<kJoinThreads>(p, z, 0, scratch);
   const Walk w(p, z);
   const int hk = u / p.chunks, chunk = u - hk * p.chunks, along = hk * (p.chunks / p.lanes) + chunk / p.lanes;
   const Rows rows(p, w, chunk);
-  if (r >= rows.n) return;
-  const int unit = line.base + along * w.tiles;
-  const int c0 = unit / line.share, c1 = (unit + w.tiles - 1) / line.share;
-  if (c0 == c1) return;      // (finished where it was formed)
+  int c0, c1;
+  pieces_of_unit(p, line, w, along, c0, c1);
+  wait_for_earlier_grids();
+  if (r >= rows.n || c0 == c1) return;      // (the unit was finished where it was formed)
   if (p.status != nullptr && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
   auto piece = [&](int c) { return partial_of(p, 2 * ((int64_t)c * p.lanes + chunk % p.lanes) + (c == c0 ? 1 : 0)); };
   const int64_t at_m = (int64_t)p.rows * p.dvo + r, at_l = at_m + p.rows;
@@ -481,19 +480,20 @@ int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
     p.rows = kGenRows;
     p.tile_log = 5;
     p.min_tiles = 2;
+    p.extra = 1;
     p.ctas = sms * 4;
   }
   const int64_t chunks = ((int64_t)p.group * p.sq + p.rows - 1) / p.rows;
   p.chunks = (int)chunks;
   // (a last tile's keys are counted in 32 bits)
   p.max_len = (int32_t)std::min<int64_t>((int64_t)p.width * p.page, 0x7fffff00);
-  const int64_t most = (p.max_len >> p.tile_log) + 2;      // tiles of a unit: a window may cross a border
+  const int64_t most = (p.max_len >> p.tile_log) + 2 + p.extra;      // tiles of a unit: a window may cross a border
   const int64_t units = (int64_t)p.batch * p.hk * chunks;
   if (units * most > 0x3fffffff) return -kPagedTooLarge;
   // A kv head's chunks side by side, so that its keys come from memory once, unless that left too few CTAs to share a line out evenly.
   p.lanes = chunks <= 8 ? (int)chunks : 1;
   p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(p.ctas / p.lanes, units / p.lanes * most / p.min_tiles + 1)) * p.lanes;
-  p.join = most > 1;
+  p.join = 1;
   return p.join ? 2 * (int64_t)p.ctas * partial_floats(p) : 0;
 }
 

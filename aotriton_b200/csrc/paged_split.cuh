@@ -5,6 +5,9 @@
 // piece of it, whatever sequences that crosses.  A unit that lies within a piece is finished there; the pieces of others leave row maximum,
 // row sum and unnormalised output in a workspace (at most two a CTA: of the unit it begins with and of the one it ends with, so that its size does not
 // depend on the lengths), which a second launch adds up in the order of the keys.  Every CTA works out its place from the lengths alone.
+//
+// A unit costs a CTA more than its tiles: queries to fetch, a result to put together.  So its place in the line is p.extra tiles longer than it is (the first ones
+// of it, which nobody works on), and a CTA gets many short sequences or few long ones for the same time.
 #pragma once
 
 #include "paged.h"
@@ -32,6 +35,9 @@ struct Walk {
   __device__ __forceinline__ bool seen(const PagedAttn& p, int n) const { return n < len && (n >= lo || n < p.sinks); }
 };
 
+// Places in the line of a unit.
+__device__ __forceinline__ int places(const PagedAttn& p, const Walk& w) { return w.tiles + p.extra; }
+
 // The line of tiles as one thread block sees it; the host has seen to it that 31 bits hold it.  `lanes` CTAs next to each other take the same piece of
 // a line without the chunks, a chunk each: they read the same keys at the same time.
 struct Line {
@@ -40,15 +46,36 @@ struct Line {
   int z;
 };
 
-// A block of NT threads (a multiple of 32) finds sequence `z`, or the one that the first tile of piece `piece` belongs to (z < 0).  `scratch`: NT / 32 + 2
-// words.  Behind the last tile, z is the batch's size.
+// A block of NT threads (a multiple of 32) finds sequence `z`, or the one that the first place of piece `piece` belongs to (z < 0).  `scratch`: NT / 32 + 2
+// words.  Behind the last place, z is the batch's size.
 template <int NT>
 __device__ __forceinline__ Line find_in_line(const PagedAttn& p, int z, int piece, int* scratch) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int units = p.hk * p.chunks / p.lanes;
+  const int units = (int)((unsigned)(p.hk * p.chunks) / (unsigned)p.lanes), pieces = (int)((unsigned)p.ctas / (unsigned)p.lanes);
+  Line r;
+  if (p.batch <= 64) {      // each warp for itself: lane i has the sequences 2i and 2i + 1
+    const int z0 = 2 * lane, a = z0 < p.batch ? places(p, Walk(p, z0)) : 0, b = z0 + 1 < p.batch ? places(p, Walk(p, z0 + 1)) : 0;
+    int up = a + b;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, up, d);
+      if (lane >= d) up += o;
+    }
+    r.total = __shfl_sync(0xffffffffu, up, 31) * units;
+    r.share = max((int)((unsigned)(r.total + pieces - 1) / (unsigned)pieces), p.min_tiles);
+    const int before = (up - a - b) * units, middle = before + a * units;
+    const int64_t at = (int64_t)piece * r.share;
+    const bool first = z >= 0 ? z == z0 : (a > 0 && at >= before && at < middle), second = z >= 0 ? z == z0 + 1 : (b > 0 && at >= middle && at < middle + b * units);
+    const uint32_t owner = __ballot_sync(0xffffffffu, first || second);
+    const int from = owner != 0u ? __ffs(owner) - 1 : 0;
+    r.z = __shfl_sync(0xffffffffu, second ? z0 + 1 : z0, from);
+    r.base = __shfl_sync(0xffffffffu, second ? middle : before, from);
+    if (owner == 0u) r.z = p.batch;
+    return r;
+  }
   const int each = (p.batch + NT - 1) / NT, z0 = min(tid * each, p.batch), z1 = min(z0 + each, p.batch);
   int mine = 0;
-  for (int i = z0; i < z1; ++i) mine += Walk(p, i).tiles;
+  for (int i = z0; i < z1; ++i) mine += places(p, Walk(p, i));
   int up = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -66,15 +93,14 @@ __device__ __forceinline__ Line find_in_line(const PagedAttn& p, int z, int piec
     total += s;
   }
   before += up - mine;
-  Line r;
   r.total = total * units;
-  r.share = max((int)((unsigned)(r.total + p.ctas / p.lanes - 1) / (unsigned)(p.ctas / p.lanes)), p.min_tiles);
+  r.share = max((int)((unsigned)(r.total + pieces - 1) / (unsigned)pieces), p.min_tiles);
   const int64_t at = (int64_t)piece * r.share;
   if (z >= 0 ? (z >= z0 && z < z1) : (mine > 0 && at >= before * units && at < (before + mine) * units)) {
     int b = before, i = z0;
     for (; i + 1 < z1; ++i) {
       if (i == z) break;
-      const int t = Walk(p, i).tiles;
+      const int t = places(p, Walk(p, i));
       if (z < 0 && at < (b + t) * units) break;
       b += t;
     }
@@ -95,24 +121,36 @@ struct Piece {
   __device__ __forceinline__ Piece(const PagedAttn& p, const Line& line)
       : at((int)(blockIdx.x / p.lanes) * line.share), end(min(at + line.share, line.total)), z(line.z), base(line.base),
         lane((int)(blockIdx.x % p.lanes)), w(p, line.z), hk(0), chunk(0), first(0), last(0) {}
-  __device__ __forceinline__ bool more() const { return at < end; }
-  // The next unit; `at` is moved behind it.
-  __device__ __forceinline__ void next(const PagedAttn& p) {
-    const int chunks = p.chunks / p.lanes, units = p.hk * chunks;
-    while (at >= base + w.tiles * units) {
-      base += w.tiles * units;
-      w = Walk(p, ++z);
+  // The next unit with tiles in this piece, if there is one; `at` is moved behind it.
+  __device__ __forceinline__ bool next(const PagedAttn& p) {
+    const int chunks = (int)((unsigned)p.chunks / (unsigned)p.lanes), units = p.hk * chunks;
+    while (at < end) {
+      int n = places(p, w);
+      while (at >= base + n * units) {
+        base += n * units;
+        w = Walk(p, ++z);
+        n = places(p, w);
+      }
+      const int u = (int)((unsigned)(at - base) / (unsigned)n);
+      hk = (int)((unsigned)u / (unsigned)chunks);
+      chunk = (u - hk * chunks) * p.lanes + lane;
+      const int unit = base + u * n + p.extra;      // its first tile's place
+      first = max(at - unit, 0);
+      last = min(end, unit + w.tiles) - unit;
+      at = unit + last;
+      if (last > 0) return true;
+      at = end;      // (the piece ends ahead of the unit's first tile)
     }
-    const int u = (int)((unsigned)(at - base) / (unsigned)w.tiles);
-    hk = (int)((unsigned)u / (unsigned)chunks);
-    chunk = (u - hk * chunks) * p.lanes + lane;
-    const int unit = base + u * w.tiles;
-    first = at - unit;
-    last = min(end, unit + w.tiles) - unit;
-    at = unit + last;
+    return false;
   }
   __device__ __forceinline__ bool whole() const { return first == 0 && last == w.tiles; }
 };
+// The pieces that have tiles of unit `along` (of its lane) of the sequence that `line` has found.
+__device__ __forceinline__ void pieces_of_unit(const PagedAttn& p, const Line& line, const Walk& w, int along, int& first, int& last) {
+  const int unit = line.base + along * places(p, w) + p.extra;
+  first = (int)((unsigned)unit / (unsigned)line.share);
+  last = (int)((unsigned)(unit + w.tiles - 1) / (unsigned)line.share);
+}
 
 // Rows of a unit's chunk: row r of it is query m of head h.
 struct Rows {

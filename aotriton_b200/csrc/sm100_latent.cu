@@ -102,14 +102,16 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbort);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) prefetch_tmap(&tm);
   wait_for_earlier_grids();
+  const unsigned int failed = tid == 0 ? *reinterpret_cast<volatile unsigned int*>(p.status) : 0u;
   if (tid == 0) {
     init_abort_and_limit(abort_flag, p.wait_limit_kcycles);
     for (int b = 0; b < L::bCount; ++b) mbar_init(&bars[b], b == L::bQ || b == L::bP ? 4 : 1);
     fence_barrier_init();
   }
   const Line line = find_in_line<kLatentThreads>(p, -1, blockIdx.x / p.lanes, reinterpret_cast<int*>(smem + L::kScratch));
-  if (__syncthreads_or(tid == 0 && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u)) return;
+  if (__syncthreads_or(failed != 0u)) return;
   if (line.z >= p.batch) return;
   if (warp == 5) {
     tmem_alloc(tmem_slot, L::kTmemCols);
@@ -129,8 +131,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
     const bool leads = lane < 16 && lane % octets == 0;
     int vi = 0, ti = 0;      // blocks and tails requested
     bool stop = false;
-    while (run.more() && !stop) {
-      run.next(p);
+    while (!stop && run.next(p)) {
       if (Rows(p, w, run.chunk).n == 0) continue;
       const int first = run.first, last = run.last;
       const int32_t* row = p.table + (int64_t)run.z * p.table_stride;
@@ -191,8 +192,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       ok = ok && __all_sync(0xffffffffu, mbar_wait(&bars[bar], parity, abort_flag, p.status, where)) != 0;
       return ok;
     };
-    while (run.more() && ok) {
-      run.next(p);
+    while (ok && run.next(p)) {
       if (Rows(p, w, run.chunk).n == 0) continue;
       const int first = run.first, last = run.last;
       if (!wait(L::bQ, (uint32_t)units & 1u, 0x7100)) break;
@@ -267,8 +267,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
     const int qboxes = (p.dqk + 63) / 64;
     int vi = 0, tiles = 0, units = 0;
     bool broken = false;
-    while (run.more() && !broken) {
-      run.next(p);
+    while (!broken && run.next(p)) {
       const int z = run.z, first = run.first, last = run.last;
       const Rows rows(p, w, run.chunk);
       if (first == 0 && run.chunk == 0) zero_rows_behind<T, kSoftmax>(p, w, z, 0, tid);
@@ -477,6 +476,7 @@ bool plan_paged_latent(int dtype, PagedAttn& p, int sms) {
   while (p.page % p.box != 0) p.box /= 2;
   p.tile_log = 7;
   p.min_tiles = 1;
+  p.extra = 2;
   p.ctas = sms;
   return true;
 }

@@ -67,7 +67,9 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbort);
   volatile uint32_t* valid = reinterpret_cast<volatile uint32_t*>(smem + L::kValid);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) { prefetch_tmap(&tm_k); prefetch_tmap(&tm_v); }
   wait_for_earlier_grids();
+  const unsigned int failed = tid == 0 ? *reinterpret_cast<volatile unsigned int*>(p.status) : 0u;
   if (tid == 0) {
     init_abort_and_limit(abort_flag, p.wait_limit_kcycles);
     for (int s = 0; s < kStages; ++s) {
@@ -77,7 +79,7 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
     fence_barrier_init();
   }
   const Line line = find_in_line<kSplitThreads>(p, -1, blockIdx.x / p.lanes, reinterpret_cast<int*>(smem + L::kScratch));
-  if (__syncthreads_or(tid == 0 && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u)) return;
+  if (__syncthreads_or(failed != 0u)) return;
   if (line.z >= p.batch) return;
   Piece run(p, line);
   const Walk& w = run.w;
@@ -88,8 +90,7 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
     const uint32_t mine = lane < 8 ? ((octets == 8 ? 0xffu : (1u << octets) - 1u) << (group * octets)) & 0xffu : 0u;
     int s = 0, ph = 1, issued = 0;
     bool stop = false;
-    while (run.more() && !stop) {
-      run.next(p);
+    while (!stop && run.next(p)) {
       if (Rows(p, w, run.chunk).n == 0) continue;
       const int first = run.first, last = run.last, hk = run.hk;
       const int32_t* row = p.table + (int64_t)run.z * p.table_stride;
@@ -147,8 +148,7 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
   float* merge = reinterpret_cast<float*>(smem + L::kMerge);
   int s = 0, ph = 0;
   bool broken = false;
-  while (run.more() && !broken) {
-    run.next(p);
+  while (!broken && run.next(p)) {
     const int z = run.z, hk = run.hk, first = run.first, last = run.last;
     const Rows rows(p, w, run.chunk);
     if (first == 0 && run.chunk == 0) zero_rows_behind<T, kConsumers * 32>(p, w, z, hk, tid);
@@ -194,11 +194,14 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
       const uint32_t vt = smem_s + L::kRing + s * (2 * L::kTile) + L::kTile + vrow * 128;
       if (key0 + 16 > w.len || (key0 < w.lo && key0 + 16 > p.sinks)) {
         // V rows that nobody sees hold whatever the cache has there: a zero weight times a non-finite value would poison the sum
-        uint8_t* vtile = smem + L::kRing + s * (2 * L::kTile) + L::kTile;
-        for (int rr = 0; rr < 16; ++rr)
+        uint8_t* vtile = smem + L::kRing + s * (2 * L::kTile) + L::kTile + warp * 16 * 128;
+#pragma unroll
+        for (int r0 = 0; r0 < 16; r0 += 4) {      // (a lane 16 bytes of a row, a warp four rows)
+          const int rr = r0 + (lane >> 3);
           if (!w.seen(p, key0 + rr))
-            for (int c = lane; c < kBoxes * 8; c += 32)
-              *reinterpret_cast<uint4*>(vtile + (c >> 3) * (kTileKeys * 128) + (warp * 16 + rr) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int b = 0; b < kBoxes; ++b) *reinterpret_cast<uint4*>(vtile + b * (kTileKeys * 128) + rr * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
         fence_proxy_async_smem();      // (ahead of the copy that overwrites the stage)
         __syncwarp();
       }
@@ -423,6 +426,7 @@ bool plan_paged_split(int dtype, PagedAttn& p, int sms) {
   while (p.page % p.box != 0) p.box /= 2;
   p.tile_log = kTileLog;
   p.min_tiles = 2;
+  p.extra = 3;
   with_split_tile(p, [&]<int HD, int MT>() {
     p.rows = SplitSmem<HD, MT>::kRows;
     p.ctas = sms * SplitSmem<HD, MT>::kCtasPerSm;
