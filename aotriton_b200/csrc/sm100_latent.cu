@@ -13,7 +13,7 @@
 // the second product has read them, so the next tile arrives under it.  (64 rows leave room for no more than one tile; the weights then take the last columns' slot,
 // which are done with once the scores are formed.)
 //
-// Roles: warps 0-3 softmax and write-out (thread = key, then = value column), warp 4 copies, warp 5 issues the products.
+// Roles: warps 0-3 (64 rows: 0-7) softmax and write-out (thread = key, then = value column), then one that copies, one that issues the products.
 #include <atomic>
 #include "launch.h"
 #include "paged.h"
@@ -24,7 +24,7 @@ namespace ab200 {
 namespace {
 using namespace ptx;
 
-constexpr int kKeys = 128, kSoftmax = 128, kLatentThreads = 192;
+constexpr int kKeys = 128;
 constexpr int kBox = kKeys * 128, kBlock = 2 * kBox;      // bytes: 64 columns of a tile, 128 columns
 constexpr float kNoReference = -3.0e38f;                  // of a row that has seen nothing
 constexpr float kSlack = 8.f;
@@ -32,12 +32,14 @@ constexpr float kSlack = 8.f;
 template <int NR>
 struct LatentSmem {
   static constexpr bool kAlias = NR > 16;                 // the weights lie in the last columns' slot
+  static constexpr int kGroups = NR > 32 ? 2 : 1;         // warpgroups that share the rows' softmax and write-out
+  static constexpr int kSoftmax = 128 * kGroups, kThreads = kSoftmax + 64, kOwn = NR / kGroups;
   static constexpr int kSlots = NR > 32 ? 4 : 5;
   static constexpr int bFull = 0, bEmpty = kSlots, bTailFull = 2 * kSlots, bTailEmpty = bTailFull + 1, bQ = bTailEmpty + 1, bS = bQ + 1, bP = bS + 1,
                        bO = bP + 1, bDrain = bO + 1, bCount = bDrain + 1;
   static constexpr int kAbort = bCount * 8, kTmem = kAbort + 8;
   static constexpr int kScratch = (kTmem + 8 + 15) & ~15;
-  static constexpr int kRef = (kScratch + (kLatentThreads / 32 + 2) * 4 + 15) & ~15;      // [NR] references, rescales, inverse sums; [4][NR] of the warps
+  static constexpr int kRef = (kScratch + (kThreads / 32 + 2) * 4 + 15) & ~15;      // [NR] references, rescales, inverse sums; [4][NR] of the warps
   static constexpr int kAlpha = kRef + NR * 4, kInv = kAlpha + NR * 4, kWarps = kInv + NR * 4;
   static constexpr int kPos = kWarps + 4 * NR * 4, kOut = kPos + NR * 4;                  // [NR] positions; offsets of the output's rows
   static constexpr int kQ = (kOut + NR * 8 + 1023) & ~1023;
@@ -50,26 +52,25 @@ struct LatentSmem {
   static_assert(kBytes <= 232448 && kQBox % 1024 == 0 && kOCol + 4 * NR <= kTmemCols, "fits");
 };
 
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kSoftmax) : "memory"); }
+template <int N>
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); }
 // ... and whether any thread says so
+template <int N>
 __device__ __forceinline__ bool softmax_any(bool x) {
   uint32_t r;
   asm volatile("{\n\t.reg .pred a, b;\n\tsetp.ne.b32 a, %1, 0;\n\tbarrier.cta.red.or.pred b, 1, %2, a;\n\tselp.b32 %0, 1, 0, b;\n\t}"
-               : "=r"(r) : "r"((uint32_t)x), "n"(kSoftmax) : "memory");
+               : "=r"(r) : "r"((uint32_t)x), "n"(N) : "memory");
   return r != 0;
 }
 
 template <int NR>
 __device__ __forceinline__ void tmem_row(uint32_t taddr, float (&x)[NR]) {
   if constexpr (NR == 16) tmem_ld16f(taddr, x);
-  else {
-    tmem_ld32f(taddr, x);
-    if constexpr (NR == 64) tmem_ld32f(taddr + 32, x + 32);
-  }
+  else tmem_ld32f(taddr, x);
   tmem_wait_ld();
 }
 
-// Combines x[c] over the lanes of a warp, halving the columns that a lane holds from step to step; column(lane) is then in x[0] (NR = 64: and the next in x[1]).
+// Combines x[c] over the lanes of a warp, halving the columns that a lane holds from step to step; that of lane_column(lane) is then in x[0].
 template <int NR, typename Op>
 __device__ __forceinline__ void across_lanes(float (&x)[NR], int lane, Op op) {
   int n = NR;
@@ -90,11 +91,11 @@ __device__ __forceinline__ void across_lanes(float (&x)[NR], int lane, Op op) {
   }
 }
 template <int NR>
-__device__ __forceinline__ int lane_column(int lane) { return NR == 64 ? 2 * lane : (NR == 32 ? lane : lane >> 1); }
+__device__ __forceinline__ int lane_column(int lane) { return NR == 32 ? lane : lane >> 1; }
 
 // p.rows = NR; p.dvo a multiple of 128 up to 512, the last 1 to 64 of p.dqk columns behind it
 template <typename T, int NR>
-__global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap tm) {
+__global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap tm) {
   using L = LatentSmem<NR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -107,13 +108,13 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
   const unsigned int failed = tid == 0 ? *reinterpret_cast<volatile unsigned int*>(p.status) : 0u;
   if (tid == 0) {
     init_abort_and_limit(abort_flag, p.wait_limit_kcycles);
-    for (int b = 0; b < L::bCount; ++b) mbar_init(&bars[b], b == L::bQ || b == L::bP ? 4 : 1);
+    for (int b = 0; b < L::bCount; ++b) mbar_init(&bars[b], b == L::bQ || b == L::bP ? 4 * L::kGroups : 1);
     fence_barrier_init();
   }
-  const Line line = find_in_line<kLatentThreads>(p, -1, blockIdx.x / p.lanes, reinterpret_cast<int*>(smem + L::kScratch));
+  const Line line = find_in_line<L::kThreads>(p, -1, blockIdx.x / p.lanes, reinterpret_cast<int*>(smem + L::kScratch));
   if (__syncthreads_or(failed != 0u)) return;
   if (line.z >= p.batch) return;
-  if (warp == 5) {
+  if (warp == 4 * L::kGroups + 1) {
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
   const Walk& w = run.w;
   const int blocks = p.dvo / 128;
 
-  if (warp == 4) {
+  if (warp == 4 * L::kGroups) {
     // ================================ TMA producer ===================================
     const int octets = p.box / 8;
     const bool leads = lane < 16 && lane % octets == 0;
@@ -145,7 +146,19 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       for (int i = first; i < last && !stop; ++i) {
         const int page = id >= 0 && id < p.num_pages ? id : p.num_pages;      // (a page that does not exist: zeros, without a read)
         const int slot = (i * kKeys + lane * 8) % p.page;
-        if (i + 1 < last) id = look(i + 1);
+        if (i + 1 < last) {
+          id = look(i + 1);
+          // the next tile towards L2: there is no room for it yet, and memory would rest until there is
+          const int next = id >= 0 && id < p.num_pages ? id : p.num_pages, at = ((i + 1) * kKeys + lane * 8) % p.page;
+          if (leads && next < p.num_pages) {
+            for (int b = run.lane; b < blocks; b += p.lanes) {
+              tma_prefetch_4d(&tm, b * 128, at, 0, next);
+              tma_prefetch_4d(&tm, b * 128 + 64, at, 0, next);
+            }
+            if (run.lane == 0) tma_prefetch_4d(&tm, p.dvo, at, 0, next);
+          }
+          __syncwarp();
+        }
         auto tail = [&] {
           if (!__all_sync(0xffffffffu, mbar_wait(&bars[L::bTailEmpty], ((uint32_t)ti & 1u) ^ 1u, abort_flag, p.status, 0x7000))) { stop = true; return; }
           if (lane == 0) mbar_expect_tx(&bars[L::bTailFull], kBox);
@@ -179,7 +192,7 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       if (ti > 0) mbar_wait_quiet(&bars[L::bTailFull], (uint32_t)(ti - 1) & 1u, abort_flag);
     }
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == 4 * L::kGroups + 1) {
     // ================================ the products ===================================
     constexpr uint32_t kIdescS = instr_desc_f16(Fmt<T>::code, 128, NR, 0, 0), kIdescO = instr_desc_f16(Fmt<T>::code, 128, NR, 1, 1);
     const uint64_t ring_k = smem_desc_sw128(smem_u32(smem + L::kRing), 16, 1024), ring_mn = smem_desc_sw128(smem_u32(smem + L::kRing), kBox, 1024);
@@ -263,7 +276,10 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
     int* pos = reinterpret_cast<int*>(smem + L::kPos);
     int64_t* out_at = reinterpret_cast<int64_t*>(smem + L::kOut);
     uint8_t* ps = smem + (L::kAlias ? L::kTail : L::kP);
-    const uint32_t mine = tmem + ((uint32_t)(warp * 32) << 16);      // this warp's lanes
+    // a warpgroup has kOwn of the rows, from `col` on; a thread of it a key, then a column of the values
+    constexpr int kSoftmax = L::kSoftmax, kOwn = L::kOwn;
+    const int col = warp / 4 * kOwn, key = tid & 127;
+    const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col;      // this warp's lanes
     const int qboxes = (p.dqk + 63) / 64;
     int vi = 0, tiles = 0, units = 0;
     bool broken = false;
@@ -273,13 +289,13 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       if (first == 0 && run.chunk == 0) zero_rows_behind<T, kSoftmax>(p, w, z, 0, tid);
       if (rows.n == 0) continue;
       // ---- the unit's queries, as the products read them ----
-      for (int i = tid; i < NR * qboxes * 8; i += kSoftmax) {
-        const int r = i % NR, c = i / NR, d = c * 8;      // 16 bytes of a row; those that there are none of are zero
-        const bool in = r < rows.n && d < p.dqk;
+      for (int r = warp; r < NR; r += 4 * L::kGroups) {      // (a warp a row, a lane 16 bytes; those that there are none of are zero)
+        const bool in = r < rows.n;
         const T* src = reinterpret_cast<const T*>(p.q.ptr);
-        if (in) src += (int64_t)z * p.q.s[0] + (int64_t)rows.head(p, 0, r) * p.q.s[1] + (int64_t)rows.query(r) * p.q.s[2] + d;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + L::kQ + (c >> 3) * L::kQBox + r * 128 + (((c ^ r) & 7) << 4))), "l"(src),
-                     "r"(in ? 16 : 0) : "memory");
+        if (in) src += (int64_t)z * p.q.s[0] + (int64_t)rows.head(p, 0, r) * p.q.s[1] + (int64_t)rows.query(r) * p.q.s[2];
+        for (int c = lane; c < qboxes * 8; c += 32)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(smem + L::kQ + (c >> 3) * L::kQBox + r * 128 + (((c ^ r) & 7) << 4))),
+                       "l"(in && c * 8 < p.dqk ? src + c * 8 : reinterpret_cast<const T*>(p.q.ptr)), "r"(in && c * 8 < p.dqk ? 16 : 0) : "memory");
       }
       if (tid < NR) {
         ref[tid] = kNoReference;
@@ -290,13 +306,13 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[L::bQ]);
-      softmax_sync();
-      float l[NR];
+      softmax_sync<kSoftmax>();
+      float l[kOwn];
 #pragma unroll
-      for (int j = 0; j < NR; ++j) l[j] = 0.f;
+      for (int j = 0; j < kOwn; ++j) l[j] = 0.f;
       const int32_t* row = p.table + (int64_t)z * p.table_stride;
       for (int i = first; i < last; ++i) {
-        const int n = i * kKeys + tid;
+        const int n = i * kKeys + key;
         bool there = n < w.len;
         if (there) {
           const int id = row[n / p.page];
@@ -307,31 +323,32 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
         const bool came = __all_sync(0xffffffffu, ok) != 0;
         tc_fence_after();
         // this key's score with each row, in base 2
-        auto scores = [&](float (&x)[NR]) {
-          tmem_row<NR>(mine, x);
+        auto scores = [&](float (&x)[kOwn]) {
+          tmem_row<kOwn>(mine, x);
 #pragma unroll
-          for (int j = 0; j < NR; ++j) x[j] = there ? x[j] * p.qk_scale : -INFINITY;
+          for (int j = 0; j < kOwn; ++j) x[j] = there ? x[j] * p.qk_scale : -INFINITY;
           if (some_hidden)
 #pragma unroll
-            for (int j = 0; j < NR; ++j)
-              if (n > pos[j]) x[j] = -INFINITY;
+            for (int j = 0; j < kOwn; ++j)
+              if (n > pos[col + j]) x[j] = -INFINITY;
         };
-        float x[NR], top = -INFINITY;
+        float x[kOwn], top = i > first ? -INFINITY : INFINITY;      // (a first tile has no reference)
+        if (i > first) {
         scores(x);
 #pragma unroll
-        for (int j = 0; j < NR; j += 4) {
-          const float4 m = *reinterpret_cast<const float4*>(ref + j);
+        for (int j = 0; j < kOwn; j += 4) {
+          const float4 m = *reinterpret_cast<const float4*>(ref + col + j);
           x[j] -= m.x; x[j + 1] -= m.y; x[j + 2] -= m.z; x[j + 3] -= m.w;
           top = fmaxf(top, fmaxf(fmaxf(x[j], x[j + 1]), fmaxf(x[j + 2], x[j + 3])));
         }
-        if (softmax_any(top > kSlack || !came)) {
+        }
+        if (softmax_any<kSoftmax>(top > kSlack || !came)) {
           // ---- a score far above its row's reference (or the first of its row): the true maxima, and everything against them ----
-          if (softmax_any(!came)) { broken = true; break; }
+          if (softmax_any<kSoftmax>(!came)) { broken = true; break; }
           scores(x);
-          across_lanes<NR>(x, lane, [](float a, float b) { return fmaxf(a, b); });
-          warps[warp * NR + lane_column<NR>(lane)] = x[0];
-          if (NR == 64) warps[warp * NR + lane_column<NR>(lane) + 1] = x[NR > 32 ? 1 : 0];
-          softmax_sync();
+          across_lanes<kOwn>(x, lane, [](float a, float b) { return fmaxf(a, b); });
+          warps[(warp & 3) * NR + col + lane_column<kOwn>(lane)] = x[0];
+          softmax_sync<kSoftmax>();
           if (tid < NR) {
             const float was = ref[tid];
             float now = fmaxf(fmaxf(warps[tid], warps[NR + tid]), fmaxf(warps[2 * NR + tid], warps[3 * NR + tid]));
@@ -339,19 +356,19 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
             alpha[tid] = ex2(was - now);
             ref[tid] = now;
           }
-          softmax_sync();
+          softmax_sync<kSoftmax>();
 #pragma unroll
-          for (int j = 0; j < NR; ++j) l[j] *= alpha[j];
+          for (int j = 0; j < kOwn; ++j) l[j] *= alpha[col + j];
           if (i > first) {      // (the last tile's product has ended: this one's scores were formed behind it)
             for (int b = 0; b < blocks; ++b) {
 #pragma unroll
-              for (int h = 0; h < NR; h += 16) {
+              for (int h = 0; h < kOwn; h += 16) {
                 float o[16];
                 uint32_t u[16];
                 tmem_ld16f(mine + L::kOCol + b * NR + h, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(o[j] * alpha[h + j]);
+                for (int j = 0; j < 16; ++j) u[j] = __float_as_uint(o[j] * alpha[col + h + j]);
                 tmem_st16(mine + L::kOCol + b * NR + h, u);
               }
             }
@@ -359,23 +376,23 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
           }
           scores(x);
 #pragma unroll
-          for (int j = 0; j < NR; ++j) x[j] -= ref[j];
+          for (int j = 0; j < kOwn; ++j) x[j] -= ref[col + j];
         }
         // ---- weights, rounded to the value type (half a step off; the sums keep 32 bits) ----
 #pragma unroll
-        for (int j = 0; j < NR; j += 8) {
+        for (int j = 0; j < kOwn; j += 8) {
           float e[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             e[k] = ex2(x[j + k]);
             l[j + k] += e[k];
           }
-          *reinterpret_cast<uint4*>(ps + tid * 128 + ((((j >> 3) ^ tid) & 7) << 4)) =
+          *reinterpret_cast<uint4*>(ps + key * 128 + (((((col + j) >> 3) ^ key) & 7) << 4)) =
               make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]), pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
         }
         if (n >= w.len)      // slots behind the sequence hold whatever the cache has there: a zero weight times a non-finite value would poison the sum
-          for (int b = 0; b < 2 * blocks; ++b) {
-            uint8_t* r = smem + L::kRing + (vi + b / 2) % L::kSlots * kBlock + (b & 1) * kBox + tid * 128;
+          for (int b = warp / 4; b < 2 * blocks; b += L::kGroups) {
+            uint8_t* r = smem + L::kRing + (vi + b / 2) % L::kSlots * kBlock + (b & 1) * kBox + key * 128;
 #pragma unroll
             for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(r + c * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
@@ -390,12 +407,11 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
       bool done = !broken;
       if (done) done = __all_sync(0xffffffffu, mbar_wait(&bars[L::bO], (uint32_t)units & 1u, abort_flag, p.status, 0x7210)) != 0;
       ++units;
-      if (broken || softmax_any(!done)) { broken = true; break; }
+      if (broken || softmax_any<kSoftmax>(!done)) { broken = true; break; }
       tc_fence_after();
-      across_lanes<NR>(l, lane, [](float a, float b) { return a + b; });
-      if (NR != 16 || (lane & 1) == 0) warps[warp * NR + lane_column<NR>(lane)] = l[0];
-      if (NR == 64) warps[warp * NR + lane_column<NR>(lane) + 1] = l[NR > 32 ? 1 : 0];
-      softmax_sync();
+      across_lanes<kOwn>(l, lane, [](float a, float b) { return a + b; });
+      if (kOwn != 16 || (lane & 1) == 0) warps[(warp & 3) * NR + col + lane_column<kOwn>(lane)] = l[0];
+      softmax_sync<kSoftmax>();
       const bool whole = run.whole();
       float* part = partial_of(p, run);
       if (tid < rows.n) {
@@ -408,29 +424,29 @@ __global__ void __launch_bounds__(kLatentThreads, 1) paged_latent_kernel(const _
           part[NR * p.dvo + NR + tid] = sum;
         }
       }
-      softmax_sync();
+      softmax_sync<kSoftmax>();
       for (int b = 0; b < blocks; ++b) {
-        float o[NR];
-        tmem_row<NR>(mine + L::kOCol + b * NR, o);
-        const int d = b * 128 + tid;
+        float o[kOwn];
+        tmem_row<kOwn>(mine + L::kOCol + b * NR, o);
+        const int d = b * 128 + key;
         if (whole) {
           T* out = reinterpret_cast<T*>(p.out.ptr) + d;
 #pragma unroll
-          for (int j = 0; j < NR; ++j)
-            if (j < rows.n) out[out_at[j]] = from_f32<T>(o[j] * inv[j]);
+          for (int j = 0; j < kOwn; ++j)
+            if (col + j < rows.n) out[out_at[col + j]] = from_f32<T>(o[j] * inv[col + j]);
         } else {
 #pragma unroll
-          for (int j = 0; j < NR; ++j)
-            if (j < rows.n) part[j * p.dvo + d] = o[j];
+          for (int j = 0; j < kOwn; ++j)
+            if (col + j < rows.n) part[(col + j) * p.dvo + d] = o[j];
         }
       }
       tc_fence_before();
-      softmax_sync();      // (the next unit's rows and queries take the place of these)
+      softmax_sync<kSoftmax>();      // (the next unit's rows and queries take the place of these)
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 4 * L::kGroups + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, L::kTmemCols);
   }
@@ -452,7 +468,7 @@ cudaError_t launch_latent_T(PagedAttn& p, cudaStream_t st) {
   CUtensorMap tm;
   const View4 k{p.k.ptr, {p.k.n[0], 1, p.k.n[1], p.dqk}, {p.k.s[0], p.k.s[2], p.k.s[1], p.k.s[3]}};
   if (!make_tile_map_16bit(&tm, k, p.dqk, p.page, p.box)) return cudaErrorInvalidValue;
-  e = launch_kernel(kernel, dim3(p.ctas), dim3(kLatentThreads), L::kBytes, st, p, tm);
+  e = launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kBytes, st, p, tm);
   if (e == cudaSuccess) count_launch();
   return e;
 }
