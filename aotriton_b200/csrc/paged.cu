@@ -294,23 +294,24 @@ __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid
 }
 
 // ---- the pieces of split units ----------------------------------------------------------------------------------------
-// grid = (batch * hk * chunks, rows / 4): a warp a row.  Weighs the pieces' rows by their maxima and adds them up in the order of the keys, a few pieces'
-// columns on the way at a time.  V: float4, or float where the columns are not a multiple of 4; K: vectors of a lane.
-constexpr int kJoinThreads = 128, kJoinRows = kJoinThreads / 32;
+// A warp takes 32 K vectors of a row; it weighs the pieces' rows by their maxima and adds them up in the order of the keys, several of them on the way at a
+// time: what bounds it is how many loads stand one behind another.  V: float4, or float where the columns are not a multiple of 4.  K: 1 while there are
+// too few rows to fill the GPU, 4 beyond (one sequence of 32768 keys, 128 heads of 512, 51 us with 4, 40 with 1; 128 short ones 70 and 78).
+// grid = (batch * hk * chunks, some): a unit's blocks take its rows' pieces, `widths` a row, in turn.
+constexpr int kJoinThreads = 128, kJoinWarps = kJoinThreads / 32, kJoinBlocks = 4736;      // (32 for each SM)
 
-template <typename V> __device__ __forceinline__ void add_weighed(V& a, float w, const V& x);
-template <> __device__ __forceinline__ void add_weighed<float>(float& a, float w, const float& x) { a = fmaf(w, x, a); }
-template <> __device__ __forceinline__ void add_weighed<float4>(float4& a, float w, const float4& x) {
+__device__ __forceinline__ void add_weighed(float& a, float w, const float& x) { a = fmaf(w, x, a); }
+__device__ __forceinline__ void add_weighed(float4& a, float w, const float4& x) {
   a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w);
 }
 
 template <typename T, typename V, int K>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttn p) {
-  constexpr int N = sizeof(V) / 4, kAhead = K > 4 ? 2 : (K > 1 ? 4 : 8);
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttn p, int widths) {
+  constexpr int N = sizeof(V) / 4, kAhead = K > 1 ? 4 : 8;
   __shared__ int scratch[kJoinThreads / 32 + 2];
   const int tid = threadIdx.x, lane = tid & 31, units = p.hk * p.chunks;
   // (the lengths are older than the attention's launch, which has waited for what was ahead of it: the places are worked out while that still runs)
-  const int z = (int)(blockIdx.x / (unsigned)units), u = (int)(blockIdx.x - (unsigned)z * units), r = blockIdx.y * kJoinRows + tid / 32;
+  const int z = (int)(blockIdx.x / (unsigned)units), u = (int)(blockIdx.x - (unsigned)z * units);
   const Line line = find_in_line<kJoinThreads>(p, z, 0, scratch);
   const Walk w(p, z);
   const int hk = u / p.chunks, chunk = u - hk * p.chunks, along = hk * (p.chunks / p.lanes) + chunk / p.lanes;
@@ -318,59 +319,69 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   int c0, c1;
   pieces_of_unit(p, line, w, along, c0, c1);
   wait_for_earlier_grids();
-  if (r >= rows.n || c0 == c1) return;      // (the unit was finished where it was formed)
-  if (p.status != nullptr && *reinterpret_cast<volatile unsigned int*>(p.status) != 0u) return;
-  auto piece = [&](int c) { return partial_of(p, 2 * ((int64_t)c * p.lanes + chunk % p.lanes) + (c == c0 ? 1 : 0)); };
-  const int64_t at_m = (int64_t)p.rows * p.dvo + r, at_l = at_m + p.rows;
-  float mx = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, piece(c)[at_m]);
+  if (c0 == c1) return;      // (the unit was finished where it was formed)
+  const unsigned int failed = p.status != nullptr ? *reinterpret_cast<volatile unsigned int*>(p.status) : 0u;
+  const int64_t step = 2 * (int64_t)p.lanes * partial_floats(p);
+  // (of the first piece the second place, of the others the first)
+  const float* head = partial_of(p, 2 * ((int64_t)c0 * p.lanes + chunk % p.lanes) + 1);
+  auto piece = [&](int i) { return i == 0 ? head : head + i * step - partial_floats(p); };
+  const int n = c1 - c0 + 1;
+  for (int job = blockIdx.y * kJoinWarps + tid / 32; job < rows.n * widths; job += gridDim.y * kJoinWarps) {
+    const int r = (int)((unsigned)job / (unsigned)widths), d = ((job - r * widths) * 32 * K + lane) * N;
+    const int64_t at_m = (int64_t)p.rows * p.dvo + r, at_l = at_m + p.rows, at_o = (int64_t)r * p.dvo;
+    // the row's maximum, and of up to 32 pieces what each lane's weighs
+    float m0 = -INFINITY, l0 = 0.f;
+    if (lane < n) { m0 = piece(lane)[at_m]; l0 = piece(lane)[at_l]; }
+    float mx = m0;
+    for (int i = lane + 32; i < n; i += 32) mx = fmaxf(mx, piece(i)[at_m]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  const float ref = mx == -INFINITY ? 0.f : mx;
-  V acc[K];
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    V acc[K];
 #pragma unroll
-  for (int k = 0; k < K; ++k) acc[k] = V{};
-  float l = 0.f;
-  for (int from = c0; from <= c1; from += 32) {
-    const int n = min(32, c1 - from + 1);
-    float weight = 0.f;
-    if (lane < n) {
-      const float* q = piece(from + lane);
-      weight = exp2f(q[at_m] - ref);
-      l = fmaf(weight, q[at_l], l);
-    }
-    for (int i = 0; i < n; i += kAhead) {
-      V x[kAhead][K];
-#pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const V* src = reinterpret_cast<const V*>(piece(from + min(i + a, n - 1)) + (int64_t)r * p.dvo);
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          if ((lane + 32 * k) * N < p.dvo) x[a][k] = src[lane + 32 * k];
+    for (int k = 0; k < K; ++k) acc[k] = V{};
+    float l = 0.f;
+    for (int from = 0; from < n; from += 32) {
+      if (from > 0) {
+        m0 = -INFINITY;
+        l0 = 0.f;
+        if (from + lane < n) { m0 = piece(from + lane)[at_m]; l0 = piece(from + lane)[at_l]; }
       }
+      const float weight = exp2f(m0 - ref);
+      l = fmaf(weight, l0, l);
+      const int here = min(32, n - from);
+      for (int i = 0; i < here; i += kAhead) {
+        V x[kAhead][K];      // (all of them asked for ahead of the first use: behind the last piece and the last column, the last again)
 #pragma unroll
-      for (int a = 0; a < kAhead; ++a) {
-        const float f = __shfl_sync(0xffffffffu, weight, (i + a) & 31);
-        if (i + a < n)
+        for (int a = 0; a < kAhead; ++a) {
+          const float* row = piece(from + min(i + a, here - 1)) + at_o;
 #pragma unroll
-          for (int k = 0; k < K; ++k)
-            if ((lane + 32 * k) * N < p.dvo) add_weighed(acc[k], f, x[a][k]);
+          for (int k = 0; k < K; ++k) x[a][k] = *reinterpret_cast<const V*>(row + min(d + 32 * N * k, p.dvo - N));
+        }
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+          const float f = __shfl_sync(0xffffffffu, weight, (i + a) & 31);
+          if (i + a < here)
+#pragma unroll
+            for (int k = 0; k < K; ++k) add_weighed(acc[k], f, x[a][k]);
+        }
       }
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (failed != 0u) return;
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const int h = rows.head(p, hk, r), m = rows.query(r);
+    T* out = out_row<T>(p, z, h, m);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const float* e = reinterpret_cast<const float*>(&acc[k]);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (d + 32 * N * k < p.dvo) out[d + 32 * N * k + j] = from_f32<T>(e[j] * inv);
+    }
+    if (d == 0) put_lse(p, z, h, m, mx, l);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const int h = rows.head(p, hk, r), m = rows.query(r);
-  T* out = out_row<T>(p, z, h, m);
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const float* e = reinterpret_cast<const float*>(&acc[k]);
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if ((lane + 32 * k) * N < p.dvo) out[(lane + 32 * k) * N + j] = from_f32<T>(e[j] * inv);
-  }
-  if (lane == 0) put_lse(p, z, h, m, mx, l);
 }
 
 // ---- keys that share columns --------------------------------------------------------------------------------------
@@ -437,14 +448,16 @@ cudaError_t launch_general_T(const PagedAttn& p, cudaStream_t st) {
 }
 template <typename T, typename V, int K>
 cudaError_t launch_join_K(const PagedAttn& p, cudaStream_t st) {
-  const int rows = (int)std::min<int64_t>(p.rows, (int64_t)p.group * p.sq);
-  return launch_counted(paged_join_kernel<T, V, K>, dim3((unsigned)((int64_t)p.batch * p.hk * p.chunks), (rows + kJoinRows - 1) / kJoinRows), kJoinThreads, 0, st, p);
+  const int per = 32 * K * (int)(sizeof(V) / 4), widths = (p.dvo + per - 1) / per;
+  const int64_t units = (int64_t)p.batch * p.hk * p.chunks, jobs = std::min<int64_t>(p.rows, (int64_t)p.group * p.sq) * widths;
+  const int64_t blocks = std::max<int64_t>(1, std::min((jobs + kJoinWarps - 1) / kJoinWarps, kJoinBlocks / units));
+  return launch_counted(paged_join_kernel<T, V, K>, dim3((unsigned)units, (unsigned)blocks), kJoinThreads, 0, st, p, widths);
 }
 template <typename T>
 cudaError_t launch_join_T(const PagedAttn& p, cudaStream_t st) {
-  if (p.dvo % 4 != 0) return launch_join_K<T, float, 32>(p, st);
-  if (p.dvo <= 128) return launch_join_K<T, float4, 1>(p, st);
-  return p.dvo <= 512 ? launch_join_K<T, float4, 4>(p, st) : launch_join_K<T, float4, 8>(p, st);
+  if (p.dvo % 4 != 0) return launch_join_K<T, float, 1>(p, st);
+  const int64_t warps = (int64_t)p.batch * p.hk * p.group * p.sq * ((p.dvo + 127) / 128);
+  return warps > kJoinBlocks && p.dvo > 128 ? launch_join_K<T, float4, 4>(p, st) : launch_join_K<T, float4, 1>(p, st);
 }
 
 template <typename F>

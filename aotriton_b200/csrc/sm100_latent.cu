@@ -36,7 +36,7 @@ struct LatentSmem {
   static constexpr int kSoftmax = 128 * kGroups, kThreads = kSoftmax + 64, kOwn = NR / kGroups;
   static constexpr int kSlots = NR > 32 ? 4 : 5;
   static constexpr int bFull = 0, bEmpty = kSlots, bTailFull = 2 * kSlots, bTailEmpty = bTailFull + 1, bQ = bTailEmpty + 1, bS = bQ + 1, bP = bS + 1,
-                       bO = bP + 1, bDrain = bO + 1, bCount = bDrain + 1;
+                       bO = bP + 1, bDrain = bO + 1, bQEmpty = bDrain + 1, bCount = bQEmpty + 1;
   static constexpr int kAbort = bCount * 8, kTmem = kAbort + 8;
   static constexpr int kScratch = (kTmem + 8 + 15) & ~15;
   static constexpr int kRef = (kScratch + (kThreads / 32 + 2) * 4 + 15) & ~15;      // [NR] references, rescales, inverse sums; [4][NR] of the warps
@@ -95,7 +95,7 @@ __device__ __forceinline__ int lane_column(int lane) { return NR == 32 ? lane : 
 
 // p.rows = NR; p.dvo a multiple of 128 up to 512, the last 1 to 64 of p.dqk columns behind it
 template <typename T, int NR>
-__global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap tm) {
+__global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ CUtensorMap tm, const __grid_constant__ CUtensorMap tm_q) {
   using L = LatentSmem<NR>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -103,12 +103,15 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
   volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kAbort);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) prefetch_tmap(&tm);
+  if (tid == 0) {
+    prefetch_tmap(&tm);
+    if (p.q_tiles) prefetch_tmap(&tm_q);
+  }
   wait_for_earlier_grids();
   const unsigned int failed = tid == 0 ? *reinterpret_cast<volatile unsigned int*>(p.status) : 0u;
   if (tid == 0) {
     init_abort_and_limit(abort_flag, p.wait_limit_kcycles);
-    for (int b = 0; b < L::bCount; ++b) mbar_init(&bars[b], b == L::bQ || b == L::bP ? 4 * L::kGroups : 1);
+    for (int b = 0; b < L::bCount; ++b) mbar_init(&bars[b], b == L::bP || (b == L::bQ && !p.q_tiles) ? 4 * L::kGroups : 1);
     fence_barrier_init();
   }
   const Line line = find_in_line<L::kThreads>(p, -1, blockIdx.x / p.lanes, reinterpret_cast<int*>(smem + L::kScratch));
@@ -124,17 +127,26 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
   const uint32_t tmem = *tmem_slot;
   Piece run(p, line);
   const Walk& w = run.w;
-  const int blocks = p.dvo / 128;
+  const int blocks = p.dvo / 128, qboxes = (p.dqk + 63) / 64;
 
   if (warp == 4 * L::kGroups) {
     // ================================ TMA producer ===================================
     const int octets = p.box / 8;
     const bool leads = lane < 16 && lane % octets == 0;
-    int vi = 0, ti = 0;      // blocks and tails requested
+    int vi = 0, ti = 0, units = 0;      // blocks, tails and units requested
     bool stop = false;
     while (!stop && run.next(p)) {
       if (Rows(p, w, run.chunk).n == 0) continue;
       const int first = run.first, last = run.last;
+      if (p.q_tiles) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars[L::bQEmpty], ((uint32_t)units & 1u) ^ 1u, abort_flag, p.status, 0x7020))) { stop = true; break; }
+        if (lane == 0) {
+          mbar_expect_tx(&bars[L::bQ], qboxes * L::kQBox);
+          for (int b = 0; b < qboxes; ++b) tma_load_4d(smem + L::kQ + b * L::kQBox, &tm_q, &bars[L::bQ], b * 64, run.chunk * NR, 0, run.z);
+        }
+        __syncwarp();
+        ++units;
+      }
       const int32_t* row = p.table + (int64_t)run.z * p.table_stride;
       auto look = [&](int i) {      // the page of this lane's eight keys in tile i
         const int n = i * kKeys + lane * 8;
@@ -189,6 +201,7 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
     if (*abort_flag && lane == 0) {      // copies that are still in flight land before the memory is used again
       for (int i = max(p.drop_copy == 1 && blockIdx.x == 0 ? 1 : 0, vi - L::kSlots); i < vi; ++i)
         mbar_wait_quiet(&bars[L::bFull + i % L::kSlots], (uint32_t)(i / L::kSlots) & 1u, abort_flag);
+      if (units > 0) mbar_wait_quiet(&bars[L::bQ], (uint32_t)(units - 1) & 1u, abort_flag);
       if (ti > 0) mbar_wait_quiet(&bars[L::bTailFull], (uint32_t)(ti - 1) & 1u, abort_flag);
     }
     __syncwarp();
@@ -239,6 +252,7 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
         if (!ok) break;
         if (elect_one()) {
           if (!L::kAlias) mma_commit(&bars[L::bTailEmpty]);
+          if (i + 1 == last) mma_commit(&bars[L::bQEmpty]);
           mma_commit(&bars[L::bS]);
         }
         __syncwarp();
@@ -280,7 +294,6 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
     constexpr int kSoftmax = L::kSoftmax, kOwn = L::kOwn;
     const int col = warp / 4 * kOwn, key = tid & 127;
     const uint32_t mine = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col;      // this warp's lanes
-    const int qboxes = (p.dqk + 63) / 64;
     int vi = 0, tiles = 0, units = 0;
     bool broken = false;
     while (!broken && run.next(p)) {
@@ -288,7 +301,8 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
       const Rows rows(p, w, run.chunk);
       if (first == 0 && run.chunk == 0) zero_rows_behind<T, kSoftmax>(p, w, z, 0, tid);
       if (rows.n == 0) continue;
-      // ---- the unit's queries, as the products read them ----
+      // ---- the unit's queries, as the products read them, where they are not rows of a tile copy ----
+      if (!p.q_tiles)
       for (int r = warp; r < NR; r += 4 * L::kGroups) {      // (a warp a row, a lane 16 bytes; those that there are none of are zero)
         const bool in = r < rows.n;
         const T* src = reinterpret_cast<const T*>(p.q.ptr);
@@ -302,10 +316,12 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
         pos[tid] = tid < rows.n ? w.len - rows.queries + rows.query(tid) : 0x7fffffff;
         out_at[tid] = tid < rows.n ? (int64_t)z * p.out.s[0] + (int64_t)rows.head(p, 0, tid) * p.out.s[1] + (int64_t)rows.query(tid) * p.out.s[2] : 0;
       }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[L::bQ]);
+      if (!p.q_tiles) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[L::bQ]);
+      }
       softmax_sync<kSoftmax>();
       float l[kOwn];
 #pragma unroll
@@ -452,6 +468,9 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
   }
 }
 
+// A call of one query each: the heads as the rows of a (batch, 1, heads, columns) view.
+View4 query_rows(const PagedAttn& p) { return View4{p.q.ptr, {p.q.n[0], 1, p.q.n[1], p.dqk}, {p.q.s[0], p.q.s[1], p.q.s[1], p.q.s[3]}}; }
+
 template <typename T, int NR>
 cudaError_t launch_latent_T(PagedAttn& p, cudaStream_t st) {
   using L = LatentSmem<NR>;
@@ -468,7 +487,9 @@ cudaError_t launch_latent_T(PagedAttn& p, cudaStream_t st) {
   CUtensorMap tm;
   const View4 k{p.k.ptr, {p.k.n[0], 1, p.k.n[1], p.dqk}, {p.k.s[0], p.k.s[2], p.k.s[1], p.k.s[3]}};
   if (!make_tile_map_16bit(&tm, k, p.dqk, p.page, p.box)) return cudaErrorInvalidValue;
-  e = launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kBytes, st, p, tm);
+  CUtensorMap tq = tm;
+  if (p.q_tiles && !make_tile_map_16bit(&tq, query_rows(p), p.dqk, p.hq, NR)) return cudaErrorInvalidValue;
+  e = launch_kernel(kernel, dim3(p.ctas), dim3(L::kThreads), L::kBytes, st, p, tm, tq);
   if (e == cudaSuccess) count_launch();
   return e;
 }
@@ -491,6 +512,7 @@ bool plan_paged_latent(int dtype, PagedAttn& p, int sms) {
   p.box = 128;
   while (p.page % p.box != 0) p.box /= 2;
   p.tile_log = 7;
+  p.q_tiles = p.sq == 1 && tma_friendly(query_rows(p));
   p.min_tiles = 1;
   p.extra = 2;
   p.ctas = sms;
