@@ -994,7 +994,7 @@ int ab200_block_tables(const ab200_block_tables_args* a, void* stream) {
   if (a->cu_seqlens == nullptr || a->taken_out == nullptr || (a->total_tokens > 0 && a->slots == nullptr)) return kErrInvalidValue;
   if (a->batch > 0 && (a->lengths == nullptr || a->new_tokens == nullptr || a->new_lengths == nullptr)) return kErrInvalidValue;
   if ((a->batch > 0 && a->table_width > 0 && a->block_table == nullptr) || (a->num_free > 0 && a->free_pages == nullptr)) return kErrInvalidValue;
-  if (a->total_tokens > INT32_MAX) return kErrNotSupported;
+  if (a->total_tokens > INT32_MAX - (1 << 20)) return kErrNotSupported;
   BlockTables b{};
   b.batch = a->batch; b.page = a->page_size; b.width = a->table_width; b.total = a->total_tokens; b.table_stride = a->table_stride; b.num_free = a->num_free;
   b.table = a->block_table; b.lengths = a->lengths; b.new_tokens = a->new_tokens; b.free_pages = a->free_pages; b.taken = a->taken;
@@ -1104,6 +1104,7 @@ static int fill_shared_columns(const ab200_shared_columns_args* a, SharedColumns
   for (const View4* v : {&r, &o})
     for (int i = 0; i < 4; ++i)
       if (v->n[i] < 0 || v->n[i] > INT32_MAX) return kErrInvalidValue;
+  if (o.n[0] > INT32_MAX / (o.n[2] > 0 ? o.n[2] : 1) || o.n[1] > INT32_MAX / (o.n[3] > 0 ? o.n[3] : 1)) return kErrNotSupported;
   if (r.n[0] != o.n[0] || r.n[1] != 1 || r.n[2] != o.n[2] || r.n[3] < 1 || r.n[3] >= o.n[3]) return kErrInvalidValue;
   if (!gradient && (s.k.n[0] != o.n[0] || s.k.n[1] != o.n[1] || s.k.n[2] != o.n[2] || s.k.n[3] != o.n[3] - r.n[3])) return kErrInvalidValue;
   const int elt = a->dtype == AB200_DTYPE_FP32 ? 4 : 2;

@@ -15,24 +15,28 @@ namespace {
 // for anything, and one launch does.
 constexpr int kTableThreads = 256, kTableTokens = 2048;
 
+// RUN: tokens next to each other that a thread takes: 4 where sequences take many, most often of one sequence and one page; 1 where most take one (48 of
+// one token 2.8 us, with 4 4.9; 590000 tokens of 300 sequences 7.0, with 1 9.6).
+template <int RUN>
 __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const __grid_constant__ BlockTables a) {
   wait_for_earlier_grids();
   __shared__ int64_t warp_tokens[kTableThreads / 32], warp_pages[kTableThreads / 32];
-  __shared__ int64_t start[kTableThreads], fresh[kTableThreads];
-  __shared__ int held[kTableThreads];
+  __shared__ int64_t fresh[kTableThreads];
+  __shared__ int start[kTableThreads], held[kTableThreads], pages_of[kTableThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t t0 = (int64_t)blockIdx.x * kTableTokens, t1 = min(t0 + kTableTokens, a.total);
   const bool sums = blockIdx.x == 0;
   int64_t tokens = 0, pages = a.taken != nullptr ? max(a.taken[0], 0) : 0;      // of the sequences so far
   for (int z0 = 0; z0 < a.batch && (sums || tokens < t1); z0 += kTableThreads) {
     const int z = z0 + tid;
-    int n = 0, m = 0;
-    int64_t need = 0;
+    int n = 0, m = 0, have = 0, need = 0;
     if (z < a.batch) {
       n = max(a.lengths[z], 0);
       m = max(a.new_tokens[z], 0);
-      const int64_t have = min(((int64_t)n + a.page - 1) / a.page, (int64_t)a.width);
-      need = min(((int64_t)n + m + a.page - 1) / a.page, (int64_t)a.width) - have;
+      // (two numbers of 31 bits and a page's worth are within 32)
+      have = (int)min((unsigned)n / (unsigned)a.page + ((unsigned)n % (unsigned)a.page != 0u), (unsigned)a.width);
+      const unsigned all = (unsigned)n + (unsigned)m;
+      need = (int)min(all / (unsigned)a.page + (all % (unsigned)a.page != 0u), (unsigned)a.width) - have;
     }
     int64_t up_t = m, up_p = need;
 #pragma unroll
@@ -49,36 +53,57 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const __gri
       all_t += warp_tokens[w];
       all_p += warp_pages[w];
     }
-    start[tid] = tokens + up_t - m;
-    fresh[tid] = pages + up_p - need;
+    start[tid] = (int)min(tokens + up_t - m, (int64_t)0x7fffffff);      // (of tokens below 2^31 alone)
+    fresh[tid] = pages + up_p - need - have;
     held[tid] = n;
+    pages_of[tid] = have;
     if (sums && z < a.batch) {
       if (z == 0) a.cu_seqlens[0] = 0;
       a.cu_seqlens[z + 1] = (int)min(tokens + up_t, (int64_t)0x7fffffff);
       a.new_lengths[z] = (int)min((int64_t)n + m, (int64_t)0x7fffffff);
     }
     __syncthreads();
-    const int64_t end = min(tokens + all_t, t1);
-    for (int64_t t = max(tokens, t0) + tid; t < end; t += kTableThreads) {
-      int lo = 0, hi = kTableThreads - 1;      // the last sequence that starts at or ahead of the token: it has tokens, those behind it start later
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (start[mid] <= t) lo = mid;
-        else hi = mid - 1;
-      }
-      const int64_t p = (int64_t)held[lo] + (t - start[lo]), page = p / a.page, have = min(((int64_t)held[lo] + a.page - 1) / a.page, (int64_t)a.width);
-      int64_t id = -1;
-      if (page < a.width) {
-        int32_t* entry = a.table + (int64_t)(z0 + lo) * a.table_stride + page;
-        if (page < have) {
-          id = *entry;
-        } else {
-          const int64_t i = fresh[lo] + page - have;
-          id = i < a.num_free ? a.free_pages[i] : -1;
-          if (p % a.page == 0) *entry = (int)id;      // (a page's first token enters it)
+    const int64_t from = max(tokens, t0), end = min(tokens + all_t, t1);
+    for (int t = from < end ? (int)from + tid * RUN : 0x7fffffff; t < (int)end; t += kTableThreads * RUN) {
+      int lo = -1, id = -1;
+      unsigned page = 0u, in = 0u;
+      bool looked = false;
+#pragma unroll
+      for (int k = 0; k < RUN; ++k) {
+        const int tk = t + k;
+        if (tk >= (int)end) break;
+        if (lo < 0 || (lo + 1 < kTableThreads && start[lo + 1] <= tk)) {
+          lo = 0;      // the last sequence that starts at or ahead of the token: it has tokens, those behind it start later
+          for (int hi = kTableThreads - 1; lo < hi;) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (start[mid] <= tk) lo = mid;
+            else hi = mid - 1;
+          }
+          const unsigned p = (unsigned)held[lo] + (unsigned)(tk - start[lo]);
+          page = p / (unsigned)a.page;
+          in = p - page * (unsigned)a.page;
+          looked = false;
+        } else if (++in == (unsigned)a.page) {
+          in = 0u;
+          ++page;
+          looked = false;
         }
+        if (!looked) {
+          looked = true;
+          id = -1;
+          if (page < (unsigned)a.width) {
+            int32_t* entry = a.table + (int64_t)(z0 + lo) * a.table_stride + page;
+            if ((int)page < pages_of[lo]) {
+              id = *entry;
+            } else {
+              const int64_t i = fresh[lo] + page;
+              id = i < a.num_free ? a.free_pages[i] : -1;
+              if (in == 0u) *entry = id;      // (a page's first token enters it)
+            }
+          }
+        }
+        a.slots[tk] = id < 0 ? -1 : (int64_t)id * a.page + in;
       }
-      a.slots[t] = id < 0 ? -1 : id * a.page + p % a.page;
     }
     tokens += all_t;
     pages += all_p;
@@ -385,20 +410,33 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 }
 
 // ---- keys that share columns --------------------------------------------------------------------------------------
-// out[b, h, s] = (k[b, h, s], shared[b, 0, s]): rows moved as they are.  V: the vector that all rows allow.
+// out[b, h, s] = (k[b, h, s], shared[b, 0, s]): rows moved as they are, bound by their bytes.  V: the vector that all rows allow.  A block takes the
+// vectors of a token's heads, each thread four at a time whose loads are on the way together; the shared ones are read again for each head, out of L1.
+// grid = (batch * tokens, some)
+constexpr int kColumnThreads = 128, kColumnBatch = 4;
+
 template <typename V>
-__global__ void __launch_bounds__(256) join_columns_kernel(const __grid_constant__ SharedColumns a, int elt) {
+__global__ void __launch_bounds__(kColumnThreads) join_columns_kernel(const __grid_constant__ SharedColumns a, int elt) {
   wait_for_earlier_grids();
-  const int per = (int)sizeof(V) / elt, vn = (int)a.k.n[3] / per, vr = (int)a.shared.n[3] / per, wide = vn + vr;
-  const int64_t rows = a.out.n[0] * a.out.n[1] * a.out.n[2], total = rows * wide;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / wide;
-    const int c = (int)(i - row * wide);
-    const int64_t bs = row / a.out.n[1], h = row - bs * a.out.n[1], b = bs / a.out.n[2], s = bs - b * a.out.n[2];      // (heads next to each other)
-    const char* src = c < vn ? reinterpret_cast<const char*>(a.k.ptr) + (b * a.k.s[0] + h * a.k.s[1] + s * a.k.s[2]) * elt + (int64_t)c * sizeof(V)
-                             : reinterpret_cast<const char*>(a.shared.ptr) + (b * a.shared.s[0] + s * a.shared.s[2]) * elt + (int64_t)(c - vn) * sizeof(V);
-    char* dst = reinterpret_cast<char*>(a.out.ptr) + (b * a.out.s[0] + h * a.out.s[1] + s * a.out.s[2]) * elt + (int64_t)c * sizeof(V);
-    *reinterpret_cast<V*>(dst) = *reinterpret_cast<const V*>(src);
+  const int per = (int)sizeof(V) / elt, vn = (int)a.k.n[3] / per, wide = vn + (int)a.shared.n[3] / per, items = (int)a.out.n[1] * wide;
+  const int b = (int)(blockIdx.x / (unsigned)a.out.n[2]), s = (int)(blockIdx.x - (unsigned)b * (unsigned)a.out.n[2]);
+  const char* k = reinterpret_cast<const char*>(a.k.ptr) + (b * a.k.s[0] + s * a.k.s[2]) * elt;
+  const char* shared = reinterpret_cast<const char*>(a.shared.ptr) + (b * a.shared.s[0] + s * a.shared.s[2]) * elt;
+  char* out = reinterpret_cast<char*>(a.out.ptr) + (b * a.out.s[0] + s * a.out.s[2]) * elt;
+  for (int i0 = blockIdx.y * kColumnThreads * kColumnBatch + threadIdx.x; i0 < items; i0 += gridDim.y * kColumnThreads * kColumnBatch) {
+    V x[kColumnBatch];
+    V* to[kColumnBatch];
+#pragma unroll
+    for (int j = 0; j < kColumnBatch; ++j) {
+      const int i = i0 + j * kColumnThreads, h = (int)((unsigned)i / (unsigned)wide), c = i - h * wide;
+      to[j] = nullptr;
+      if (i >= items) continue;
+      x[j] = *reinterpret_cast<const V*>(c < vn ? k + h * a.k.s[1] * elt + (int64_t)c * sizeof(V) : shared + (int64_t)(c - vn) * sizeof(V));
+      to[j] = reinterpret_cast<V*>(out + h * a.out.s[1] * elt + (int64_t)c * sizeof(V));
+    }
+#pragma unroll
+    for (int j = 0; j < kColumnBatch; ++j)
+      if (to[j] != nullptr) *to[j] = x[j];
   }
 }
 
@@ -472,7 +510,8 @@ auto with_type(int dtype, F f) {
 }  // namespace
 
 cudaError_t launch_block_tables(const BlockTables& a, cudaStream_t st) {
-  return launch_counted(block_tables_kernel, dim3(std::max(1u, grid_for(a.total, kTableTokens))), kTableThreads, 0, st, a);
+  return launch_counted(a.total > (int64_t)8 * a.batch ? block_tables_kernel<4> : block_tables_kernel<1>, dim3(std::max(1u, grid_for(a.total, kTableTokens))),
+                        kTableThreads, 0, st, a);
 }
 
 cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st) {
@@ -519,12 +558,13 @@ cudaError_t launch_paged(int dtype, PagedAttn& p, cudaStream_t st) {
 }
 
 cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t st) {
-  const int elt = dtype == 1 ? 4 : 2, per = 16 / elt;
-  const int64_t elements = a.out.n[0] * a.out.n[1] * a.out.n[2] * a.out.n[3];
-  if (vec_rows(a.k, per) && vec_rows(a.shared, per) && vec_rows(a.out, per))
-    return launch_counted(join_columns_kernel<uint4>, dim3(grid_for(elements / per, 256)), 256, 0, st, a, elt);
-  if (elt == 4) return launch_counted(join_columns_kernel<uint32_t>, dim3(grid_for(elements, 256)), 256, 0, st, a, elt);
-  return launch_counted(join_columns_kernel<uint16_t>, dim3(grid_for(elements, 256)), 256, 0, st, a, elt);
+  const int elt = dtype == 1 ? 4 : 2;
+  const bool vec = vec_rows(a.k, 16 / elt) && vec_rows(a.shared, 16 / elt) && vec_rows(a.out, 16 / elt);
+  const int64_t items = a.out.n[1] * (a.out.n[3] / (vec ? 16 / elt : 1));
+  const dim3 grid((unsigned)(a.out.n[0] * a.out.n[2]), (unsigned)std::min<int64_t>(65535, (items + kColumnThreads * kColumnBatch - 1) / (kColumnThreads * kColumnBatch)));
+  if (vec) return launch_counted(join_columns_kernel<uint4>, grid, kColumnThreads, 0, st, a, elt);
+  if (elt == 4) return launch_counted(join_columns_kernel<uint32_t>, grid, kColumnThreads, 0, st, a, elt);
+  return launch_counted(join_columns_kernel<uint16_t>, grid, kColumnThreads, 0, st, a, elt);
 }
 
 cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st) {
