@@ -74,17 +74,22 @@ constexpr float kRescaleThreshold = 8.0f;
 // a tile is 64 KB, so one query tile per CTA (S in 128 and O in 256 tensor-memory columns) and one
 // stage each for K and V; the K copy of block j+1 then runs under the softmax and P V of block j,
 // the V copy under Q K^T and the softmax of block j+1.
+// HD = 192: head dims up to 192 of Q and K and up to 128 of V, as latent attention has them.  Two query tiles, whose S and O fill tensor memory, one
+// stage for K (49 KB) and two for V.  32 heads x 4096, 192 and 128, causal, keys joined first: 188 us (1.0 PFLOP/s without the joining);
+// on HD = 256's one tile of 128 queries 282.
 template <int HD>
 struct FwdSmem {
-  static constexpr int kTiles = HD > 128 ? 1 : 2;
-  static constexpr int kStages = HD > 128 ? 1 : 2;
+  static constexpr int kTiles = HD > 192 ? 1 : 2;
+  static constexpr int kStages = HD > 128 ? 1 : 2, kVStages = HD == 192 ? 2 : kStages;      // of K, of V
   static constexpr int kCtaRows = kTiles * kBM;
-  static constexpr int kHalves = HD / 64;
+  static constexpr int kVD = HD == 192 ? 128 : HD;           // columns of V and O
+  static constexpr int kHalves = HD / 64, kVHalves = kVD / 64;
   static constexpr int kTileBytes = kHalves * 128 * 128;     // 128 rows x HD x 2 bytes
+  static constexpr int kVBytes = kVHalves * 128 * 128;
   static constexpr int kQ = 0;                               // kTiles tiles
   static constexpr int kK = kQ + kTiles * kTileBytes;
   static constexpr int kV = kK + kStages * kTileBytes;
-  static constexpr int kBars = kV + kStages * kTileBytes;
+  static constexpr int kBars = kV + kVStages * kVBytes;
   // barrier slots (8 bytes each)
   static constexpr int bQFull = 0 /*2*/, bKFull = 2, bKEmpty = 4, bVFull = 6, bVEmpty = 8, bSFull = 10 /*2*/,
                        bPFull = 12 /*2*/, bPvDone = 14 /*2*/, bPHalf = 16 /*2*/, bKeepFull = 18 /*2*/,
@@ -264,23 +269,23 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
               tma_load_4d(smem + L::kK + s * L::kTileBytes + hf * 16384, &tm_k, &bars[L::bKFull + s], hf * 64, krow, hk,
                           sq.bidx);
           }
-          if (!mbar_wait(&bars[L::bVEmpty + s], ph ^ 1u, abort_flag, status, 0x200 + j)) { issued = j * 2 + 1; break; }
+          const int sv = j % L::kVStages;
+          if (!mbar_wait(&bars[L::bVEmpty + sv], ((uint32_t)(j / L::kVStages) & 1u) ^ 1u, abort_flag, status, 0x200 + j)) { issued = j * 2 + 1; break; }
           if (p.drop_copy == 1 && j == 0) { issued = 2; continue; }   // test hook: this block's V never arrives
-          mbar_expect_tx(&bars[L::bVFull + s], L::kTileBytes);
-          for (int hf = 0; hf < L::kHalves; ++hf)
-            tma_load_4d(smem + L::kV + s * L::kTileBytes + hf * 16384, &tm_v, &bars[L::bVFull + s], hf * 64, krow, hk,
+          mbar_expect_tx(&bars[L::bVFull + sv], L::kVBytes);
+          for (int hf = 0; hf < L::kVHalves; ++hf)
+            tma_load_4d(smem + L::kV + sv * L::kVBytes + hf * 16384, &tm_v, &bars[L::bVFull + sv], hf * 64, krow, hk,
                         sq.bidx);
           issued = j * 2 + 2;
         }
         if (*abort_flag) {
           // Let copies that are still in flight land before the CTA gives its shared memory back.
           for (int t = 0; t < ntile; ++t) mbar_wait_quiet(&bars[L::bQFull + t], 0, abort_flag);
-          for (int i = max(0, issued - 2 * kStages); i < issued; ++i) {
-            int j = i >> 1, s = j % kStages;
-            uint32_t ph = (uint32_t)(j / kStages) & 1u;
-            if (p.drop_copy == 1 && i == 1) continue;   // (never issued)
-            mbar_wait_quiet((i & 1) ? &bars[L::bVFull + s] : &bars[L::bKFull + s], ph, abort_flag);
-          }
+          const int copied_k = (issued + 1) / 2, copied_v = issued / 2;
+          for (int j = max(0, copied_k - kStages); j < copied_k; ++j)
+            mbar_wait_quiet(&bars[L::bKFull + j % kStages], (uint32_t)(j / kStages) & 1u, abort_flag);
+          for (int j = max(p.drop_copy == 1 ? 1 : 0, copied_v - L::kVStages); j < copied_v; ++j)      // (1: the first was never issued)
+            mbar_wait_quiet(&bars[L::bVFull + j % L::kVStages], (uint32_t)(j / L::kVStages) & 1u, abort_flag);
         }
       }
       __syncwarp();
@@ -293,14 +298,14 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       // padded head dimension costs its own size, not the kernel's.
       constexpr uint32_t kIdescQK = instr_desc_f16(Fmt<T>::code, 128, 128, 0, 0);
       // (EXACT: both equal the kernel's head dimension, known at compile time)
-      const uint32_t kIdescPV = instr_desc_f16(Fmt<T>::code, 128, EXACT ? (uint32_t)HD : (uint32_t)((p.dvo + 15) & ~15), 0, 1);
+      const uint32_t kIdescPV = instr_desc_f16(Fmt<T>::code, 128, EXACT ? (uint32_t)L::kVD : (uint32_t)((p.dvo + 15) & ~15), 0, 1);
       const int ksteps = EXACT ? HD / 16 : (p.dqk + 15) >> 4;
       // Descriptors are built once; a k-step, a tile or a ring stage only moves the 14-bit
       // start-address field (units of 16 bytes), which cannot carry out of the field.
       const uint64_t q_desc = smem_desc_sw128(smem_u32(smem + L::kQ), 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(smem_u32(smem + L::kK), 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + L::kV), 16384, 1024);
-      constexpr uint32_t kStageStep = L::kTileBytes >> 4;
+      constexpr uint32_t kStageStep = L::kTileBytes >> 4, kVStep = L::kVBytes >> 4;
       auto wait = [&](int bar, uint32_t parity, uint32_t where) {
         return __all_sync(0xffffffffu, mbar_wait(&bars[bar], parity, abort_flag, status, where)) != 0;
       };
@@ -331,25 +336,27 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
         for (int t = 0; t < ntile; ++t) issue_qk(t, 0, t == ntile - 1);
       }
       for (int j = 0; ok && j < nblk; ++j) {
-        const int s = j % kStages;
+        const int s = j % L::kVStages;
         const uint32_t par = (uint32_t)j & 1u;
-        if (!wait(L::bVFull + s, (uint32_t)(j / kStages) & 1u, 0x600 + j)) break;
+        if (!wait(L::bVFull + s, (uint32_t)(j / L::kVStages) & 1u, 0x600 + j)) break;
         // Last, partial block of the sequence: the rows of V beyond its end must not reach P V.
         if constexpr (!EXACT) {
           if (j == tail_j)
-            zero_tail_rows(smem + L::kV + s * L::kTileBytes, sq.sk - block(j) * kBN, L::kHalves, lane);
+            zero_tail_rows(smem + L::kV + s * L::kVBytes, sq.sk - block(j) * kBN, L::kVHalves, lane);
         }
         if constexpr ((FEAT & kSinks) != 0) {
           int from, to;
           hidden_keys(p, sq, from, to);
           from = max(from - block(j) * kBN, 0);
           to = min(to - block(j) * kBN, kBN);
-          if (from < to) zero_rows_between(smem + L::kV + s * L::kTileBytes, from, to, L::kHalves, 16384, lane);
+          if (from < to) zero_rows_between(smem + L::kV + s * L::kVBytes, from, to, L::kVHalves, 16384, lane);
         }
-        if (j + 1 < nblk) {
+        // (one K stage for two tiles: its copy still runs under the softmax, P V need not wait for it)
+        constexpr bool kLateK = L::kTiles == 2 && kStages == 1;
+        if (!kLateK && j + 1 < nblk) {
           if (!wait(L::bKFull + ((j + 1) % kStages), (uint32_t)((j + 1) / kStages) & 1u, 0x400 + j + 1)) break;
         }
-        const uint64_t vd = v_desc + (uint64_t)((uint32_t)s * kStageStep);
+        const uint64_t vd = v_desc + (uint64_t)((uint32_t)s * kVStep);
         const uint32_t first = (j > 0) ? 1u : 0u;
         for (int t = 0; ok && t < ntile; ++t) {
           // P arrives in two halves of 64 keys: the first half of P V runs while the softmax warps
@@ -376,6 +383,10 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
             if (t == ntile - 1) mma_commit(&bars[L::bVEmpty + s]);
           }
           __syncwarp();
+          if constexpr (kLateK) {
+            if (t == 0 && j + 1 < nblk && !wait(L::bKFull, (uint32_t)(j + 1) & 1u, 0x400 + j + 1)) { ok = false; break; }
+            tc_fence_after();
+          }
           // the tile's S buffer is free again: PV_t(j), just issued, runs first
           if (j + 1 < nblk) issue_qk(t, j + 1, t == ntile - 1);
         }
@@ -536,7 +547,7 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
         if (!mbar_wait(&bars[L::bPvDone + t], (uint32_t)(j - 1) & 1u, abort_flag, status, 0x800 + 2 * j + t)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
+        for (int c = 0; c < L::kVD / 32; ++c) {
           if (c * 32 >= p.dvo) break;          // columns the P V product never writes
           uint32_t o[32];
           tmem_ld32(o_addr + c * 32, o);
@@ -672,19 +683,19 @@ sm100_fwd_kernel(const __grid_constant__ Params p, const __grid_constant__ CUten
       // (Two 32-column pieces of O at a time, so that a piece is on its way while the one before it is packed.)
       const uint32_t stage = smem_u32(smem + L::kQ + t * L::kTileBytes);
 #pragma unroll
-      for (int c = 0; c < HD / 32; c += 2) {
+      for (int c = 0; c < L::kVD / 32; c += 2) {
         if (c * 32 >= p.dvo) break;
         float o[2][32];
         tmem_ld32f(o_addr + c * 32, o[0]);
         tmem_ld32f(o_addr + c * 32 + 32, o[1]);
         tmem_wait_ld();
-        stage_put32<T>(stage, r, c * 32, o[0], inv, HD * 2);
-        if (c * 32 + 32 < p.dvo) stage_put32<T>(stage, r, c * 32 + 32, o[1], inv, HD * 2);
+        stage_put32<T>(stage, r, c * 32, o[0], inv, L::kVD * 2);
+        if (c * 32 + 32 < p.dvo) stage_put32<T>(stage, r, c * 32 + 32, o[1], inv, L::kVD * 2);
       }
       __syncwarp();
-      warp_copy_out<T, HD / 8>(stage, reinterpret_cast<T*>(p.out.ptr) + (int64_t)sq.bidx * p.out.s[0] +
+      warp_copy_out<T, L::kVD / 8>(stage, reinterpret_cast<T*>(p.out.ptr) + (int64_t)sq.bidx * p.out.s[0] +
                                           (int64_t)h * p.out.s[1] + (sq.q0 + m0 + t * kBM) * p.out.s[2],
-                               p.out.s[2], min(kBM, sq.sq - (m0 + t * kBM)), p.dvo, quarter * 32, 0, lane, HD * 2);
+                               p.out.s[2], min(kBM, sq.sq - (m0 + t * kBM)), p.dvo, quarter * 32, 0, lane, L::kVD * 2);
       if (p.lse != nullptr && m < sq.sq)
         p.lse[lse_offset(p, sq, h) + m] = (l > 0.f) ? (m_used + log2f(l)) * kLn2 : INFINITY;
     }
@@ -729,7 +740,7 @@ cudaError_t fwd_device_facts(int* dev, unsigned int** status, int* sms, bool* re
 #include "sm100_fwd_sink.cuh"
 
 inline bool exact_tiles(const Params& p, int hd) {
-  return p.varlen_mode == 0 && p.max_sq % 128 == 0 && p.max_sk % 128 == 0 && p.dqk == hd && p.dvo == hd;
+  return p.varlen_mode == 0 && p.max_sq % 128 == 0 && p.max_sk % 128 == 0 && p.dqk == hd && p.dvo == (hd == 192 ? 128 : hd);
 }
 
 template <typename T, int HD, bool EXACT, int FEAT>
@@ -777,6 +788,11 @@ cudaError_t launch_fwd_T(const Params& p, cudaStream_t st) {
   }
 }
 
+template <typename T>
+cudaError_t launch_fwd_192(const Params& p, cudaStream_t st) {
+  return exact_tiles(p, 192) ? launch_fwd_TE<T, 192, true, kPlain>(p, st) : launch_fwd_TE<T, 192, false, kPlain>(p, st);
+}
+
 }  // namespace
 
 bool sm100_fwd_supported(int dtype, const Params& p) {
@@ -799,6 +815,15 @@ bool sm100_fwd_split(const Params& p, int sms, SplitPlan* plan) {
 cudaError_t launch_sm100_fwd(int dtype, const Params& p, cudaStream_t st) {
   if (decode_shape(p)) return dtype == 2 ? launch_decode_T<__half>(p, st) : launch_decode_T<__nv_bfloat16>(p, st);
   const int dmax = p.dqk > p.dvo ? p.dqk : p.dvo;
+  if (p.dqk > 128 && p.dqk <= 192 && p.dvo <= 128 && features(p) == kPlain) {
+    // (a CTA a query tile while all of them start at once: 2 x 16 heads x 391 of 192 and 128 18.9 us, two tiles a CTA 19.8)
+    int dev = 0, sms = 0;
+    unsigned int* status = nullptr;
+    bool remember = false;
+    const cudaError_t e = fwd_device_facts(&dev, &status, &sms, &remember);
+    if (e != cudaSuccess) return e;
+    if (((int64_t)p.max_sq + kBM - 1) / kBM * p.hq * p.batch > sms) return dtype == 2 ? launch_fwd_192<__half>(p, st) : launch_fwd_192<__nv_bfloat16>(p, st);
+  }
   if (dtype == 2)
     return dmax <= 64 ? launch_fwd_T<__half, 64>(p, st)
                       : (dmax <= 128 ? launch_fwd_T<__half, 128>(p, st) : launch_fwd_T<__half, 256>(p, st));
