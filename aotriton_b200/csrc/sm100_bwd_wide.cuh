@@ -22,12 +22,17 @@
 // eight compute warps (thread = one row of the 128 x 64 score tile, two warpgroups split its columns
 // 32 apiece); dV with bias and dropout has eight more and two S' buffers (wide_groups).  The arithmetic is that of the 128-wide kernels (see the head of sm100_bwd.cu); dK and dV
 // recompute the probabilities separately, which is the price of the one-accumulator form.
+//
+// Head dims up to 192 of Q and K and up to 128 of V, as latent attention has them, leave room for both accumulators: the mode dKV forms dK and dV in one
+// launch, dV += P'^T dO_i beside dK += dS' Q_i.  dO feeds two products, so it has two stages (of 16 KB), and P' is packed into the other half of
+// the columns that dP' leaves behind.  32 heads x 4096 of 192 and 128, causal: dV 315 and dK 412 us apart.
 // Every wait is bounded.
 
 constexpr int kWideCompute = 8;        // warps of a compute group: 4..11, and 12..19 where there are two
 constexpr int kNB = 64;                // rows of a streamed block
 constexpr uint32_t kWColS = 0, kWColDP = 64, kWColAcc = 256;      // (two compute groups: kColDPW)
-constexpr int kWideDV = 0, kWideDK = 1, kWideDQ = 2;
+constexpr int kWideDV = 0, kWideDK = 1, kWideDQ = 2, kWideDKV = 3;
+constexpr uint32_t kWColDK = 192, kWColDV = 384;      // (dKV)
 // Compute groups.  dV with dropout and bias is bound by its compute warps (they read the bias and draw the bits that the later
 // kernels get from it): two groups take every other streamed block, with a buffer of S' each, so that one's loads and
 // generator run beside the other's.  Measured, 8 x 16 heads x 2048 of 256, bias, dropout 0.2: 1448 -> 1237 us.  Elsewhere it
@@ -56,11 +61,11 @@ struct WideSmem {
 static_assert(WideSmem::kDynamic <= 232448, "shared memory of the wide backward kernel");
 static_assert(WideSmem::kBars % 8 == 0, "barrier alignment");
 
-// zero_tail_rows (sm100_ptx.cuh) for a streamed tile: rows [valid_rows, 64) of its four boxes.
-static __device__ __noinline__ void zero_tail_rows_streamed(uint8_t* tile, int valid_rows, int lane) {
+// zero_tail_rows (sm100_ptx.cuh) for a streamed tile: rows [valid_rows, 64) of its boxes.
+static __device__ __noinline__ void zero_tail_rows_streamed(uint8_t* tile, int valid_rows, int lane, int boxes = WideSmem::kBoxes) {
   const uint4 z = make_uint4(0u, 0u, 0u, 0u);
   if (valid_rows < 0) valid_rows = 0;
-  for (int b = 0; b < WideSmem::kBoxes; ++b)
+  for (int b = 0; b < boxes; ++b)
     for (int o = valid_rows * 128 + lane * 16; o < WideSmem::kStrBox; o += 512)
       *reinterpret_cast<uint4*>(tile + b * WideSmem::kStrBox + o) = z;
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -81,7 +86,12 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
   constexpr uint32_t kColDPW = kGroups == 2 ? 128 : kWColDP;      // (behind two S' buffers)
   // The early tile has one stage; dV, which keeps only K resident, gives it two in the second
   // resident tile's place.
-  constexpr int kEarlyStages = MODE == kWideDV ? 2 : 1;
+  constexpr bool kBoth = MODE == kWideDKV;
+  constexpr int kEarlyStages = MODE == kWideDV || kBoth ? 2 : 1;
+  // 64-column boxes of the resident tiles and the streamed ones, and where the accumulator of d_out columns lies
+  constexpr int kBoxesA = kBoth ? 3 : L::kBoxes, kBoxesB = kBoth ? 2 : L::kBoxes, kBoxesLate = kBoxesA, kBoxesEarly = kBoxesB;
+  constexpr int kEarlyStr = kBoth ? L::kStr / 2 : L::kStr;
+  constexpr uint32_t kColAcc = kBoth ? kWColDK : kWColAcc;
   constexpr int kEarlyBase = MODE == kWideDV ? WideSmem::kResB : WideSmem::kEarly;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -139,7 +149,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       }
     }
   }
-  const View4& outv = MODE == kWideDV ? p.dv : (MODE == kWideDK ? p.dk : p.dq);
+  const View4& outv = MODE == kWideDV ? p.dv : (MODE == kWideDQ ? p.dq : p.dk);
   const int d_out = MODE == kWideDV ? p.dvo : p.dqk;
   const int64_t row_tok0 = kKeys ? sq.k0 : sq.q0, col_tok0 = kKeys ? sq.q0 : sq.k0;
   if (c_hi < c_lo) {      // rows nothing attends to / that attend to nothing: the gradient is zero
@@ -151,6 +161,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       if (chunk > 0) return;
     }
     zero_rows<T>(outv, sq.bidx, hrow, row_tok0, r0, rows_total, d_out);
+    if constexpr (kBoth) zero_rows<T>(p.dv, sq.bidx, hrow, row_tok0, r0, rows_total, p.dvo);
     if constexpr (MODE == kWideDQ) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, 0, 0); }
     return;
   }
@@ -196,10 +207,10 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     // ================================ TMA producer ===================================
     if (lane == 0) {
       const int rrow = (int)(row_tok0 + r0);
-      mbar_expect_tx(&bars[L::bResFull], (kHasDp ? 2 : 1) * L::kRes);
-      for (int b = 0; b < L::kBoxes; ++b) {
+      mbar_expect_tx(&bars[L::bResFull], (kBoxesA + (kHasDp ? kBoxesB : 0)) * L::kResBox);
+      for (int b = 0; b < kBoxesA; ++b) {
         tma_load_4d(smem + L::kResA + b * L::kResBox, &tm_r1, &bars[L::bResFull], b * 64, rrow, hrow, sq.bidx);
-        if constexpr (kHasDp)
+        if (kHasDp && b < kBoxesB)
           tma_load_4d(smem + L::kResB + b * L::kResBox, &tm_r2, &bars[L::bResFull], b * 64, rrow, hrow, sq.bidx);
       }
       // test hook of the bounded waits: the first early tile never arrives
@@ -214,15 +225,15 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         const int es = i % kEarlyStages;
         if (!mbar_wait(&bars[L::bEarlyEmpty + es], ((uint32_t)(i / kEarlyStages) & 1u) ^ 1u, abort_flag, status, 0x3100)) break;
         if (!(drop_first && i == 0)) {
-          mbar_expect_tx(&bars[L::bEarlyFull + es], L::kStr);
-          for (int b = 0; b < L::kBoxes; ++b)
-            tma_load_4d(smem + kEarlyBase + es * L::kStr + b * L::kStrBox, &tm_early, &bars[L::bEarlyFull + es], b * 64, srow,
+          mbar_expect_tx(&bars[L::bEarlyFull + es], kBoxesEarly * L::kStrBox);
+          for (int b = 0; b < kBoxesEarly; ++b)
+            tma_load_4d(smem + kEarlyBase + es * kEarlyStr + b * L::kStrBox, &tm_early, &bars[L::bEarlyFull + es], b * 64, srow,
                         hs, sq.bidx);
           issued_e = i + 1;
         }
         if (!mbar_wait(&bars[L::bLateEmpty + s], ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, status, 0x3000)) break;
-        mbar_expect_tx(&bars[L::bLateFull + s], L::kStr);
-        for (int b = 0; b < L::kBoxes; ++b)
+        mbar_expect_tx(&bars[L::bLateFull + s], kBoxesLate * L::kStrBox);
+        for (int b = 0; b < kBoxesLate; ++b)
           tma_load_4d(smem + L::kLate + s * L::kStr + b * L::kStrBox, &tm_late, &bars[L::bLateFull + s], b * 64, srow, hs,
                       sq.bidx);
         issued_l = i + 1;
@@ -260,7 +271,9 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     const uint64_t late_km = smem_desc_sw128(smem_u32(smem + L::kLate), 16, 1024);
     const uint64_t late_mn = smem_desc_sw128(smem_u32(smem + L::kLate), L::kStrBox, 1024);
     const uint64_t early_km = smem_desc_sw128(smem_u32(smem + kEarlyBase), 16, 1024);
-    constexpr uint32_t kStageStep = L::kStr >> 4;
+    const uint64_t early_mn = smem_desc_sw128(smem_u32(smem + kEarlyBase), L::kStrBox, 1024);      // (dKV)
+    const uint32_t idesc_dv = instr_desc_f16(Fmt<T>::code, 128, (uint32_t)((p.dvo + 15) & ~15), 0, 1);
+    constexpr uint32_t kStageStep = L::kStr >> 4, kEarlyStep = kEarlyStr >> 4;
     // k-step kk of a K-major tile: head-dim columns 16kk..16kk+15 (box kk / 4, 32 bytes per step inside it)
     auto res_step = [](int kk) { return (uint32_t)(kk >> 2) * (uint32_t)(L::kResBox >> 4) + (uint32_t)(kk & 3) * 2u; };
     auto str_step = [](int kk) { return (uint32_t)(kk >> 2) * (uint32_t)(L::kStrBox >> 4) + (uint32_t)(kk & 3) * 2u; };
@@ -291,7 +304,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         if (i >= kGroups && !wait(L::bSRead + sb, (uint32_t)(kGroups == 2 ? (i >> 1) - 1 : i - 1) & 1u, 0x3800)) return false;
         if (!wait(L::bEarlyFull + es, epar, 0x3200)) return false;
         tc_fence_after();
-        const uint64_t ea = early_km + (uint64_t)(es * kStageStep);
+        const uint64_t ea = early_km + (uint64_t)(es * kEarlyStep);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 16; ++kk)
@@ -305,17 +318,17 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       } else {
         const int valid = valid_rows(i);
         if (!wait(L::bEarlyFull + es, epar, 0x3400)) return false;
-        if (valid < kNB) zero_tail_rows_streamed(smem + kEarlyBase + es * L::kStr, valid, lane);
-        zero_hidden(i, smem + kEarlyBase + es * L::kStr);
+        if (valid < kNB) zero_tail_rows_streamed(smem + kEarlyBase + es * kEarlyStr, valid, lane, kBoxesEarly);
+        zero_hidden(i, smem + kEarlyBase + es * kEarlyStr);
         tc_fence_after();
-        const uint64_t ea = early_km + (uint64_t)(es * kStageStep);
+        const uint64_t ea = early_km + (uint64_t)(es * kEarlyStep);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 16; ++kk)
             if (kk < ksteps_vo)
               mma_ss(tmem_base + kColDPW + s * 64u, r2_km + res_step(kk), ea + str_step(kk), kIdescS, kk > 0 ? 1u : 0u);
           mma_commit(&bars[L::bDpFull + s]);
-          mma_commit(&bars[L::bEarlyEmpty + es]);
+          if (!kBoth) mma_commit(&bars[L::bEarlyEmpty + es]);      // (dKV: dO feeds dV's product too)
         }
         __syncwarp();
         if (i > 0 && !wait(L::bSRead, (uint32_t)(i - 1) & 1u, 0x3800)) return false;
@@ -350,7 +363,14 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kNB / 16; ++kk)
-          mma_ts(tmem_base + kWColAcc, a_col + split_a_col(kk), lb + (uint32_t)kk * (2048u >> 4), idesc_acc, kk > 0 ? 1u : first);
+          mma_ts(tmem_base + kColAcc, a_col + split_a_col(kk), lb + (uint32_t)kk * (2048u >> 4), idesc_acc, kk > 0 ? 1u : first);
+        if constexpr (kBoth) {
+          const uint64_t eb = early_mn + (uint64_t)(s * kEarlyStep);
+#pragma unroll
+          for (int kk = 0; kk < kNB / 16; ++kk)
+            mma_ts(tmem_base + kWColDV, a_col + 16u + split_a_col(kk), eb + (uint32_t)kk * (2048u >> 4), idesc_dv, kk > 0 ? 1u : first);
+          mma_commit(&bars[L::bEarlyEmpty + s]);
+        }
         mma_commit(&bars[L::bLateEmpty + s]);
         if (i + 1 == niter) mma_commit(&bars[L::bAccDone]);
       }
@@ -554,6 +574,11 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           }
         }
         tmem_st16(a_col, pk);
+        if constexpr (kBoth) {      // P', in the other columns that dP' left behind
+#pragma unroll
+          for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(pr[2 * c], pr[2 * c + 1]);
+          tmem_st16(a_col + 16u, pk);
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -679,7 +704,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       const float scale = MODE != kWideDV ? p.sm_scale : 1.0f;
       for (int c = (warp - 4) >> 2; c * 32 < d_out; c += 2 * kGroups) {
         float v[32];
-        tmem_ld32f(tmem_base + lane_addr + kWColAcc + c * 32, v);
+        tmem_ld32f(tmem_base + lane_addr + kColAcc + c * 32, v);
         tmem_wait_ld();
         if constexpr (kKeys && (FEAT & kSinks) != 0) {      // a first key's sums (the 16-bit row written below is overwritten by the last launch)
           if (p.sink_chunks > 0 && r0 + r < min(p.sinks, sq.sk)) {
@@ -695,6 +720,18 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         warp_copy_out<T, 4>(stage, dst, outv.s[2], nrows, d_out, quarter * 32, c * 4, lane, 512);
         __syncwarp();
       }
+      if constexpr (kBoth) {
+        dst = reinterpret_cast<T*>(p.dv.ptr) + (int64_t)sq.bidx * p.dv.s[0] + (int64_t)hrow * p.dv.s[1] + (row_tok0 + r0) * p.dv.s[2];
+        for (int c = (warp - 4) >> 2; c * 32 < p.dvo; c += 2) {
+          float v[32];
+          tmem_ld32f(tmem_base + lane_addr + kWColDV + c * 32, v);
+          tmem_wait_ld();
+          stage_put32<T>(stage, r, c * 32, v, 1.0f, 512);
+          __syncwarp();
+          warp_copy_out<T, 4>(stage, dst, p.dv.s[2], nrows, p.dvo, quarter * 32, c * 4, lane, 512);
+          __syncwarp();
+        }
+      }
     }
   }
 
@@ -707,6 +744,9 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
 }
 
 #include "sm100_bwd_dk_db.cuh"
+
+// Whether dK and dV are formed in one launch.
+inline bool wide_both(const Params& p) { return p.dqk <= 192 && p.dvo <= 128 && features(p) == kPlain; }
 
 // which: 1 dV and dK (two launches), 2 dQ(+dBias); p.dk_from_db: 1 dV, 2 dQ and dBias, then dK from dBias
 template <typename T>
@@ -753,7 +793,15 @@ cudaError_t launch_bwd_wide_T(int which, const Params& p, cudaStream_t st) {
        sm100_bwd_wide_kernel<T, 1, kSinks>},
       {sm100_bwd_wide_kernel<T, 2, kPlain>, sm100_bwd_wide_kernel<T, 2, kBias>, sm100_bwd_wide_kernel<T, 2, kDropout>, sm100_bwd_wide_kernel<T, 2, kAll>,
        sm100_bwd_wide_kernel<T, 2, kSinks>}};
-  if (which == 1) {
+  if (which == 1 && wide_both(p)) {
+    auto kern = sm100_bwd_wide_kernel<T, kWideDKV, kPlain>;
+    static std::atomic<bool> both_set[64];
+    if (pretend || !both_set[dev].load(std::memory_order_acquire)) {
+      if ((e = host().func_set_smem(reinterpret_cast<const void*>(kern), L::kDynamic)) != cudaSuccess) return e;
+      if (!pretend) both_set[dev].store(true, std::memory_order_release);
+    }
+    e = launch_kernel(kern, dim3((p.max_sk + kBlk - 1) / kBlk, p.hk, p.batch), dim3(wide_threads(kWideDKV, kPlain)), L::kDynamic, st, p, k128, v128, q64, do64, status);
+  } else if (which == 1) {
     const Kernel kern_dv = kKernels[kWideDV][feat], kern_dk = kKernels[kWideDK][feat];
     if ((e = set_smem(feat == kSinks ? 13 + kWideDV : 4 * kWideDV + feat, reinterpret_cast<const void*>(kern_dv))) != cudaSuccess) return e;
     if ((e = set_smem(feat == kSinks ? 13 + kWideDK : 4 * kWideDK + feat, reinterpret_cast<const void*>(kern_dk))) != cudaSuccess) return e;
