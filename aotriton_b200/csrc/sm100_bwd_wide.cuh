@@ -24,14 +24,13 @@
 // recompute the probabilities separately, which is the price of the one-accumulator form.
 //
 // Head dims up to 192 of Q and K and up to 128 of V, as latent attention has them, leave room for both accumulators: the mode dKV forms dK and dV in one
-// launch, dV += P'^T dO_i beside dK += dS' Q_i.  dO feeds two products, so it has two stages (of 16 KB), and P' is packed into the other half of
-// the columns that dP' leaves behind.  32 heads x 4096 of 192 and 128, causal: dV 315 and dK 412 us apart.
+// launch, dV += P'^T dO_i beside dK += dS' Q_i; P' is packed into the other half of the columns that dP' leaves behind.  Their tiles, and those of dQ, have three stages.  32 heads x 4096 of 192 and 128, causal: dV 315 and dK 412 us apart.
 // Every wait is bounded.
 
 constexpr int kWideCompute = 8;        // warps of a compute group: 4..11, and 12..19 where there are two
 constexpr int kNB = 64;                // rows of a streamed block
 constexpr uint32_t kWColS = 0, kWColDP = 64, kWColAcc = 256;      // (two compute groups: kColDPW)
-constexpr int kWideDV = 0, kWideDK = 1, kWideDQ = 2, kWideDKV = 3;
+constexpr int kWideDV = 0, kWideDK = 1, kWideDQ = 2, kWideDKV = 3, kWideDQN = 4;      // (N: narrow, as dKV)
 constexpr uint32_t kWColDK = 192, kWColDV = 384;      // (dKV)
 // Compute groups.  dV with dropout and bias is bound by its compute warps (they read the bias and draw the bits that the later
 // kernels get from it): two groups take every other streamed block, with a buffer of S' each, so that one's loads and
@@ -52,11 +51,15 @@ struct WideSmem {
   static constexpr int kAuxFlag = kAux + 2 * 2 * kNB * 4;
   static constexpr int kBars = kAuxFlag + 16;
   static constexpr int bResFull = 0, bLateFull = 1, bLateEmpty = 3, bEarlyFull = 5, bEarlyEmpty = 7, bSFull = 9,
-                       bSRead = 11, bDpFull = 13, bDsFull = 15, bAccDone = 17, bAuxFull = 18, bAuxEmpty = 20, bCount = 22;
+                       bSRead = 11, bDpFull = 13, bDsFull = 15, bAccDone = 17, bAuxFull = 18, bAuxEmpty = 20, bThird = 22 /* the third stages' */, bCount = 26;
   static constexpr int kTmemSlot = kBars + bCount * 8;
   static constexpr int kAbort = kTmemSlot + 8;
   static constexpr int kUsed = kAbort + 8;
   static constexpr int kDynamic = kUsed + 512;
+  static constexpr int late_full(int s) { return s < 2 ? bLateFull + s : bThird; }
+  static constexpr int late_empty(int s) { return s < 2 ? bLateEmpty + s : bThird + 1; }
+  static constexpr int early_full(int s) { return s < 2 ? bEarlyFull + s : bThird + 2; }
+  static constexpr int early_empty(int s) { return s < 2 ? bEarlyEmpty + s : bThird + 3; }
 };
 static_assert(WideSmem::kDynamic <= 232448, "shared memory of the wide backward kernel");
 static_assert(WideSmem::kBars % 8 == 0, "barrier alignment");
@@ -80,19 +83,22 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
                       const __grid_constant__ CUtensorMap tm_early, unsigned int* status) {
   wait_for_earlier_grids();
   using L = WideSmem;
-  constexpr bool kKeys = MODE != kWideDQ;      // the CTA's rows are keys
+  constexpr bool kBoth = MODE == kWideDKV, kNarrow = MODE == kWideDKV || MODE == kWideDQN;
+  constexpr bool kKeys = MODE != kWideDQ && MODE != kWideDQN;      // the CTA's rows are keys
   constexpr bool kHasDp = MODE != kWideDV;
   constexpr int kGroups = wide_groups(MODE, FEAT);
   constexpr uint32_t kColDPW = kGroups == 2 ? 128 : kWColDP;      // (behind two S' buffers)
-  // The early tile has one stage; dV, which keeps only K resident, gives it two in the second
-  // resident tile's place.
-  constexpr bool kBoth = MODE == kWideDKV;
-  constexpr int kEarlyStages = MODE == kWideDV || kBoth ? 2 : 1;
-  // 64-column boxes of the resident tiles and the streamed ones, and where the accumulator of d_out columns lies
-  constexpr int kBoxesA = kBoth ? 3 : L::kBoxes, kBoxesB = kBoth ? 2 : L::kBoxes, kBoxesLate = kBoxesA, kBoxesEarly = kBoxesB;
-  constexpr int kEarlyStr = kBoth ? L::kStr / 2 : L::kStr;
+  // Stages and places of the tiles.  The early tile has one stage; dV, which keeps only K resident, gives it two in the second resident tile's place.  Narrow
+  // tiles (64-column boxes: 3 of Q and K, 2 of V and dO) have three each: a block's first GEMMs, which go out ahead of the accumulating GEMM of the one before,
+  // then find their tiles there, where with two stages they waited for a copy that had been requested behind the accumulating GEMM of two blocks back.
+  constexpr int kBoxesA = kNarrow ? 3 : L::kBoxes, kBoxesB = kNarrow ? 2 : L::kBoxes, kBoxesLate = kBoxesA, kBoxesEarly = kBoxesB;
+  constexpr int kLateStages = kNarrow ? 3 : 2, kEarlyStages = kNarrow ? 3 : (MODE == kWideDV ? 2 : 1);
+  constexpr int kLateStr = kBoxesLate * L::kStrBox, kEarlyStr = kBoxesEarly * L::kStrBox;
+  constexpr int kResA = L::kResA, kResB = kNarrow ? kBoxesA * L::kResBox : L::kResB;
+  constexpr int kLateBase = kNarrow ? kResB + kBoxesB * L::kResBox : L::kLate;
+  constexpr int kEarlyBase = kNarrow ? kLateBase + kLateStages * kLateStr : (MODE == kWideDV ? L::kResB : L::kEarly);
+  static_assert(kEarlyBase + kEarlyStages * kEarlyStr <= L::kAux, "stages end ahead of what is staged");
   constexpr uint32_t kColAcc = kBoth ? kWColDK : kWColAcc;
-  constexpr int kEarlyBase = MODE == kWideDV ? WideSmem::kResB : WideSmem::kEarly;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBars);
@@ -149,7 +155,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       }
     }
   }
-  const View4& outv = MODE == kWideDV ? p.dv : (MODE == kWideDQ ? p.dq : p.dk);
+  const View4& outv = MODE == kWideDV ? p.dv : (kKeys ? p.dk : p.dq);
   const int d_out = MODE == kWideDV ? p.dvo : p.dqk;
   const int64_t row_tok0 = kKeys ? sq.k0 : sq.q0, col_tok0 = kKeys ? sq.q0 : sq.k0;
   if (c_hi < c_lo) {      // rows nothing attends to / that attend to nothing: the gradient is zero
@@ -162,14 +168,14 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     }
     zero_rows<T>(outv, sq.bidx, hrow, row_tok0, r0, rows_total, d_out);
     if constexpr (kBoth) zero_rows<T>(p.dv, sq.bidx, hrow, row_tok0, r0, rows_total, p.dvo);
-    if constexpr (MODE == kWideDQ) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, 0, 0); }
+    if constexpr (!kKeys) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, 0, 0); }
     return;
   }
   const int cb_lo = c_lo / kNB;
   const int before = kKeys ? 0 : blocks_before<FEAT>(p, c_hi, cb_lo, kNB);
   const int ncb = before + c_hi / kNB - cb_lo + 1;
   auto block = [&](int c) { return kKeys ? cb_lo + c : block_at<FEAT>(c, before, cb_lo); };
-  if constexpr (MODE == kWideDQ) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, cb_lo * kNB, (cb_lo + ncb) * kNB); }
+  if constexpr (!kKeys) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, cb_lo * kNB, (cb_lo + ncb) * kNB); }
   const int niter = kKeys ? ncb * p.group : ncb;      // dV / dK walk the q heads of the kv head's group
   const int hk = kKeys ? hrow : hrow / p.group;
 
@@ -177,18 +183,20 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     init_abort_and_limit(abort_flag, p.wait_limit_kcycles);
     mbar_init(&bars[L::bResFull], 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars[L::bLateFull + s], 1);
-      mbar_init(&bars[L::bLateEmpty + s], 1);
       mbar_init(&bars[L::bDpFull + s], 1);
       mbar_init(&bars[L::bDsFull + s], kWideCompute);
       mbar_init(&bars[L::bAuxFull + s], 1);
       mbar_init(&bars[L::bAuxEmpty + s], kWideCompute);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars[L::bEarlyFull + s], 1);
-      mbar_init(&bars[L::bEarlyEmpty + s], 1);
       mbar_init(&bars[L::bSFull + s], 1);
       mbar_init(&bars[L::bSRead + s], kWideCompute);
+    }
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&bars[L::late_full(s)], 1);
+      mbar_init(&bars[L::late_empty(s)], 1);
+      mbar_init(&bars[L::early_full(s)], 1);
+      mbar_init(&bars[L::early_empty(s)], 1);
     }
     mbar_init(&bars[L::bAccDone], 1);
     fence_barrier_init();
@@ -209,42 +217,42 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       const int rrow = (int)(row_tok0 + r0);
       mbar_expect_tx(&bars[L::bResFull], (kBoxesA + (kHasDp ? kBoxesB : 0)) * L::kResBox);
       for (int b = 0; b < kBoxesA; ++b) {
-        tma_load_4d(smem + L::kResA + b * L::kResBox, &tm_r1, &bars[L::bResFull], b * 64, rrow, hrow, sq.bidx);
+        tma_load_4d(smem + kResA + b * L::kResBox, &tm_r1, &bars[L::bResFull], b * 64, rrow, hrow, sq.bidx);
         if (kHasDp && b < kBoxesB)
-          tma_load_4d(smem + L::kResB + b * L::kResBox, &tm_r2, &bars[L::bResFull], b * 64, rrow, hrow, sq.bidx);
+          tma_load_4d(smem + kResB + b * L::kResBox, &tm_r2, &bars[L::bResFull], b * 64, rrow, hrow, sq.bidx);
       }
       // test hook of the bounded waits: the first early tile never arrives
       const bool drop_first = kKeys ? p.drop_copy == 2 : p.drop_copy == 3;
       int issued_l = 0, issued_e = 0;
       for (int i = 0, hg = 0, cb = 0; i < niter; ++i) {      // hg, cb: i / ncb, i % ncb
-        const int s = i & 1;
+        const int s = i % kLateStages;
         const int hs = kKeys ? hk * p.group + hg : hk;
         const int srow = (int)(col_tok0 + (int64_t)block(cb) * kNB);
         if (++cb == ncb) { cb = 0; ++hg; }
         // the early tile first: it is what the block's first GEMM waits for
         const int es = i % kEarlyStages;
-        if (!mbar_wait(&bars[L::bEarlyEmpty + es], ((uint32_t)(i / kEarlyStages) & 1u) ^ 1u, abort_flag, status, 0x3100)) break;
+        if (!mbar_wait(&bars[L::early_empty(es)], ((uint32_t)(i / kEarlyStages) & 1u) ^ 1u, abort_flag, status, 0x3100)) break;
         if (!(drop_first && i == 0)) {
-          mbar_expect_tx(&bars[L::bEarlyFull + es], kBoxesEarly * L::kStrBox);
+          mbar_expect_tx(&bars[L::early_full(es)], kEarlyStr);
           for (int b = 0; b < kBoxesEarly; ++b)
-            tma_load_4d(smem + kEarlyBase + es * kEarlyStr + b * L::kStrBox, &tm_early, &bars[L::bEarlyFull + es], b * 64, srow,
+            tma_load_4d(smem + kEarlyBase + es * kEarlyStr + b * L::kStrBox, &tm_early, &bars[L::early_full(es)], b * 64, srow,
                         hs, sq.bidx);
           issued_e = i + 1;
         }
-        if (!mbar_wait(&bars[L::bLateEmpty + s], ((uint32_t)(i >> 1) & 1u) ^ 1u, abort_flag, status, 0x3000)) break;
-        mbar_expect_tx(&bars[L::bLateFull + s], kBoxesLate * L::kStrBox);
+        if (!mbar_wait(&bars[L::late_empty(s)], ((uint32_t)(i / kLateStages) & 1u) ^ 1u, abort_flag, status, 0x3000)) break;
+        mbar_expect_tx(&bars[L::late_full(s)], kLateStr);
         for (int b = 0; b < kBoxesLate; ++b)
-          tma_load_4d(smem + L::kLate + s * L::kStr + b * L::kStrBox, &tm_late, &bars[L::bLateFull + s], b * 64, srow, hs,
+          tma_load_4d(smem + kLateBase + s * kLateStr + b * L::kStrBox, &tm_late, &bars[L::late_full(s)], b * 64, srow, hs,
                       sq.bidx);
         issued_l = i + 1;
-        if constexpr (MODE == kWideDQ) {
+        if constexpr (!kKeys) {
           // the next block's K and V towards L2 (their slots free up a block from now; measured: dQ 6 %
           // faster, while for dV and dK, whose streamed Q and dO are shared by fewer CTAs, it did not pay)
           if (i + 1 < niter) {
             const int nrow = (int)(col_tok0 + (int64_t)block(cb) * kNB);
-            for (int b = 0; b < L::kBoxes; ++b) {
+            for (int b = 0; b < kBoxesLate; ++b) {
               tma_prefetch_4d(&tm_late, b * 64, nrow, hk, sq.bidx);
-              tma_prefetch_4d(&tm_early, b * 64, nrow, hk, sq.bidx);
+              if (b < kBoxesEarly) tma_prefetch_4d(&tm_early, b * 64, nrow, hk, sq.bidx);
             }
           }
         }
@@ -252,10 +260,10 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       if (*abort_flag) {
         // Let copies that are still in flight land before the CTA gives its shared memory back.
         mbar_wait_quiet(&bars[L::bResFull], 0, abort_flag);
-        for (int i = max(0, issued_l - 2); i < issued_l; ++i)
-          mbar_wait_quiet(&bars[L::bLateFull + (i & 1)], (uint32_t)(i >> 1) & 1u, abort_flag);
+        for (int i = max(0, issued_l - kLateStages); i < issued_l; ++i)
+          mbar_wait_quiet(&bars[L::late_full(i % kLateStages)], (uint32_t)(i / kLateStages) & 1u, abort_flag);
         for (int i = max(drop_first ? 1 : 0, issued_e - kEarlyStages); i < issued_e; ++i)
-          mbar_wait_quiet(&bars[L::bEarlyFull + i % kEarlyStages], (uint32_t)(i / kEarlyStages) & 1u, abort_flag);
+          mbar_wait_quiet(&bars[L::early_full(i % kEarlyStages)], (uint32_t)(i / kEarlyStages) & 1u, abort_flag);
       }
     }
     __syncwarp();
@@ -266,14 +274,14 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     constexpr uint32_t kIdescS = instr_desc_f16(Fmt<T>::code, 128, kNB, 0, 0);
     const uint32_t idesc_acc = instr_desc_f16(Fmt<T>::code, 128, (uint32_t)((d_out + 15) & ~15), 0, 1);
     const int ksteps_qk = (p.dqk + 15) >> 4, ksteps_vo = (p.dvo + 15) >> 4;
-    const uint64_t r1_km = smem_desc_sw128(smem_u32(smem + L::kResA), 16, 1024);
-    const uint64_t r2_km = smem_desc_sw128(smem_u32(smem + L::kResB), 16, 1024);
-    const uint64_t late_km = smem_desc_sw128(smem_u32(smem + L::kLate), 16, 1024);
-    const uint64_t late_mn = smem_desc_sw128(smem_u32(smem + L::kLate), L::kStrBox, 1024);
+    const uint64_t r1_km = smem_desc_sw128(smem_u32(smem + kResA), 16, 1024);
+    const uint64_t r2_km = smem_desc_sw128(smem_u32(smem + kResB), 16, 1024);
+    const uint64_t late_km = smem_desc_sw128(smem_u32(smem + kLateBase), 16, 1024);
+    const uint64_t late_mn = smem_desc_sw128(smem_u32(smem + kLateBase), L::kStrBox, 1024);
     const uint64_t early_km = smem_desc_sw128(smem_u32(smem + kEarlyBase), 16, 1024);
     const uint64_t early_mn = smem_desc_sw128(smem_u32(smem + kEarlyBase), L::kStrBox, 1024);      // (dKV)
     const uint32_t idesc_dv = instr_desc_f16(Fmt<T>::code, 128, (uint32_t)((p.dvo + 15) & ~15), 0, 1);
-    constexpr uint32_t kStageStep = L::kStr >> 4, kEarlyStep = kEarlyStr >> 4;
+    constexpr uint32_t kStageStep = kLateStr >> 4, kEarlyStep = kEarlyStr >> 4;
     // k-step kk of a K-major tile: head-dim columns 16kk..16kk+15 (box kk / 4, 32 bytes per step inside it)
     auto res_step = [](int kk) { return (uint32_t)(kk >> 2) * (uint32_t)(L::kResBox >> 4) + (uint32_t)(kk & 3) * 2u; };
     auto str_step = [](int kk) { return (uint32_t)(kk >> 2) * (uint32_t)(L::kStrBox >> 4) + (uint32_t)(kk & 3) * 2u; };
@@ -302,7 +310,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
       const uint32_t sb = kGroups == 2 ? s : 0u;      // S' buffer
       if constexpr (MODE == kWideDV) {
         if (i >= kGroups && !wait(L::bSRead + sb, (uint32_t)(kGroups == 2 ? (i >> 1) - 1 : i - 1) & 1u, 0x3800)) return false;
-        if (!wait(L::bEarlyFull + es, epar, 0x3200)) return false;
+        if (!wait(L::early_full(es), epar, 0x3200)) return false;
         tc_fence_after();
         const uint64_t ea = early_km + (uint64_t)(es * kEarlyStep);
         if (elect_one()) {
@@ -310,14 +318,14 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           for (int kk = 0; kk < 16; ++kk)
             if (kk < ksteps_qk) mma_ss(tmem_base + kWColS + sb * 64u, r1_km + res_step(kk), ea + str_step(kk), kIdescS, kk > 0 ? 1u : 0u);
           mma_commit(&bars[L::bSFull + sb]);
-          mma_commit(&bars[L::bEarlyEmpty + es]);
+          mma_commit(&bars[L::early_empty(es)]);
           // the accumulating GEMM of block i-2 has run: its P' buffer can be written again
           mma_commit(&bars[L::bDpFull + s]);
         }
         __syncwarp();
       } else {
         const int valid = valid_rows(i);
-        if (!wait(L::bEarlyFull + es, epar, 0x3400)) return false;
+        if (!wait(L::early_full(es), epar, 0x3400)) return false;
         if (valid < kNB) zero_tail_rows_streamed(smem + kEarlyBase + es * kEarlyStr, valid, lane, kBoxesEarly);
         zero_hidden(i, smem + kEarlyBase + es * kEarlyStr);
         tc_fence_after();
@@ -328,15 +336,16 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
             if (kk < ksteps_vo)
               mma_ss(tmem_base + kColDPW + s * 64u, r2_km + res_step(kk), ea + str_step(kk), kIdescS, kk > 0 ? 1u : 0u);
           mma_commit(&bars[L::bDpFull + s]);
-          if (!kBoth) mma_commit(&bars[L::bEarlyEmpty + es]);      // (dKV: dO feeds dV's product too)
+          if (!kBoth) mma_commit(&bars[L::early_empty(es)]);      // (dKV: dO feeds dV's product too)
         }
         __syncwarp();
         if (i > 0 && !wait(L::bSRead, (uint32_t)(i - 1) & 1u, 0x3800)) return false;
-        if (!wait(L::bLateFull + s, (uint32_t)(i >> 1) & 1u, 0x3300)) return false;
-        if (valid < kNB) zero_tail_rows_streamed(smem + L::kLate + s * L::kStr, valid, lane);
-        zero_hidden(i, smem + L::kLate + s * L::kStr);
+        const uint32_t ls = (uint32_t)(i % kLateStages);
+        if (!wait(L::late_full(ls), (uint32_t)(i / kLateStages) & 1u, 0x3300)) return false;
+        if (valid < kNB) zero_tail_rows_streamed(smem + kLateBase + ls * kLateStr, valid, lane, kBoxesLate);
+        zero_hidden(i, smem + kLateBase + ls * kLateStr);
         tc_fence_after();
-        const uint64_t la = late_km + (uint64_t)(s * kStageStep);
+        const uint64_t la = late_km + (uint64_t)(ls * kStageStep);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 16; ++kk)
@@ -351,13 +360,14 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     auto issue_acc = [&](int i) -> bool {
       const uint32_t s = (uint32_t)i & 1u;
       if (!wait(L::bDsFull + s, (uint32_t)(i >> 1) & 1u, 0x3500)) return false;
+      const uint32_t ls = (uint32_t)(i % kLateStages);
       if constexpr (MODE == kWideDV) {
-        if (!wait(L::bLateFull + s, (uint32_t)(i >> 1) & 1u, 0x3600)) return false;
+        if (!wait(L::late_full(ls), (uint32_t)(i / kLateStages) & 1u, 0x3600)) return false;
         const int valid = valid_rows(i);
-        if (valid < kNB) zero_tail_rows_streamed(smem + L::kLate + s * L::kStr, valid, lane);
+        if (valid < kNB) zero_tail_rows_streamed(smem + kLateBase + ls * kLateStr, valid, lane);
       }
       tc_fence_after();
-      const uint64_t lb = late_mn + (uint64_t)(s * kStageStep);
+      const uint64_t lb = late_mn + (uint64_t)(ls * kStageStep);
       const uint32_t a_col = tmem_base + kColDPW + s * 64u;
       const uint32_t first = i > 0 ? 1u : 0u;
       if (elect_one()) {
@@ -365,13 +375,13 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         for (int kk = 0; kk < kNB / 16; ++kk)
           mma_ts(tmem_base + kColAcc, a_col + split_a_col(kk), lb + (uint32_t)kk * (2048u >> 4), idesc_acc, kk > 0 ? 1u : first);
         if constexpr (kBoth) {
-          const uint64_t eb = early_mn + (uint64_t)(s * kEarlyStep);
+          const uint64_t eb = early_mn + (uint64_t)((uint32_t)(i % kEarlyStages) * kEarlyStep);
 #pragma unroll
           for (int kk = 0; kk < kNB / 16; ++kk)
             mma_ts(tmem_base + kWColDV, a_col + 16u + split_a_col(kk), eb + (uint32_t)kk * (2048u >> 4), idesc_dv, kk > 0 ? 1u : first);
-          mma_commit(&bars[L::bEarlyEmpty + s]);
+          mma_commit(&bars[L::early_empty(i % kEarlyStages)]);
         }
-        mma_commit(&bars[L::bLateEmpty + s]);
+        mma_commit(&bars[L::late_empty(ls)]);
         if (i + 1 == niter) mma_commit(&bars[L::bAccDone]);
       }
       __syncwarp();
@@ -697,7 +707,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     if (ok) ok = mbar_wait(&bars[L::bAccDone], 0, abort_flag, status, 0x3E00);
     if (ok) {
       tc_fence_after();
-      const uint32_t stage = smem_u32(smem + L::kResA);
+      const uint32_t stage = smem_u32(smem + kResA);      // (64 KB, all of them of tiles that are done with)
       const int nrows = kKeys && (FEAT & kSinks) != 0 && chunk > 0 ? 0 : min(kBlk, rows_total - r0);
       T* dst = reinterpret_cast<T*>(outv.ptr) + (int64_t)sq.bidx * outv.s[0] + (int64_t)hrow * outv.s[1] +
                (row_tok0 + r0) * outv.s[2];
@@ -745,8 +755,8 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
 
 #include "sm100_bwd_dk_db.cuh"
 
-// Whether dK and dV are formed in one launch.
-inline bool wide_both(const Params& p) { return p.dqk <= 192 && p.dvo <= 128 && features(p) == kPlain; }
+// Whether the narrow tiles do: dK and dV in one launch, and dQ.
+inline bool wide_narrow(const Params& p) { return p.dqk <= 192 && p.dvo <= 128 && features(p) == kPlain; }
 
 // which: 1 dV and dK (two launches), 2 dQ(+dBias); p.dk_from_db: 1 dV, 2 dQ and dBias, then dK from dBias
 template <typename T>
@@ -767,7 +777,7 @@ cudaError_t launch_bwd_wide_T(int which, const Params& p, cudaStream_t st) {
       return cudaErrorInvalidValue;
   }
   static std::atomic<unsigned int*> status_of[64];
-  static std::atomic<bool> attr_set[64][16];
+  static std::atomic<bool> attr_set[64][18];
   const int feat = features(p);
   int dev = 0;
   cudaError_t e = host().get_device(&dev);
@@ -793,14 +803,11 @@ cudaError_t launch_bwd_wide_T(int which, const Params& p, cudaStream_t st) {
        sm100_bwd_wide_kernel<T, 1, kSinks>},
       {sm100_bwd_wide_kernel<T, 2, kPlain>, sm100_bwd_wide_kernel<T, 2, kBias>, sm100_bwd_wide_kernel<T, 2, kDropout>, sm100_bwd_wide_kernel<T, 2, kAll>,
        sm100_bwd_wide_kernel<T, 2, kSinks>}};
-  if (which == 1 && wide_both(p)) {
-    auto kern = sm100_bwd_wide_kernel<T, kWideDKV, kPlain>;
-    static std::atomic<bool> both_set[64];
-    if (pretend || !both_set[dev].load(std::memory_order_acquire)) {
-      if ((e = host().func_set_smem(reinterpret_cast<const void*>(kern), L::kDynamic)) != cudaSuccess) return e;
-      if (!pretend) both_set[dev].store(true, std::memory_order_release);
-    }
-    e = launch_kernel(kern, dim3((p.max_sk + kBlk - 1) / kBlk, p.hk, p.batch), dim3(wide_threads(kWideDKV, kPlain)), L::kDynamic, st, p, k128, v128, q64, do64, status);
+  if (wide_narrow(p)) {
+    const Kernel kern = which == 1 ? sm100_bwd_wide_kernel<T, kWideDKV, kPlain> : sm100_bwd_wide_kernel<T, kWideDQN, kPlain>;
+    if ((e = set_smem(15 + which, reinterpret_cast<const void*>(kern))) != cudaSuccess) return e;
+    e = which == 1 ? launch_kernel(kern, dim3((p.max_sk + kBlk - 1) / kBlk, p.hk, p.batch), dim3(wide_threads(kWideDKV, kPlain)), L::kDynamic, st, p, k128, v128, q64, do64, status)
+                   : launch_kernel(kern, dim3((p.max_sq + kBlk - 1) / kBlk, p.hq, p.batch), dim3(wide_threads(kWideDQN, kPlain)), L::kDynamic, st, p, q128, do128, k64, v64, status);
   } else if (which == 1) {
     const Kernel kern_dv = kKernels[kWideDV][feat], kern_dk = kKernels[kWideDK][feat];
     if ((e = set_smem(feat == kSinks ? 13 + kWideDV : 4 * kWideDV + feat, reinterpret_cast<const void*>(kern_dv))) != cudaSuccess) return e;
