@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
     const int octets = p.box / 8;
     const bool leads = lane < 16 && lane % octets == 0;
     int vi = 0, ti = 0, units = 0;      // blocks, tails and units requested
-    bool stop = false;
+    bool stop = false, dropped = false;
     while (!stop && run.next(p)) {
       if (Rows(p, w, run.chunk).n == 0) continue;
       const int first = run.first, last = run.last;
@@ -183,7 +183,9 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
           if (stop) break;
           const int s = vi % L::kSlots;
           if (!__all_sync(0xffffffffu, mbar_wait(&bars[L::bEmpty + s], ((uint32_t)(vi / L::kSlots) & 1u) ^ 1u, abort_flag, p.status, 0x7010))) { stop = true; break; }
-          if (!(p.drop_copy == 1 && vi == 0 && blockIdx.x == 0)) {      // (test hook: the first block never arrives)
+          const bool drop = p.drop_copy == 1 && run.z == 0 && run.chunk == 0 && i == 0 && b == 0;      // (test hook: the first block never arrives)
+          dropped |= drop;
+          if (!drop) {
             uint8_t* dst = smem + L::kRing + s * kBlock;
             if (lane == 0) mbar_expect_tx(&bars[L::bFull + s], kBlock);
             __syncwarp();
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(LatentSmem<NR>::kThreads, 1) paged_latent_kern
     }
     __syncwarp();
     if (*abort_flag && lane == 0) {      // copies that are still in flight land before the memory is used again
-      for (int i = max(p.drop_copy == 1 && blockIdx.x == 0 ? 1 : 0, vi - L::kSlots); i < vi; ++i)
+      for (int i = max(dropped ? 1 : 0, vi - L::kSlots); i < vi; ++i)
         mbar_wait_quiet(&bars[L::bFull + i % L::kSlots], (uint32_t)(i / L::kSlots) & 1u, abort_flag);
       if (units > 0) mbar_wait_quiet(&bars[L::bQ], (uint32_t)(units - 1) & 1u, abort_flag);
       if (ti > 0) mbar_wait_quiet(&bars[L::bTailFull], (uint32_t)(ti - 1) & 1u, abort_flag);

@@ -89,7 +89,7 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
     const int octets = p.box / 8, group = lane / octets;      // a box's eights of keys
     const uint32_t mine = lane < 8 ? ((octets == 8 ? 0xffu : (1u << octets) - 1u) << (group * octets)) & 0xffu : 0u;
     int s = 0, ph = 1, issued = 0;
-    bool stop = false;
+    bool stop = false, dropped = false;
     while (!stop && run.next(p)) {
       if (Rows(p, w, run.chunk).n == 0) continue;
       const int first = run.first, last = run.last, hk = run.hk;
@@ -111,7 +111,9 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
         const int slot = (w.tile(i) * kTileKeys + lane * 8) % p.page;
         if (i + 1 < last) id = look(i + 1, seen);
         if (!__all_sync(0xffffffffu, mbar_wait(&bars[L::bEmpty + s], (uint32_t)ph, abort_flag, p.status, 0x6000))) { stop = true; break; }
-        if (!(p.drop_copy == 1 && issued == 0 && blockIdx.x == 0)) {      // (test hook: the first tile never arrives)
+        const bool drop = p.drop_copy == 1 && run.z == 0 && run.hk == 0 && run.chunk == 0 && i == 0;      // (test hook: the first tile never arrives)
+        dropped |= drop;
+        if (!drop) {
           uint8_t* kt = smem + L::kRing + s * (2 * L::kTile);
           if (lane == 0) {
             valid[s] = bits;
@@ -132,7 +134,7 @@ paged_split_kernel(const __grid_constant__ PagedAttn p, const __grid_constant__ 
     }
     __syncwarp();
     if (*abort_flag && lane == 0) {      // copies that are still in flight land before the memory is used again
-      for (int i = max(p.drop_copy == 1 && blockIdx.x == 0 ? 1 : 0, issued - kStages); i < issued; ++i)
+      for (int i = max(dropped ? 1 : 0, issued - kStages); i < issued; ++i)
         mbar_wait_quiet(&bars[L::bFull + i % kStages], (uint32_t)(i / kStages) & 1u, abort_flag);
     }
     return;

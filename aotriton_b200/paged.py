@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import cabi
 from .autograd import _FLOATS, _check, _native, _on_its_device, _unit_rows
@@ -33,6 +34,8 @@ class BlockTables(NamedTuple):
 def _no_gradient(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or on detached tensors")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode gradient")
 
 
 def _int32(t, dim, device):
