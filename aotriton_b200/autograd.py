@@ -43,7 +43,7 @@ except ImportError as e:      # (built where torch was missing, had no CUDA or w
             return None
 
         @staticmethod
-        def join_columns(*args):
+        def latent_attend(*args):
             return None
 
         @staticmethod
@@ -712,83 +712,131 @@ def dropout(x, dropout_p, residual=None, philox_seed=DEFAULT_PHILOX_SEED, philox
     return _apply(_Dropout, x, residual, float(dropout_p), seed, offset)
 
 
-class _JoinColumns(torch.autograd.Function):
-    """(k, shared) head by head: keys whose last columns all heads share."""
+def _latent_problem(cu_q, cu_k, max_q, max_k, causal_type, window_left, window_right, sm_scale):
+    kw = dict(sm_scale=sm_scale, causal_type=causal_type, window_left=window_left, window_right=window_right)
+    if cu_q is not None:
+        kw.update(cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=max_q, max_seqlen_k=max_k, varlen_type=cabi.VARLEN_COMPACT)
+    return kw
+
+
+class _LatentAttention(torch.autograd.Function):
+    """Attention over keys whose last columns all heads share.  (Of packed tokens, rows behind the last sequence are zero, in the gradients too.)"""
 
     @staticmethod
     @_on_its_device
-    def forward(ctx, k, shared):
-        b, h, s, dn = k.shape
-        joined = torch.empty((b, s, h, dn + shared.shape[3]), device=k.device, dtype=k.dtype).transpose(1, 2)
+    def forward(ctx, q, k, shared, v, cu_q, cu_k, max_q, max_k, causal_type, window_left, window_right, sm_scale, return_lse):
+        b, hq, sq, _ = q.shape
+        joined = torch.empty((k.shape[0], k.shape[2], k.shape[1], q.shape[3]), device=k.device, dtype=k.dtype).transpose(1, 2)
+        if cu_q is not None:      # (1, H, tokens, D) views of (tokens, H, D) storage
+            o = torch.zeros((1, sq, hq, v.shape[3]), device=q.device, dtype=q.dtype).transpose(1, 2)
+            lse = torch.empty((hq, sq), device=q.device, dtype=torch.float32)
+        else:
+            o = torch.empty((b, hq, sq, v.shape[3]), device=q.device, dtype=q.dtype)
+            lse = torch.empty((b * hq, sq), device=q.device, dtype=torch.float32)
+        stream = torch.cuda.current_stream(q.device).cuda_stream
         if joined.numel():
-            stream = torch.cuda.current_stream(k.device).cuda_stream
             _check(hipError_t(cabi.shared_columns("join", k, shared, joined, stream=stream)), "join_columns")
-        ctx.width = dn
-        return joined
+        if not q.numel() or not joined.numel():      # nobody, or nothing to see
+            o.zero_()
+            lse.fill_(float("inf"))
+        else:
+            kw = _latent_problem(cu_q, cu_k, max_q, max_k, causal_type, window_left, window_right, sm_scale)
+            _check(hipError_t(cabi.attn_fwd(q, joined, v, o, lse, stream=stream, **kw)), "latent_attention")
+        ctx.save_for_backward(q, joined, v, o, lse, cu_q, cu_k)
+        ctx.args = (shared.shape[3], max_q, max_k, causal_type, window_left, window_right, sm_scale)
+        ctx.mark_non_differentiable(lse)
+        return (o, lse) if return_lse else o
 
     @staticmethod
-    def backward(ctx, grad):
-        return grad[..., :ctx.width], _SumColumns.apply(grad, ctx.width) if ctx.needs_input_grad[1] else None
+    def backward(ctx, do, *unused):
+        q, joined, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        return _latent_grad(q, joined, v, o, do, lse, cu_q, cu_k, *ctx.args) + (None,) * 9
 
 
-class _SumColumns(torch.autograd.Function):
-    """The sum over the heads of the columns from `width` on."""
+class _LatentAttentionGrad(torch.autograd.Function):
+    """(dq, dk, dshared, dv): an operator of its own, which knows that it has no derivative."""
 
     @staticmethod
     @_on_its_device
-    def forward(ctx, grad, width):
-        grad = _unit_rows(grad)
-        b, h, s, d = grad.shape
-        ctx.args = (h, width)
-        shared = torch.empty((b, 1, s, d - width), device=grad.device, dtype=grad.dtype)
-        if shared.numel():
-            stream = torch.cuda.current_stream(grad.device).cuda_stream
-            _check(hipError_t(cabi.shared_columns("sum", None, shared, grad, stream=stream)), "sum_columns")
-        return shared
+    def forward(ctx, q, joined, v, o, do, lse, cu_q, cu_k, columns, max_q, max_k, causal_type, window_left, window_right, sm_scale):
+        like = torch.empty_like if cu_q is None else torch.zeros_like
+        dq, dk, dv = like(q), like(joined), like(v)
+        shared = torch.empty((joined.shape[0], 1, joined.shape[2], columns), device=q.device, dtype=q.dtype)
+        if not q.numel() or not joined.numel():
+            return dq.zero_(), dk.zero_()[..., :-columns], shared.zero_(), dv.zero_()
+        delta = torch.empty_like(lse)
+        kw = _latent_problem(cu_q, cu_k, max_q, max_k, causal_type, window_left, window_right, sm_scale)
+        args = (q, joined, v, o, _unit_rows(do), dq, dk, dv, lse, delta)
+        stream = torch.cuda.current_stream(q.device).cuda_stream
+        need = cabi.attn_bwd_shared_workspace(*args, columns, stream=stream, **kw)
+        if need < 0:
+            _check(hipError_t(-need), "latent_attention backward")
+        workspace = (torch.empty if cu_q is None else torch.zeros)([need], device=q.device, dtype=torch.float32) if need else None
+        _check(hipError_t(cabi.attn_bwd_shared(*args, shared, workspace=workspace, stream=stream, **kw)), "latent_attention backward")
+        _native.note_bwd_family()
+        return dq, dk[..., :-columns], shared, dv
 
     @staticmethod
-    def backward(ctx, grad):
-        h, width = ctx.args
-        return torch.nn.functional.pad(grad.expand(-1, h, -1, -1), (width, 0)), None
+    def backward(ctx, *grads):
+        raise RuntimeError("latent_attention has no second derivative")
 
 
-def _python_sum_columns(grad, width):
-    """The gradient of a native call whose own gradient or modes are not ordinary ones (csrc/torch_ops.cc)."""
-    return _SumColumns.apply(grad, width)
+def _latent_grad(q, joined, v, o, do, lse, cu_q, cu_k, columns, *numbers):
+    """The gradients, of a Python call or of a native one whose own gradient or modes are not ordinary ones (csrc/torch_ops.cc).  What a saved-tensor hook handed
+    back is looked at first, as in _sink_grad."""
+    bad = [t for t in (q, joined, v, o) if t.dim() != 4 or t.dtype != do.dtype or t.device != do.device or (t.shape[3] > 1 and t.stride(3) != 1)]
+    bad += [t for t in (cu_q, cu_k) if t is not None and (t.dtype != torch.int32 or t.device != do.device or t.shape != cu_q.shape or not t.is_contiguous())]
+    if (bad or lse.dim() != 2 or lse.dtype != torch.float32 or lse.device != do.device or not lse.is_contiguous()
+            or lse.numel() != q.shape[0] * q.shape[1] * q.shape[2] or not o.shape == do.shape == (*q.shape[:3], v.shape[3])
+            or joined.shape[:3] != v.shape[:3] or joined.shape[0] != q.shape[0] or joined.shape[3] != q.shape[3] or columns >= joined.shape[3]
+            or joined.shape[1] and q.shape[1] % joined.shape[1]):
+        raise ValueError("latent_attention: what was saved for the backward came back with other types, sizes or devices")
+    return _LatentAttentionGrad.apply(q, joined, v, o, do, lse, cu_q, cu_k, columns, *numbers)
 
 
-_native.set_python_function("sum_columns", _python_sum_columns)
+_native.set_python_function("latent_attention", _latent_grad)
 
 
-def _join_shared(q, k, k_shared, v, what):
+def _latent_attention(q, k, k_shared, v, cu_q, cu_k, max_q, max_k, causal, sm_scale, return_lse, what):
+    causal_type, left, right = flash.translate_causal(causal)
+    sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
+    if not torch.compiler.is_compiling():
+        r = _native.latent_attend(q, k, k_shared, v, cu_q, cu_k, max_q, max_k, causal_type, left, right, sm_scale, return_lse)
+        if r is not None:
+            return r
     for t in (q, k, k_shared, v):
         if t.dim() != 4 or t.dtype not in _FLOATS or not t.is_cuda or t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"{what}: q, k, k_shared and v are (batch, heads, tokens, dim) CUDA tensors of one device and type, fp32, fp16 or bf16")
     if (k_shared.shape[0], *k_shared.shape[1:3]) != (k.shape[0], 1, k.shape[2]) or v.shape[:3] != k.shape[:3] or k.shape[0] != q.shape[0]:
         raise ValueError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(k_shared.shape)}, {tuple(v.shape)} do not go together")
-    if not k.shape[1] or q.shape[1] % k.shape[1] or not k.shape[3] or not k_shared.shape[3] or q.shape[3] != k.shape[3] + k_shared.shape[3]:
+    if not q.shape[1] or not k.shape[1] or q.shape[1] % k.shape[1] or not k.shape[3] or not k_shared.shape[3] or q.shape[3] != k.shape[3] + k_shared.shape[3]:
         raise ValueError(f"{what}: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(k_shared.shape)} do not go together: a query is as wide as a head's key and the "
                          "shared columns")
     if q.shape[3] > 512 or not 1 <= v.shape[3] <= 512:
         raise ValueError(f"{what}: head dims from 1 to 512 are supported")
-    if not torch.compiler.is_compiling():
-        r = _native.join_columns(k, k_shared)
-        if r is not None:
-            return r
-    return _apply(_JoinColumns, _unit_rows(k), _unit_rows(k_shared))
+    if cu_q is not None:
+        for t in (cu_q, cu_k):
+            if t.dim() != 1 or t.numel() < 2 or t.numel() != cu_q.numel() or t.dtype != torch.int32 or t.device != q.device or t.stride(0) != 1:
+                raise ValueError(f"{what}: the cumulative lengths are contiguous int32 tensors on q's device, one entry more than there are sequences")
+        if q.shape[0] != 1:
+            raise ValueError(f"{what}: packed tokens are (1, heads, tokens, dim)")
+        if not 0 <= max_q <= q.shape[2] or not 0 <= max_k <= k.shape[2]:
+            raise ValueError(f"{what}: longest sequences {max_q} and {max_k} do not fit {q.shape[2]} and {k.shape[2]} tokens")
+        max_q, max_k = max(max_q, 1), max(max_k, 1)
+    q, k, k_shared, v = map(_unit_rows, (q, k, k_shared, v))
+    return _apply(_LatentAttention, q, k, k_shared, v, cu_q, cu_k, max_q, max_k, causal_type, left, right, float(sm_scale), bool(return_lse))
 
 
 def latent_attention(q, k, k_shared, v, causal=False, sm_scale=None, return_lse=False):
     """Latent attention in its expanded form, for prompts and training: `attention` whose heads' keys are their own columns, expanded from a token's latent
     vector, followed by columns that all heads share (its position columns).  q: (B, H, Sq, dn + dr), k: (B, Hk, Sk, dn), k_shared: (B, 1, Sk, dr),
     v: (B, Hk, Sk, dv), of any strides; causal as for `attention`; sm_scale: (dn + dr) ** -0.5 where not given.  The gradient of k_shared is summed over the heads in fp32, in
-    their order.  paged.paged_latent_attention decodes from the latent vectors themselves."""
-    joined = _join_shared(q, k, k_shared, v, "latent_attention")
-    return attention(_unit_rows(q), joined, _unit_rows(v), causal=causal, sm_scale=sm_scale, return_lse=return_lse)
+    their order, and rounded once (where the general kernels take 16-bit tensors, each head's share is rounded before).  The log-sum-exp has no gradient.
+    paged.paged_latent_attention decodes from the latent vectors themselves."""
+    return _latent_attention(q, k, k_shared, v, None, None, 0, 0, causal, sm_scale, return_lse, "latent_attention")
 
 
 def varlen_latent_attention(q, k, k_shared, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=False, sm_scale=None, return_lse=False):
-    """latent_attention over token-packed sequences, (1, H, tokens, dim) tensors, as varlen_attention has them."""
-    joined = _join_shared(q, k, k_shared, v, "varlen_latent_attention")
-    return varlen_attention(_unit_rows(q), joined, _unit_rows(v), cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal=causal, sm_scale=sm_scale,
-                            return_lse=return_lse)
+    """latent_attention over token-packed sequences, (1, H, tokens, dim) tensors, as varlen_attention has them.  Rows behind the last sequence are zero, in the
+    gradients too; the log-sum-exp, (H, tokens), is laid out for sequences that fill the tensors.  max_seqlen_q and _k are at least the longest lengths."""
+    return _latent_attention(q, k, k_shared, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal, sm_scale, return_lse, "varlen_latent_attention")

@@ -25,7 +25,8 @@ SYMBOLS = [
     "ab200_debug_simulate_encoded_softmax", "ab200_sink_attn_fwd", "ab200_sink_attn_bwd",
     "ab200_sink_attn_bwd_workspace", "ab200_relative_bias_fwd", "ab200_relative_bias_bwd",
     "ab200_relative_bias_workspace", "ab200_dropout", "ab200_block_tables", "ab200_paged_write", "ab200_paged_attn",
-    "ab200_paged_attn_workspace", "ab200_join_columns", "ab200_sum_columns", "ab200_check_gpu", "ab200_multiprocessor_count",
+    "ab200_paged_attn_workspace", "ab200_join_columns", "ab200_sum_columns", "ab200_attn_bwd_shared", "ab200_attn_bwd_shared_workspace",
+    "ab200_check_gpu", "ab200_multiprocessor_count",
     "ab200_set_kernel_family", "ab200_select_variant", "ab200_last_fwd_family", "ab200_last_bwd_family",
     "ab200_kernel_status", "ab200_stream_check", "ab200_debug_bounded_wait_test", "ab200_debug_keep_tiles",
     "ab200_debug_dk_from_dbias", "ab200_debug_split_keys",
@@ -146,6 +147,9 @@ def lib() -> C.CDLL:
         L.ab200_paged_attn.argtypes = L.ab200_paged_attn_workspace.argtypes = [C.POINTER(PagedAttnArgs), C.c_void_p]
         L.ab200_paged_attn_workspace.restype = C.c_int64
         L.ab200_join_columns.argtypes = L.ab200_sum_columns.argtypes = [C.POINTER(SharedColumnsArgs), C.c_void_p]
+        L.ab200_attn_bwd_shared.argtypes = [C.POINTER(BwdArgs), C.c_int32, C.POINTER(View4), C.c_void_p, C.c_uint64, C.c_void_p]
+        L.ab200_attn_bwd_shared_workspace.argtypes = [C.POINTER(BwdArgs), C.c_int32, C.c_void_p]
+        L.ab200_attn_bwd_shared_workspace.restype = C.c_int64
         L.ab200_check_gpu.argtypes = [C.c_void_p]
         L.ab200_multiprocessor_count.argtypes = [C.c_void_p]
         L.ab200_select_variant.argtypes = [C.c_int] * 5
@@ -394,3 +398,16 @@ def shared_columns(entry, k, shared, joined, *, stream=None) -> int:
     a = SharedColumnsArgs()
     a.dtype, a.k, a.shared, a.joined = _torch_dtype_code(joined), view4(k), view4(shared), view4(joined)
     return getattr(lib(), f"ab200_{entry}_columns")(C.byref(a), stream if stream is not None else current_stream_handle())
+
+
+def attn_bwd_shared_workspace(q, k, v, out, dout, dq, dk, dv, lse, delta, columns, *, stream=None, **kw) -> int:
+    """Floats the call needs; negative: an error code."""
+    a = make_bwd_args(q, k, v, out, dout, dq, dk, dv, lse, delta, **kw)
+    return lib().ab200_attn_bwd_shared_workspace(C.byref(a), columns, stream if stream is not None else current_stream_handle())
+
+
+def attn_bwd_shared(q, k, v, out, dout, dq, dk, dv, lse, delta, shared, *, workspace=None, stream=None, **kw) -> int:
+    """attn_bwd for joined keys; `shared`, (B, 1, S, columns), gets the sum of dk's last columns over the heads."""
+    a, s = make_bwd_args(q, k, v, out, dout, dq, dk, dv, lse, delta, **kw), view4(shared)
+    return lib().ab200_attn_bwd_shared(C.byref(a), shared.shape[3], C.byref(s), _ptr(workspace), workspace.numel() if workspace is not None else 0,
+                                       stream if stream is not None else current_stream_handle())

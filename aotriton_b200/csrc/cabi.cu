@@ -668,10 +668,11 @@ int ab200_bwd_postprocess(const ab200_attn_bwd_args* a, void* stream) {
   return (int)launch_postprocess(a->prob.dtype, dq, a->dq_acc, a->prob.sm_scale, st);
 }
 
-int ab200_attn_bwd(const ab200_attn_bwd_args* a, void* stream) {
+// tail: dK's columns from tail_from on in 32 bits (Params::dk_tail), or null.
+static int attn_bwd(const ab200_attn_bwd_args* a, float* tail, int tail_from, void* stream) {
   if (a == nullptr) return kErrInvalidValue;
   if (!a->dq.ptr || !a->dk.ptr || !a->dv.ptr) return kErrInvalidValue;
-  if (a->dq_acc != nullptr && ab200_bwd_uses_dq_acc(a, stream)) {
+  if (tail == nullptr && a->dq_acc != nullptr && ab200_bwd_uses_dq_acc(a, stream)) {
     if (int e = ab200_bwd_preprocess(a, stream)) return e;
     if (int e = ab200_bwd_fused(a, stream)) return e;
     return ab200_bwd_postprocess(a, stream);
@@ -700,6 +701,8 @@ int ab200_attn_bwd(const ab200_attn_bwd_args* a, void* stream) {
   if (tc) {
     keep_share_setup(p);
     p.dk_from_db = dk_from_db_possible(p);
+    p.dk_tail = tail;
+    p.dk_tail_from = tail_from;
     if ((e = launch_sm100_bwd_dkdv(dtype, p, st)) != cudaSuccess) return (int)e;
     return (int)launch_sm100_bwd_dq(dtype, p, st);
   }
@@ -709,6 +712,8 @@ int ab200_attn_bwd(const ab200_attn_bwd_args* a, void* stream) {
   if ((e = launch_general(1, dtype, p, st)) != cudaSuccess) return (int)e;
   return (int)launch_general(2, dtype, p, st);
 }
+
+int ab200_attn_bwd(const ab200_attn_bwd_args* a, void* stream) { return attn_bwd(a, nullptr, 0, stream); }
 
 // Whether ab200_attn_bwd would run the two-kernel tcgen05 backward, the device apart: 1, 0, or a negative error.
 static int two_kernel_bwd(const ab200_attn_bwd_args* a, const Params& p) {
@@ -1134,6 +1139,48 @@ int ab200_sum_columns(const ab200_shared_columns_args* a, void* stream) {
   if (s.shared.n[0] == 0 || s.shared.n[2] == 0) return 0;
   DeviceGuard guard(st);
   return (int)launch_sum_columns(a->dtype, s, st);
+}
+
+// The backward for joined keys, with the shared columns' gradient.  Floats of dK's last columns in 32 bits; 0 where the kernels that take the call have none
+// (fp32 tensors, whose dK has 32 bits already; bias, dropout; head dims that the general kernels take).
+static int64_t plan_bwd_shared(const ab200_attn_bwd_args* a, int columns, Params& p) {
+  if (int e = fill_bwd(a, p, true)) return -e;
+  if (columns < 1 || columns >= p.dqk) return -kErrInvalidValue;
+  const int sel = ab200_select_variant(kOpBwd, a->prob.dtype, p.dqk, p.dvo, family_flags(g_family) | (sm100_bwd_supported(a->prob.dtype, p) ? AB200_SELECT_ALIGNED : 0));
+  if (sel < 0) return sel;
+  if ((sel & 0xff) < kVarTcgen05 || features(p) != kPlain || columns % 4 != 0) return 0;
+  for (int i = 0; i < 3; ++i)
+    if (p.k.n[i] < 0 || p.k.n[i] > INT32_MAX) return -kErrInvalidValue;
+  return p.k.n[0] * p.hk * p.k.n[2] * columns;
+}
+
+int64_t ab200_attn_bwd_shared_workspace(const ab200_attn_bwd_args* a, int32_t columns, void* stream) {
+  Params p{};
+  const int64_t floats = plan_bwd_shared(a, columns, p);
+  if (floats < 0) return floats;
+  if (int e = check_device(static_cast<cudaStream_t>(stream))) return -e;
+  return floats;
+}
+
+int ab200_attn_bwd_shared(const ab200_attn_bwd_args* a, int32_t columns, const ab200_view4* shared, float* workspace, uint64_t workspace_floats, void* stream) {
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Params p{};
+  const int64_t floats = plan_bwd_shared(a, columns, p);
+  if (floats < 0) return (int)-floats;
+  if (shared == nullptr || shared->size[3] != columns) return kErrInvalidValue;
+  if (floats > 0 && (workspace == nullptr || workspace_floats < (uint64_t)floats || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)) return kErrInvalidValue;
+  ab200_shared_columns_args c{};
+  c.dtype = a->prob.dtype;
+  c.shared = *shared;
+  c.joined = a->dk;
+  for (int i = 0; i < 3; ++i) c.joined.size[i] = a->k.size[i];
+  c.joined.size[3] = p.dqk;
+  SharedColumns s{};
+  if (int e = fill_shared_columns(&c, s, true)) return e;
+  if (int e = attn_bwd(a, floats > 0 ? workspace : nullptr, p.dqk - columns, stream)) return e;
+  if (s.shared.n[0] == 0 || s.shared.n[2] == 0) return 0;
+  DeviceGuard guard(st);
+  return (int)(floats > 0 ? launch_sum_tail(a->prob.dtype, s.shared, workspace, p.hk, st) : launch_sum_columns(a->prob.dtype, s, st));
 }
 
 // --- HIP-named runtime helpers used by the Python tests of the reference

@@ -64,6 +64,10 @@ struct Params {
   int32_t packed_tiles;           // token-packed: the grid counts row tiles of all sequences instead of max_sq's per sequence
   int32_t hw_order;               // the forward's CTAs in the hardware's order: a grid of 2^24 or more, beyond quick_div
   unsigned int* ticket;           // dK/dV's ticket counter, zeroed by the preprocess kernel of the same call (null: by the launch itself)
+  // dK's columns from dk_tail_from on once more, in 32 bits, (batch, kv head, token, columns): keys whose last columns all heads share sum them over the heads
+  // (null: not wanted; tcgen05 kernels with neither bias nor dropout alone)
+  float* dk_tail;
+  int32_t dk_tail_from;
   int32_t dk_from_db;             // dK = sm_scale * dBias^T Q, after the dQ kernel has written dBias (sm100_bwd_dk_db.cuh)
   int32_t keep_tiles, keep_shift; // keep bits of the first keep_tiles 32-key tiles pass through dQ's rows (0: none), or, with
                                   // keep_shift kKeepInDbias, through dBias; see KeepShare

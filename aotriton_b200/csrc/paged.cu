@@ -457,6 +457,22 @@ __global__ void __launch_bounds__(256) sum_columns_kernel(const __grid_constant_
   }
 }
 
+// ... from columns in 32 bits, heads * rows * dr of them a batch element.
+template <typename T>
+__global__ void __launch_bounds__(256) sum_tail_kernel(const __grid_constant__ View4 shared, const float* __restrict__ tail, int heads) {
+  wait_for_earlier_grids();
+  const int dr = (int)shared.n[3];
+  const int64_t a_head = shared.n[2] * dr, total = shared.n[0] * a_head;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const int64_t b = i / a_head, at = i - b * a_head, s = at / dr;
+    const float* src = tail + b * heads * a_head + at;
+    float sum = 0.f;
+#pragma unroll 8
+    for (int h = 0; h < heads; ++h) sum += src[h * a_head];
+    reinterpret_cast<T*>(shared.ptr)[b * shared.s[0] + s * shared.s[2] + (at - s * dr)] = from_f32<T>(sum);
+  }
+}
+
 unsigned grid_for(int64_t items, int64_t per) { return (unsigned)std::min<int64_t>((items + per - 1) / per, 0x7fffffff); }
 
 template <typename... K, typename... A>
@@ -565,6 +581,11 @@ cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t 
   if (vec) return launch_counted(join_columns_kernel<uint4>, grid, kColumnThreads, 0, st, a, elt);
   if (elt == 4) return launch_counted(join_columns_kernel<uint32_t>, grid, kColumnThreads, 0, st, a, elt);
   return launch_counted(join_columns_kernel<uint16_t>, grid, kColumnThreads, 0, st, a, elt);
+}
+
+cudaError_t launch_sum_tail(int dtype, const View4& shared, const float* tail, int heads, cudaStream_t st) {
+  const dim3 grid(grid_for(shared.n[0] * shared.n[2] * shared.n[3], 256));
+  return with_type(dtype, [&]<typename T>() { return launch_counted(sum_tail_kernel<T>, grid, 256, 0, st, shared, tail, heads); });
 }
 
 cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st) {

@@ -74,4 +74,7 @@ unsigned int sm100_paged_status(bool reset);
 cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t st);
 cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st);      // shared = sum over heads of out's last columns
 
+// ... from dK's last columns in 32 bits, (batch, kv heads, tokens, columns).
+cudaError_t launch_sum_tail(int dtype, const View4& shared, const float* tail, int heads, cudaStream_t st);
+
 }  // namespace ab200

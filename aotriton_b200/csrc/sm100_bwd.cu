@@ -151,6 +151,22 @@ __device__ void zero_rows(const View4& v, int b, int h, int64_t tok0, int row0, 
   }
 }
 
+// Columns d0..d0 + 31 of row n of dK towards dk_tail: those that belong there.
+__device__ __forceinline__ void keep_tail(const Params& p, const Seq& sq, int hk, int n, int d0, const float (&v)[32], float scale) {
+  if (n >= sq.sk) return;
+  const int width = p.dqk - p.dk_tail_from;
+  float* dst = p.dk_tail + (((int64_t)sq.bidx * p.hk + hk) * p.k.n[2] + sq.k0 + n) * width - p.dk_tail_from + d0;
+#pragma unroll
+  for (int c = 0; c < 32; c += 4)
+    if (d0 + c >= p.dk_tail_from && d0 + c < p.dqk)
+      *reinterpret_cast<float4*>(dst + c) = make_float4(v[c] * scale, v[c + 1] * scale, v[c + 2] * scale, v[c + 3] * scale);
+}
+__device__ __forceinline__ void zero_tail(const Params& p, const Seq& sq, int hk, int n) {
+  const int width = p.dqk - p.dk_tail_from;
+  float* dst = p.dk_tail + (((int64_t)sq.bidx * p.hk + hk) * p.k.n[2] + sq.k0 + n) * width;
+  for (int c = 0; c < width; ++c) dst[c] = 0.f;
+}
+
 template <int HD>
 __device__ __forceinline__ void init_barriers(uint64_t* bars, volatile uint32_t* abort_flag, uint32_t limit_kcycles) {
   using L = BwdSmem<HD>;
@@ -613,6 +629,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
                    (sq.k0 + n) * p.dv.s[2];
           for (int c = 0; c < p.dqk; ++c) dkp[c] = from_f32<T>(0.f);
           for (int c = 0; c < p.dvo; ++c) dvp[c] = from_f32<T>(0.f);
+          if constexpr (FEAT == kPlain && !FUSED) { if (p.dk_tail != nullptr) zero_tail(p, sq, hk, n); }
         }
         __syncwarp();
         continue;
@@ -909,6 +926,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         tc_fence_before();
         __syncwarp();
         keep_sums(0, p.dqk);
+        if constexpr (FEAT == kPlain && !FUSED) { if (p.dk_tail != nullptr) keep_tail(p, sq, hk, n, d0, v, p.sm_scale); }
         stage_put32<T>(stage, r, d0, v, p.sm_scale, HD * 2);
         __syncwarp();
         warp_copy_out<T, 4>(stage, reinterpret_cast<T*>(p.dk.ptr) + (int64_t)sq.bidx * p.dk.s[0] + (int64_t)hk * p.dk.s[1] +

@@ -85,7 +85,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
   using L = WideSmem;
   constexpr bool kBoth = MODE == kWideDKV, kNarrow = MODE == kWideDKV || MODE == kWideDQN;
   constexpr bool kKeys = MODE != kWideDQ && MODE != kWideDQN;      // the CTA's rows are keys
-  constexpr bool kHasDp = MODE != kWideDV;
+  constexpr bool kHasDp = MODE != kWideDV, kTail = FEAT == kPlain && (MODE == kWideDK || MODE == kWideDKV);
   constexpr int kGroups = wide_groups(MODE, FEAT);
   constexpr uint32_t kColDPW = kGroups == 2 ? 128 : kWColDP;      // (behind two S' buffers)
   // Stages and places of the tiles.  The early tile has one stage; dV, which keeps only K resident, gives it two in the second resident tile's place.  Narrow
@@ -168,6 +168,10 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
     }
     zero_rows<T>(outv, sq.bidx, hrow, row_tok0, r0, rows_total, d_out);
     if constexpr (kBoth) zero_rows<T>(p.dv, sq.bidx, hrow, row_tok0, r0, rows_total, p.dvo);
+    if constexpr (kTail) {
+      if (p.dk_tail != nullptr)
+        for (int n = r0 + (int)threadIdx.x; n < min(r0 + kBlk, rows_total); n += (int)blockDim.x) zero_tail(p, sq, hrow, n);
+    }
     if constexpr (!kKeys) { if (dbias_on) zero_dbias_outside<T>(p, sq, hrow, r0, kBlk, 0, 0); }
     return;
   }
@@ -725,6 +729,7 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           }
           __syncwarp();
         }
+        if constexpr (kTail) { if (p.dk_tail != nullptr) keep_tail(p, sq, hrow, r0 + r, c * 32, v, scale); }
         stage_put32<T>(stage, r, c * 32, v, scale, 512);
         __syncwarp();
         warp_copy_out<T, 4>(stage, dst, outv.s[2], nrows, d_out, quarter * 32, c * 4, lane, 512);

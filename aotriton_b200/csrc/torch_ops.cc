@@ -1,5 +1,5 @@
 // The autograd entry points' native route: attention on ordinary torch tensors, forward and backward, without Python in
-// between; in the same way sink attention, the relative position bias, dropout of hidden states, the operators over a paged cache and keys that share columns.  Outputs, gradients and scratch
+// between; in the same way sink attention, the relative position bias, dropout of hidden states, the operators over a paged cache and latent attention.  Outputs, gradients and scratch
 // come from torch's caching allocator, launches go to torch's current stream through the C++ operator API (include/aotriton/flash.h), the backward is a torch::autograd::Function: version checks and CUDA-graph
 // capture see what they see of the Python Function, saved-tensor hooks the inputs, the output and the log-sum-exp.
 //
@@ -561,28 +561,90 @@ Tensor join_columns(const Tensor& k, const Tensor& shared) {
   check((hipError_t)ab200_join_columns(&a, stream_handle()), "join_columns");
   return joined;
 }
-struct JoinColumns : torch::autograd::Function<JoinColumns> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& k, const Tensor& shared) {
-    ctx->saved_data["numbers"] = std::vector<int64_t>{k.size(3), (int64_t)k.scalar_type()};
+// Attention over them.  cu_q, cu_k: of token-packed sequences, whose rows behind the last one are zero.
+struct LatentCall {
+  int64_t columns, max_q, max_k, causal_type, left, right;
+  double sm_scale;
+};
+ab200_attn_problem latent_problem(const LatentCall& c, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k) {
+  SinkCall s{};
+  s.max_q = c.max_q;
+  s.max_k = c.max_k;
+  s.varlen = cu_q.defined() ? AB200_VARLEN_COMPACT : AB200_VARLEN_NONE;
+  s.sm_scale = c.sm_scale;
+  ab200_attn_problem p = sink_problem(s, q, k, v, cu_q, cu_k);
+  p.causal_type = (int32_t)c.causal_type;
+  p.window_left = (int32_t)c.left;
+  p.window_right = (int32_t)c.right;
+  return p;
+}
+void latent_forward(const LatentCall& c, const Tensor& q, const Tensor& joined, const Tensor& v, const Tensor& cu_q, const Tensor& cu_k, bool want_lse, Tensor& out,
+                    Tensor& lse) {
+  at::AutoDispatchBelowADInplaceOrView guard;
+  if (cu_q.defined()) out = fresh({1, q.size(2), q.size(1), v.size(3)}, q.scalar_type()).zero_().transpose(1, 2);
+  else out = fresh({q.size(0), q.size(1), q.size(2), v.size(3)}, q.scalar_type());
+  if (want_lse) lse = fresh({q.size(0) * q.size(1), q.size(2)}, at::kFloat);
+  ab200_attn_fwd_args a{};
+  a.prob = latent_problem(c, q, joined, v, cu_q, cu_k);
+  a.q = c_view(q); a.k = c_view(joined); a.v = c_view(v); a.out = c_view(out);
+  a.lse = want_lse ? lse.data_ptr<float>() : nullptr;
+  check((hipError_t)ab200_attn_fwd(&a, stream_handle()), "latent_attention");
+}
+struct LatentAttend : torch::autograd::Function<LatentAttend> {
+  using Maybe = std::optional<Tensor>;
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& shared, const Tensor& v, const Maybe& seqs_q, const Maybe& seqs_k,
+                               const LatentCall& c, bool return_lse) {
+    const Tensor cu_q = seqs_q.value_or(Tensor()), cu_k = seqs_k.value_or(Tensor());
+    const Tensor joined = join_columns(k, shared);
+    Tensor out, lse;
+    latent_forward(c, q, joined, v, cu_q, cu_k, true, out, lse);
+    ctx->save_for_backward({q, joined, v, out, lse, cu_q, cu_k});
+    ctx->saved_data["numbers"] = std::vector<int64_t>{c.columns, c.max_q, c.max_k, c.causal_type, c.left, c.right};
+    ctx->saved_data["scale"] = c.sm_scale;
+    ctx->mark_non_differentiable({lse});
     ctx->set_materialize_grads(false);
-    return join_columns(k, shared);
+    return return_lse ? variable_list{out, lse} : variable_list{out};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list r(2);
-    Tensor g = grads[0];
-    if (!g.defined()) return r;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &cu_q = saved[5], &cu_k = saved[6];
     const auto n = ctx->saved_data["numbers"].toIntVector();
-    if (ctx->needs_input_grad(0)) r[0] = g.narrow(3, 0, n[0]);
-    if (!ctx->needs_input_grad(1)) return r;
-    if (ordinary_gradient(g, (at::ScalarType)n[1])) {
-      if (g.stride(-1) != 1) g = g.contiguous();
-      r[1] = fresh({g.size(0), 1, g.size(2), g.size(3) - n[0]}, g.scalar_type());
-      const auto a = columns_args(Tensor(), r[1], g);
-      check((hipError_t)ab200_sum_columns(&a, stream_handle()), "sum_columns");
-    } else {
+    const LatentCall c{n[0], n[1], n[2], n[3], n[4], n[5], ctx->saved_data["scale"].toDouble()};
+    variable_list r(8);
+    if (!grads[0].defined()) return r;
+    Tensor dout = grads[0];
+    // (as in SinkAttend::backward)
+    if (at::GradMode::is_enabled() || !Attend::as_saved(q, k, v, Tensor(), out, dout, lse, cu_q, cu_k) || !SinkAttend::sizes_match(q, k, v, out, cu_q, cu_k) ||
+        k.size(3) <= c.columns) {
       pybind11::gil_scoped_acquire gil;
-      r[1] = THPVariable_Unpack(call_python("sum_columns", pybind11::make_tuple(wrapped(g), n[0])).ptr());
+      const auto o = call_python("latent_attention", pybind11::make_tuple(wrapped(q), wrapped(k), wrapped(v), wrapped(out), wrapped(dout), wrapped(lse), wrapped(cu_q),
+                                                                          wrapped(cu_k), c.columns, c.max_q, c.max_k, c.causal_type, c.left, c.right, c.sm_scale));
+      for (int i = 0; i < 4; ++i) r[i] = THPVariable_Unpack(PyTuple_GET_ITEM(o.ptr(), i));
+      return r;
     }
+    if (dout.stride(-1) != 1) dout = dout.size(-1) == 1 ? dout.squeeze(-1).unsqueeze(-1) : dout.contiguous();
+    const Tensor dk = gradient_of(k);
+    r[0] = gradient_of(q);
+    r[1] = dk.narrow(3, 0, k.size(3) - c.columns);
+    r[2] = fresh({k.size(0), 1, k.size(2), c.columns}, k.scalar_type());
+    r[3] = gradient_of(v);
+    if (cu_q.defined())
+      for (const Tensor& t : {r[0], dk, r[3]}) t.zero_();
+    const Tensor delta = fresh(lse.sizes(), at::kFloat);
+    ab200_attn_bwd_args a{};
+    a.prob = latent_problem(c, q, k, v, cu_q, cu_k);
+    a.q = c_view(q); a.k = c_view(k); a.v = c_view(v); a.out = c_view(out); a.dout = c_view(dout);
+    a.dq = c_view(r[0]); a.dk = c_view(dk); a.dv = c_view(r[3]);
+    a.lse = lse.data_ptr<float>();
+    a.delta = delta.data_ptr<float>();
+    const ab200_view4 shared = c_view(r[2]);
+    const int64_t need = ab200_attn_bwd_shared_workspace(&a, (int32_t)c.columns, stream_handle());
+    if (need < 0) check((hipError_t)-need, "latent_attention backward");
+    const Tensor workspace = need > 0 ? fresh({need}, at::kFloat) : Tensor();
+    if (need > 0 && cu_q.defined()) workspace.zero_();
+    check((hipError_t)ab200_attn_bwd_shared(&a, (int32_t)c.columns, &shared, need > 0 ? workspace.data_ptr<float>() : nullptr, (uint64_t)need, stream_handle()),
+          "latent_attention backward");
+    g_last_bwd_family.store(ab200_last_bwd_family(), std::memory_order_relaxed);
     return r;
   }
 };
@@ -838,24 +900,51 @@ PyObject* relative_bias(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// join_columns(k, shared): the joined keys, or None: not an ordinary call.  (The caller has looked at types and shapes.)
-PyObject* join_columns_from(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// latent_attend(q, k, shared, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, causal_type, window_left, window_right, sm_scale, return_lse): out, or (out, lse),
+// or None: not an ordinary call, or one whose arguments the caller is to look at.
+PyObject* latent_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 2) {
-    PyErr_SetString(PyExc_TypeError, "join_columns takes 2 arguments");
+  if (n != 13) {
+    PyErr_SetString(PyExc_TypeError, "latent_attend takes 13 arguments");
     return nullptr;
   }
   if (!ordinary_first(a[0])) Py_RETURN_NONE;
   const int dev = c10::cuda::current_device();
-  Tensor k, shared;
-  if (!attention_operand(a[0], dev, &k) || !attention_operand(a[1], dev, &shared)) Py_RETURN_NONE;
-  if (shared.scalar_type() != k.scalar_type() || shared.size(0) != k.size(0) || shared.size(1) != 1 || shared.size(2) != k.size(2)) Py_RETURN_NONE;
-  Tensor out;
+  LatentCall c{};
+  Tensor q, k, shared, v, cu_q, cu_k;
+  if (!attention_operand(a[0], dev, &q) || !attention_operand(a[1], dev, &k) || !attention_operand(a[2], dev, &shared) || !attention_operand(a[3], dev, &v)) Py_RETURN_NONE;
+  for (const Tensor* t : {&k, &shared, &v})
+    if (t->scalar_type() != q.scalar_type() || t->size(0) != q.size(0) || t->size(2) != k.size(2)) Py_RETURN_NONE;
+  if (shared.size(1) != 1 || v.size(1) != k.size(1) || q.size(1) % k.size(1) != 0 || q.size(3) != k.size(3) + shared.size(3) || q.size(3) > 512 || v.size(3) > 512)
+    Py_RETURN_NONE;
+  if (!small_int(a[8], &c.causal_type) || !small_int(a[9], &c.left) || !small_int(a[10], &c.right) || !number(a[11], &c.sm_scale)) Py_RETURN_NONE;
+  const bool return_lse = a[12] == Py_True;
+  if (!return_lse && a[12] != Py_False) Py_RETURN_NONE;
+  c.columns = shared.size(3);
+  if (a[4] != Py_None) {
+    for (int i = 0; i < 2; ++i) {
+      Tensor& cu = i ? cu_k : cu_q;
+      if (!plain_tensor(a[4 + i], dev, &cu) || cu.dim() != 1 || cu.numel() < 2 || cu.scalar_type() != at::kInt) Py_RETURN_NONE;
+    }
+    if (cu_q.numel() != cu_k.numel() || q.size(0) != 1 || !small_int(a[6], &c.max_q) || !small_int(a[7], &c.max_k) || c.max_q < 1 || c.max_q > q.size(2) || c.max_k < 1 ||
+        c.max_k > k.size(2))
+      Py_RETURN_NONE;
+  }
+  Tensor out, lse;
   {
     pybind11::gil_scoped_release release;
-    out = at::GradMode::is_enabled() && (k.requires_grad() || shared.requires_grad()) ? JoinColumns::apply(k, shared) : join_columns(k, shared);
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || shared.requires_grad() || v.requires_grad())) {
+      auto maybe = [](const Tensor& t) { return t.defined() ? LatentAttend::Maybe(t) : LatentAttend::Maybe(); };
+      variable_list r = LatentAttend::apply(q, k, shared, v, maybe(cu_q), maybe(cu_k), c, return_lse);
+      out = std::move(r[0]);
+      if (return_lse) lse = std::move(r[1]);
+    } else {
+      latent_forward(c, q, join_columns(k, shared), v, cu_q, cu_k, return_lse, out, lse);
+    }
   }
-  return THPVariable_Wrap(std::move(out));
+  if (!return_lse) return THPVariable_Wrap(std::move(out));
+  return PyTuple_Pack(2, pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(out))).ptr(),
+                      pybind11::reinterpret_steal<pybind11::object>(THPVariable_Wrap(std::move(lse))).ptr());
   END_HANDLE_TH_ERRORS
 }
 
@@ -1053,7 +1142,7 @@ PyMethodDef kMethods[] = {{"attend", reinterpret_cast<PyCFunction>(reinterpret_c
                           {"sink_attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&sink_attend)), METH_FASTCALL, nullptr},
                           {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&dropout)), METH_FASTCALL, nullptr},
                           {"relative_bias", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&relative_bias)), METH_FASTCALL, nullptr},
-                          {"join_columns", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&join_columns_from)), METH_FASTCALL, nullptr},
+                          {"latent_attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&latent_attend)), METH_FASTCALL, nullptr},
                           {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&paged_attention)), METH_FASTCALL, nullptr},
                           {"block_tables", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&block_tables)), METH_FASTCALL, nullptr},
                           {"paged_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&paged_write)), METH_FASTCALL, nullptr},

@@ -342,6 +342,14 @@ typedef struct ab200_shared_columns_args {
 AB200_API int ab200_join_columns(const ab200_shared_columns_args* args, void* stream);
 AB200_API int ab200_sum_columns(const ab200_shared_columns_args* args, void* stream);
 
+/* ab200_attn_bwd for joined keys whose last `columns` columns all heads share: dK as there, and `shared`, (B, 1, S, columns), the sum of its last columns over the kv
+ * heads.  The sums are taken from 32 bits, for which the workspace has room (16-byte aligned; contents do not matter, calls that may overlap need one each); where it is
+ * of no floats, from dK itself.  The fused form does not apply. */
+AB200_API int ab200_attn_bwd_shared(const ab200_attn_bwd_args* args, int32_t columns, const ab200_view4* shared, float* workspace, uint64_t workspace_floats,
+                                    void* stream);
+/* Floats of workspace that call needs (0: none), or the negated error code.  Launches nothing. */
+AB200_API int64_t ab200_attn_bwd_shared_workspace(const ab200_attn_bwd_args* args, int32_t columns, void* stream);
+
 /* Replaces aotriton::v2::flash::check_gpu (modules/flash/csrc/attn_check.cc:36-46):
  * 0 when the stream's device is an sm_100 part, hipErrorNoBinaryForGpu (209) otherwise. */
 AB200_API int ab200_check_gpu(void* stream);

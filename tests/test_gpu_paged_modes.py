@@ -119,32 +119,53 @@ def _inputs(seed=0):
     return [torch.randn(2, h, 100, d, generator=g, device="cuda").half().requires_grad_() for h, d in ((4, 192), (2, 128), (1, 64), (2, 128))]
 
 
-def test_joined_keys_the_python_way(monkeypatch):
+@pytest.mark.parametrize("packed", [False, True])
+def test_latent_attention_the_python_way(packed, monkeypatch):
     ins = _inputs()
-    out = autograd.latent_attention(*ins, causal=True)
+    if packed:
+        ins = [t.detach()[:1].requires_grad_() for t in ins]
+        ends = torch.tensor([0, 30, 90], dtype=torch.int32, device="cuda")      # (ten rows behind the last sequence)
+        call = lambda: autograd.varlen_latent_attention(*ins, ends, ends, 60, 60, causal=True, return_lse=True)
+    else:
+        call = lambda: autograd.latent_attention(*ins, causal=True, return_lse=True)
+    out, lse = call()
     do = torch.randn_like(out)
     want = torch.autograd.grad(out, ins, do)
-    monkeypatch.setattr(autograd._native, "join_columns", lambda *a: None)
-    again = autograd.latent_attention(*ins, causal=True)
-    assert torch.equal(again, out)
+    monkeypatch.setattr(autograd._native, "latent_attend", lambda *a: None)
+    again, lse2 = call()
+    assert torch.equal(again, out) and (packed or torch.equal(lse, lse2))
     for a, b in zip(torch.autograd.grad(again, ins, do), want):
         assert torch.equal(a, b)
+    if packed:
+        assert (out[:, :, 90:] == 0).all() and all((g[:, :, 90:] == 0).all() for g in want)
 
 
 @pytest.mark.parametrize("native", [True, False])
-def test_joined_keys_differentiated_twice(native, monkeypatch):
-    """The gradient is linear in the gradient that comes in: its own derivative is the joining again."""
+def test_hooks_modes_and_second_derivatives(native, monkeypatch):
     if not native:
-        monkeypatch.setattr(autograd._native, "join_columns", lambda *a: None)
-    k, r = torch.randn(2, 3, 5, 8, device="cuda", requires_grad=True), torch.randn(2, 1, 5, 4, device="cuda", requires_grad=True)
-    joined = autograd._join_shared(torch.randn(2, 3, 5, 12, device="cuda"), k, r, k, "test")
-    assert torch.equal(joined, torch.cat([k, r.expand(-1, 3, -1, -1)], -1))
-    up = torch.randn_like(joined).requires_grad_()
-    gk, gr = torch.autograd.grad(joined, (k, r), up, create_graph=True)
-    assert torch.equal(gk, up[..., :8]) and torch.allclose(gr, up[..., 8:].sum(1, keepdim=True), atol=1e-6)
-    a, b = torch.randn_like(gk), torch.randn_like(gr)
-    (back,) = torch.autograd.grad((gk, gr), up, (a, b))
-    assert torch.equal(back, torch.cat([a, b.expand(-1, 3, -1, -1)], -1))
+        monkeypatch.setattr(autograd._native, "latent_attend", lambda *a: None)
+    ins = _inputs()
+    call = lambda: autograd.latent_attention(*ins, causal=True)
+    out = call()
+    do = torch.randn_like(out)
+    want = torch.autograd.grad(out, ins, do)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
+        out = call()
+    for a, b in zip(torch.autograd.grad(out, ins, do), want):
+        assert torch.equal(a, b)
+    for change in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t[..., : t.shape[-1] // 2], lambda t: t.flatten()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+            out = call()
+        with pytest.raises(ValueError, match="came back"):
+            torch.autograd.grad(out, ins, do)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(call(), ins, torch.stack([do] * 2), is_grads_batched=True)
+    grads = torch.autograd.grad(call(), ins, do.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(grads[0].float().sum(), ins[0])
+    turned = torch.randn(2, 4, 128, 100, device="cuda").half().transpose(2, 3)      # a gradient without unit stride
+    for a, b in zip(torch.autograd.grad(call(), ins, turned), torch.autograd.grad(call(), ins, turned.contiguous())):
+        assert torch.equal(a, b)
 
 
 def test_a_captured_training_step_beside_an_eager_graph():

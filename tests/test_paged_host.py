@@ -179,6 +179,38 @@ def test_shared_columns_entries(fake):
     assert join(None, None) == 1 and add(None, None) == 1 and count() == 5
 
 
+def test_backward_of_joined_keys_entry(fake):
+    f, size, count = fake.ab200_attn_bwd_shared, fake.ab200_attn_bwd_shared_workspace, lambda: fake.ab200_debug_host_call_count(7)
+
+    def args(dtype=cabi.DTYPE_BF16, B=2, H=4, Hk=2, S=300, D=192, Dv=128, **kw):
+        a = cabi.BwdArgs()
+        p = a.prob
+        p.dtype, p.batch, p.num_head_q, p.num_head_k, p.max_seqlen_q, p.max_seqlen_k, p.head_dim_qk, p.head_dim_vo, p.sm_scale = dtype, B, H, Hk, S, S, D, Dv, 0.1
+        a.q, a.k, a.v, a.out, a.dout, a.dq, a.dk, a.dv = (_view(0x10000000 * (i + 1), (B, h, S, d)) for i, (h, d) in
+                                                          enumerate(((H, D), (Hk, D), (Hk, Dv), (H, Dv), (H, Dv), (H, D), (Hk, D), (Hk, Dv))))
+        a.lse, a.delta = 0xa0000000, 0xb0000000
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    for kw, columns, launches in ((dict(), 64, 4), (dict(D=96, Dv=64), 32, 4), (dict(D=256, Dv=256), 64, 5)):      # delta, dK and dV (256: apart), dQ, the sum
+        a = args(**kw)
+        shared = _view(0xc0000000, (2, 1, 300, columns))
+        need = size(a, columns, None)
+        assert need == 2 * 2 * 300 * columns
+        n = count()
+        for ptr, floats in ((None, need), (0x5000, need - 1), (0x5004, need)):
+            assert f(a, columns, shared, ptr, floats, None) == 1
+        assert count() == n and f(a, columns, shared, 0x5000, need, None) == 0 and count() == n + launches, kw
+    for kw, columns in ((dict(dtype=cabi.DTYPE_FP32), 64), (dict(D=40, Dv=24), 6), (dict(D=13, Dv=10), 3)):      # from dK itself
+        assert size(args(**kw), columns, None) == 0 and f(args(**kw), columns, _view(0xc0000000, (2, 1, 300, columns)), None, 0, None) == 0, kw
+    n, good = count(), _view(0xc0000000, (2, 1, 300, 64))
+    for columns, shared in ((0, good), (192, good), (-1, good), (32, good), (64, None), (64, _view(0xc0000000, (2, 2, 300, 64))), (64, _view(0xc0000000, (2, 1, 299, 64))),
+                            (64, _view(None, (2, 1, 300, 64)))):
+        assert f(args(), columns, shared, 0x5000, 1 << 30, None) == 1
+    assert size(args(), 192, None) == -1 and size(None, 64, None) == -1 and count() == n
+
+
 class T:
     """What the checks look at: they come before anything touches the device."""
     def __init__(self, *shape, dtype=torch.float16, cuda=True, device="cuda:0", unit=1, grad=False):
@@ -295,15 +327,18 @@ def test_they_run_on_their_tensors_device(monkeypatch):
 
     monkeypatch.setattr(torch.cuda, "device", Device)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: SimpleNamespace(cuda_stream=0))
-    for name, result in (("block_tables", 0), ("paged_write", 0), ("paged_attn", 0), ("paged_attn_workspace", 8), ("shared_columns", 0)):
+    for name, result in (("block_tables", 0), ("paged_write", 0), ("paged_attn", 0), ("paged_attn_workspace", 8), ("shared_columns", 0), ("attn_fwd", 0), ("attn_bwd_shared", 0),
+                         ("attn_bwd_shared_workspace", 8)):
         monkeypatch.setattr(cabi, name, lambda *a, name=name, result=result, **kw: (seen.append((name, current[-1])), result)[1])
     monkeypatch.setattr(paged, "_check", lambda err, what: None)
     monkeypatch.setattr(autograd, "_check", lambda err, what: None)
+    monkeypatch.setattr(autograd._native, "note_bwd_family", lambda: None)
     here = torch.device("cpu")
     paged._block_tables(_ints(2, 5), _ints(2), _ints(2), _ints(5), 16, 10, None)
     k, cache = torch.zeros(5, 2, 8), torch.zeros(9, 16, 2, 8)
     paged._paged_write(k, None, cache, None, torch.zeros(5, dtype=torch.int64))
     paged._paged_attention(torch.zeros(2, 4, 1, 8), cache, cache, _ints(2, 5), _ints(2), None, 0, 0, 1.0, False, "x")
-    k, r = torch.zeros(1, 2, 5, 8, requires_grad=True), torch.zeros(1, 1, 5, 4, requires_grad=True)
-    autograd._JoinColumns.apply(k, r).sum().backward()
-    assert seen == [(n, here) for n in ("block_tables", "paged_write", "paged_attn_workspace", "paged_attn", "shared_columns", "shared_columns")]
+    q, k, r = torch.zeros(1, 2, 5, 12), torch.zeros(1, 2, 5, 8, requires_grad=True), torch.zeros(1, 1, 5, 4, requires_grad=True)
+    autograd._LatentAttention.apply(q, k, r, k, None, None, 0, 0, 0, 0, 0, 1.0, False).sum().backward()
+    assert seen == [(n, here) for n in ("block_tables", "paged_write", "paged_attn_workspace", "paged_attn", "shared_columns", "attn_fwd", "attn_bwd_shared_workspace",
+                                        "attn_bwd_shared")]
