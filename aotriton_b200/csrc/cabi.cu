@@ -1148,7 +1148,7 @@ static int64_t plan_bwd_shared(const ab200_attn_bwd_args* a, int columns, Params
   if (columns < 1 || columns >= p.dqk) return -kErrInvalidValue;
   const int sel = ab200_select_variant(kOpBwd, a->prob.dtype, p.dqk, p.dvo, family_flags(g_family) | (sm100_bwd_supported(a->prob.dtype, p) ? AB200_SELECT_ALIGNED : 0));
   if (sel < 0) return sel;
-  if ((sel & 0xff) < kVarTcgen05 || features(p) != kPlain || columns % 4 != 0) return 0;
+  if ((sel & 0xff) < kVarTcgen05 || features(p) != kPlain || columns % 8 != 0) return 0;
   for (int i = 0; i < 3; ++i)
     if (p.k.n[i] < 0 || p.k.n[i] > INT32_MAX) return -kErrInvalidValue;
   return p.k.n[0] * p.hk * p.k.n[2] * columns;

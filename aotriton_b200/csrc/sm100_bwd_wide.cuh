@@ -729,10 +729,10 @@ sm100_bwd_wide_kernel(const __grid_constant__ Params p, const __grid_constant__ 
           }
           __syncwarp();
         }
-        if constexpr (kTail) { if (p.dk_tail != nullptr) keep_tail(p, sq, hrow, r0 + r, c * 32, v, scale); }
+        if constexpr (kTail) { if (p.dk_tail != nullptr) keep_tail(p, sq, hrow, r0 + r, c * 32, v, scale); __syncwarp(); }
         stage_put32<T>(stage, r, c * 32, v, scale, 512);
         __syncwarp();
-        warp_copy_out<T, 4>(stage, dst, outv.s[2], nrows, d_out, quarter * 32, c * 4, lane, 512);
+        warp_copy_out<T, 4>(stage, dst, outv.s[2], nrows, kTail ? dk_columns(p) : d_out, quarter * 32, c * 4, lane, 512);
         __syncwarp();
       }
       if constexpr (kBoth) {
