@@ -999,6 +999,7 @@ int ab200_block_tables(const ab200_block_tables_args* a, void* stream) {
   if (a->cu_seqlens == nullptr || a->taken_out == nullptr || (a->total_tokens > 0 && a->slots == nullptr)) return kErrInvalidValue;
   if (a->batch > 0 && (a->lengths == nullptr || a->new_tokens == nullptr || a->new_lengths == nullptr)) return kErrInvalidValue;
   if ((a->batch > 0 && a->table_width > 0 && a->block_table == nullptr) || (a->num_free > 0 && a->free_pages == nullptr)) return kErrInvalidValue;
+  if (a->batch > 1 && a->table_stride < a->table_width) return kErrInvalidValue;      // (rows are written: none over another)
   if (a->total_tokens > INT32_MAX - (1 << 20)) return kErrNotSupported;
   BlockTables b{};
   b.batch = a->batch; b.page = a->page_size; b.width = a->table_width; b.total = a->total_tokens; b.table_stride = a->table_stride; b.num_free = a->num_free;

@@ -120,29 +120,31 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const __gri
 // loads are on the way together.
 constexpr int kWriteThreads = 256, kWriteBatch = 4;
 
-template <typename V>
-__global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const __grid_constant__ PagedWrite a, int elt, int64_t vectors) {
+// I: what counts the vectors; 32 bits where they do (20000 latent rows of 576 11.9 us in 64 bits).
+template <typename V, typename I>
+__global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const __grid_constant__ PagedWrite a, int elt, I vectors) {
   wait_for_earlier_grids();
   const int per = (int)sizeof(V) / elt;      // elements of a vector
   const int vk = a.dk / per, vv = a.dv / per, of_k = a.heads * vk, of_token = of_k + a.heads * vv;
-  const int64_t first = ((int64_t)blockIdx.x * kWriteBatch * kWriteThreads) + threadIdx.x;
+  const I first = (I)blockIdx.x * (kWriteBatch * kWriteThreads) + threadIdx.x;
   V value[kWriteBatch];
   V* to[kWriteBatch];
 #pragma unroll
   for (int b = 0; b < kWriteBatch; ++b) {
-    const int64_t i = first + b * kWriteThreads;
+    const I i = first + b * kWriteThreads;
     to[b] = nullptr;
     if (i >= vectors) continue;
-    const int64_t t = i / of_token;
-    int e = (int)(i - t * of_token);
+    const int64_t t = i / (I)of_token;
+    int e = (int)(i - (I)t * (I)of_token);
     const int64_t slot = a.slots[t];
     if (slot < 0 || slot >= a.slots_total) continue;
-    const int64_t page = slot / a.page, in = slot - page * a.page;
+    const I page = (I)slot / (I)a.page;      // (slots of a cache that 32 bits do not count: 64)
+    const int in = (int)((I)slot - page * (I)a.page);
     const bool is_k = e < of_k;
     if (!is_k) e -= of_k;
-    const int wide = is_k ? vk : vv, h = e / wide, c = e - h * wide;
+    const int wide = is_k ? vk : vv, h = (int)((unsigned)e / (unsigned)wide), c = e - h * wide;
     const int64_t from = t * (is_k ? a.sk[0] : a.sv[0]) + h * (is_k ? a.sk[1] : a.sv[1]) + (int64_t)c * per;
-    const int64_t dst = page * (is_k ? a.ck[0] : a.cv[0]) + in * (is_k ? a.ck[1] : a.cv[1]) + h * (is_k ? a.ck[2] : a.cv[2]) + (int64_t)c * per;
+    const int64_t dst = (int64_t)page * (is_k ? a.ck[0] : a.cv[0]) + in * (is_k ? a.ck[1] : a.cv[1]) + h * (is_k ? a.ck[2] : a.cv[2]) + (int64_t)c * per;
     value[b] = *reinterpret_cast<const V*>(reinterpret_cast<const char*>(is_k ? a.k : a.v) + from * elt);
     to[b] = reinterpret_cast<V*>(reinterpret_cast<char*>(is_k ? a.k_cache : a.v_cache) + dst * elt);
   }
@@ -540,11 +542,15 @@ cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st) 
   const int64_t vectors = a.tokens * a.heads * ((a.dk + a.dv) / per);
   if (vectors == 0) return cudaSuccess;
   const dim3 grid(grid_for(vectors, (int64_t)kWriteThreads * kWriteBatch));
-  switch (a.vec) {
-    case 16: return launch_counted(paged_write_kernel<uint4>, grid, kWriteThreads, 0, st, a, elt, vectors);
-    case 4: return launch_counted(paged_write_kernel<uint32_t>, grid, kWriteThreads, 0, st, a, elt, vectors);
-    default: return launch_counted(paged_write_kernel<uint16_t>, grid, kWriteThreads, 0, st, a, elt, vectors);
-  }
+  auto launch = [&]<typename I>() {
+    switch (a.vec) {
+      case 16: return launch_counted(paged_write_kernel<uint4, I>, grid, kWriteThreads, 0, st, a, elt, (I)vectors);
+      case 4: return launch_counted(paged_write_kernel<uint32_t, I>, grid, kWriteThreads, 0, st, a, elt, (I)vectors);
+      default: return launch_counted(paged_write_kernel<uint16_t, I>, grid, kWriteThreads, 0, st, a, elt, (I)vectors);
+    }
+  };
+  // (room for the last block's indices)
+  return vectors < 0x7fff0000 && a.slots_total < 0x7fff0000 ? launch.template operator()<uint32_t>() : launch.template operator()<int64_t>();
 }
 
 int64_t plan_paged(int dtype, PagedAttn& p, int sms) {

@@ -1029,7 +1029,9 @@ PyObject* block_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   if (a[6] != Py_None && (!whole_numbers(a[6], dev, at::kInt, 1, &taken) || taken.numel() != 1)) Py_RETURN_NONE;
   const int64_t batch = table.size(0);
-  if (lengths.size(0) != batch || new_tokens.size(0) != batch || batch > INT32_MAX || table.size(1) > INT32_MAX || page < 1 || total < 1) Py_RETURN_NONE;
+  if (lengths.size(0) != batch || new_tokens.size(0) != batch || batch > INT32_MAX || table.size(1) > INT32_MAX || page < 1 || total < 1 ||
+      (batch > 1 && table.stride(0) < table.size(1)))
+    Py_RETURN_NONE;
   Tensor out[4];
   {
     pybind11::gil_scoped_release release;

@@ -79,6 +79,8 @@ def block_tables(block_table, lengths, new_tokens, free_pages, page_size, total_
         raise ValueError("block_tables: lengths and new_tokens are contiguous int32 tensors on the table's device, one entry a row of it")
     if not _int32(free_pages, 1, device) or (taken is not None and not (_int32(taken, 1, device) and taken.numel() == 1)):
         raise ValueError("block_tables: free_pages and taken are contiguous int32 tensors on the table's device, taken of one element")
+    if batch > 1 and block_table.stride(0) < block_table.shape[1]:
+        raise ValueError("block_tables: rows of the block table overlap")
     if not _whole(page_size, 1) or not _whole(total_tokens, 0):
         raise ValueError(f"block_tables: page_size {page_size} and total_tokens {total_tokens}: whole numbers, 1 or more and 0 or more")
     return _block_tables(block_table, lengths, new_tokens, free_pages, page_size, total_tokens, taken)

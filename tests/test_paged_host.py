@@ -55,7 +55,7 @@ def test_block_tables_entry(fake):
     assert f(_tables_args(table_width=0, block_table=None), None) == 0 and count() == 5
     for bad, code in ((dict(batch=-1), 1), (dict(page_size=0), 1), (dict(table_width=-1), 1), (dict(num_free=-1), 1), (dict(total_tokens=-1), 1), (dict(cu_seqlens=None), 1),
                       (dict(taken_out=None), 1), (dict(slots=None), 1), (dict(lengths=None), 1), (dict(new_tokens=None), 1), (dict(new_lengths=None), 1),
-                      (dict(block_table=None), 1), (dict(free_pages=None), 1), (dict(total_tokens=1 << 31), 801)):
+                      (dict(block_table=None), 1), (dict(free_pages=None), 1), (dict(table_stride=9), 1), (dict(total_tokens=1 << 31), 801)):
         assert f(_tables_args(**bad), None) == code, bad
     assert f(None, None) == 1 and count() == 5
 
@@ -295,6 +295,8 @@ def test_block_tables_refusals():
 
     table = _ints(2, 5).as_subclass(Table)
     good = dict(lengths=_ints(2), new_tokens=_ints(2), free_pages=_ints(5), page_size=16, total_tokens=10, taken=_ints(1))
+    with pytest.raises(ValueError, match="overlap"):
+        paged.block_tables(_ints(1, 5).as_subclass(Table).expand(2, 5), **good)
     for bad in (dict(lengths=_ints(3)), dict(lengths=_ints(2).long()), dict(new_tokens=_ints(2, 1)), dict(new_tokens=_ints(1)), dict(free_pages=_ints(5).float()), dict(free_pages=_ints(10)[::2]),
                 dict(page_size=0), dict(page_size=16.0), dict(page_size=True), dict(total_tokens=-1), dict(total_tokens=1 << 31), dict(taken=_ints(2)), dict(taken=3), dict(lengths=None)):
         with pytest.raises(ValueError):
