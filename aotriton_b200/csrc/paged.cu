@@ -175,10 +175,12 @@ __device__ __forceinline__ void load_vec(const T* src, float (&x)[N]) {
 template <typename T, int N, int J>
 __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid_constant__ PagedAttn p) {
   wait_for_earlier_grids();
-  extern __shared__ float q_s[];      // [kGenRows][dqk]
-  __shared__ float s[kGenRows][kGenKeys], alpha[kGenRows], m_s[kGenRows], l_s[kGenRows];
+  extern __shared__ __align__(16) float q_s[];      // [kGenRows][dqk]
+  __shared__ float scores[2][kGenRows][kGenKeys], alphas[2][kGenRows], m_s[kGenRows], l_s[kGenRows];      // (of a tile and the next one)
   __shared__ float meet[J == 1 ? kGenThreads * kGenRows : 1];
-  __shared__ int64_t page_of[kGenKeys];
+  // where a key and its value start in the caches (-1: nobody sees it), worked out once (a thread each divided by the page's size 32 times a tile before: 16 sequences of
+  // up to 2000 fp32 keys 166 us); a tile's, the last one's, which some may still read, and the next one's
+  __shared__ int64_t places_k[3][kGenKeys], places_v[3][kGenKeys];
   __shared__ int scratch[kGenThreads / 32 + 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Line line = find_in_line<kGenThreads>(p, -1, blockIdx.x / p.lanes, scratch);
@@ -205,49 +207,79 @@ __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid
     for (int r = 0; r < kGenRows; ++r)
 #pragma unroll
       for (int j = 0; j < J; ++j) acc[r][j] = 0.f;
+    auto place_of = [&](int n, int64_t& at_k, int64_t& at_v) {
+      at_k = at_v = -1;
+      if (!w.seen(p, n)) return;
+      const int page = (int)((unsigned)n / (unsigned)p.page), in = n - page * p.page, id = p.table[(int64_t)z * p.table_stride + page];
+      if (id < 0 || id >= p.num_pages) return;
+      at_k = id * p.k.s[0] + in * p.k.s[1] + hk * p.k.s[2];
+      at_v = id * p.v.s[0] + in * p.v.s[1] + hk * p.v.s[2];
+    };
+    if (tid < kGenKeys) place_of(w.tile(first) * kGenKeys + tid, places_k[first % 3][tid], places_v[first % 3][tid]);
+    __syncthreads();
     for (int i = first; i < last; ++i) {
       const int n0 = w.tile(i) * kGenKeys;
-      __syncthreads();
-      if (tid < kGenKeys) {      // a key's place in the cache in slots, or -1: nobody sees it
-        int64_t place = -1;
-        const int n = n0 + tid;
-        if (w.seen(p, n)) {
-          const int id = p.table[(int64_t)z * p.table_stride + n / p.page];
-          if (id >= 0 && id < p.num_pages) place = (int64_t)id * p.page + n % p.page;
-        }
-        page_of[tid] = place;
-      }
-      __syncthreads();
+      const int64_t *at_k = places_k[i % 3], *at_v = places_v[i % 3];
+      float(*s)[kGenKeys] = scores[i & 1];
+      float* alpha = alphas[i & 1];
+      int64_t next_k = -1, next_v = -1;      // (looked up while the keys are on their way)
+      if (tid < kGenKeys && i + 1 < last) place_of(w.tile(i + 1) * kGenKeys + tid, next_k, next_v);
       {
         const int key = tid >> 3, l8 = tid & 7;
-        const int64_t place = page_of[key];
+        const int64_t place = at_k[key];
         float dot[kGenRows];
 #pragma unroll
         for (int r = 0; r < kGenRows; ++r) dot[r] = 0.f;
         if (place >= 0) {
-          const T* kr = reinterpret_cast<const T*>(p.k.ptr) + place / p.page * p.k.s[0] + place % p.page * p.k.s[1] + (int64_t)hk * p.k.s[2];
-          for (int d = l8 * N; d < p.dqk; d += 8 * N) {
-            float x[N];
-            load_vec<T, N>(kr + d, x);
+          const T* kr = reinterpret_cast<const T*>(p.k.ptr) + place;
+          constexpr int kAhead = 4;      // vectors of a lane on the way at a time
+          for (int d0 = l8 * N; d0 < p.dqk; d0 += 8 * N * kAhead) {
+            float x[kAhead][N];
 #pragma unroll
-            for (int r = 0; r < kGenRows; ++r)
-              if (r < rows.n)
+            for (int a = 0; a < kAhead; ++a)
+              if (d0 + 8 * N * a < p.dqk) load_vec<T, N>(kr + d0 + 8 * N * a, x[a]);
+              else
 #pragma unroll
-                for (int e = 0; e < N; ++e) dot[r] = fmaf(q_s[r * p.dqk + d + e], x[e], dot[r]);
+                for (int e = 0; e < N; ++e) x[a][e] = 0.f;
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+              const int d = d0 + 8 * N * a;
+              if (d >= p.dqk) break;
+#pragma unroll
+              for (int r = 0; r < kGenRows; ++r) {
+                if (r >= rows.n) break;
+                const float* q = q_s + r * p.dqk + d;
+                if constexpr (N % 4 == 0) {
+#pragma unroll
+                  for (int e = 0; e < N; e += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(q + e);
+                    dot[r] = fmaf(y.x, x[a][e], dot[r]);
+                    dot[r] = fmaf(y.y, x[a][e + 1], dot[r]);
+                    dot[r] = fmaf(y.z, x[a][e + 2], dot[r]);
+                    dot[r] = fmaf(y.w, x[a][e + 3], dot[r]);
+                  }
+                } else {
+#pragma unroll
+                  for (int e = 0; e < N; ++e) dot[r] = fmaf(q[e], x[a][e], dot[r]);
+                }
+              }
+            }
           }
         }
 #pragma unroll
         for (int r = 0; r < kGenRows; ++r) {
+          if (r >= rows.n) break;
 #pragma unroll
           for (int o = 1; o < 8; o <<= 1) dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], o);
           if (l8 == 0) s[r][key] = dot[r];
         }
       }
+      if (tid < kGenKeys) { places_k[(i + 1) % 3][tid] = next_k; places_v[(i + 1) % 3][tid] = next_v; }
       __syncthreads();
       for (int r = warp; r < rows.n; r += kGenThreads / 32) {
         const int n = n0 + lane;
         const int64_t pos = (int64_t)w.len - w.queries + rows.query(r);
-        const bool ok = page_of[lane] >= 0 && n <= pos && (n > pos - p.window || n < p.sinks);
+        const bool ok = at_k[lane] >= 0 && n <= pos && (n > pos - p.window || n < p.sinks);
         const float x = ok ? s[r][lane] * p.qk_scale : -INFINITY;
         float mx = x;
 #pragma unroll
@@ -271,18 +303,30 @@ __global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid
         if (r < rows.n)
 #pragma unroll
           for (int j = 0; j < J; ++j) acc[r][j] *= alpha[r];
-      for (int key = group; key < kGenKeys; key += groups) {
-        const int64_t place = page_of[key];
-        if (place < 0) continue;
-        const T* vr = reinterpret_cast<const T*>(p.v.ptr) + place / p.page * p.v.s[0] + place % p.page * p.v.s[1] + (int64_t)hk * p.v.s[2];
+      constexpr int kKeysAhead = J > 1 ? 4 : 8;      // values of a thread on the way at a time
+      for (int k0 = group; k0 < kGenKeys; k0 += groups * kKeysAhead) {
+        float x[kKeysAhead][J];
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int d = col + j * kGenThreads;
-          if (d < p.dvo) {
-            const float x = to_f32<T>(vr[d]);
+        for (int u = 0; u < kKeysAhead; ++u) {
+          const int key = k0 + u * groups;
+          const int64_t place = key < kGenKeys ? at_v[key] : -1;
+          const T* vr = reinterpret_cast<const T*>(p.v.ptr) + place;
 #pragma unroll
-            for (int r = 0; r < kGenRows; ++r)
-              if (r < rows.n) acc[r][j] = fmaf(s[r][key], x, acc[r][j]);
+          for (int j = 0; j < J; ++j) {
+            const int d = col + j * kGenThreads;
+            x[u][j] = place >= 0 && d < p.dvo ? to_f32<T>(vr[d]) : 0.f;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kKeysAhead; ++u) {
+          const int key = k0 + u * groups;
+          if (key >= kGenKeys) break;
+#pragma unroll
+          for (int r = 0; r < kGenRows; ++r) {
+            if (r >= rows.n) break;
+            const float e = s[r][key];
+#pragma unroll
+            for (int j = 0; j < J; ++j) acc[r][j] = fmaf(e, x[u][j], acc[r][j]);
           }
         }
       }
