@@ -154,7 +154,8 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const __grid
 }
 
 // ---- attention, any type and size up to 1024 ----------------------------------------------------------------------
-// Bound by latency: what has no tensor-core kernel (fp32, odd head dims and pages) is small or rare; 16 sequences of 2000 fp32 keys take 20 to 30 us.
+// For what has no tensor-core kernel: fp32, odd head dims and pages.  Bound by instructions (a fused multiply-add a score and column on the ordinary pipe, and its
+// operands from shared memory).  16 sequences of 40 to 2000 fp32 keys, 32:8 heads of 128, 71 us (floor 21; three blocks an SM, with 112 registers and two 111).
 // Tiles of 32 keys: eight lanes form a key's scores with the unit's rows, a warp a row takes their softmax on, and a thread a column adds up
 // the values; with fewer columns than threads, groups of threads share the keys.
 constexpr int kGenThreads = 256, kGenRows = 8, kGenKeys = 32;
@@ -173,13 +174,13 @@ __device__ __forceinline__ void load_vec(const T* src, float (&x)[N]) {
 
 // J: columns of a thread.  N: elements of K that a lane reads at a time.
 template <typename T, int N, int J>
-__global__ void __launch_bounds__(kGenThreads) paged_general_kernel(const __grid_constant__ PagedAttn p) {
+__global__ void __launch_bounds__(kGenThreads, J == 1 ? 3 : 2) paged_general_kernel(const __grid_constant__ PagedAttn p) {
   wait_for_earlier_grids();
   extern __shared__ __align__(16) float q_s[];      // [kGenRows][dqk]
   __shared__ float scores[2][kGenRows][kGenKeys], alphas[2][kGenRows], m_s[kGenRows], l_s[kGenRows];      // (of a tile and the next one)
   __shared__ float meet[J == 1 ? kGenThreads * kGenRows : 1];
-  // where a key and its value start in the caches (-1: nobody sees it), worked out once (a thread each divided by the page's size 32 times a tile before: 16 sequences of
-  // up to 2000 fp32 keys 166 us); a tile's, the last one's, which some may still read, and the next one's
+  // where a key and its value start in the caches (-1: nobody sees it), worked out once (with a division in every thread for every key the
+  // sequences above took 166 us and not 112); a tile's, the last one's, which some may still read, and the next one's
   __shared__ int64_t places_k[3][kGenKeys], places_v[3][kGenKeys];
   __shared__ int scratch[kGenThreads / 32 + 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -605,7 +606,7 @@ int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
     p.tile_log = 5;
     p.min_tiles = 2;
     p.extra = 1;
-    p.ctas = sms * 4;
+    p.ctas = sms * 3;
   }
   const int64_t chunks = ((int64_t)p.group * p.sq + p.rows - 1) / p.rows;
   p.chunks = (int)chunks;

@@ -57,6 +57,16 @@ def test_long_and_ragged(h):
     run(40, h, 1, 576, 512, 16, [(i * 37) % 300 + (3000 if i == 7 else 0) for i in range(40)], torch.float16)
 
 
+@pytest.mark.parametrize("dtype,h", [(torch.bfloat16, 16), (torch.float16, 32), (torch.bfloat16, 64), (torch.float16, 100), (torch.float32, 4)])
+def test_many_sequences(dtype, h):
+    run(130, h, 1, 192, 128, 16, [(i * 53) % 200 + (900 if i in (3, 129) else 0) for i in range(130)], dtype)
+    run(65, h, 2, 288, 256, 32, [(i * 53) % 100 for i in range(65)], dtype, query_lengths=[i % 3 for i in range(65)])
+
+
+def test_many_rows_a_sequence():
+    run(2, 128, 11, 192, 128, 16, [300, 40], torch.bfloat16)      # more chunks of rows than stand side by side
+
+
 @pytest.mark.parametrize("dtype", HALF)
 def test_weights_that_grow_along_the_sequence(dtype):
     # each tile's largest score is above the last one's: what has been summed is rescaled again and again

@@ -82,6 +82,23 @@ def test_batches_of_very_different_lengths(dtype, b):
     run(b, 4, 1, 1, 64, 64, 16, lengths, dtype)
 
 
+@pytest.mark.parametrize("dtype", ALL)
+def test_two_streams_at_once(dtype):
+    """Calls that overlap, each with a workspace of its own."""
+    cases = [make(4, 8, 2, 1, 128, 128, 16, [1000, 3, 500, 2000], dtype, seed=i) for i in range(2)]
+    want = [paged.paged_attention(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(paged.paged_attention(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
 def test_one_long_sequence():
     run(1, 8, 1, 1, 128, 128, 64, [40001], torch.bfloat16)
     run(1, 8, 1, 2, 64, 64, 16, [30000], torch.float16, window=20000, sinks=3)
