@@ -618,15 +618,14 @@ int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
   // A kv head's chunks side by side, so that its keys come from memory once, unless that left too few CTAs to share a line out evenly.
   p.lanes = chunks <= 8 ? (int)chunks : 1;
   p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(p.ctas / p.lanes, units / p.lanes * most / p.min_tiles + 1)) * p.lanes;
-  p.join = 1;
-  return p.join ? 2 * (int64_t)p.ctas * partial_floats(p) : 0;
+  return 2 * (int64_t)p.ctas * partial_floats(p);
 }
 
 cudaError_t launch_paged(int dtype, PagedAttn& p, cudaStream_t st) {
   cudaError_t e = p.kind == kPagedSplit    ? launch_paged_split(dtype, p, st)
                   : p.kind == kPagedLatent ? launch_paged_latent(dtype, p, st)
                                            : with_type(dtype, [&]<typename T>() { return launch_general_T<T>(p, st); });
-  if (e == cudaSuccess && p.join) e = with_type(dtype, [&]<typename T>() { return launch_join_T<T>(p, st); });
+  if (e == cudaSuccess) e = with_type(dtype, [&]<typename T>() { return launch_join_T<T>(p, st); });
   return e;
 }
 

@@ -42,8 +42,9 @@ struct PagedAttn {
   int32_t window, sinks;             // window INT32_MAX: none
   int32_t max_len;                   // what the table has room for
   // How the call is cut (plan_paged, paged_split.cuh): into units -- (sequence, kv head, chunk of `rows` query rows) -- and tiles of 2^tile_log keys, for `ctas`
-  // CTAs, min_tiles a CTA at least, a unit counted as `extra` tiles more than it has; `lanes` chunks side by side (a divisor of the chunks, and of the CTAs).  box: slots of a tile copy.
-  int32_t kind, ctas, lanes, rows, chunks, tile_log, min_tiles, extra, join, box;
+  // CTAs, min_tiles a CTA at least, a unit counted as `extra` tiles more than it has; `lanes` chunks side by side (a divisor of the chunks, and of the CTAs).
+  // box: slots of a tile copy.
+  int32_t kind, ctas, lanes, rows, chunks, tile_log, min_tiles, extra, box;
   int32_t q_tiles;                   // latent attention: the queries come as tile copies
   unsigned int* status;              // the word in which a kernel records a wait that ran out (null: the general kernel has none)
   float* partial;                    // two partial results a CTA: of the unit that it starts with, of the one that it ends with

@@ -266,7 +266,7 @@ typedef struct ab200_block_tables_args {
   int32_t page_size;
   int32_t table_width;          /* entries of a row                                                      */
   int32_t* block_table;         /* (batch, table_width)                                                  */
-  int64_t table_stride;         /* between rows                                                          */
+  int64_t table_stride;         /* between rows, at least table_width                                    */
   const int32_t* lengths;
   const int32_t* new_tokens;
   const int32_t* free_pages;
