@@ -771,7 +771,7 @@ class _LatentAttentionGrad(torch.autograd.Function):
         need = cabi.attn_bwd_shared_workspace(*args, columns, stream=stream, **kw)
         if need < 0:
             _check(hipError_t(-need), "latent_attention backward")
-        workspace = (torch.empty if cu_q is None else torch.zeros)([need], device=q.device, dtype=torch.float32) if need else None
+        workspace = torch.empty([need], device=q.device, dtype=torch.float32) if need else None
         _check(hipError_t(cabi.attn_bwd_shared(*args, shared, workspace=workspace, stream=stream, **kw)), "latent_attention backward")
         _native.note_bwd_family()
         return dq, dk[..., :-columns], shared, dv

@@ -1138,6 +1138,7 @@ int ab200_sum_columns(const ab200_shared_columns_args* a, void* stream) {
   if (int e = fill_shared_columns(a, s, true)) return e;
   if (int e = check_device(st)) return e;
   if (s.shared.n[0] == 0 || s.shared.n[2] == 0) return 0;
+  s.tokens = KeyTokens{0, (int32_t)s.shared.n[0], (int32_t)s.shared.n[2], nullptr, nullptr};      // all of them
   DeviceGuard guard(st);
   return (int)launch_sum_columns(a->dtype, s, st);
 }
@@ -1180,8 +1181,9 @@ int ab200_attn_bwd_shared(const ab200_attn_bwd_args* a, int32_t columns, const a
   if (int e = fill_shared_columns(&c, s, true)) return e;
   if (int e = attn_bwd(a, floats > 0 ? workspace : nullptr, p.dqk - columns, stream)) return e;
   if (s.shared.n[0] == 0 || s.shared.n[2] == 0) return 0;
+  s.tokens = KeyTokens{p.varlen_mode, p.batch, p.max_sk, p.cu_k, p.ss_k};
   DeviceGuard guard(st);
-  return (int)(floats > 0 ? launch_sum_tail(a->prob.dtype, s.shared, workspace, p.hk, st) : launch_sum_columns(a->prob.dtype, s, st));
+  return (int)(floats > 0 ? launch_sum_tail(a->prob.dtype, s, workspace, p.hk, st) : launch_sum_columns(a->prob.dtype, s, st));
 }
 
 // --- HIP-named runtime helpers used by the Python tests of the reference

@@ -488,6 +488,20 @@ __global__ void __launch_bounds__(kColumnThreads) join_columns_kernel(const __gr
   }
 }
 
+// Whether token `s` of batch element `b` is a key of a sequence.  dK's kernels write those alone, so that nothing is summed for the others.
+__device__ __forceinline__ bool of_a_sequence(const KeyTokens& t, int64_t b, int64_t s) {
+  if (t.varlen_mode == 0) return b < t.batch && s < t.max_sk;
+  if (t.varlen_mode == 2) return b < t.batch && s < min(t.cu_k[b + 1] - t.cu_k[b], t.max_sk);
+  const int32_t* starts = t.ss_k != nullptr ? t.ss_k : t.cu_k;
+  int lo = 0;      // the last sequence that starts at or ahead of the token: of those that start together all but the last are empty
+  for (int hi = t.batch - 1; lo < hi;) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (starts[mid] <= s) lo = mid;
+    else hi = mid - 1;
+  }
+  return b == 0 && t.batch > 0 && s >= starts[lo] && s - starts[lo] < min(t.cu_k[lo + 1] - t.cu_k[lo], t.max_sk);
+}
+
 // shared[b, 0, s, c] = sum over the heads of out[b, h, s, dn + c], in their order, in 32 bits, rounded once.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_columns_kernel(const __grid_constant__ SharedColumns a) {
@@ -499,8 +513,9 @@ __global__ void __launch_bounds__(256) sum_columns_kernel(const __grid_constant_
     const int c = (int)(i - row * dr);
     const T* src = reinterpret_cast<const T*>(a.out.ptr) + b * a.out.s[0] + s * a.out.s[2] + dn + c;
     float sum = 0.f;
+    const int heads = of_a_sequence(a.tokens, b, s) ? (int)a.out.n[1] : 0;
 #pragma unroll 8
-    for (int h = 0; h < (int)a.out.n[1]; ++h) sum += to_f32<T>(src[(int64_t)h * a.out.s[1]]);
+    for (int h = 0; h < heads; ++h) sum += to_f32<T>(src[(int64_t)h * a.out.s[1]]);
     reinterpret_cast<T*>(a.shared.ptr)[b * a.shared.s[0] + s * a.shared.s[2] + c] = from_f32<T>(sum);
   }
 }
@@ -508,16 +523,18 @@ __global__ void __launch_bounds__(256) sum_columns_kernel(const __grid_constant_
 // ... from columns in 32 bits, heads * rows * dr of them a batch element, dr a multiple of 4.  Many heads' loads on the way at a time: one by one and four bytes
 // each, 32 heads x 4096 x 64 took 23 us.
 template <typename T>
-__global__ void __launch_bounds__(128) sum_tail_kernel(const __grid_constant__ View4 shared, const float* __restrict__ tail, int heads) {
+__global__ void __launch_bounds__(128) sum_tail_kernel(const __grid_constant__ SharedColumns a, const float* __restrict__ tail, int heads) {
   wait_for_earlier_grids();
+  const View4& shared = a.shared;
   const int dr = (int)shared.n[3];
   const int64_t a_head = shared.n[2] * dr / 4, total = shared.n[0] * a_head;
   for (int64_t i = (int64_t)blockIdx.x * 128 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 128) {
     const int64_t b = i / a_head, at = i - b * a_head, s = at * 4 / dr;
     const float4* src = reinterpret_cast<const float4*>(tail) + b * heads * a_head + at;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int terms = of_a_sequence(a.tokens, b, s) ? heads : 0;
 #pragma unroll 16
-    for (int h = 0; h < heads; ++h) {
+    for (int h = 0; h < terms; ++h) {
       const float4 x = __ldcs(src + h * a_head);
       sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
     }
@@ -639,9 +656,9 @@ cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t 
   return launch_counted(join_columns_kernel<uint16_t>, grid, kColumnThreads, 0, st, a, elt);
 }
 
-cudaError_t launch_sum_tail(int dtype, const View4& shared, const float* tail, int heads, cudaStream_t st) {
-  const dim3 grid(grid_for(shared.n[0] * shared.n[2] * shared.n[3], 512));
-  return with_type(dtype, [&]<typename T>() { return launch_counted(sum_tail_kernel<T>, grid, 128, 0, st, shared, tail, heads); });
+cudaError_t launch_sum_tail(int dtype, const SharedColumns& a, const float* tail, int heads, cudaStream_t st) {
+  const dim3 grid(grid_for(a.shared.n[0] * a.shared.n[2] * a.shared.n[3], 512));
+  return with_type(dtype, [&]<typename T>() { return launch_counted(sum_tail_kernel<T>, grid, 128, 0, st, a, tail, heads); });
 }
 
 cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st) {

@@ -54,8 +54,14 @@ struct PagedAttn {
 
 enum PagedKind : int { kPagedGeneral = 1, kPagedSplit = 2, kPagedLatent = 3 };
 
+// Which tokens of keys are of a sequence (Params' fields of the same names), of no more than max_sk keys.
+struct KeyTokens {
+  int32_t varlen_mode, batch, max_sk;
+  const int32_t *cu_k, *ss_k;
+};
 struct SharedColumns {
   View4 k, shared, out;              // (B, H, S, dn), (B, 1, S, dr), (B, H, S, dn + dr)
+  KeyTokens tokens;                  // the gradient's: rows of no sequence are zero
 };
 
 cudaError_t launch_block_tables(const BlockTables& a, cudaStream_t st);
@@ -76,6 +82,6 @@ cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t 
 cudaError_t launch_sum_columns(int dtype, const SharedColumns& a, cudaStream_t st);      // shared = sum over heads of out's last columns
 
 // ... from dK's last columns in 32 bits, (batch, kv heads, tokens, columns).
-cudaError_t launch_sum_tail(int dtype, const View4& shared, const float* tail, int heads, cudaStream_t st);
+cudaError_t launch_sum_tail(int dtype, const SharedColumns& a, const float* tail, int heads, cudaStream_t st);
 
 }  // namespace ab200

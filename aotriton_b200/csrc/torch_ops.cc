@@ -641,7 +641,6 @@ struct LatentAttend : torch::autograd::Function<LatentAttend> {
     const int64_t need = ab200_attn_bwd_shared_workspace(&a, (int32_t)c.columns, stream_handle());
     if (need < 0) check((hipError_t)-need, "latent_attention backward");
     const Tensor workspace = need > 0 ? fresh({need}, at::kFloat) : Tensor();
-    if (need > 0 && cu_q.defined()) workspace.zero_();
     check((hipError_t)ab200_attn_bwd_shared(&a, (int32_t)c.columns, &shared, need > 0 ? workspace.data_ptr<float>() : nullptr, (uint64_t)need, stream_handle()),
           "latent_attention backward");
     g_last_bwd_family.store(ab200_last_bwd_family(), std::memory_order_relaxed);
