@@ -281,7 +281,9 @@ __device__ __forceinline__ DkdvItem dkdv_item(const Params& p, int w) {
 // call's own: neither, dense causal 4 x 32 heads x 4096 of 128 1875 -> 1768, 64:8 heads x 16384, window 4096, 6530 -> 6200; bias,
 // 4 x 8 heads x 1024 of 64 131.5 -> 113.1, 4 x 8:2 heads x 1024 of 128 with dBias 228 -> 207; dropout, 16 packed sequences of 64 to 8192
 // tokens, 32:8 heads of 128, dK/dV 8980 -> 8713, dQ 5450 -> 4960; 16 x 12 x 391 of 64, training step, 324 -> 303.
-template <typename T, int HD, bool FUSED, bool EXACT, int FEAT>
+// TAIL: dK's last columns in 32 bits (Params::dk_tail).  An instantiation of its own: asked for at run time, it cost the backward of calls without
+// them 0.3 % (4 x 32 heads x 2048 of 128, causal, 533.8 -> 535.4 us; now 530.4 and 530.9 on another box).
+template <typename T, int HD, bool FUSED, bool EXACT, int FEAT, bool TAIL = false>
 __global__ void __launch_bounds__(FUSED ? kFusedThreads : kBwdThreads, 1)
 sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ CUtensorMap tm_q,
                       const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
@@ -632,7 +634,7 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
                    (sq.k0 + n) * p.dv.s[2];
           for (int c = 0; c < p.dqk; ++c) dkp[c] = from_f32<T>(0.f);
           for (int c = 0; c < p.dvo; ++c) dvp[c] = from_f32<T>(0.f);
-          if constexpr (FEAT == kPlain && !FUSED) { if (p.dk_tail != nullptr) zero_tail(p, sq, hk, n); }
+          if constexpr (TAIL) zero_tail(p, sq, hk, n);
         }
         __syncwarp();
         continue;
@@ -929,12 +931,15 @@ sm100_bwd_dkdv_kernel(const __grid_constant__ Params p, const __grid_constant__ 
         tc_fence_before();
         __syncwarp();
         keep_sums(0, p.dqk);
-        if constexpr (FEAT == kPlain && !FUSED) { if (p.dk_tail != nullptr) keep_tail(p, sq, hk, n, d0, v, p.sm_scale); __syncwarp(); }
+        if constexpr (TAIL) {
+          keep_tail(p, sq, hk, n, d0, v, p.sm_scale);
+          __syncwarp();
+        }
         stage_put32<T>(stage, r, d0, v, p.sm_scale, HD * 2);
         __syncwarp();
         warp_copy_out<T, 4>(stage, reinterpret_cast<T*>(p.dk.ptr) + (int64_t)sq.bidx * p.dk.s[0] + (int64_t)hk * p.dk.s[1] +
                                        (sq.k0 + it.n0) * p.dk.s[2],
-                            p.dk.s[2], nrows, FEAT == kPlain && !FUSED ? dk_columns(p) : p.dqk, quarter * 32, wg * 4, lane, HD * 2);
+                            p.dk.s[2], nrows, TAIL ? p.dk_tail_from : p.dqk, quarter * 32, wg * 4, lane, HD * 2);
         __syncwarp();
       }
       // The staging tile is the next item's dS^T tile: no compute warp may write dS^T there while
@@ -1449,7 +1454,7 @@ cudaError_t launch_bwd_T(int which, const Params& p, cudaStream_t st, float* dq_
   // make the stream's device, and remembered.
   struct PerDevice { std::atomic<unsigned int*> status{nullptr}; std::atomic<int> sms{0}; };
   static PerDevice per_device[64];
-  static std::atomic<bool> attr_set[64][24];
+  static std::atomic<bool> attr_set[64][26];
   const bool exact = p.varlen_mode == 0 && p.max_sq % 128 == 0 && p.max_sk % 128 == 0 && p.dqk == HD && p.dvo == HD;
   const int feat = features(p);
   int dev = 0;
@@ -1484,9 +1489,11 @@ cudaError_t launch_bwd_T(int which, const Params& p, cudaStream_t st, float* dq_
          sm100_bwd_dkdv_kernel<T, HD, false, true, kSinks>}};
     static constexpr Kernel kFused[4] = {sm100_bwd_dkdv_kernel<T, 128, true, false, kPlain>, sm100_bwd_dkdv_kernel<T, 128, true, false, kBias>,
                                          sm100_bwd_dkdv_kernel<T, 128, true, false, kDropout>, sm100_bwd_dkdv_kernel<T, 128, true, false, kAll>};
-    const Kernel kern_split = kSplit[exact][feat], kern_fused = kFused[feat & 3];
+    static constexpr Kernel kTail[2] = {sm100_bwd_dkdv_kernel<T, HD, false, false, kPlain, true>, sm100_bwd_dkdv_kernel<T, HD, false, true, kPlain, true>};
+    const bool tail = p.dk_tail != nullptr;      // (features are kPlain then)
+    const Kernel kern_split = tail ? kTail[exact] : kSplit[exact][feat], kern_fused = kFused[feat & 3];
     e = fused ? set_smem(16 + feat, reinterpret_cast<const void*>(kern_fused), BwdSmem<128>::kDynamic)
-              : set_smem(feat == kSinks ? 20 + exact : 2 * feat + exact, reinterpret_cast<const void*>(kern_split), L::kDynamic);
+              : set_smem(tail ? 24 + exact : (feat == kSinks ? 20 + exact : 2 * feat + exact), reinterpret_cast<const void*>(kern_split), L::kDynamic);
     if (e != cudaSuccess) return e;
     const int nitems = ((p.max_sk + kBlk - 1) / kBlk) * ((p.hk * p.batch + 7) / 8) * 8 +
                        (feat == kSinks ? p.batch * p.hk * ((p.sinks + kBlk - 1) / kBlk) * p.sink_chunks : 0);
