@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kWriteThreads) paged_write_kernel(const __grid
 
 // ---- attention, any type and size up to 1024 ----------------------------------------------------------------------
 // For what has no tensor-core kernel: fp32, odd head dims and pages.  Bound by instructions (a fused multiply-add a score and column on the ordinary pipe, and its
-// operands from shared memory).  16 sequences of 40 to 2000 fp32 keys, 32:8 heads of 128, 71 us (floor 21; three blocks an SM, with 112 registers and two 111).
+// operands from shared memory).  16 sequences of 40 to 2000 fp32 keys, 32:8 heads of 128, 72 us (floor 21).
 // Tiles of 32 keys: eight lanes form a key's scores with the unit's rows, a warp a row takes their softmax on, and a thread a column adds up
 // the values; with fewer columns than threads, groups of threads share the keys.
 constexpr int kGenThreads = 256, kGenRows = 8, kGenKeys = 32;
@@ -172,9 +172,15 @@ __device__ __forceinline__ void load_vec(const T* src, float (&x)[N]) {
   }
 }
 
+// Blocks an SM, for which a call is cut.  Values of one column a thread: three, 80 registers (the case above with 112 and two blocks 111 us; 16-bit rows read 16 bytes at a
+// time then keep 56 to 76 bytes in memory, and are faster all the same: 32 sequences of 100 to 4000 bf16 keys, 16:4 heads of 256, 291 us, with two blocks
+// and nothing there 368).  More columns: two, 102 to 123 registers (cut for three, which do not fit, a wave and a half: heads of 512 1434 us for 1091, 8 sequences
+// of 500 to 4000 fp32 latent rows x 16 heads 125 for 99).
+__host__ __device__ constexpr int gen_blocks(int columns) { return columns == 1 ? 3 : 2; }
+
 // J: columns of a thread.  N: elements of K that a lane reads at a time.
 template <typename T, int N, int J>
-__global__ void __launch_bounds__(kGenThreads, J == 1 ? 3 : 2) paged_general_kernel(const __grid_constant__ PagedAttn p) {
+__global__ void __launch_bounds__(kGenThreads, gen_blocks(J)) paged_general_kernel(const __grid_constant__ PagedAttn p) {
   wait_for_earlier_grids();
   extern __shared__ __align__(16) float q_s[];      // [kGenRows][dqk]
   __shared__ float scores[2][kGenRows][kGenKeys], alphas[2][kGenRows], m_s[kGenRows], l_s[kGenRows];      // (of a tile and the next one)
@@ -623,7 +629,7 @@ int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
     p.tile_log = 5;
     p.min_tiles = 2;
     p.extra = 1;
-    p.ctas = sms * 3;
+    p.ctas = sms * gen_blocks(p.dvo <= kGenThreads ? 1 : 4);
   }
   const int64_t chunks = ((int64_t)p.group * p.sq + p.rows - 1) / p.rows;
   p.chunks = (int)chunks;
