@@ -30,13 +30,13 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const __gri
   for (int z0 = 0; z0 < a.batch && (sums || tokens < t1); z0 += kTableThreads) {
     const int z = z0 + tid;
     int n = 0, m = 0, have = 0, need = 0;
+    // (of so many tokens; two numbers of 31 bits and a page's worth are within 32)
+    auto pages_for = [&](unsigned count) { return (int)min(count / (unsigned)a.page + (count % (unsigned)a.page != 0u), (unsigned)a.width); };
     if (z < a.batch) {
       n = max(a.lengths[z], 0);
       m = max(a.new_tokens[z], 0);
-      // (two numbers of 31 bits and a page's worth are within 32)
-      have = (int)min((unsigned)n / (unsigned)a.page + ((unsigned)n % (unsigned)a.page != 0u), (unsigned)a.width);
-      const unsigned all = (unsigned)n + (unsigned)m;
-      need = (int)min(all / (unsigned)a.page + (all % (unsigned)a.page != 0u), (unsigned)a.width) - have;
+      have = pages_for((unsigned)n);
+      need = pages_for((unsigned)n + (unsigned)m) - have;
     }
     int64_t up_t = m, up_p = need;
 #pragma unroll
@@ -57,10 +57,21 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const __gri
     fresh[tid] = pages + up_p - need - have;
     held[tid] = n;
     pages_of[tid] = have;
+    int got = m;      // its tokens with room among the slots: it holds those, and their pages are taken
+    if (sums && tokens + all_t > a.total) {
+      got = (int)min((int64_t)m, max(a.total - (tokens + up_t - m), (int64_t)0));
+      int64_t fewer = (int64_t)pages_for((unsigned)n + (unsigned)got) - have - need;
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) fewer += __shfl_xor_sync(0xffffffffu, fewer, d);
+      __syncthreads();      // (the warps' pages have been added up)
+      if (lane == 0) warp_pages[warp] = fewer;
+      __syncthreads();
+      for (int w = 0; w < kTableThreads / 32; ++w) all_p += warp_pages[w];
+    }
     if (sums && z < a.batch) {
       if (z == 0) a.cu_seqlens[0] = 0;
       a.cu_seqlens[z + 1] = (int)min(tokens + up_t, (int64_t)0x7fffffff);
-      a.new_lengths[z] = (int)min((int64_t)n + m, (int64_t)0x7fffffff);
+      a.new_lengths[z] = (int)min((int64_t)n + got, (int64_t)0x7fffffff);
     }
     __syncthreads();
     const int64_t from = max(tokens, t0), end = min(tokens + all_t, t1);

@@ -27,7 +27,7 @@ class BlockTables(NamedTuple):
     """What block_tables returns, all on the device."""
     slots: torch.Tensor         # (total_tokens,) int64: the slot of each new token, packed in order of sequence; -1: none
     cu_seqlens: torch.Tensor    # (batch + 1,) int32: running sums of the new tokens, as varlen_attention takes them
-    lengths: torch.Tensor       # (batch,) int32: the sequences' lengths with the new tokens
+    lengths: torch.Tensor       # (batch,) int32: the sequences' lengths with the new tokens that had room in total_tokens
     taken: torch.Tensor         # (1,) int32: pages of the free list that are gone now; more than it has: there were too few
 
 
@@ -66,8 +66,9 @@ def block_tables(block_table, lengths, new_tokens, free_pages, page_size, total_
     first ceil(lengths[z] / page_size) entries are its own; the pages it needs beyond them are taken off the free list in order of sequence and position
     and entered into its row, the rest of which is left as it is.  Calling it again on the same arguments gives the same.
 
-    total_tokens, a number, is at least the sum of new_tokens (what is beyond it gets neither slot nor page); slots behind that sum are -1.  Where the row is too
-    short or the free list used up, tokens have the slot -1 (paged_write skips them), and `taken` exceeds the length of the free list in the second case."""
+    total_tokens, a number, is the room for slots, at least the sum of new_tokens as a rule; slots behind that sum are -1.  Tokens beyond it get neither slot nor page,
+    and `lengths` and `taken` do not count them (cu_seqlens does): a later step can take them.  Where the row is too short or the free list used up, tokens have the
+    slot -1 (paged_write skips them) and count, and `taken` exceeds the length of the free list in the second case."""
     if not torch.compiler.is_compiling():
         r = _native.block_tables(block_table, lengths, new_tokens, free_pages, page_size, total_tokens, taken)
         if r is not None:

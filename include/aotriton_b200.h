@@ -272,10 +272,10 @@ typedef struct ab200_block_tables_args {
   const int32_t* free_pages;
   int64_t num_free;
   const int32_t* taken;         /* device scalar: how many of free_pages are gone already; NULL -> 0     */
-  int64_t total_tokens;         /* room of `slots`, at least the sum of new_tokens (what is beyond gets neither slot nor page) */
+  int64_t total_tokens;         /* room of `slots`; tokens beyond it get neither slot nor page, and new_lengths and taken_out leave them out */
   int64_t* slots;               /* packed in order of sequence; -1 behind the last token                 */
   int32_t* cu_seqlens;          /* batch + 1: running sums of new_tokens                                 */
-  int32_t* new_lengths;         /* lengths + new_tokens                                                  */
+  int32_t* new_lengths;         /* lengths and the new tokens that had room                              */
   int32_t* taken_out;           /* taken + pages taken now; above num_free: there were too few           */
 } ab200_block_tables_args;
 
