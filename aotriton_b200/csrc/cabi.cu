@@ -1148,11 +1148,14 @@ int ab200_sum_columns(const ab200_shared_columns_args* a, void* stream) {
 static int64_t plan_bwd_shared(const ab200_attn_bwd_args* a, int columns, Params& p) {
   if (int e = fill_bwd(a, p, true)) return -e;
   if (columns < 1 || columns >= p.dqk) return -kErrInvalidValue;
+  for (int i = 0; i < 3; ++i)
+    if (p.k.n[i] < 0 || p.k.n[i] > INT32_MAX) return -kErrInvalidValue;
+  // (the workspace's rows are those of k: what the kernels write has to be among them)
+  const bool packed = p.varlen_mode == 1;
+  if (p.batch > 0 && (p.k.n[0] < (packed ? 1 : p.batch) || (!packed && p.k.n[2] < p.max_sk))) return -kErrInvalidValue;
   const int sel = ab200_select_variant(kOpBwd, a->prob.dtype, p.dqk, p.dvo, family_flags(g_family) | (sm100_bwd_supported(a->prob.dtype, p) ? AB200_SELECT_ALIGNED : 0));
   if (sel < 0) return sel;
   if ((sel & 0xff) < kVarTcgen05 || features(p) != kPlain || columns % 8 != 0) return 0;
-  for (int i = 0; i < 3; ++i)
-    if (p.k.n[i] < 0 || p.k.n[i] > INT32_MAX) return -kErrInvalidValue;
   return p.k.n[0] * p.hk * p.k.n[2] * columns;
 }
 

@@ -344,7 +344,8 @@ AB200_API int ab200_sum_columns(const ab200_shared_columns_args* args, void* str
 
 /* ab200_attn_bwd for joined keys whose last `columns` columns all heads share: dK as there, but that its last columns may be left unwritten, and `shared`,
  * (B, 1, S, columns), their sum over the kv heads, zero for tokens of no sequence (whatever dK and the workspace hold there).  The sums are taken from 32 bits, for which the workspace has room (16-byte aligned; contents do not matter, calls that may overlap need one each); where it is
- * of no floats, from dK itself.  The fused form does not apply. */
+ * of no floats, from dK itself.  k.size says how many batch elements and tokens there are, at least the
+ * problem's (packed: one, and its tokens).  The fused form does not apply. */
 AB200_API int ab200_attn_bwd_shared(const ab200_attn_bwd_args* args, int32_t columns, const ab200_view4* shared, float* workspace, uint64_t workspace_floats,
                                     void* stream);
 /* Floats of workspace that call needs (0: none), or the negated error code.  Launches nothing. */
