@@ -647,20 +647,42 @@ int64_t plan_paged(int dtype, PagedAttn& p, int sms) {
   // (a last tile's keys are counted in 32 bits)
   p.max_len = (int32_t)std::min<int64_t>((int64_t)p.width * p.page, 0x7fffff00);
   const int64_t most = (p.max_len >> p.tile_log) + 2 + p.extra;      // tiles of a unit: a window may cross a border
-  const int64_t units = (int64_t)p.batch * p.hk * chunks;
-  if (units * most > 0x3fffffff) return -kPagedTooLarge;
+  // What the tables have room for is all that is known here of the lengths: where that is more than 31 bits count, a few launches take some sequences each.
+  const int64_t fit = 0x3fffffff / ((int64_t)p.hk * chunks * most);
+  if (fit == 0) return -kPagedTooLarge;
+  const int64_t launches = (p.batch + fit - 1) / fit;
+  p.slice = (int32_t)((p.batch + launches - 1) / launches);
+  const int64_t units = (int64_t)p.slice * p.hk * chunks;
   // A kv head's chunks side by side, so that its keys come from memory once, unless that left too few CTAs to share a line out evenly.
   p.lanes = chunks <= 8 ? (int)chunks : 1;
   p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(p.ctas / p.lanes, units / p.lanes * most / p.min_tiles + 1)) * p.lanes;
   return 2 * (int64_t)p.ctas * partial_floats(p);
 }
 
-cudaError_t launch_paged(int dtype, PagedAttn& p, cudaStream_t st) {
+static cudaError_t launch_paged_slice(int dtype, PagedAttn& p, cudaStream_t st) {
   cudaError_t e = p.kind == kPagedSplit    ? launch_paged_split(dtype, p, st)
                   : p.kind == kPagedLatent ? launch_paged_latent(dtype, p, st)
                                            : with_type(dtype, [&]<typename T>() { return launch_general_T<T>(p, st); });
   if (e == cudaSuccess) e = with_type(dtype, [&]<typename T>() { return launch_join_T<T>(p, st); });
   return e;
+}
+cudaError_t launch_paged(int dtype, PagedAttn& p, cudaStream_t st) {
+  if (p.slice >= p.batch) return launch_paged_slice(dtype, p, st);
+  const int64_t elt = dtype == 1 ? 4 : 2;
+  for (int z = 0; z < p.batch; z += p.slice) {      // (one behind the other: they share the workspace)
+    PagedAttn s = p;
+    s.batch = std::min(p.slice, p.batch - z);
+    for (View4* v : {&s.q, &s.out}) {
+      v->ptr = static_cast<char*>(v->ptr) + z * v->s[0] * elt;
+      v->n[0] = s.batch;
+    }
+    s.table += z * p.table_stride;
+    s.lengths += z;
+    if (s.query_lengths != nullptr) s.query_lengths += z;
+    if (s.lse != nullptr) s.lse += (int64_t)z * p.hq * p.sq;
+    if (const cudaError_t e = launch_paged_slice(dtype, s, st)) return e;
+  }
+  return cudaSuccess;
 }
 
 cudaError_t launch_join_columns(int dtype, const SharedColumns& a, cudaStream_t st) {

@@ -43,8 +43,8 @@ struct PagedAttn {
   int32_t max_len;                   // what the table has room for
   // How the call is cut (plan_paged, paged_split.cuh): into units -- (sequence, kv head, chunk of `rows` query rows) -- and tiles of 2^tile_log keys, for `ctas`
   // CTAs, min_tiles a CTA at least, a unit counted as `extra` tiles more than it has; `lanes` chunks side by side (a divisor of the chunks, and of the CTAs).
-  // box: slots of a tile copy.
-  int32_t kind, ctas, lanes, rows, chunks, tile_log, min_tiles, extra, box;
+  // box: slots of a tile copy.  slice: sequences of a launch, fewer than all where their tables have room for more tiles than are counted.
+  int32_t kind, ctas, lanes, rows, chunks, tile_log, min_tiles, extra, box, slice;
   int32_t q_tiles;                   // latent attention: the queries come as tile copies
   unsigned int* status;              // the word in which a kernel records a wait that ran out (null: the general kernel has none)
   float* partial;                    // two partial results a CTA: of the unit that it starts with, of the one that it ends with
@@ -66,7 +66,8 @@ struct SharedColumns {
 
 cudaError_t launch_block_tables(const BlockTables& a, cudaStream_t st);
 cudaError_t launch_paged_write(int dtype, const PagedWrite& a, cudaStream_t st);
-// Chooses the kernel and how the call is cut for `sms` SMs; returns the floats of workspace it needs, or -kPagedTooLarge: more tiles than are counted.
+// Chooses the kernel and how the call is cut for `sms` SMs; returns the floats of workspace it needs, or -kPagedTooLarge: a table row with room for more tiles than
+// are counted.
 constexpr int64_t kPagedTooLarge = 1;
 int64_t plan_paged(int dtype, PagedAttn& a, int sms);
 cudaError_t launch_paged(int dtype, PagedAttn& a, cudaStream_t st);
