@@ -187,12 +187,13 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sink
 
     fp16 and bf16 with head dims up to 128 that are multiples of 8, 16-byte aligned caches, pages of a multiple of 8 slots and few queries are fastest."""
     sm_scale = q.shape[-1] ** -0.5 if sm_scale is None else sm_scale
-    if not torch.compiler.is_compiling():
+    number = type(v_cache) is int      # (which the native route takes for a latent cache's value_dim)
+    if not number and not torch.compiler.is_compiling():
         r = _native.paged_attention(q, k_cache, v_cache, block_table, lengths, query_lengths, window, sinks, sm_scale, return_lse)
         if r is not None:
             return r
     for t in (k_cache, v_cache):
-        if not _is_cache(t, q) or t.shape[:3] != k_cache.shape[:3]:
+        if number or not _is_cache(t, q) or t.shape[:3] != k_cache.shape[:3]:
             raise ValueError("paged_attention: the caches are (pages, page_size, heads, dim) tensors of q's device and type with unit innermost stride")
     if k_cache.shape[3] != q.shape[-1]:
         raise ValueError(f"paged_attention: head dims {q.shape[-1]} of q and {k_cache.shape[3]} of the keys")

@@ -1,8 +1,9 @@
-"""CPU: how calls over pages are cut, on a pretended device."""
+"""CPU: how calls over pages are cut, on a pretended device; a refusal."""
 import pytest
+import torch
 
-from aotriton_b200 import cabi
-from test_paged_host import _attn_args, fake  # noqa: F401  (a fixture)
+from aotriton_b200 import cabi, paged
+from test_paged_host import T, _attn_args, _ints, fake  # noqa: F401  (a fixture)
 
 
 @pytest.mark.parametrize("dtype", [cabi.DTYPE_FP32, cabi.DTYPE_BF16])
@@ -29,3 +30,9 @@ def test_tables_with_room_for_more_tiles_than_are_counted(fake):  # noqa: F811
     for after, launches in ((0, 1), (1, 2), (2, 3)):      # an error on the way comes back, with nothing launched after it
         fake.ab200_debug_host_calls(1, 7, 98, after)
         assert f(a, None) == 98 and count() == launches
+
+
+def test_a_number_for_the_values_is_no_latent_cache():
+    dev = torch.device("cpu")
+    with pytest.raises(ValueError, match="paged_attention: the caches"):
+        paged.paged_attention(T(2, 16, 1, 576, device=dev), T(9, 16, 576, device=dev), 512, _ints(2, 5), _ints(2))
