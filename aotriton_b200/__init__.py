@@ -6,7 +6,10 @@ API of ROCm/aotriton.
                           bindings, argument-for-argument like the reference's
                           modules/flash/tests/aotriton_flash.py
   aotriton_b200.autograd  torch.autograd.Function wrappers (attention, varlen_attention; sink_attention,
-                          varlen_sink_attention, relative_position_bias, dropout)
+                          varlen_sink_attention, relative_position_bias, dropout; latent_attention,
+                          varlen_latent_attention)
+  aotriton_b200.paged     serving from a cache in pages (block_tables, paged_write, paged_attention,
+                          paged_latent_attention)
   aotriton_b200.sharding  batch x head partitioning for multi-GPU runs
   aotriton_b200.build     in-tree nvcc build
 

@@ -178,8 +178,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, window=None, sink
     """Attention of the last Sq tokens of each sequence over its pages.  q: (B, Hq, Sq, D) of any strides; caches (pages, page_size, Hk, D), fewer heads than q's
     for GQA; block_table: (B, width) int32; lengths: (B,) int32, keys of each sequence, the queries' own among them (block_tables' lengths
     of this step).  Query m stands at position P = lengths - Sq + m and sees the keys n <= P; with a window those with n > P - window
-    or n < sinks, as in sink_attention.  query_lengths: (B,) int32, where sequences have fewer queries than Sq, the first of their rows; the others' output is
-    zero.  Returns (B, Hq, Sq, Dv) and, if asked for, the log-sum-exp (B * Hq, Sq).
+    or n < sinks, as in sink_attention.  query_lengths: (B,) int32, where sequences have fewer queries than Sq: theirs are the first of their rows, at
+    P = lengths - query_lengths + m, and the other rows' output is zero.  Returns (B, Hq, Sq, Dv) and, if asked for, the log-sum-exp (B * Hq, Sq).
 
     Rows that see nothing give zeros (log-sum-exp +inf), positions below 0 among them.  Keys of pages outside the cache (table entries below 0, say) are seen by nobody;
     what slots hold that nobody sees, NaN included, does not matter.  The work is shared out on the device by the lengths, so that

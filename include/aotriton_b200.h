@@ -327,7 +327,8 @@ typedef struct ab200_paged_attn_args {
 } ab200_paged_attn_args;
 
 AB200_API int ab200_paged_attn(const ab200_paged_attn_args* args, void* stream);
-/* Floats of workspace the call needs (it does not depend on the lengths), or the negated error code.  Launches nothing. */
+/* Floats of workspace the call needs, or the negated error code.  It does not depend on what the lengths hold, but on the kernel that takes the call, which pointers,
+ * strides and the window have a say in beside the shape: ask with the arguments of the call itself.  Launches nothing. */
 AB200_API int64_t ab200_paged_attn_workspace(const ab200_paged_attn_args* args, void* stream);
 
 /* Keys whose last columns all heads share: joined[b, h, s] = (k[b, h, s], shared[b, 0, s]); and the gradient of the shared columns, shared[b, 0, s] = the sum
