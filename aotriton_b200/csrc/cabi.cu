@@ -1184,7 +1184,7 @@ int ab200_attn_bwd_shared(const ab200_attn_bwd_args* a, int32_t columns, const a
   if (int e = fill_shared_columns(&c, s, true)) return e;
   if (int e = attn_bwd(a, floats > 0 ? workspace : nullptr, p.dqk - columns, stream)) return e;
   if (s.shared.n[0] == 0 || s.shared.n[2] == 0) return 0;
-  s.tokens = KeyTokens{p.varlen_mode, p.batch, p.max_sk, p.cu_k, p.ss_k};
+  s.tokens = KeyTokens{p.varlen_mode, p.batch, p.max_sq > 0 ? p.max_sk : 0, p.cu_k, p.ss_k};      // (no queries: no kernel has written dK)
   DeviceGuard guard(st);
   return (int)(floats > 0 ? launch_sum_tail(a->prob.dtype, s, workspace, p.hk, st) : launch_sum_columns(a->prob.dtype, s, st));
 }

@@ -99,3 +99,26 @@ def test_rows_of_no_sequence_are_zero(dtype, dn, dr, dv, tail, layout):
         w, most = _want(q[z, :, q0:q0 + mq], k[z, :, k0:k0 + mk], v[z, :, k0:k0 + mk], do[z, :, q0:q0 + mq], scale, dr, not tail)
         assert ((got - w).abs() <= most + 1e-30).all(), float((got - w).abs().max())
     assert (shared[:, 0][~inside] == 0).all()
+
+
+@pytest.mark.parametrize("layout", ["dense", "compact", "padded"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_problem_without_queries(dtype, layout):
+    """No kernel runs, dK is left as it is, and nothing of it is summed."""
+    h, hk, d, dv, dr, nk = 4, 2, 192, 128, 64, 40
+    q, k, v, do = (torch.randn(1, n, s, w, device="cuda").to(dtype) for n, s, w in ((h, 5, d), (hk, nk, d), (hk, nk, dv), (h, 5, dv)))
+    dq, dk, dv_ = (torch.full_like(t, math.nan) for t in (q, k, v))
+    lse, delta = (torch.zeros(h, 5, device="cuda") for _ in range(2))
+    kw = dict(sm_scale=0.1)
+    if layout != "dense":
+        ends = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 0], [0, nk])]
+        kw.update(cu_seqlens_q=ends[0], cu_seqlens_k=ends[1], max_seqlen_q=0, max_seqlen_k=nk, varlen_type=cabi.VARLEN_PADDED if layout == "padded" else cabi.VARLEN_COMPACT)
+    a = cabi.make_bwd_args(q, k, v, do, do, dq, dk, dv_, lse, delta, **kw)
+    a.prob.max_seqlen_q = 0
+    shared = torch.full((1, 1, nk, dr), math.nan, device="cuda", dtype=dtype)
+    L, stream = cabi.lib(), cabi.current_stream_handle()
+    need = L.ab200_attn_bwd_shared_workspace(a, dr, stream)
+    assert need >= 0
+    workspace = torch.full([max(need, 4)], math.nan, device="cuda")
+    assert L.ab200_attn_bwd_shared(a, dr, cabi.view4(shared), workspace.data_ptr(), need, stream) == 0
+    assert (shared == 0).all()
